@@ -239,13 +239,19 @@ def _plain_orth(x):
     return (x.transpose(-1, -2) if tall else x).to(torch.bfloat16)
 
 
+def _row_scales(x):
+    """Largest magnitude of each row over 127, an IEEE division (by a tensor: by a number torch takes its reciprocal)."""
+    most = x.float().abs().amax(dim=1)
+    return most / torch.full_like(most, 127.0)
+
+
 def _plain_int8(s):
     x = s["x"]
     if s["case"]["x"] == "ram":
         xq, xs, out = x.float(), 1.0 / 255.0, {}
     else:
         xf = x.float()
-        scale = xf.abs().amax(dim=1) / 127.0
+        scale = _row_scales(x)
         xq = torch.round(xf / torch.where(scale > 0, scale, 1.0)[:, None])
         xs, out = scale[:, None], {"q": xq.to(torch.int8), "scale": scale}
     y = (xq @ s["w_q"].float().T) * xs * s["w_scale"] + s["bias"]
@@ -375,7 +381,8 @@ def exact(case, seed):
     if case["x"] == "ram":
         y, out = torch.einsum("mk,nk->mn", x, w) / 255.0, {}
     else:
-        scale = s["x"].float().abs().amax(dim=1) / 127.0
+        most = s["x"].float().abs().amax(dim=1)
+        scale = most / torch.full_like(most, 127.0)
         q = torch.round(s["x"].float() / torch.where(scale > 0, scale, 1.0)[:, None])
         y = torch.einsum("mk,nk->mn", q.double(), w) * scale.double()[:, None]
         out = {"q": None, "scale": scale.double()}
