@@ -1,0 +1,70 @@
+/*
+ * nesle_ops.h -- C ABI of the policy-learning operators.
+ *
+ * Operators of a recurrent actor-critic on the batched core: the 8-bit product
+ * that reads RAM observations as they are, the gated delta rule that gives the
+ * policy a memory over time, and the Newton-Schulz orthogonalisation of matrix
+ * updates.  No counterpart in the reference.
+ *
+ * All pointers are device memory of `device`.  Calls are asynchronous on
+ * `stream` (a cudaStream_t as void*, NULL = the legacy default stream), allocate
+ * nothing and can be captured in a CUDA graph; scratch memory is the caller's.
+ * Status codes and nesle_last_error() are those of nesle_b200.h.
+ */
+#ifndef NESLE_OPS_H
+#define NESLE_OPS_H
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define NESLE_F32 0
+#define NESLE_BF16 1
+#define NESLE_F16 2
+
+/* Times that a kernel of this file gave up on an internal wait on `device`
+ * (its outputs are then invalid); 0 unless something is broken.  Synchronous. */
+int nesle_ops_stalls(int device, uint32_t* count);
+
+/* Symmetric quantisation of each row to 8 bits: scale = max|x| / 127, q =
+ * round-half-even(x / scale), both divisions in IEEE fp32; a row of zeros gets
+ * scale 0 and zeros.  A row that holds a NaN or an infinity gets that scale, and
+ * zeros where x / scale is not a number.  Columns cols..ld_q-1 of q are set to
+ * zero (ld_q - cols < 16).  ld_* in elements. */
+int nesle_quantize_rows(const void* x, int dtype, uint64_t rows, uint64_t cols, int64_t ld_x, int8_t* q, int64_t ld_q,
+                        float* scale, int device, void* stream);
+
+typedef struct nesle_int8_args {
+    const void* x;         /* [m][k] 8-bit integers, rows ld_x bytes apart */
+    int x_unsigned;        /* x is uint8 (else int8) */
+    int64_t ld_x;
+    const float* x_scale;  /* [m], or NULL: x_scale_value for every token */
+    float x_scale_value;
+    const int8_t* w;       /* [n][ld_w] int8, zeros from k to ld_w; ld_w a multiple of 16, 16-byte aligned */
+    const uint8_t* w_biased; /* [n][ld_w] the same weights + 128 (read where x is unsigned) */
+    int64_t ld_w;
+    const float* w_scale;  /* [n] */
+    const float* bias;     /* [n] or NULL */
+    void* y;               /* [m][n], rows ld_y elements apart */
+    int y_dtype;           /* NESLE_F32, NESLE_BF16 or NESLE_F16 */
+    int64_t ld_y;
+    uint64_t m, k, n;
+    int relu;
+    void* workspace;       /* nesle_int8_workspace bytes, 16-byte aligned */
+    uint64_t workspace_bytes;
+    int device;
+} nesle_int8_args;
+
+/* y[m][n] = act(x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]); the sum is exact in 32-bit integers, which
+ * bounds k: 33,025 for unsigned x (255 * 255 k < 2^31), 131,072 for signed. */
+int nesle_int8_linear(const nesle_int8_args* args, void* stream);
+/* Scratch bytes that the call needs (0 where x is 16-byte aligned with rows a multiple of 16 bytes apart). */
+uint64_t nesle_int8_workspace(const nesle_int8_args* args);
+
+#ifdef __cplusplus
+}
+#endif
+#endif

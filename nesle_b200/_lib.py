@@ -1,4 +1,4 @@
-"""ctypes binding of libnesle_b200.so (include/nesle_b200.h).
+"""ctypes binding of libnesle_b200.so (include/nesle_b200.h, include/nesle_ops.h).
 
 Loading fails loudly: there is no CPU fallback.  The library is built in-tree
 by ``python -m nesle_b200.build`` (``__graft_entry__.build()``).
@@ -19,6 +19,8 @@ ACTIONS_U8, ACTIONS_I64 = 0, 1
 RENDER_RGB, RENDER_INDEX, RENDER_GRAY84 = 0, 1, 2
 PTR_RAM, PTR_LAST_REWARDS, PTR_LAST_DONE, PTR_FRAMES_RGB, PTR_FRAMES_INDEX, PTR_OBS_GRAY84, PTR_REWARDS, \
     PTR_DONE = range(8)
+
+F32, BF16, F16 = 0, 1, 2
 
 _u8p = ctypes.POINTER(ctypes.c_uint8)
 
@@ -54,7 +56,16 @@ class FcsState(ctypes.Structure):
                 ("oam", ctypes.c_uint8 * 256)]
 
 
-# Exported symbols and their ctypes signatures (every function include/nesle_b200.h declares).
+class Int8Args(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("x_unsigned", ctypes.c_int), ("ld_x", ctypes.c_int64),
+                ("x_scale", ctypes.c_void_p), ("x_scale_value", ctypes.c_float), ("w", ctypes.c_void_p),
+                ("w_biased", ctypes.c_void_p), ("ld_w", ctypes.c_int64), ("w_scale", ctypes.c_void_p),
+                ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_dtype", ctypes.c_int), ("ld_y", ctypes.c_int64),
+                ("m", ctypes.c_uint64), ("k", ctypes.c_uint64), ("n", ctypes.c_uint64), ("relu", ctypes.c_int),
+                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("device", ctypes.c_int)]
+
+
+# Exported symbols and their ctypes signatures (every function include/*.h declares).
 SIGNATURES = {
     "nesle_create": (ctypes.c_int, [ctypes.POINTER(CreateArgs), ctypes.POINTER(ctypes.c_void_p)]),
     "nesle_destroy": (ctypes.c_int, [ctypes.c_void_p]),
@@ -87,6 +98,12 @@ SIGNATURES = {
     "nesle_parse_fcs": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_size_t, ctypes.POINTER(FcsState)]),
     "nesle_last_error": (ctypes.c_char_p, []),
     "nesle_abi_version": (ctypes.c_int, []),
+    "nesle_ops_stalls": (ctypes.c_int, [ctypes.c_int, ctypes.POINTER(ctypes.c_uint32)]),
+    "nesle_quantize_rows": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint64,
+                                           ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
+                                           ctypes.c_int, ctypes.c_void_p]),
+    "nesle_int8_linear": (ctypes.c_int, [ctypes.POINTER(Int8Args), ctypes.c_void_p]),
+    "nesle_int8_workspace": (ctypes.c_uint64, [ctypes.POINTER(Int8Args)]),
 }
 
 # EnvRecord (csrc/nesle_state.h), the first 128 bytes of a saved state blob.

@@ -10,14 +10,19 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 ROOT = PKG.parent
 LIB = PKG / "libnesle_b200.so"
-SOURCES = ["kernels.cu", "capi.cu", "formats.cpp"]
-DEPS = SOURCES + ["kernels.h", "nes_core.cuh", "nes_render.cuh", "nes_v2.cuh", "nesle_state.h", "formats.h"]
+OBJ = CSRC / "_build"
+_CORE = ["kernels.h", "nes_core.cuh", "nes_render.cuh", "nes_v2.cuh", "nesle_state.h", "formats.h"]
+_OPS = ["ops_common.h", "tc05.cuh"]
+# source -> the headers it includes; each source is one object, compiled when it or a header is newer
+SOURCES = {"kernels.cu": _CORE, "capi.cu": _CORE, "formats.cpp": _CORE, "ops_common.cu": _OPS, "ops_int8.cu": _OPS}
+HEADERS = [ROOT / "include" / "nesle_b200.h", ROOT / "include" / "nesle_ops.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 
@@ -28,24 +33,37 @@ def nvcc() -> str:
     return exe
 
 
+def _newest(src: str) -> float:
+    return max(p.stat().st_mtime for p in [CSRC / src, *(CSRC / h for h in SOURCES[src]), *HEADERS])
+
+
 def needs_build() -> bool:
-    if not LIB.exists():
-        return True
-    t = LIB.stat().st_mtime
-    deps = [CSRC / d for d in DEPS] + [ROOT / "include" / "nesle_b200.h"]
-    return any(d.stat().st_mtime > t for d in deps)
+    return not LIB.exists() or any(_newest(s) > LIB.stat().st_mtime for s in SOURCES)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     if not force and not needs_build():
         return LIB
-    tmp = LIB.with_suffix(".so.tmp")
-    cmd = [nvcc(), "-std=c++20", "-O3", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC", "-shared",
-           "-I", str(ROOT / "include"), "-o", str(tmp), *[str(CSRC / s) for s in SOURCES]]
+    OBJ.mkdir(exist_ok=True)
+    flags = ["-std=c++20", "-O3", *ARCH, "-lineinfo", "-Xcompiler", "-fPIC", "-I", str(ROOT / "include")]
     if verbose:
-        cmd.insert(1, "-Xptxas=-v")
-        print(" ".join(cmd), flush=True)
-    subprocess.run(cmd, check=True, cwd=str(CSRC))
+        flags.insert(0, "-Xptxas=-v")
+
+    def compile_one(src: str) -> Path:
+        obj = OBJ / (src + ".o")
+        if force or not obj.exists() or _newest(src) > obj.stat().st_mtime:
+            tmp = OBJ / f"{src}.{os.getpid()}.tmp.o"
+            cmd = [nvcc(), *flags, "-c", "-o", str(tmp), str(CSRC / src)]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            subprocess.run(cmd, check=True, cwd=str(CSRC))
+            os.replace(tmp, obj)
+        return obj
+
+    with ThreadPoolExecutor(len(SOURCES)) as pool:
+        objects = list(pool.map(compile_one, SOURCES))
+    tmp = LIB.with_suffix(".so.tmp")
+    subprocess.run([nvcc(), *ARCH, "-shared", "-o", str(tmp), *map(str, objects)], check=True, cwd=str(CSRC))
     os.replace(tmp, LIB)
     return LIB
 

@@ -49,6 +49,17 @@ int bcd3(const uint8_t* ram, int a) { return (ram[a] & 0xF) * 100 + (ram[a + 1] 
 
 }  // namespace
 
+namespace nesle {
+// The operator files (ops_*.cu) report through the same thread-local message.
+int set_error(int code, const char* message) noexcept {
+    try {
+        g_err = message;
+    } catch (...) {  // out of host memory: the code alone
+    }
+    return code;
+}
+}  // namespace nesle
+
 constexpr uint32_t kRenderChunks = 8;  // env ranges of nesle_render_copy
 
 struct nesle_batch {

@@ -1,0 +1,90 @@
+// ops_common.h -- what the operator files (ops_*.cu) share: error reporting,
+// the device guard, element types and tensor-map encoding.
+#pragma once
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include <exception>
+#include <string>
+
+#include "../../include/nesle_b200.h"
+#include "../../include/nesle_ops.h"
+
+namespace nesle {
+
+// Sets the thread's last error (nesle_last_error) and returns `code`; in capi.cu.
+int set_error(int code, const char* message) noexcept;
+
+namespace ops {
+
+inline int invalid(const char* m) { return set_error(NESLE_ERR_INVALID, m); }
+
+inline int cuda_status(cudaError_t e, const char* where) {
+    if (e == cudaSuccess) return NESLE_OK;
+    return set_error(NESLE_ERR_CUDA, (std::string(where) + ": " + cudaGetErrorString(e)).c_str());
+}
+
+// Runs a C entry's body: no C++ exception leaves the library.
+template <class F>
+int guarded(F&& body) noexcept {
+    try {
+        return body();
+    } catch (const std::exception& e) {
+        return set_error(NESLE_ERR_RUNTIME, e.what());
+    } catch (...) {
+        return set_error(NESLE_ERR_RUNTIME, "unknown C++ exception");
+    }
+}
+
+// Makes `device` current for the scope.
+struct OnDevice {
+    int prev = -1;
+    bool ok = true;
+    explicit OnDevice(int device) {
+        ok = cudaGetDevice(&prev) == cudaSuccess && (prev == device || cudaSetDevice(device) == cudaSuccess);
+    }
+    ~OnDevice() {
+        int cur = -1;
+        if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);
+    }
+};
+
+int sm_count(int device);
+
+// The device address of the stall counter, which kernels add to when a wait gives up.
+int stall_counter(int device, unsigned int** out);
+
+// A tiled tensor map over `rank` dimensions, innermost first; `strides` are the
+// byte strides of dimensions 1..rank-1.  128-byte swizzle, zero fill.
+int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
+               const uint64_t* strides, const uint32_t* box);
+
+// Allows a kernel its dynamic shared memory (an attribute of the function on the current device).
+template <class K>
+cudaError_t allow_smem(K* kernel, int bytes) {
+    return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
+template <class T>
+__device__ __forceinline__ float to_f32(T x);
+template <>
+__device__ __forceinline__ float to_f32(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f32(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <>
+__device__ __forceinline__ float to_f32(__half x) { return __half2float(x); }
+
+template <class T>
+__device__ __forceinline__ T from_f32(float x);
+template <>
+__device__ __forceinline__ float from_f32(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_f32(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x); }
+
+}  // namespace ops
+}  // namespace nesle

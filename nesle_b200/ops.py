@@ -1,0 +1,175 @@
+"""Policy-learning operators on the GPU (include/nesle_ops.h): what a recurrent
+actor-critic on the batched core computes beside the env step.
+
+* ``int8_linear`` / ``quantize_rows`` / ``Int8Weight`` -- product of 8-bit
+  integers with a scale for each token and channel.  RAM observations are bytes
+  already and go in as they are.
+
+Calls go on the caller's current torch stream, return before the work is done,
+and never synchronise the host.  Argument errors raise ValueError, CUDA errors
+RuntimeError.  There is no CPU fallback: tensors must be on a CUDA device.
+No counterpart in the reference.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _lib
+
+__all__ = ["Int8Weight", "int8_linear", "quantize_rows", "stalls"]
+
+_DTYPE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _require(ok: bool, message: str) -> None:
+    if not ok:
+        raise ValueError(message)
+
+
+def _on(x: torch.Tensor, device: torch.device, name: str) -> None:
+    _require(isinstance(x, torch.Tensor) and x.device == device, f"{name} must be a tensor on {device}")
+
+
+def _cuda_device(x, name: str) -> torch.device:
+    _require(isinstance(x, torch.Tensor) and x.is_cuda, f"{name} must be a CUDA tensor")
+    return x.device
+
+
+def _stream(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _no_grad_path(name: str, *tensors) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError(f"{name} has no gradient; call it under torch.no_grad() or on detached tensors")
+
+
+def stalls(device: int = 0) -> int:
+    """Times that a kernel gave up on an internal wait (0 unless something is broken); synchronises."""
+    n = ctypes.c_uint32()
+    _lib.check(_lib.load().nesle_ops_stalls(device, ctypes.byref(n)))
+    return n.value
+
+
+# ------------------------------------------------------------------ 8-bit product
+
+def _rows(x: torch.Tensor) -> torch.Tensor:
+    """(..., cols) as (rows, cols) with unit column stride; copies only where the layout has to change."""
+    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
+    return x if x.stride(1) == 1 or x.shape[1] <= 1 else x.contiguous()
+
+
+def _ld(x: torch.Tensor) -> int:
+    """Row stride of a 2-D tensor; where a stride carries no meaning (one row, or none) the row length."""
+    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1)
+
+
+def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Symmetric 8-bit quantisation of the last dimension: ``(q, scale)`` with ``q = round(x / scale)`` (half to even)
+    in [-127, 127], ``scale = max|x| / 127`` in fp32, of shapes ``x.shape`` and ``x.shape[:-1]``.  A zero row has scale
+    0.  A NaN or an infinity in a row becomes the row's scale.  ``q``'s rows lie a multiple of 16 bytes apart, as
+    :func:`int8_linear` reads them best."""
+    dev = _cuda_device(x, "x")
+    _require(x.dtype in _DTYPE, "x must be float32, bfloat16 or float16")
+    _require(x.dim() >= 1, "x needs at least one dimension")
+    _no_grad_path("quantize_rows", x)
+    shape, x = x.shape, x if x.dim() > 1 else x[None]
+    cols = shape[-1]
+    if cols == 0:
+        return x.new_empty(shape, dtype=torch.int8), x.new_zeros(shape[:-1], dtype=torch.float32)
+    x2 = _rows(x)
+    if x2.stride(0) < cols and x2.shape[0] > 1:  # rows that overlap or repeat (an expanded tensor)
+        x2 = x2.contiguous()
+    ld = -(-cols // 16) * 16
+    q = torch.empty((x2.shape[0], ld), dtype=torch.int8, device=dev)[:, :cols]
+    scale = torch.empty(x2.shape[0], dtype=torch.float32, device=dev)
+    _lib.check(_lib.load().nesle_quantize_rows(x2.data_ptr(), _DTYPE[x2.dtype], x2.shape[0], cols, _ld(x2), q.data_ptr(),
+                                               ld, scale.data_ptr(), dev.index, _stream(dev)))
+    return (q if len(shape) == 2 else q.unflatten(0, shape[:-1]) if len(shape) > 2 else q[0]), scale.view(shape[:-1])
+
+
+class Int8Weight:
+    """A weight matrix ``(n, k)`` in 8 bits with a scale for each channel, laid out once for :func:`int8_linear`: rows
+    padded with zeros to a multiple of 16 bytes, and the same matrix + 128 as unsigned bytes for unsigned tokens."""
+
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor):
+        dev = _cuda_device(q, "q")
+        _require(q.dtype == torch.int8 and q.dim() == 2, "q must be a 2-D int8 tensor")
+        _on(scale, dev, "scale")
+        _require(scale.dtype == torch.float32 and scale.shape == q.shape[:1], "scale must be float32 of shape (n,)")
+        self.n, self.k = q.shape
+        self.ld = max(16, -(-self.k // 16) * 16)
+        self.q = torch.zeros((self.n, self.ld), dtype=torch.int8, device=dev)
+        self.q[:, :self.k] = q
+        self.biased = self.q.view(torch.uint8) ^ 128  # two's complement: flipping the top bit adds 128
+        self.scale = scale.detach().contiguous().clone()
+        self.device = dev
+
+    @classmethod
+    def from_float(cls, weight: torch.Tensor) -> "Int8Weight":
+        """Quantises a floating ``(n, k)`` matrix, each channel by its own largest magnitude."""
+        return cls(*quantize_rows(weight.detach()))
+
+    @property
+    def shape(self) -> tuple[int, int]:
+        return self.n, self.k
+
+
+def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | float | None = None,
+                bias: torch.Tensor | None = None, *, relu: bool = False, out_dtype: torch.dtype = torch.bfloat16,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(x_scale * weight.scale * (x @ weight.q.T) + bias)`` with the integer product exact in 32 bits.
+
+    ``x`` is ``(..., k)``: uint8 (RAM bytes) or int8 with ``x_scale`` a number or a float32 tensor ``x.shape[:-1]``; or
+    floating, which is quantised per token first (:func:`quantize_rows`; ``x_scale`` stays None).  ``bias`` is float32
+    ``(n,)``.  The result is ``(..., n)`` in ``out_dtype`` (bfloat16, float16 or float32), or written to ``out``."""
+    dev = _cuda_device(x, "x")
+    _require(isinstance(weight, Int8Weight) and weight.device == dev, f"weight must be an Int8Weight on {dev}")
+    _require(x.dim() >= 1 and x.shape[-1] == weight.k, f"x must have {weight.k} columns, has shape {tuple(x.shape)}")
+    _no_grad_path("int8_linear", x, bias)
+    if x.dtype in _DTYPE:
+        _require(x_scale is None, "x_scale is computed where x is floating")
+        x, x_scale = quantize_rows(x)
+    _require(x.dtype in (torch.uint8, torch.int8), "x must be uint8, int8 or floating")
+    shape = x.shape[:-1]
+    x2 = _rows(x if x.dim() > 1 else x[None])
+    if x2.stride(0) < x2.shape[1] and x2.shape[0] > 1:
+        x2 = x2.contiguous()
+    m, k = x2.shape
+    a = _lib.Int8Args()
+    if isinstance(x_scale, torch.Tensor):
+        _on(x_scale, dev, "x_scale")
+        _require(x_scale.dtype == torch.float32 and x_scale.shape == shape, f"x_scale must be float32 of shape {tuple(shape)}")
+        x_scale = x_scale.contiguous()
+        a.x_scale = x_scale.data_ptr()
+    else:
+        _require(x_scale is not None, "x_scale is needed where x is integer")
+        a.x_scale_value = float(x_scale)
+    if bias is not None:
+        _on(bias, dev, "bias")
+        _require(bias.dtype == torch.float32 and bias.shape == (weight.n,), f"bias must be float32 of shape ({weight.n},)")
+        bias = bias.detach().contiguous()
+        a.bias = bias.data_ptr()
+    if out is None:
+        _require(out_dtype in _DTYPE, "out_dtype must be float32, bfloat16 or float16")
+        out = torch.empty((*shape, weight.n), dtype=out_dtype, device=dev)
+    else:
+        _on(out, dev, "out")
+        _require(out.dtype in _DTYPE and out.shape == (*shape, weight.n), f"out must be floating of shape {(*shape, weight.n)}")
+        _require(out.dim() < 3 or out.is_contiguous(), "out of more than two dimensions must be contiguous")
+    y = out.view(-1, weight.n) if out.dim() != 2 else out
+    _require(y.stride(1) == 1 or y.shape[1] <= 1, "out must have unit column stride")
+    _require(y.shape[0] <= 1 or y.stride(0) >= weight.n, "out's rows must not overlap")
+    a.x, a.x_unsigned, a.ld_x = x2.data_ptr(), x2.dtype == torch.uint8, _ld(x2)
+    a.w, a.w_biased, a.ld_w, a.w_scale = weight.q.data_ptr(), weight.biased.data_ptr(), weight.ld, weight.scale.data_ptr()
+    a.y, a.y_dtype, a.ld_y = y.data_ptr(), _DTYPE[y.dtype], _ld(y)
+    a.m, a.k, a.n, a.relu, a.device = m, k, weight.n, relu, dev.index
+    lib = _lib.load()
+    need = lib.nesle_int8_workspace(ctypes.byref(a))
+    if need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = scratch.data_ptr(), need
+    _lib.check(lib.nesle_int8_linear(ctypes.byref(a), _stream(dev)))
+    return out

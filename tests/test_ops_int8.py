@@ -1,0 +1,208 @@
+"""8-bit product (nesle_b200.ops.int8_linear, quantize_rows) against 64 bits.
+
+The integer sum is exact, so an output differs from the 64-bit value by the
+rounding of the epilogue alone: the sum to fp32 and three fp32 operations (at
+most 4 * 2^-24 of the largest term) and one rounding to the output type."""
+from __future__ import annotations
+
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from nesle_b200 import ops  # noqa: E402
+
+UNIT = {t: torch.finfo(t).eps / 2 for t in (torch.float32, torch.bfloat16, torch.float16)}  # one rounding to nearest
+
+
+def _gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+@pytest.fixture(autouse=True, scope="module")
+def _cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from nesle_b200 import build
+
+    build.build()
+
+
+def _weight(n, k, seed):
+    g = _gen(seed)
+    q = torch.randint(-127, 128, (n, k), generator=g, device="cuda", dtype=torch.int8)
+    return q, torch.rand(n, generator=g, device="cuda") * 0.01 + 1e-4
+
+
+def _check(y, xq, xs, q, ws, bias, relu):
+    acc = xq.double() @ q.double().T
+    terms = acc * xs * ws.double()
+    want = terms + (bias.double() if bias is not None else 0.0)
+    size = terms.abs() + (bias.double().abs() if bias is not None else 0.0)
+    if relu:
+        want = want.clamp(min=0)
+    tol = want.abs() * UNIT[y.dtype] + size * 4 * 2.0 ** -24 + (2.0 ** -25 if y.dtype == torch.float16 else 0.0)
+    assert y.shape == want.shape
+    assert bool(((y.double() - want).abs() <= tol).all()), float(((y.double() - want).abs() - tol).max())
+
+
+def _quantized(x):
+    """IEEE divisions by tensors (torch turns a division by a number into a product with its reciprocal)."""
+    most = x.float().abs().amax(1)
+    scale = most / torch.full_like(most, 127.0)
+    return torch.round(x.float() / torch.where(scale > 0, scale, 1.0)[:, None]).to(torch.int8), scale
+
+
+SIZES = [(1, 2048, 512), (1, 1, 1), (2, 17, 3), (16, 64, 8), (17, 100, 9), (64, 256, 130), (65, 128, 16), (128, 128, 64),
+         (129, 127, 65), (200, 130, 129), (257, 2048, 512), (1000, 300, 257), (300, 96, 2048), (20000, 64, 33)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", SIZES)
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8])
+def test_product_matches_64_bits(m, k, n, dtype):
+    g = _gen(m * 7 + k)
+    lo, hi = (0, 256) if dtype == torch.uint8 else (-128, 128)
+    x = torch.randint(lo, hi, (m, k), generator=g, device="cuda", dtype=dtype)
+    q, ws = _weight(n, k, 1)
+    xs = torch.rand(m, generator=g, device="cuda") + 0.01
+    bias = torch.randn(n, generator=g, device="cuda")
+    w = ops.Int8Weight(q, ws)
+    for out_dtype in (torch.bfloat16, torch.float32):
+        _check(ops.int8_linear(x, w, xs, bias, out_dtype=out_dtype), x, xs.double()[:, None], q, ws, bias, False)
+    _check(ops.int8_linear(x, w, 1 / 255, relu=True, out_dtype=torch.float16), x,
+           float(torch.tensor(1 / 255, dtype=torch.float32)), q, ws, None, True)
+    assert ops.stalls() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,value", [(torch.uint8, 255), (torch.int8, -128), (torch.int8, 127)])
+def test_extreme_sums_are_exact(dtype, value):
+    """Every byte at its extreme: the largest sums that the accumulators meet."""
+    for m in (3, 130):
+        k = 8192
+        x = torch.full((m, k), value, dtype=dtype, device="cuda")
+        q = torch.full((70, k), 127, dtype=torch.int8, device="cuda")
+        q[1::2] = -127
+        y = ops.int8_linear(x, ops.Int8Weight(q, torch.ones(70, device="cuda")), 1.0, out_dtype=torch.float32)
+        want = (x.double() @ q.double().T).float()
+        assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [5, 300])
+def test_strided_and_unaligned_operands(m):
+    """Slices of a wider observation: rows further apart than they are long, starts off 16 bytes."""
+    ram = torch.randint(0, 256, (m, 2048), generator=_gen(3), device="cuda", dtype=torch.uint8)
+    for start, k in ((0, 100), (16, 1000), (1, 255), (2000, 48), (7, 2041)):
+        x = ram[:, start:start + k]
+        q, ws = _weight(40, k, start)
+        out = torch.full((m, 64), 7.0, device="cuda", dtype=torch.bfloat16)
+        ops.int8_linear(x, ops.Int8Weight(q, ws), 0.5, out=out[:, 3:43])
+        _check(out[:, 3:43], x, 0.5, q, ws, None, False)
+        assert bool((out[:, :3] == 7).all()) and bool((out[:, 43:] == 7).all())
+    x = ram.T  # not unit stride: laid out again
+    q, ws = _weight(40, m, 5)
+    _check(ops.int8_linear(x, ops.Int8Weight(q, ws), 0.5), x, 0.5, q, ws, None, False)
+    one = ram[:1].expand(m, 2048)
+    q, ws = _weight(40, 2048, 6)
+    _check(ops.int8_linear(one, ops.Int8Weight(q, ws), 0.5), one, 0.5, q, ws, None, False)
+
+
+@pytest.mark.gpu
+def test_empty_sizes():
+    q, ws = _weight(6, 32, 1)
+    w = ops.Int8Weight(q, ws)
+    assert ops.int8_linear(torch.empty((0, 32), dtype=torch.uint8, device="cuda"), w, 1.0).shape == (0, 6)
+    none = ops.Int8Weight(q[:, :0], ws)
+    y = ops.int8_linear(torch.empty((5, 0), dtype=torch.int8, device="cuda"), none, 1.0, torch.arange(6.0, device="cuda"))
+    assert torch.equal(y, torch.arange(6.0, device="cuda", dtype=torch.bfloat16).expand(5, 6))
+    qq, ss = ops.quantize_rows(torch.empty((3, 0), device="cuda"))
+    assert qq.shape == (3, 0) and torch.equal(ss, torch.zeros(3, device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (3, 7), (5, 64), (9, 1000), (4, 1024), (2, 4097), (3, 20000), (70, 512)])
+def test_quantize_rows_is_exact(dtype, rows, cols):
+    x = (torch.randn((rows, cols), generator=_gen(cols), device="cuda") * 3).to(dtype)
+    if rows > 1:
+        x[1] = 0
+    q, s = ops.quantize_rows(x)
+    want_q, want_s = _quantized(x)
+    assert torch.equal(s, want_s) and torch.equal(q, want_q)
+    wide = torch.randn((rows, 3 * cols + 5), generator=_gen(1), device="cuda").to(dtype)[:, 3:3 + cols]
+    q, s = ops.quantize_rows(wide)
+    want_q, want_s = _quantized(wide)
+    assert torch.equal(s, want_s) and torch.equal(q, want_q)
+
+
+@pytest.mark.gpu
+def test_quantize_rows_with_infinities_and_nan():
+    x = torch.randn((4, 33), generator=_gen(0), device="cuda")
+    x[1, 5], x[2, 6] = float("inf"), float("nan")
+    q, s = ops.quantize_rows(x)
+    assert torch.isinf(s[1]) and torch.isnan(s[2]) and torch.isfinite(s[[0, 3]]).all()
+    assert int(q[1].abs().sum()) == 0 and int(q[2].abs().sum()) == 0
+    qw, ws = _weight(8, 33, 1)
+    y = ops.int8_linear(x, ops.Int8Weight(qw, ws))
+    assert not torch.isfinite(y[1]).any() and not torch.isfinite(y[2]).any()
+    assert torch.isfinite(y[[0, 3]]).all()
+
+
+@pytest.mark.gpu
+def test_floating_tokens_are_quantised_per_token():
+    x = torch.randn((2, 70, 48), generator=_gen(2), device="cuda", dtype=torch.bfloat16)
+    w = ops.Int8Weight.from_float(torch.randn((24, 48), generator=_gen(3), device="cuda"))
+    q, s = ops.quantize_rows(x)
+    assert q.shape == x.shape and s.shape == (2, 70)
+    assert torch.equal(ops.int8_linear(x, w), ops.int8_linear(q, w, s))
+    assert torch.equal(ops.int8_linear(x[0, 0], w), ops.int8_linear(x, w)[0, 0])
+
+
+@pytest.mark.gpu
+def test_on_another_stream_and_in_a_graph():
+    x = torch.randint(0, 256, (500, 200), generator=_gen(2), device="cuda", dtype=torch.uint8)
+    q, ws = _weight(96, 200, 4)
+    w = ops.Int8Weight(q, ws)
+    want = ops.int8_linear(x, w, 0.25)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        y = ops.int8_linear(x, w, 0.25)
+    side.synchronize()
+    assert torch.equal(y, want)
+    out = torch.empty_like(want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.int8_linear(x, w, 0.25, out=out)
+    x.fill_(3)
+    graph.replay()
+    assert torch.equal(out, ops.int8_linear(x, w, 0.25))
+
+
+@pytest.mark.gpu
+def test_refusals():
+    q, ws = _weight(8, 32, 1)
+    w = ops.Int8Weight(q, ws)
+    x = torch.zeros((4, 32), dtype=torch.uint8, device="cuda")
+    for call in (
+        lambda: ops.int8_linear(x.cpu(), w, 1.0),
+        lambda: ops.int8_linear(x[:, :31], w, 1.0),
+        lambda: ops.int8_linear(x, w),
+        lambda: ops.int8_linear(x.to(torch.int16), w, 1.0),
+        lambda: ops.int8_linear(x, w, torch.ones(3, device="cuda")),
+        lambda: ops.int8_linear(x, w, torch.ones(4, device="cuda", dtype=torch.float64)),
+        lambda: ops.int8_linear(x, w, 1.0, torch.ones(7, device="cuda")),
+        lambda: ops.int8_linear(x, w, 1.0, out_dtype=torch.float64),
+        lambda: ops.int8_linear(x, w, 1.0, out=torch.empty((4, 7), device="cuda")),
+        lambda: ops.int8_linear(x, w, 1.0, out=torch.empty((8, 4), device="cuda").T),
+        lambda: ops.int8_linear(x.float(), w, 1.0),
+        lambda: ops.int8_linear(x.float().requires_grad_(), w),
+        lambda: ops.Int8Weight(q.float(), ws),
+        lambda: ops.Int8Weight(q, ws[:-1]),
+        lambda: ops.quantize_rows(x),
+        lambda: ops.int8_linear(torch.zeros((2, 40000), dtype=torch.uint8, device="cuda"),
+                                ops.Int8Weight(torch.zeros((8, 40000), dtype=torch.int8, device="cuda"), ws), 1.0),
+    ):
+        with pytest.raises(ValueError):
+            call()
