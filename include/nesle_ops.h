@@ -64,6 +64,26 @@ int nesle_int8_linear(const nesle_int8_args* args, void* stream);
 /* Scratch bytes that the call needs (0 where x is 16-byte aligned with rows a multiple of 16 bytes apart). */
 uint64_t nesle_int8_workspace(const nesle_int8_args* args);
 
+typedef struct nesle_orth_args {
+    const void* x;       /* [batch][rows][cols], any strides (elements) */
+    int dtype;           /* NESLE_F32, NESLE_BF16 or NESLE_F16 */
+    int64_t stride_b, stride_r, stride_c;
+    uint64_t batch, rows, cols;
+    int steps;           /* products' rounds, at least 1 */
+    double eps;          /* added to the norm */
+    void* out;           /* [batch][rows][cols] bf16, contiguous, 16-byte aligned */
+    void* workspace;     /* nesle_orth_workspace bytes, 256-byte aligned */
+    uint64_t workspace_bytes;
+    int device;
+} nesle_orth_args;
+
+/* Each matrix divided by its Frobenius norm plus eps, then `steps` times X <- aX + (bA + cA^2) X with A = X X^T (of the
+ * smaller side) and (a, b, c) = (3.4445, -4.7750, 2.0315): the singular values move towards 1, the singular vectors stay.
+ * Products carry 22 bits.  A matrix whose norm is far below eps keeps fewer, and ends as zero.  A NaN or an infinity makes
+ * its matrix NaN. */
+int nesle_orthogonalize(const nesle_orth_args* args, void* stream);
+uint64_t nesle_orth_workspace(const nesle_orth_args* args);
+
 #ifdef __cplusplus
 }
 #endif

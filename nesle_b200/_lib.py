@@ -65,6 +65,14 @@ class Int8Args(ctypes.Structure):
                 ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("device", ctypes.c_int)]
 
 
+class OrthArgs(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("dtype", ctypes.c_int), ("stride_b", ctypes.c_int64),
+                ("stride_r", ctypes.c_int64), ("stride_c", ctypes.c_int64), ("batch", ctypes.c_uint64),
+                ("rows", ctypes.c_uint64), ("cols", ctypes.c_uint64), ("steps", ctypes.c_int), ("eps", ctypes.c_double),
+                ("out", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
+                ("device", ctypes.c_int)]
+
+
 # Exported symbols and their ctypes signatures (every function include/*.h declares).
 SIGNATURES = {
     "nesle_create": (ctypes.c_int, [ctypes.POINTER(CreateArgs), ctypes.POINTER(ctypes.c_void_p)]),
@@ -104,6 +112,8 @@ SIGNATURES = {
                                            ctypes.c_int, ctypes.c_void_p]),
     "nesle_int8_linear": (ctypes.c_int, [ctypes.POINTER(Int8Args), ctypes.c_void_p]),
     "nesle_int8_workspace": (ctypes.c_uint64, [ctypes.POINTER(Int8Args)]),
+    "nesle_orthogonalize": (ctypes.c_int, [ctypes.POINTER(OrthArgs), ctypes.c_void_p]),
+    "nesle_orth_workspace": (ctypes.c_uint64, [ctypes.POINTER(OrthArgs)]),
 }
 
 # EnvRecord (csrc/nesle_state.h), the first 128 bytes of a saved state blob.

@@ -4,6 +4,8 @@ actor-critic on the batched core computes beside the env step.
 * ``int8_linear`` / ``quantize_rows`` / ``Int8Weight`` -- product of 8-bit
   integers with a scale for each token and channel.  RAM observations are bytes
   already and go in as they are.
+* ``orthogonalize`` -- Newton-Schulz orthogonalisation of matrix updates, for
+  the ``Muon`` optimiser (nesle_b200.muon).
 
 Calls go on the caller's current torch stream, return before the work is done,
 and never synchronise the host.  Argument errors raise ValueError, CUDA errors
@@ -18,7 +20,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["Int8Weight", "int8_linear", "quantize_rows", "stalls"]
+__all__ = ["Int8Weight", "int8_linear", "orthogonalize", "quantize_rows", "stalls"]
 
 _DTYPE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
@@ -172,4 +174,35 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
         scratch = torch.empty(need, dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = scratch.data_ptr(), need
     _lib.check(lib.nesle_int8_linear(ctypes.byref(a), _stream(dev)))
+    return out
+
+
+# ------------------------------------------------------------------ Newton-Schulz
+
+def orthogonalize(update: torch.Tensor, *, steps: int = 5, eps: float = 1e-7,
+                  out: torch.Tensor | None = None) -> torch.Tensor:
+    """Orthogonalises each matrix of ``update`` (``(..., rows, cols)``, float32, bfloat16 or float16, any strides):
+    divided by its Frobenius norm plus ``eps``, then ``steps`` Newton-Schulz rounds X <- aX + (bA + cA^2)X with
+    A = X X^T on the smaller side and (a, b, c) = (3.4445, -4.7750, 2.0315).  Singular values end between about 0.7 and
+    1.2, singular vectors stay.  The result is bfloat16 of the same shape, or written to ``out`` (contiguous bfloat16).
+    Products carry 22 bits of both operands; a zero matrix stays zero, a NaN or an infinity makes its matrix NaN."""
+    dev = _cuda_device(update, "update")
+    _require(update.dtype in _DTYPE, "update must be float32, bfloat16 or float16")
+    _require(update.dim() >= 2, "update must have at least two dimensions")
+    _no_grad_path("orthogonalize", update)
+    rows, cols = update.shape[-2:]
+    if out is None:
+        out = torch.empty(update.shape, dtype=torch.bfloat16, device=dev)
+    else:
+        _on(out, dev, "out")
+        _require(out.dtype == torch.bfloat16 and out.shape == update.shape and out.is_contiguous(),
+                 f"out must be contiguous bfloat16 of shape {tuple(update.shape)}")
+    x = update if update.dim() == 3 else update.reshape(-1, rows, cols) if out.numel() else update.new_empty((0, rows, cols))
+    a = _lib.OrthArgs(x.data_ptr(), _DTYPE[x.dtype], *x.stride(), *x.shape, steps, eps, out.data_ptr(), None, 0, dev.index)
+    lib = _lib.load()
+    need = lib.nesle_orth_workspace(ctypes.byref(a))
+    if need:
+        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = scratch.data_ptr(), need
+    _lib.check(lib.nesle_orthogonalize(ctypes.byref(a), _stream(dev)))
     return out
