@@ -84,6 +84,58 @@ typedef struct nesle_orth_args {
 int nesle_orthogonalize(const nesle_orth_args* args, void* stream);
 uint64_t nesle_orth_workspace(const nesle_orth_args* args);
 
+/* The gated delta rule.  Strides are in elements; the last dimension of q, k and v has stride 1; q, k, v and o have one
+ * type.  dk and dv are 1 to 128.  States are fp32, [n][h][dk][dv]. */
+typedef struct nesle_delta_step_args {
+    const void *q, *k, *v; /* [n][h][dk], [n][h][dk], [n][h][dv] */
+    int64_t q_n, q_h, k_n, k_h, v_n, v_h;
+    int dtype;
+    const float *g, *beta; /* [n][h]: log of the decay, write strength */
+    int64_t g_n, g_h, beta_n, beta_h;
+    const uint8_t* reset;  /* [n], nonzero: the state counts as zero; or NULL */
+    int64_t reset_n;
+    float* state;          /* in and out; its dk x dv matrices are contiguous */
+    int64_t state_n, state_h;
+    void* o;               /* [n][h][dv], contiguous */
+    uint64_t n, h, dk, dv;
+    float scale;
+    int device;
+} nesle_delta_step_args;
+
+/* One token of every env and head, with the state updated in place:
+ * S0 = reset ? 0 : exp(g) S;  u = beta (v - S0^T k);  S = S0 + k u^T;  o = scale S^T q. */
+int nesle_delta_step(const nesle_delta_step_args* args, void* stream);
+
+typedef struct nesle_delta_args {
+    const void *q, *k, *v; /* [t][n][h][dk], [t][n][h][dk], [t][n][h][dv] */
+    int64_t q_t, q_n, q_h, k_t, k_n, k_h, v_t, v_n, v_h;
+    int dtype;
+    const float *g, *beta; /* [t][n][h] */
+    int64_t g_t, g_n, g_h, beta_t, beta_n, beta_h;
+    const uint8_t* reset;  /* [t][n], nonzero: token t starts an episode; or NULL */
+    int64_t reset_t, reset_n;
+    const float* state;    /* before the first token, contiguous; NULL for zeros */
+    uint64_t t, n, h, dk, dv;
+    float scale;
+    void* o;               /* [t][n][h][dv], contiguous */
+    float* final_state;    /* or NULL */
+    float* errors;         /* [t][n][h][dv] and nesle_delta_checkpoint_floats floats that the backward pass reads; both NULL */
+    float* checkpoints;    /* where no gradient is wanted */
+    /* backward only; contiguous */
+    const void* d_o;       /* like o */
+    const float* d_final;  /* or NULL for zeros */
+    void *dq, *d_k, *d_v;
+    float *dg, *dbeta;
+    float* dstate;         /* or NULL */
+    int device;
+} nesle_delta_args;
+
+/* The same over t tokens; and its gradients, of all inputs, from those of o and of the final state.  The backward call
+ * takes the forward call's inputs, errors and checkpoints.  The gradient of g is zero at tokens that start an episode. */
+uint64_t nesle_delta_checkpoint_floats(const nesle_delta_args* args);
+int nesle_delta_scan(const nesle_delta_args* args, void* stream);
+int nesle_delta_scan_backward(const nesle_delta_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

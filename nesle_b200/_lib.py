@@ -73,6 +73,28 @@ class OrthArgs(ctypes.Structure):
                 ("device", ctypes.c_int)]
 
 
+_void, _i64, _u64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint64
+
+
+class DeltaStepArgs(ctypes.Structure):
+    _fields_ = [*((x, _void) for x in ("q", "k", "v")), *((x, _i64) for x in ("q_n", "q_h", "k_n", "k_h", "v_n", "v_h")),
+                ("dtype", ctypes.c_int), ("g", _void), ("beta", _void),
+                *((x, _i64) for x in ("g_n", "g_h", "beta_n", "beta_h")), ("reset", _void), ("reset_n", _i64),
+                ("state", _void), ("state_n", _i64), ("state_h", _i64), ("o", _void),
+                *((x, _u64) for x in ("n", "h", "dk", "dv")), ("scale", ctypes.c_float), ("device", ctypes.c_int)]
+
+
+class DeltaArgs(ctypes.Structure):
+    _fields_ = [*((x, _void) for x in ("q", "k", "v")),
+                *((x, _i64) for x in ("q_t", "q_n", "q_h", "k_t", "k_n", "k_h", "v_t", "v_n", "v_h")),
+                ("dtype", ctypes.c_int), ("g", _void), ("beta", _void),
+                *((x, _i64) for x in ("g_t", "g_n", "g_h", "beta_t", "beta_n", "beta_h")), ("reset", _void),
+                ("reset_t", _i64), ("reset_n", _i64), ("state", _void),
+                *((x, _u64) for x in ("t", "n", "h", "dk", "dv")), ("scale", ctypes.c_float),
+                *((x, _void) for x in ("o", "final_state", "errors", "checkpoints", "d_o", "d_final", "dq", "d_k", "d_v",
+                                       "dg", "dbeta", "dstate")), ("device", ctypes.c_int)]
+
+
 # Exported symbols and their ctypes signatures (every function include/*.h declares).
 SIGNATURES = {
     "nesle_create": (ctypes.c_int, [ctypes.POINTER(CreateArgs), ctypes.POINTER(ctypes.c_void_p)]),
@@ -112,6 +134,10 @@ SIGNATURES = {
                                            ctypes.c_int, ctypes.c_void_p]),
     "nesle_int8_linear": (ctypes.c_int, [ctypes.POINTER(Int8Args), ctypes.c_void_p]),
     "nesle_int8_workspace": (ctypes.c_uint64, [ctypes.POINTER(Int8Args)]),
+    "nesle_delta_step": (ctypes.c_int, [ctypes.POINTER(DeltaStepArgs), ctypes.c_void_p]),
+    "nesle_delta_scan": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), ctypes.c_void_p]),
+    "nesle_delta_scan_backward": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), ctypes.c_void_p]),
+    "nesle_delta_checkpoint_floats": (ctypes.c_uint64, [ctypes.POINTER(DeltaArgs)]),
     "nesle_orthogonalize": (ctypes.c_int, [ctypes.POINTER(OrthArgs), ctypes.c_void_p]),
     "nesle_orth_workspace": (ctypes.c_uint64, [ctypes.POINTER(OrthArgs)]),
 }

@@ -1,0 +1,11 @@
+// ops_delta_f32.cu -- the gated delta rule's kernels for one input type.
+#include "ops_delta.cuh"
+
+namespace nesle {
+namespace ops {
+namespace delta {
+template int launch_forward<float>(const Scan&, cudaStream_t);
+template int launch_backward<float>(const Scan&, cudaStream_t);
+}  // namespace delta
+}  // namespace ops
+}  // namespace nesle

@@ -4,6 +4,9 @@ actor-critic on the batched core computes beside the env step.
 * ``int8_linear`` / ``quantize_rows`` / ``Int8Weight`` -- product of 8-bit
   integers with a scale for each token and channel.  RAM observations are bytes
   already and go in as they are.
+* ``delta_step`` / ``delta_scan`` -- the gated delta rule, a memory of fixed
+  size for every env and head: one token in place (rollout), and a whole
+  rollout with its gradients (update).
 * ``orthogonalize`` -- Newton-Schulz orthogonalisation of matrix updates, for
   the ``Muon`` optimiser (nesle_b200.muon).
 
@@ -20,7 +23,7 @@ import torch
 
 from . import _lib
 
-__all__ = ["Int8Weight", "int8_linear", "orthogonalize", "quantize_rows", "stalls"]
+__all__ = ["Int8Weight", "delta_scan", "delta_step", "int8_linear", "orthogonalize", "quantize_rows", "stalls"]
 
 _DTYPE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
@@ -206,3 +209,145 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, eps: float = 1e-7,
         a.workspace, a.workspace_bytes = scratch.data_ptr(), need
     _lib.check(lib.nesle_orthogonalize(ctypes.byref(a), _stream(dev)))
     return out
+
+
+# ------------------------------------------------------------------ gated delta rule
+
+def _delta_inputs(q, k, v, g, beta, reset, lead: str):
+    """Checks what delta_step and delta_scan share; ``lead`` names the dimensions before the head size."""
+    dev = _cuda_device(q, "q")
+    dims = len(lead) + 1
+    _require(q.dtype in _DTYPE, "q must be float32, bfloat16 or float16")
+    _require(q.dim() == dims, f"q must have shape ({', '.join(lead)}, dk)")
+    for name, x in (("k", k), ("v", v), ("g", g), ("beta", beta)):
+        _on(x, dev, name)
+    _require(k.shape == q.shape and k.dtype == q.dtype, f"k must be {q.dtype} of shape {tuple(q.shape)}")
+    _require(v.dim() == dims and v.shape[:-1] == q.shape[:-1] and v.dtype == q.dtype,
+             f"v must be {q.dtype} of shape {tuple(q.shape[:-1])} + (dv,)")
+    for name, x in (("g", g), ("beta", beta)):
+        _require(x.dtype == torch.float32 and x.shape == q.shape[:-1], f"{name} must be float32 of shape {tuple(q.shape[:-1])}")
+    _require(1 <= q.shape[-1] <= 128 and 1 <= v.shape[-1] <= 128, "head sizes must be 1 to 128")
+    if reset is not None:
+        _on(reset, dev, "reset")
+        _require(reset.dtype in (torch.bool, torch.uint8) and reset.shape == q.shape[:-2],
+                 f"reset must be bool or uint8 of shape {tuple(q.shape[:-2])}")
+    return dev
+
+
+def _unit(x: torch.Tensor) -> torch.Tensor:
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
+def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+               state: torch.Tensor, reset: torch.Tensor | None = None, *, scale: float | None = None,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """One token of the gated delta rule for every env and head; ``state`` is updated in place:
+
+        S0 = 0 where reset else exp(g) S;  u = beta (v - S0^T k);  S = S0 + k u^T;  o = scale S^T q
+
+    ``q, k``: (n, h, dk), ``v``: (n, h, dv), float32, bfloat16 or float16; ``g, beta``: (n, h) float32; ``state``:
+    (n, h, dk, dv) float32 with contiguous matrices; ``reset``: (n,) bool or uint8.  ``scale`` is dk ** -0.5 unless
+    given.  Returns ``o`` (n, h, dv) in q's type, or writes it to ``out`` (contiguous).  Without gradients: for a
+    sequence with gradients see :func:`delta_scan`."""
+    dev = _delta_inputs(q, k, v, g, beta, reset, "nh")
+    _no_grad_path("delta_step", q, k, v, g, beta, state)
+    n, h, dk = q.shape
+    dv = v.shape[-1]
+    _on(state, dev, "state")
+    _require(state.dtype == torch.float32 and state.shape == (n, h, dk, dv), f"state must be float32 of shape {(n, h, dk, dv)}")
+    _require((state.stride(3) == 1 or dv == 1) and (state.stride(2) == dv or dk == 1), "state's matrices must be contiguous")
+    _require((n <= 1 or state.stride(0) >= dk * dv) and (h <= 1 or state.stride(1) >= dk * dv), "state's matrices must not overlap")
+    if out is None:
+        out = torch.empty((n, h, dv), dtype=q.dtype, device=dev)
+    else:
+        _on(out, dev, "out")
+        _require(out.dtype == q.dtype and out.shape == (n, h, dv) and out.is_contiguous(),
+                 f"out must be contiguous {q.dtype} of shape {(n, h, dv)}")
+    q, k, v = _unit(q), _unit(k), _unit(v)
+    a = _lib.DeltaStepArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+                           v.stride(0), v.stride(1), _DTYPE[q.dtype], g.data_ptr(), beta.data_ptr(), g.stride(0), g.stride(1),
+                           beta.stride(0), beta.stride(1), None if reset is None else reset.data_ptr(),
+                           0 if reset is None else reset.stride(0), state.data_ptr(), state.stride(0), state.stride(1),
+                           out.data_ptr(), n, h, dk, dv, dk ** -0.5 if scale is None else scale, dev.index)
+    _lib.check(_lib.load().nesle_delta_step(ctypes.byref(a), _stream(dev)))
+    return out
+
+
+def _scan_args(q, k, v, g, beta, reset, state, scale, dev):
+    t, n, h, dk = q.shape
+    return _lib.DeltaArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_t=q.stride(0), q_n=q.stride(1), q_h=q.stride(2),
+                          k_t=k.stride(0), k_n=k.stride(1), k_h=k.stride(2), v_t=v.stride(0), v_n=v.stride(1),
+                          v_h=v.stride(2), dtype=_DTYPE[q.dtype], g=g.data_ptr(), beta=beta.data_ptr(), g_t=g.stride(0),
+                          g_n=g.stride(1), g_h=g.stride(2), beta_t=beta.stride(0), beta_n=beta.stride(1),
+                          beta_h=beta.stride(2), reset=None if reset is None else reset.data_ptr(),
+                          reset_t=0 if reset is None else reset.stride(0), reset_n=0 if reset is None else reset.stride(1),
+                          state=None if state is None else state.data_ptr(), t=t, n=n, h=h, dk=dk, dv=v.shape[-1],
+                          scale=scale, device=dev.index)
+
+
+class _DeltaScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, g, beta, state, reset, scale, grad):
+        dev, (t, n, h, dk), dv = q.device, q.shape, v.shape[-1]
+        o = torch.empty((t, n, h, dv), dtype=q.dtype, device=dev)
+        final = torch.empty((n, h, dk, dv), dtype=torch.float32, device=dev)
+        a = _scan_args(q, k, v, g, beta, reset, state, scale, dev)
+        a.o, a.final_state = o.data_ptr(), final.data_ptr()
+        lib = _lib.load()
+        if grad:
+            errors = torch.empty((t, n, h, dv), dtype=torch.float32, device=dev)
+            checkpoints = torch.empty(lib.nesle_delta_checkpoint_floats(ctypes.byref(a)), dtype=torch.float32, device=dev)
+            a.errors, a.checkpoints = errors.data_ptr(), checkpoints.data_ptr()
+            ctx.save_for_backward(q, k, v, g, beta, reset, errors, checkpoints)
+            ctx.scale, ctx.has_state = scale, state is not None
+            ctx.set_materialize_grads(False)
+        _lib.check(lib.nesle_delta_scan(ctypes.byref(a), _stream(dev)))
+        return o, final
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, d_o, d_final):
+        q, k, v, g, beta, reset, errors, checkpoints = ctx.saved_tensors
+        dev, (t, n, h, dk) = q.device, q.shape
+        d_o = torch.zeros_like(v, memory_format=torch.contiguous_format) if d_o is None else d_o.contiguous()
+        if d_final is not None:
+            d_final = d_final.contiguous()
+        dq, dk_, dv_ = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
+        dg, dbeta = (torch.empty(x.shape, dtype=torch.float32, device=dev) for x in (g, beta))
+        dstate = None
+        if ctx.has_state and ctx.needs_input_grad[5]:
+            dstate = torch.empty((n, h, dk, v.shape[-1]), dtype=torch.float32, device=dev)
+        if t == 0:
+            if dstate is not None:
+                dstate = torch.zeros_like(dstate) if d_final is None else d_final.clone()
+            return dq, dk_, dv_, dg, dbeta, dstate, None, None, None
+        a = _scan_args(q, k, v, g, beta, reset, None, ctx.scale, dev)
+        a.errors, a.checkpoints, a.d_o = errors.data_ptr(), checkpoints.data_ptr(), d_o.data_ptr()
+        a.d_final = None if d_final is None else d_final.data_ptr()
+        a.dq, a.d_k, a.d_v, a.dg, a.dbeta = (x.data_ptr() for x in (dq, dk_, dv_, dg, dbeta))
+        a.dstate = None if dstate is None else dstate.data_ptr()
+        _lib.check(_lib.load().nesle_delta_scan_backward(ctypes.byref(a), _stream(dev)))
+        return dq, dk_, dv_, dg, dbeta, dstate, None, None, None
+
+
+def delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
+               state: torch.Tensor | None = None, reset: torch.Tensor | None = None, *,
+               scale: float | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The gated delta rule over t tokens, time first as rollouts are stored: ``(o, final_state)``, both differentiable
+    in all floating inputs.  It is :func:`delta_step` token by token (up to rounding).
+
+    ``q, k``: (t, n, h, dk), ``v``: (t, n, h, dv), one of float32, bfloat16 and float16, any strides (rows copied unless
+    the last is 1); ``g, beta``: (t, n, h) float32; ``state``: (n, h, dk, dv) float32 before the first token, or None for
+    zeros; ``reset``: (t, n) bool or uint8, True where a token starts an episode: nothing before it, not even a NaN,
+    reaches it, and no gradient passes.  States and sums are fp32 throughout.  With gradients a call keeps one state for
+    every 16 tokens until its backward pass."""
+    dev = _delta_inputs(q, k, v, g, beta, reset, "tnh")
+    t, n, h, dk = q.shape
+    if state is not None:
+        _on(state, dev, "state")
+        _require(state.dtype == torch.float32 and state.shape == (n, h, dk, v.shape[-1]),
+                 f"state must be float32 of shape {(n, h, dk, v.shape[-1])}")
+        state = state.contiguous()
+    grad = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, state))
+    return _DeltaScan.apply(_unit(q), _unit(k), _unit(v), g, beta, state, reset, dk ** -0.5 if scale is None else float(scale),
+                            grad)
