@@ -23,7 +23,7 @@ _OPS = ["ops_common.h", "tc05.cuh"]
 # source -> the headers it includes; each source is one object, compiled when it or a header is newer
 SOURCES = {"kernels.cu": _CORE, "capi.cu": _CORE, "formats.cpp": _CORE, "ops_common.cu": _OPS, "ops_int8.cu": _OPS,
            "ops_orth.cu": _OPS,
-           **{f"ops_delta{t}.cu": ["ops_common.h", "ops_delta.cuh"] for t in ("", "_bf16", "_f16", "_f32")}}
+           **{f"ops_delta{t}.cu": [*_OPS, "ops_delta.cuh"] for t in ("", "_bf16", "_f16", "_f32")}}
 HEADERS = [ROOT / "include" / "nesle_b200.h", ROOT / "include" / "nesle_ops.h"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 

@@ -164,7 +164,7 @@ Scan to_scan(const nesle_delta_args& a, bool backward) {
     p.t = (int64_t)a.t, p.n = (int64_t)a.n, p.h = (int64_t)a.h, p.dk = (int)a.dk, p.dv = (int)a.dv;
     p.scale = a.scale;
     const int size = a.dtype == NESLE_F32 ? 4 : 2;
-    p.aligned = rows_aligned(a.q, a.q_t, a.q_n, a.q_h, size) && rows_aligned(a.k, a.k_t, a.k_n, a.k_h, size) &&
+    p.aligned = a.dk * size % 16 == 0 && a.dv * size % 16 == 0 && rows_aligned(a.q, a.q_t, a.q_n, a.q_h, size) && rows_aligned(a.k, a.k_t, a.k_n, a.k_h, size) &&
                 (backward ? rows_aligned(a.d_o, (int64_t)a.dv, 0, 0, size) : rows_aligned(a.v, a.v_t, a.v_n, a.v_h, size));
     p.o = a.o, p.final_state = a.final_state, p.errors = a.errors, p.checkpoints = a.checkpoints;
     p.d_o = a.d_o, p.d_final = a.d_final, p.dq = a.dq, p.dk_out = a.d_k, p.dv_out = a.d_v, p.dg = a.dg, p.dbeta = a.dbeta;
@@ -219,7 +219,8 @@ int nesle_delta_scan(const nesle_delta_args* args, void* stream) {
         if (a.t && (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.o)) return invalid("delta_scan: null argument");
         OnDevice on(a.device);
         if (!on.ok) return invalid("delta_scan: device ordinal out of range");
-        const delta::Scan p = delta::to_scan(a, false);
+        delta::Scan p = delta::to_scan(a, false);
+        if (int rc = stall_counter(a.device, &p.stalls)) return rc;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         if (a.dtype == NESLE_F32) return delta::launch_forward<float>(p, st);
         if (a.dtype == NESLE_BF16) return delta::launch_forward<__nv_bfloat16>(p, st);

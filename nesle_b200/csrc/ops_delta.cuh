@@ -31,6 +31,7 @@
 #include <stddef.h>
 
 #include "ops_common.h"
+#include "tc05.cuh"
 
 namespace nesle {
 namespace ops {
@@ -53,7 +54,7 @@ struct Scan {
     int64_t t, n, h;
     int dk, dv;
     float scale;
-    bool aligned;  // every row of q, k, v (and d_o) starts on 16 bytes
+    bool aligned;  // every row of q, k, v (and d_o) is whole 16-byte chunks and starts on 16 bytes
     void* o;
     float* final_state;
     float* errors;       // [t][n][h][dv], NULL where no gradient is wanted
@@ -62,6 +63,7 @@ struct Scan {
     const float* d_final;
     void *dq, *dk_out, *dv_out;
     float *dg, *dbeta, *dstate;
+    unsigned int* stalls;
 };
 
 template <class T>
@@ -141,12 +143,22 @@ __device__ __forceinline__ void load_columns(uint32_t (&r)[4], const __nv_bfloat
     ldmatrix4_t(r, tile + (lane % 8 + lane / 16 * 8) * ld + c0 + lane / 8 % 2 * 8);
 }
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_at(dst)), "l"(src), "r"(bytes) : "memory");
+// 16 bytes, or zeros where not `in`.  (A byte count in a register instead of the predicate took 180 clocks a copy.)
+__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool in) {
+    asm volatile("{\n\t.reg .pred P;\n\tsetp.eq.u32 P, %2, 0;\n\tcp.async.cg.shared.global [%0], [%1], 16, P;\n\t}" ::"r"(smem_at(dst)),
+                 "l"(src), "r"((uint32_t)in)
+                 : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// `bytes` (a multiple of 16, both ends on 16 bytes) by the copy engine, counted on `bar`.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_at(dst)), "l"(src),
+                 "r"(bytes), "r"(smem_at(bar))
+                 : "memory");
+}
 
 // Rows t0.. of a (tokens, d) tensor into a tile of 16 x D with rows `ld` apart; zeros past the sequence and past d.
 template <class T, int D>
@@ -158,7 +170,7 @@ __device__ __forceinline__ void stage(T* tile, int ld, const T* src, int64_t str
         T* to = tile + r * ld + c;
         const T* from = src + (in ? (t0 + r) * stride_t + c : 0);
         if (aligned) {
-            cp_async16(to, from, in ? min(kPer, d - c) * (int)sizeof(T) : 0);
+            cp_async16(to, from, in);
         } else {
 #pragma unroll
             for (int j = 0; j < kPer; ++j) to[j] = in && c + j < d ? from[j] : from_f32<T>(0.f);
@@ -214,24 +226,31 @@ __device__ __forceinline__ void fill_decays(Decays& w, float a, float beta, int 
     __syncwarp();
 }
 
-// Gate scalars of the 16 tokens of a block, lane i < 16 holding token i.
+// Gate scalars of the 16 tokens of a block, lane i < 16 holding token i: loads only, so that they can be on their way
+// while the block before is worked on.
 struct Gates {
-    float a, beta;
-    uint32_t resets;  // bit i: token i starts an episode
+    float g, beta;
+    uint32_t reset;
+    __device__ __forceinline__ float decay() const { return expf(g); }
+    __device__ __forceinline__ uint32_t starts() const { return __ballot_sync(0xffffffffu, reset != 0); }  // bit i: token i starts an episode
 };
-__device__ __forceinline__ Gates load_gates(const Scan& p, int64_t n, int64_t h, int64_t t0, int lane) {
-    Gates s{1.f, 0.f, 0u};
-    const int64_t t = t0 + lane;
-    const bool in = lane < kC && t < p.t;
-    bool reset = false;
-    if (in) {
-        s.a = expf(p.g[t * p.sg.t + n * p.sg.n + h * p.sg.h]);
-        s.beta = p.beta[t * p.sb.t + n * p.sb.n + h * p.sb.h];
-        reset = p.reset && p.reset[t * p.reset_t + n * p.reset_n] != 0;
+struct GatePointers {
+    const float *g, *beta;
+    const uint8_t* reset;
+    int64_t g_t, b_t, r_t;
+    __device__ __forceinline__ GatePointers(const Scan& p, int64_t n, int64_t h, int lane)
+        : g(p.g + lane * p.sg.t + n * p.sg.n + h * p.sg.h), beta(p.beta + lane * p.sb.t + n * p.sb.n + h * p.sb.h),
+          reset(p.reset ? p.reset + lane * p.reset_t + n * p.reset_n : nullptr), g_t(p.sg.t), b_t(p.sb.t), r_t(p.reset_t) {}
+    __device__ __forceinline__ Gates load(int64_t t0, int64_t t_end, int lane) const {
+        Gates s{0.f, 0.f, 0u};
+        if (lane < kC && t0 + lane < t_end) {
+            s.g = g[t0 * g_t];
+            s.beta = beta[t0 * b_t];
+            if (reset) s.reset = reset[t0 * r_t];
+        }
+        return s;
     }
-    s.resets = __ballot_sync(0xffffffffu, reset);
-    return s;
-}
+};
 
 __device__ __forceinline__ bool within(int i, int r0, int r1) { return i >= r0 && i < r1; }
 // Halves of a register that holds tokens i and i + 1 of an operand: zero those outside the chunk, whatever they hold.
@@ -241,129 +260,273 @@ __device__ __forceinline__ uint32_t pair_mask(int i, int r0, int r1) {
 
 // ---------------------------------------------------------------- forward
 //
-// A block takes one (env, head); each warp 16 columns of the state, which need
-// nothing of one another.  A warp holds its columns transposed (dv x dk) as
-// accumulators of S^T += U^T K, which is also the register layout of the B
-// operand of K S and Q S: the state never leaves the registers.  Inputs are
-// fetched one block of 16 tokens ahead (cp.async), one barrier a block.
+// A block takes 64 columns of one (env, head)'s state: four warps with 16 each,
+// and one helper.  Columns need nothing of one another, so a state warp keeps its
+// columns, transposed (dv x dk), in registers for the whole sequence, and works
+// in transposed form throughout,
+//
+//   R^T = V^T - (S^T K^T) gamma    E^T = R^T M^T    U = beta E
+//   O^T = (S^T Q^T) gamma + U^T (D o Q K^T)^T       S^T <- Gamma S^T + (eta U)^T K
+//
+// because the accumulators of one product are then the A operand of the next:
+// no state, error or update passes through shared memory.
+//
+// What the warps would all compute alike is the helper's, one chunk ahead: the
+// loads (a bulk copy for each row, two blocks of 16 tokens ahead), the decays, Q K^T and K K^T,
+// and M = (I + (D o K K^T) beta)^-1 by substitution, so that the triangular
+// solve is a product too.  One barrier a chunk.
 
-constexpr int kRowPad = 20;  // floats of a row of a warp's 16 x 16 scratch
+constexpr int kLdM = kC + 8;  // bf16 of a row of a 16 x 16 operand tile
 
-struct alignas(16) WarpScratch {
-    Decays w;
-    float lt[kC][kC];         // D_ij k_i.k_j (i > j) at [j][i]
-    float r[kC][kRowPad];     // K S, then U
+struct alignas(16) Chunk {  // a chunk as the helper leaves it
+    __nv_bfloat16 m[3][kC][kLdM];    // M, by terms
+    __nv_bfloat16 att[3][kC][kLdM];  // D_ij q_i.k_j (i >= j), by terms
+    float gamma[kC], eta[kC], beta[kC];
+    float keep;
+    int block, r0, r1;               // tokens 16 block + r0 .. r1 - 1; block < 0: the sequence is over
+    int fresh;                       // starts an episode
 };
-static_assert(offsetof(WarpScratch, r) % 16 == 0, "rows are accessed two floats at a time");
+
+constexpr int kLdD = 34;
+
+struct alignas(16) HelperScratch {
+    float d[kC][kLdD];    // D_ij; column 16: gamma_i; the rest is not read
+    float b[kC][kC + 4];  // strictly lower part of the system
+    float x[8][8];
+};
+
+// Decays of tokens r0..r1-1 (lane i holds a_i; 1 outside): D to scratch, gamma, eta, beta and keep to the chunk.
+__device__ __forceinline__ void chunk_decays(float (&d)[kC][kLdD], float (&gamma)[kC], float (&eta)[kC], float (&beta_out)[kC],
+                                             float& keep, float a, float beta, int r0, int r1, bool fresh, int lane) {
+    // lane j < 16 runs down column j of D from its diagonal, lane 16 down the column before the chunk, which is gamma
+    const int start = lane == 16 ? r0 : lane;
+    float run = 0.f, last = 0.f;
+#pragma unroll
+    for (int i = 0; i < kC; ++i) {
+        const float ai = __shfl_sync(0xffffffffu, a, i);
+        const float begin = lane == 16 ? (fresh ? 0.f : ai) : 1.f;
+        run = i == start ? begin : run * ai;
+        d[i][lane] = run;
+        last = i == r1 - 1 ? run : last;
+    }
+    __syncwarp();
+    const bool in = within(lane, r0, r1);
+    if (lane < 16) {
+        gamma[lane] = in ? d[lane][16] : 0.f;
+        eta[lane] = in ? last : 0.f;
+        beta_out[lane] = in ? beta : 0.f;
+    } else if (lane == 16) {
+        keep = last;
+    }
+}
+
+// The inverse of I + b, b strictly lower triangular 16 x 16, into b: two 8 x 8 inverses by substitution (lanes 0..7 and
+// 8..15, a column each), then the block below them, -M22 b21 M11.
+__device__ __forceinline__ void invert_lower(HelperScratch& hs, int lane) {
+    if (lane < 16) {
+        const int o = lane & 8, c = lane & 7;
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = i == c ? 1.f : 0.f;
+#pragma unroll
+        for (int j = 0; j < 7; ++j)
+#pragma unroll
+            for (int i = j + 1; i < 8; ++i) x[i] = fmaf(-hs.b[o + i][o + j], x[j], x[i]);
+        __syncwarp(0xffffu);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) hs.b[o + i][o + c] = x[i];
+    }
+    __syncwarp();
+    const int i = lane / 4, j = lane % 4 * 2;  // 64 entries, two a lane
+    float y0 = 0.f, y1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float l = hs.b[8 + i][k];
+        y0 = fmaf(l, hs.b[k][j], y0);
+        y1 = fmaf(l, hs.b[k][j + 1], y1);
+    }
+    hs.x[i][j] = y0;
+    hs.x[i][j + 1] = y1;
+    __syncwarp();
+    y0 = y1 = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+        const float l = hs.b[8 + i][8 + k];
+        y0 = fmaf(-l, hs.x[k][j], y0);
+        y1 = fmaf(-l, hs.x[k][j + 1], y1);
+    }
+    hs.b[8 + i][j] = y0;
+    hs.b[8 + i][j + 1] = y1;
+    hs.b[i][8 + j] = 0.f;
+    hs.b[i][8 + j + 1] = 0.f;
+    __syncwarp();
+}
+
+// A 16 x 16 fp32 matrix in scratch as N bf16 terms.
+template <int N>
+__device__ __forceinline__ void store_terms(__nv_bfloat16 (&out)[3][kC][kLdM], const float (&in)[kC][kC + 4], int lane) {
+#pragma unroll
+    for (int z = 0; z < 4; ++z) {
+        const int i = z * 4 + lane / 8, j = lane % 8 * 2;
+        const float2 v = *reinterpret_cast<const float2*>(&in[i][j]);
+        uint32_t s[N];
+        split(v.x, v.y, s);
+#pragma unroll
+        for (int x = 0; x < N; ++x) *reinterpret_cast<uint32_t*>(&out[x][i][j]) = s[x];
+    }
+}
+
+// 16 x 16 operand tile as a B operand whose columns are the tile's rows.
+template <int N>
+__device__ __forceinline__ void load_operand(uint32_t (&r)[N][4], const __nv_bfloat16 (&tile)[3][kC][kLdM], int lane) {
+#pragma unroll
+    for (int x = 0; x < N; ++x) load_rows(r[x], &tile[x][0][0], kLdM, 0, lane);
+}
+
+// Up to 16 rows of a (tokens, d) tensor into a tile by one warp: where rows are whole 16-byte chunks a lane asks the copy
+// engine for a row (and the warp has told `bar` to expect the bytes), else the warp loads them.  Columns past d and rows
+// past the sequence keep what they hold.
+template <class T>
+__device__ __forceinline__ void stage_rows(T* tile, int ld, const T* src, int64_t stride_t, int rows, int d, bool aligned, uint64_t* bar,
+                                           int lane) {
+    if (aligned) {
+        if (lane < rows) bulk_load(tile + lane * ld, src + lane * stride_t, d * (uint32_t)sizeof(T), bar);
+    } else {
+        for (int r = 0; r < rows; ++r)
+            for (int c = lane; c < d; c += 32) tile[r * ld + c] = src[r * stride_t + c];
+    }
+}
+
+template <class T, int D>
+__device__ __forceinline__ void to_terms_warp(__nv_bfloat16* terms, int ld, const T* raw, int ld_raw, int lane) {
+    constexpr int N = Terms<T>::n;
+    for (int i = lane; i < kC * D / 2; i += 32) {
+        const int r = i / (D / 2), c = i % (D / 2) * 2;
+        uint32_t s[N];
+        split(to_f32(raw[r * ld_raw + c]), to_f32(raw[r * ld_raw + c + 1]), s);
+#pragma unroll
+        for (int j = 0; j < N; ++j) *reinterpret_cast<uint32_t*>(terms + (j * kC + r) * ld + c) = s[j];
+    }
+}
+
+constexpr int kLdOut = 24;  // 16-bit elements of a row of a warp's 16 x 16 tile on its way out
+
+constexpr int kForwardWarps = 4;  // state warps of a block: 64 columns
 
 template <class T, int DK>
 struct ForwardSmem {
-    static constexpr int kLd = DK + 16 / sizeof(T);      // raw rows
-    static constexpr int kLdTerm = DK + 8;               // rows of terms; the same for bf16
+    static constexpr int kWidth = kForwardWarps * 16;
+    static constexpr int kLd = DK + 16 / sizeof(T), kLdV = kWidth + 16 / sizeof(T);  // raw rows
+    static constexpr int kLdTerm = DK + 8;                                           // rows of terms; the same for bf16
     static constexpr bool kInPlace = Terms<T>::n == 1;
-    __host__ __device__ static constexpr size_t raw(int dv16) { return 2 * kC * (2 * kLd + (size_t)dv16) * sizeof(T); }
-    __host__ __device__ static constexpr size_t terms() { return kInPlace ? 0 : 2 * Terms<T>::n * kC * kLdTerm * 2; }
-    static size_t bytes(int warps) { return raw(warps * 16 + 16) + terms() + warps * sizeof(WarpScratch); }
+    static constexpr int kBuffers = 4;  // state warps on one block, the helper on the next, two on their way
+    static constexpr size_t kRaw = (size_t)kC * (2 * kLd + kLdV) * sizeof(T);        // a buffer
+    static constexpr size_t kTerms = kInPlace ? 0 : (size_t)2 * 2 * Terms<T>::n * kC * kLdTerm * 2;  // of two blocks
+    static constexpr int kLdS = 20;  // floats of a row of a warp's columns of the state on their way out
+    static constexpr size_t kOut = (size_t)DK * kLdS * 4;  // of a warp: that, or its 16 x 16 outputs
+    static constexpr size_t kBytes = kBuffers * kRaw + kTerms + 2 * sizeof(Chunk) + sizeof(HelperScratch) + kForwardWarps * kOut + 8 * kBuffers;
+    static_assert(kRaw % 16 == 0 && kTerms % 16 == 0 && kOut % 16 == 0 && kOut >= kC * kLdOut * 2, "layout");
 };
 
 template <class T, int DK>
-__global__ void __launch_bounds__(256) scan_forward_kernel(const Scan p) {
+__global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) scan_forward_kernel(const Scan p) {
     using L = ForwardSmem<T, DK>;
     constexpr int NT = Terms<T>::n, kTiles = DK / 8, kSteps = DK / 16;
     constexpr int NO = NT == 3 ? 3 : 2;  // terms that o needs: 16 bits and more against its own 8 or 11
     extern __shared__ __align__(16) uint8_t smem[];
-    const int warps = blockDim.x / 32, warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = lane / 4, quad = lane % 4;
-    const int ldv = warps * 16 + 16;
-    T* raw = reinterpret_cast<T*>(smem);
-    constexpr int kRaw = kC * L::kLd;
-    const int raw_v = kC * ldv, raw_all = 2 * kRaw + raw_v;
-    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(smem + L::raw(ldv));
-    WarpScratch& ws = reinterpret_cast<WarpScratch*>(smem + L::raw(ldv) + L::terms())[warp];
+    constexpr int warps = kForwardWarps, ldv = L::kLdV;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = lane / 4, quad = lane % 4;
+    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(smem + L::kBuffers * L::kRaw);
+    Chunk* chunks = reinterpret_cast<Chunk*>(smem + L::kBuffers * L::kRaw + L::kTerms);
+    HelperScratch& hs = *reinterpret_cast<HelperScratch*>(chunks + 2);
+    float* out_tiles = reinterpret_cast<float*>(&hs + 1);
+    uint64_t* arrived = reinterpret_cast<uint64_t*>(out_tiles + warps * L::kOut / 4);  // a buffer's rows are there
     const int64_t seq = blockIdx.x, n = seq / p.h, h = seq % p.h;
-    const T* q = static_cast<const T*>(p.q) + n * p.sq.n + h * p.sq.h;
-    const T* k = static_cast<const T*>(p.k) + n * p.sk.n + h * p.sk.h;
-    const T* v = static_cast<const T*>(p.v) + n * p.sv.n + h * p.sv.h;
+    const int first_col = blockIdx.y * L::kWidth, cols = min(L::kWidth, p.dv - first_col);
     const int64_t blocks = (p.t + kC - 1) / kC;
-    const int c0 = warp * 16;  // this warp's columns of the state
-
-    auto fetch = [&](int64_t b, int buf) {
-        T* to = raw + buf * raw_all;
-        stage<T, DK>(to, L::kLd, k, p.sk.t, b * kC, p.t, p.dk, p.aligned);
-        stage<T, DK>(to + kRaw, L::kLd, q, p.sq.t, b * kC, p.t, p.dk, p.aligned);
-        constexpr int kPer = 16 / sizeof(T);
-        const int per_row = warps * 16 / kPer;
-        for (int i = threadIdx.x; i < kC * per_row; i += blockDim.x) {
-            const int r = i / per_row, c = i % per_row * kPer;
-            const bool in = b * kC + r < p.t && c < p.dv;
-            T* dst = to + 2 * kRaw + r * ldv + c;
-            const T* from = v + (in ? (b * kC + r) * p.sv.t + c : 0);
-            if (p.aligned) {
-                cp_async16(dst, from, in ? min(kPer, p.dv - c) * (int)sizeof(T) : 0);
-            } else {
-#pragma unroll
-                for (int j = 0; j < kPer; ++j) dst[j] = in && c + j < p.dv ? from[j] : from_f32<T>(0.f);
-            }
-        }
-        cp_async_commit();
+    auto raw_tile = [&](int64_t b) { return reinterpret_cast<T*>(smem + b % L::kBuffers * L::kRaw); };
+    // K and Q of a block as operand tiles
+    auto k_tile = [&](int64_t b) -> const __nv_bfloat16* {
+        return L::kInPlace ? reinterpret_cast<const __nv_bfloat16*>(raw_tile(b)) : terms + (b & 1) * (L::kTerms / 4);
     };
+    auto q_tile = [&](int64_t b) -> const __nv_bfloat16* {
+        return k_tile(b) + (L::kInPlace ? kC * L::kLd : NT * kC * L::kLdTerm);
+    };
+    for (int i = threadIdx.x; i < (int)(L::kBuffers * L::kRaw / 16); i += blockDim.x)
+        reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);  // columns past dk and dv stay zero
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kBuffers; ++i) tc::mbar_init(&arrived[i], 1);
+        tc::mbar_init_fence();
+    }
+    tc::fence_async_smem();
+    __syncthreads();
 
-    Acc s[kTiles];  // S^T: rows = columns c0.. of the state, columns = dk
-    const float* s0 = p.state ? p.state + seq * p.dk * p.dv : nullptr;
-#pragma unroll
-    for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int kk = i * 8 + quad * 2 + e % 2, c = c0 + row + e / 2 * 8;
-            s[i].v[e] = s0 && kk < p.dk && c < p.dv ? s0[(int64_t)kk * p.dv + c] : 0.f;
-        }
-
-    fetch(0, 0);
-    Gates next = load_gates(p, n, h, 0, lane);
-    for (int64_t b = 0; b < blocks; ++b) {
-        const int buf = b & 1;
-        cp_async_wait<0>();
-        __syncthreads();
-        if (b + 1 < blocks) fetch(b + 1, buf ^ 1);
-        const Gates gates = next;
-        if (b + 1 < blocks) next = load_gates(p, n, h, (b + 1) * kC, lane);
-        const T* tk = raw + buf * raw_all;
-        const T* tv = tk + 2 * kRaw;
-        const __nv_bfloat16 *kt, *qt;
-        if constexpr (L::kInPlace) {
-            kt = reinterpret_cast<const __nv_bfloat16*>(tk);
-            qt = kt + kRaw;
-        } else {
-            to_terms<T, DK>(terms, L::kLdTerm, tk, L::kLd);
-            to_terms<T, DK>(terms + NT * kC * L::kLdTerm, L::kLdTerm, tk + kRaw, L::kLd);
-            kt = terms;
-            qt = terms + NT * kC * L::kLdTerm;
-            __syncthreads();
-        }
-        if (p.checkpoints) {
-            float* to = p.checkpoints + (seq * blocks + b) * p.dk * p.dv;
-#pragma unroll
-            for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const int kk = i * 8 + quad * 2 + e % 2, c = c0 + row + e / 2 * 8;
-                    if (kk < p.dk && c < p.dv) to[(int64_t)kk * p.dv + c] = s[i].v[e];
-                }
-        }
-        const int count = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
-        for (int r0 = 0; r0 < count;) {
-            const bool fresh = gates.resets >> r0 & 1;
-            const uint32_t later = gates.resets & ~((2u << r0) - 1);
-            const int r1 = later ? min(count, __ffs(later) - 1) : count;
-            if (fresh) {
-#pragma unroll
-                for (int i = 0; i < kTiles; ++i) s[i].zero();
+    if (warp == warps) {
+        const T* q = static_cast<const T*>(p.q) + n * p.sq.n + h * p.sq.h;
+        const T* k = static_cast<const T*>(p.k) + n * p.sk.n + h * p.sk.h;
+        const T* v = static_cast<const T*>(p.v) + n * p.sv.n + h * p.sv.h + first_col;
+        auto fetch = [&](int64_t b) {
+            if (b >= blocks) return;
+            T* to = raw_tile(b);
+            uint64_t* bar = &arrived[b % L::kBuffers];
+            const int rows = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
+            if (p.aligned) {
+                if (lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(rows * (2 * p.dk + cols) * sizeof(T)));
+                __syncwarp();
             }
-            __syncwarp();
-            fill_decays(ws.w, within(lane, r0, r1) ? gates.a : 1.f, gates.beta, r0, r1, fresh, lane);
-
-            Acc kk[2], qk[2], ks[2], qs[2];
+            stage_rows(to, L::kLd, k + b * kC * p.sk.t, p.sk.t, rows, p.dk, p.aligned, bar, lane);
+            stage_rows(to + kC * L::kLd, L::kLd, q + b * kC * p.sq.t, p.sq.t, rows, p.dk, p.aligned, bar, lane);
+            stage_rows(to + 2 * kC * L::kLd, ldv, v + b * kC * p.sv.t, p.sv.t, rows, cols, p.aligned, bar, lane);
+        };
+        fetch(0);
+        fetch(1);
+        const GatePointers get_gates(p, n, h, lane);
+        Gates gates{}, next = get_gates.load(0, p.t, lane);
+        float decay = 1.f;
+        uint32_t starts = 0;
+        int64_t b = -1;
+        int r0 = 0, count = 0;
+        for (int turn = 0;; ++turn) {
+            Chunk& ch = chunks[turn & 1];
+            if (r0 >= count) {  // the next block of 16 tokens
+                ++b;
+                r0 = 0;
+                if (b >= blocks) {
+                    if (lane == 0) ch.block = -1;
+                    __syncthreads();
+                    break;
+                }
+                count = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
+                gates = next;
+                next = get_gates.load((b + 1) * kC, p.t, lane);
+                decay = gates.decay();
+                starts = gates.starts();
+                if (p.aligned && !tc::mbar_wait_warp(&arrived[b % L::kBuffers], b / L::kBuffers & 1)) {
+                    if (lane == 0) {
+                        atomicAdd(p.stalls, 1u);
+                        ch.block = -1;
+                    }
+                    __syncthreads();
+                    break;
+                }
+                __syncwarp();
+                fetch(b + 2);
+                if constexpr (!L::kInPlace) {
+                    __nv_bfloat16* to = terms + (b & 1) * (L::kTerms / 4);
+                    to_terms_warp<T, DK>(to, L::kLdTerm, raw_tile(b), L::kLd, lane);
+                    to_terms_warp<T, DK>(to + NT * kC * L::kLdTerm, L::kLdTerm, raw_tile(b) + kC * L::kLd, L::kLd, lane);
+                    __syncwarp();
+                }
+            }
+            const bool fresh = starts >> r0 & 1;
+            const uint32_t later = starts & ~((2u << r0) - 1);
+            const int r1 = later ? min(count, __ffs(later) - 1) : count;
+            chunk_decays(hs.d, ch.gamma, ch.eta, ch.beta, ch.keep, within(lane, r0, r1) ? decay : 1.f, gates.beta, r0, r1, fresh, lane);
+            if (lane == 0) ch.block = (int)b, ch.r0 = r0, ch.r1 = r1, ch.fresh = fresh;
+            const __nv_bfloat16 *kt = k_tile(b), *qt = q_tile(b);
+            Acc kk[2], qk[2];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) kk[i].zero(), qk[i].zero(), ks[i].zero(), qs[i].zero();
+            for (int i = 0; i < 2; ++i) kk[i].zero(), qk[i].zero();
 #pragma unroll
             for (int st = 0; st < kSteps; ++st) {
                 uint32_t ka[NT][4], qa[NT][4];
@@ -374,120 +537,243 @@ __global__ void __launch_bounds__(256) scan_forward_kernel(const Scan p) {
                 }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    uint32_t kb[NT][2], sb[3][2], lo[3], hi[3];
+                    uint32_t kb[NT][2];
 #pragma unroll
                     for (int x = 0; x < NT; ++x) kb[x][0] = ka[x][c], kb[x][1] = ka[x][c + 2];
                     mma_terms<3>(kk[c], ka, kb);
                     mma_terms<NO>(qk[c], qa, kb);
-                    split(s[2 * st].v[2 * c], s[2 * st].v[2 * c + 1], lo);
-                    split(s[2 * st + 1].v[2 * c], s[2 * st + 1].v[2 * c + 1], hi);
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) sb[x][0] = lo[x], sb[x][1] = hi[x];
-                    mma_terms<3>(ks[c], ka, sb);
-                    mma_terms<NO>(qs[c], qa, sb);
                 }
             }
-            // the triangular part to shared memory, D o Q K^T as the A operand of (D o Q K^T) U
-            uint32_t att[NO][4];
+            __syncwarp();
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int i = row + half * 8, j = c * 8 + quad * 2;
-                    float at[2];
+                    const float2 d = *reinterpret_cast<const float2*>(&hs.d[i][j]);
+                    const float2 be = *reinterpret_cast<const float2*>(&ch.beta[j]);
+                    const bool in0 = within(i, r0, r1) && j >= r0, in1 = within(i, r0, r1) && j + 1 >= r0;  // and j <= i
+                    *reinterpret_cast<float2*>(&hs.b[i][j]) = make_float2(in0 && i > j ? d.x * be.x * kk[c].v[half * 2] : 0.f,
+                                                                          in1 && i > j + 1 ? d.y * be.y * kk[c].v[half * 2 + 1] : 0.f);
+                    uint32_t s[NO];
+                    split(in0 && i >= j ? d.x * qk[c].v[half * 2] : 0.f, in1 && i >= j + 1 ? d.y * qk[c].v[half * 2 + 1] : 0.f, s);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const float d = ws.w.d[i][j + e];
-                        const bool in = within(i, r0, r1) && within(j + e, r0, r1);
-                        ws.lt[j + e][i] = in && i > j + e ? d * kk[c].v[half * 2 + e] : 0.f;
-                        at[e] = in && i >= j + e ? d * qk[c].v[half * 2 + e] : 0.f;
-                    }
-                    uint32_t tmp[NO];
-                    split(at[0], at[1], tmp);
-#pragma unroll
-                    for (int x = 0; x < NO; ++x) att[x][c * 2 + half] = tmp[x];
-                    *reinterpret_cast<float2*>(&ws.r[i][j]) = make_float2(ks[c].v[half * 2], ks[c].v[half * 2 + 1]);
+                    for (int x = 0; x < NO; ++x) *reinterpret_cast<uint32_t*>(&ch.att[x][i][j]) = s[x];
                 }
             __syncwarp();
-            if (lane < 16) {  // one column of the state each: forward substitution
-                float x[kC];
-#pragma unroll
-                for (int i = 0; i < kC; ++i) x[i] = to_f32(tv[i * ldv + c0 + lane]) - ws.w.gamma[i] * ws.r[i][lane];
-                float* er = p.errors && c0 + lane < p.dv ? p.errors + ((b * kC * p.n + n) * p.h + h) * p.dv + c0 + lane : nullptr;
-                const int64_t er_t = p.n * p.h * p.dv;
-#pragma unroll
-                for (int i = 0; i < kC; ++i) {
-                    const bool in = within(i, r0, r1);
-                    const float u = in ? ws.w.beta[i] * x[i] : 0.f;
-                    if (er && in) er[i * er_t] = x[i];
-                    ws.r[i][lane] = u;
-#pragma unroll
-                    for (int j = i + 1; j < kC; ++j) x[j] = fmaf(-ws.lt[i][j], u, x[j]);
-                }
-            }
-            __syncwarp();
-            // U as the B operand (tokens x columns) of (D o Q K^T) U, and eta U transposed as the A operand of the update
-            uint32_t ua[3][4];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t ub[NO][2];
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int i = quad * 2 + half * 8;
-                    const float x = ws.r[i][c * 8 + row], y = ws.r[i + 1][c * 8 + row];
-                    uint32_t tmp[NO], tmp3[3];
-                    split(x, y, tmp);
-                    split(x * ws.w.eta[i], y * ws.w.eta[i + 1], tmp3);
-#pragma unroll
-                    for (int z = 0; z < NO; ++z) ub[z][half] = tmp[z];
-#pragma unroll
-                    for (int z = 0; z < 3; ++z) ua[z][half * 2 + c] = tmp3[z];
-                }
-                const float g0 = ws.w.gamma[row], g1 = ws.w.gamma[row + 8];
-                qs[c].v[0] *= g0, qs[c].v[1] *= g0, qs[c].v[2] *= g1, qs[c].v[3] *= g1;
-                mma_terms<NO>(qs[c], att, ub);
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int i = row + half * 8, col = c0 + c * 8 + quad * 2;
-                    if (within(i, r0, r1)) {
-                        T* o = static_cast<T*>(p.o) + (((b * kC + i) * p.n + n) * p.h + h) * p.dv + col;
-#pragma unroll
-                        for (int e = 0; e < 2; ++e)
-                            if (col + e < p.dv) o[e] = from_f32<T>(p.scale * qs[c].v[half * 2 + e]);
-                    }
-                }
-            }
-            const float keep = ws.w.keep;
-            const uint32_t m0 = pair_mask(quad * 2, r0, r1), m1 = pair_mask(quad * 2 + 8, r0, r1);
-#pragma unroll
-            for (int st = 0; st < kSteps; ++st) {
-                uint32_t kb[NT][4];
-#pragma unroll
-                for (int x = 0; x < NT; ++x) load_tokens(kb[x], kt + x * kC * L::kLdTerm, L::kLdTerm, st * 16, lane);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    Acc& acc = s[2 * st + c];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) acc.v[e] *= keep;
-                    uint32_t bb[NT][2];
-#pragma unroll
-                    for (int x = 0; x < NT; ++x) bb[x][0] = kb[x][2 * c] & m0, bb[x][1] = kb[x][2 * c + 1] & m1;
-                    mma_terms<3>(acc, ua, bb);
-                }
-            }
+            invert_lower(hs, lane);
+            store_terms<3>(ch.m, hs.b, lane);
+            __syncwarp();  // scratch is free
             r0 = r1;
+            __syncthreads();
         }
+        return;
     }
-    if (p.final_state) {
-        float* to = p.final_state + seq * p.dk * p.dv;
+
+    const int v0 = warp * 16, c0 = first_col + v0;  // this warp's columns of the state
+    const bool whole = p.dk == DK && c0 + 16 <= p.dv;
+    float* state_tile = out_tiles + warp * L::kOut / 4;
+    __nv_bfloat16* out_tile = reinterpret_cast<__nv_bfloat16*>(state_tile);
+    const bool s_aligned = p.dv % 4 == 0 && reinterpret_cast<uintptr_t>(p.checkpoints) % 16 == 0 &&
+                           reinterpret_cast<uintptr_t>(p.final_state) % 16 == 0;
+    const bool o_aligned = sizeof(T) == 2 && p.dv % 8 == 0 && reinterpret_cast<uintptr_t>(p.o) % 16 == 0;
+    Acc s[kTiles];  // S^T: rows = columns c0.. of the state, columns = dk
+    // where this thread's values of a (dk, dv) matrix lie: value e of tile i at i * 8 * dv + at(e)
+    auto each_state = [&](auto&& f) {
 #pragma unroll
         for (int i = 0; i < kTiles; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int kk = i * 8 + quad * 2 + e % 2, c = c0 + row + e / 2 * 8;
-                if (kk < p.dk && c < p.dv) to[(int64_t)kk * p.dv + c] = s[i].v[e];
+                f(s[i].v[e], kk * p.dv + c, whole || (kk < p.dk && c < p.dv));
             }
+    };
+    {
+        const float* s0 = p.state ? p.state + seq * p.dk * p.dv : nullptr;
+        each_state([&](float& x, int at, bool in) { x = s0 && in ? s0[at] : 0.f; });
     }
+    // The state to a (dk, dv) matrix: through shared memory, 16 columns of a row at a time, so that stores are 16 bytes.
+    auto put_state = [&](float* to) {
+        if (whole && s_aligned) {
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) state_tile[(i * 8 + quad * 2 + e % 2) * L::kLdS + row + e / 2 * 8] = s[i].v[e];
+            __syncwarp();
+            float4* out = reinterpret_cast<float4*>(to + (lane / 4) * p.dv + c0 + lane % 4 * 4);
+#pragma unroll
+            for (int i = 0; i < DK / 8; ++i)
+                __stcs(out + i * 2 * p.dv, *reinterpret_cast<const float4*>(state_tile + (i * 8 + lane / 4) * L::kLdS + lane % 4 * 4));
+            __syncwarp();
+        } else {
+            each_state([&](float& x, int at, bool in) {
+                if (in) to[at] = x;
+            });
+        }
+    };
+    const int64_t step_t = p.n * p.h * p.dv, first = (n * p.h + h) * p.dv + c0;
+    for (int turn = 0;; ++turn) {
+        __syncthreads();
+        const Chunk& ch = chunks[turn & 1];
+        const int64_t b = ch.block;
+        if (b < 0) break;
+        if (p.aligned) tc::mbar_wait_warp(&arrived[b % L::kBuffers], b / L::kBuffers & 1);  // long since; it makes the copies visible here
+        const int r0 = ch.r0, r1 = ch.r1;
+        const __nv_bfloat16 *kt = k_tile(b), *qt = q_tile(b);
+        if (p.checkpoints && r0 == 0) put_state(p.checkpoints + (seq * blocks + b) * p.dk * p.dv);
+        if (ch.fresh) {
+#pragma unroll
+            for (int i = 0; i < kTiles; ++i) s[i].zero();
+        }
+        Acc ks[2], qs[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) ks[i].zero(), qs[i].zero();
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+            uint32_t sa[3][4];
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                uint32_t tmp[3];
+                const Acc& t = s[2 * st + z / 2];
+                split(t.v[z % 2 * 2], t.v[z % 2 * 2 + 1], tmp);
+#pragma unroll
+                for (int x = 0; x < 3; ++x) sa[x][z] = tmp[x];
+            }
+            uint32_t ka[NT][4], qa[NT][4];
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                load_rows(ka[x], kt + x * kC * L::kLdTerm, L::kLdTerm, st * 16, lane);
+                load_rows(qa[x], qt + x * kC * L::kLdTerm, L::kLdTerm, st * 16, lane);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t kb[NT][2], qb[NT][2];
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    kb[x][0] = ka[x][c], kb[x][1] = ka[x][c + 2];
+                    qb[x][0] = qa[x][c], qb[x][1] = qa[x][c + 2];
+                }
+                mma_terms<3>(ks[c], sa, kb);
+                mma_terms<NO>(qs[c], sa, qb);
+            }
+        }
+        // R^T; tokens outside the chunk are zero whatever their inputs hold
+        uint32_t ra[3][4];
+        {
+            const T* tv = raw_tile(b) + 2 * kC * L::kLd;
+            uint32_t vv[4];
+            if constexpr (L::kInPlace) load_columns(vv, reinterpret_cast<const __nv_bfloat16*>(tv), ldv, v0, lane);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int j = c * 8 + quad * 2;
+                const float2 ga = *reinterpret_cast<const float2*>(&ch.gamma[j]);
+                const bool in0 = within(j, r0, r1), in1 = within(j + 1, r0, r1);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    float x0, x1;
+                    if constexpr (L::kInPlace) {
+                        x0 = __uint_as_float(vv[c * 2 + half] << 16);
+                        x1 = __uint_as_float(vv[c * 2 + half] & 0xFFFF0000u);
+                    } else {
+                        x0 = to_f32(tv[j * ldv + v0 + row + half * 8]);
+                        x1 = to_f32(tv[(j + 1) * ldv + v0 + row + half * 8]);
+                    }
+                    uint32_t tmp[3];
+                    split(in0 ? fmaf(-ga.x, ks[c].v[half * 2], x0) : 0.f, in1 ? fmaf(-ga.y, ks[c].v[half * 2 + 1], x1) : 0.f, tmp);
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) ra[x][c * 2 + half] = tmp[x];
+                }
+                qs[c].v[0] *= ga.x, qs[c].v[1] *= ga.y, qs[c].v[2] *= ga.x, qs[c].v[3] *= ga.y;
+            }
+        }
+        uint32_t uo[NO][4], ue[3][4];  // U^T and (eta U)^T
+        {
+            uint32_t mb[3][4];
+            load_operand(mb, ch.m, lane);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t bb[3][2];
+#pragma unroll
+                for (int x = 0; x < 3; ++x) bb[x][0] = mb[x][c], bb[x][1] = mb[x][c + 2];
+                Acc e;
+                e.zero();
+                mma_terms<3>(e, ra, bb);
+                const int j = c * 8 + quad * 2;
+                if (p.errors) {
+                    float* er = p.errors + (b * kC + j) * step_t + first + row;
+#pragma unroll
+                    for (int z = 0; z < 4; ++z)
+                        if (within(j + z % 2, r0, r1) && (whole || c0 + row + z / 2 * 8 < p.dv)) __stcs(er + z % 2 * step_t + z / 2 * 8, e.v[z]);
+                }
+                const float2 be = *reinterpret_cast<const float2*>(&ch.beta[j]), et = *reinterpret_cast<const float2*>(&ch.eta[j]);
+                const float h0 = be.x * et.x, h1 = be.y * et.y;  // rounded once more than beta e, then eta: 2^-24
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t t2[NO], t3[3];
+                    split(be.x * e.v[half * 2], be.y * e.v[half * 2 + 1], t2);
+                    split(h0 * e.v[half * 2], h1 * e.v[half * 2 + 1], t3);
+#pragma unroll
+                    for (int x = 0; x < NO; ++x) uo[x][c * 2 + half] = t2[x];
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) ue[x][c * 2 + half] = t3[x];
+                }
+            }
+        }
+        {
+            uint32_t ab[NO][4];
+            load_operand(ab, ch.att, lane);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t bb[NO][2];
+#pragma unroll
+                for (int x = 0; x < NO; ++x) bb[x][0] = ab[x][c], bb[x][1] = ab[x][c + 2];
+                mma_terms<NO>(qs[c], uo, bb);
+            }
+        }
+        if (o_aligned && whole) {  // by a transposed tile in shared memory, 16 bytes a lane
+            if constexpr (sizeof(T) == 2) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                    for (int z = 0; z < 4; ++z)
+                        reinterpret_cast<T*>(out_tile)[(c * 8 + quad * 2 + z % 2) * kLdOut + row + z / 2 * 8] = from_f32<T>(p.scale * qs[c].v[z]);
+                __syncwarp();
+                const int i = lane / 2;
+                if (within(i, r0, r1))
+                    *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + (b * kC + i) * step_t + first + lane % 2 * 8) =
+                        *reinterpret_cast<const uint4*>(out_tile + i * kLdOut + lane % 2 * 8);
+                __syncwarp();
+            }
+        } else {
+            T* o = static_cast<T*>(p.o) + b * kC * step_t + first + row;
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    const int i = c * 8 + quad * 2 + z % 2;
+                    if (within(i, r0, r1) && (whole || c0 + row + z / 2 * 8 < p.dv)) o[i * step_t + z / 2 * 8] = from_f32<T>(p.scale * qs[c].v[z]);
+                }
+        }
+        const float keep = ch.keep;
+        const uint32_t m0 = pair_mask(quad * 2, r0, r1), m1 = pair_mask(quad * 2 + 8, r0, r1);
+#pragma unroll
+        for (int st = 0; st < kSteps; ++st) {
+            uint32_t kb[NT][4];
+#pragma unroll
+            for (int x = 0; x < NT; ++x) load_tokens(kb[x], kt + x * kC * L::kLdTerm, L::kLdTerm, st * 16, lane);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                Acc& acc = s[2 * st + c];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc.v[e] *= keep;
+                uint32_t bb[NT][2];
+#pragma unroll
+                for (int x = 0; x < NT; ++x) bb[x][0] = kb[x][2 * c] & m0, bb[x][1] = kb[x][2 * c + 1] & m1;
+                mma_terms<3>(acc, ue, bb);
+            }
+        }
+    }
+    if (p.final_state) put_state(p.final_state + seq * p.dk * p.dv);
 }
 
 // --------------------------------------------------------------- backward
@@ -509,6 +795,8 @@ __global__ void __launch_bounds__(256) scan_forward_kernel(const Scan p) {
 // for what sums over dk (dU), and 16 rows of dS for what sums over dv (dQ, dK);
 // both copies stay in registers.  X = -beta gamma dR, Y = scale gamma dO and U
 // go through shared memory as bf16 terms.
+
+constexpr int kRowPad = 20;  // floats of a row of a warp's 16 x 16 scratch
 
 template <class T, int DK, int DV>
 struct BackwardSmem {
@@ -589,14 +877,16 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
         }
 
     if (blocks) fetch(blocks - 1, (blocks - 1) & 1);
-    Gates next = load_gates(p, n, h, (blocks - 1) * kC, lane);
+    const GatePointers get_gates(p, n, h, lane);
+    Gates next = get_gates.load((blocks - 1) * kC, p.t, lane);
     for (int64_t b = blocks - 1; b >= 0; --b) {
         const int buf = b & 1;
         cp_async_wait<0>();
         __syncthreads();
         if (b > 0) fetch(b - 1, buf ^ 1);
         const Gates gates = next;
-        if (b > 0) next = load_gates(p, n, h, (b - 1) * kC, lane);
+        if (b > 0) next = get_gates.load((b - 1) * kC, p.t, lane);
+        const uint32_t starts = gates.starts();
         const T* rk = reinterpret_cast<const T*>(smem + buf * L::kRaw);
         const T* rq = rk + kC * L::kLdK;
         const T* ro = rq + kC * L::kLdK;
@@ -617,10 +907,10 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
         }
         const int count = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
         for (int r1 = count; r1 > 0;) {
-            const uint32_t earlier = gates.resets & ((1u << r1) - 1);
+            const uint32_t earlier = starts & ((1u << r1) - 1);
             const int r0 = earlier ? 31 - __clz(earlier) : 0;
-            const bool fresh = gates.resets >> r0 & 1;
-            fill_decays(ws.w, within(lane, r0, r1) ? gates.a : 1.f, gates.beta, r0, r1, fresh, lane);
+            const bool fresh = starts >> r0 & 1;
+            fill_decays(ws.w, within(lane, r0, r1) ? gates.decay() : 1.f, gates.beta, r0, r1, fresh, lane);
             const uint32_t m0 = pair_mask(quad * 2, r0, r1), m1 = pair_mask(quad * 2 + 8, r0, r1);
 
             // k_i.k_j, and k_j.q_i with tokens j as rows; dU through dS
@@ -1040,11 +1330,11 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
 
 template <class T, int DK>
 int launch_forward_dk(const Scan& p, cudaStream_t st) {
-    const int warps = (p.dv + 15) / 16;
-    const size_t bytes = ForwardSmem<T, DK>::bytes(warps);
+    using L = ForwardSmem<T, DK>;
     auto* kernel = scan_forward_kernel<T, DK>;
-    if (int rc = cuda_status(allow_smem(kernel, (int)bytes), "delta_scan")) return rc;
-    kernel<<<static_cast<unsigned>(p.n * p.h), warps * 32, bytes, st>>>(p);
+    if (int rc = cuda_status(allow_smem(kernel, (int)L::kBytes), "delta_scan")) return rc;
+    const dim3 grid(static_cast<unsigned>(p.n * p.h), (p.dv + L::kWidth - 1) / L::kWidth);
+    kernel<<<grid, (kForwardWarps + 1) * 32, L::kBytes, st>>>(p);
     return cuda_status(cudaGetLastError(), "delta_scan");
 }
 
