@@ -149,8 +149,13 @@ const char* check_common(int dtype, uint64_t n, uint64_t h, uint64_t dk, uint64_
     return nullptr;
 }
 
-bool rows_aligned(const void* p, int64_t a, int64_t b, int64_t c, int size) {
-    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && a * size % 16 == 0 && b * size % 16 == 0 && c * size % 16 == 0;
+// What a tensor map takes: base and strides on 16 bytes, strides positive and below 2^40 bytes (dimensions of one element
+// have none).
+bool rows_aligned(const nesle_delta_args& x, const void* p, int64_t st, int64_t sn, int64_t sh, int size) {
+    auto ok = [&](uint64_t count, int64_t stride) {
+        return count <= 1 || (stride > 0 && stride * size % 16 == 0 && stride < (int64_t(1) << 40) / size);
+    };
+    return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ok(x.t, st) && ok(x.n, sn) && ok(x.h, sh) && x.t <= 0x7FFFFFFFull;
 }
 
 Scan to_scan(const nesle_delta_args& a, bool backward) {
@@ -164,8 +169,10 @@ Scan to_scan(const nesle_delta_args& a, bool backward) {
     p.t = (int64_t)a.t, p.n = (int64_t)a.n, p.h = (int64_t)a.h, p.dk = (int)a.dk, p.dv = (int)a.dv;
     p.scale = a.scale;
     const int size = a.dtype == NESLE_F32 ? 4 : 2;
-    p.aligned = a.dk * size % 16 == 0 && a.dv * size % 16 == 0 && rows_aligned(a.q, a.q_t, a.q_n, a.q_h, size) && rows_aligned(a.k, a.k_t, a.k_n, a.k_h, size) &&
-                (backward ? rows_aligned(a.d_o, (int64_t)a.dv, 0, 0, size) : rows_aligned(a.v, a.v_t, a.v_n, a.v_h, size));
+    const int64_t dv = (int64_t)a.dv;
+    p.aligned = a.dk * size % 16 == 0 && a.dv * size % 16 == 0 && rows_aligned(a, a.q, a.q_t, a.q_n, a.q_h, size) &&
+                rows_aligned(a, a.k, a.k_t, a.k_n, a.k_h, size) &&
+                (backward ? rows_aligned(a, a.d_o, p.n * p.h * dv, p.h * dv, dv, size) : rows_aligned(a, a.v, a.v_t, a.v_n, a.v_h, size));
     p.o = a.o, p.final_state = a.final_state, p.errors = a.errors, p.checkpoints = a.checkpoints;
     p.d_o = a.d_o, p.d_final = a.d_final, p.dq = a.dq, p.dk_out = a.d_k, p.dv_out = a.d_v, p.dg = a.dg, p.dbeta = a.dbeta;
     p.dstate = a.dstate;

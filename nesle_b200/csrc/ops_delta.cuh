@@ -128,19 +128,38 @@ __device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], const void* p) {
                  : "r"(smem_at(p)));
 }
 
-// Tiles are 16 tokens x columns of bf16 in shared memory, rows `ld` elements apart.
+// Tiles of 16 tokens x columns in shared memory come in two layouts.  As fetched (TMA): panels of 16 rows of 128 bytes, a
+// row's eight 16-byte chunks permuted by the row (chunk c of row r at c ^ (r % 8)), so that eight rows of one chunk fall on
+// all banks.  As bf16 terms: rows `ld` elements apart, ld * 2 an odd multiple of 16 bytes.
+template <class T>
+__device__ __forceinline__ int panel_at(int r, int c) {  // element (r, c) of a fetched tile
+    constexpr int kPer = 16 / sizeof(T), kWide = 8 * kPer;
+    return c / kWide * (kC * kWide) + r * kWide + ((c / kPer % 8) ^ (r & 7)) * kPer + c % kPer;
+}
+struct Panels {  // a fetched bf16 tile as an operand
+    const __nv_bfloat16* tile;
+    __device__ __forceinline__ const __nv_bfloat16* at(int r, int c) const { return tile + panel_at<__nv_bfloat16>(r, c); }
+};
+struct Rows {  // a tile of terms
+    const __nv_bfloat16* tile;
+    int ld;
+    __device__ __forceinline__ const __nv_bfloat16* at(int r, int c) const { return tile + r * ld + c; }
+};
 // A operand, rows = tokens, k = columns c0..c0+15.  As a B operand with columns = tokens (K K^T) the same registers
 // are {r0, r2} for tokens 0..7 and {r1, r3} for tokens 8..15.
-__device__ __forceinline__ void load_rows(uint32_t (&r)[4], const __nv_bfloat16* tile, int ld, int c0, int lane) {
-    ldmatrix4(r, tile + (lane % 16) * ld + c0 + lane / 16 * 8);
+template <class Tile>
+__device__ __forceinline__ void load_rows(uint32_t (&r)[4], const Tile& t, int c0, int lane) {
+    ldmatrix4(r, t.at(lane % 16, c0 + lane / 16 * 8));
 }
 // B operand, k = tokens, columns c0..c0+15: {r0, r1} for the first 8 columns, {r2, r3} for the next.
-__device__ __forceinline__ void load_tokens(uint32_t (&r)[4], const __nv_bfloat16* tile, int ld, int c0, int lane) {
-    ldmatrix4_t(r, tile + (lane % 16) * ld + c0 + lane / 16 * 8);
+template <class Tile>
+__device__ __forceinline__ void load_tokens(uint32_t (&r)[4], const Tile& t, int c0, int lane) {
+    ldmatrix4_t(r, t.at(lane % 16, c0 + lane / 16 * 8));
 }
 // A operand, rows = columns c0..c0+15 of the tile, k = tokens.
-__device__ __forceinline__ void load_columns(uint32_t (&r)[4], const __nv_bfloat16* tile, int ld, int c0, int lane) {
-    ldmatrix4_t(r, tile + (lane % 8 + lane / 16 * 8) * ld + c0 + lane / 8 % 2 * 8);
+template <class Tile>
+__device__ __forceinline__ void load_columns(uint32_t (&r)[4], const Tile& t, int c0, int lane) {
+    ldmatrix4_t(r, t.at(lane % 8 + lane / 16 * 8, c0 + lane / 8 % 2 * 8));
 }
 
 // 16 bytes, or zeros where not `in`.  (A byte count in a register instead of the predicate took 180 clocks a copy.)
@@ -152,13 +171,6 @@ __device__ __forceinline__ void cp_async16(void* dst, const void* src, bool in) 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// `bytes` (a multiple of 16, both ends on 16 bytes) by the copy engine, counted on `bar`.
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_at(dst)), "l"(src),
-                 "r"(bytes), "r"(smem_at(bar))
-                 : "memory");
-}
 
 // Rows t0.. of a (tokens, d) tensor into a tile of 16 x D with rows `ld` apart; zeros past the sequence and past d.
 template <class T, int D>
@@ -272,7 +284,7 @@ __device__ __forceinline__ uint32_t pair_mask(int i, int r0, int r1) {
 // no state, error or update passes through shared memory.
 //
 // What the warps would all compute alike is the helper's, one chunk ahead: the
-// loads (a bulk copy for each row, two blocks of 16 tokens ahead), the decays, Q K^T and K K^T,
+// loads (TMA, two blocks of 16 tokens ahead), the decays, Q K^T and K K^T,
 // and M = (I + (D o K K^T) beta)^-1 by substitution, so that the triangular
 // solve is a product too.  One barrier a chunk.
 
@@ -380,30 +392,41 @@ __device__ __forceinline__ void store_terms(__nv_bfloat16 (&out)[3][kC][kLdM], c
 template <int N>
 __device__ __forceinline__ void load_operand(uint32_t (&r)[N][4], const __nv_bfloat16 (&tile)[3][kC][kLdM], int lane) {
 #pragma unroll
-    for (int x = 0; x < N; ++x) load_rows(r[x], &tile[x][0][0], kLdM, 0, lane);
+    for (int x = 0; x < N; ++x) load_rows(r[x], Rows{&tile[x][0][0], kLdM}, 0, lane);
 }
 
-// Up to 16 rows of a (tokens, d) tensor into a tile by one warp: where rows are whole 16-byte chunks a lane asks the copy
-// engine for a row (and the warp has told `bar` to expect the bytes), else the warp loads them.  Columns past d and rows
-// past the sequence keep what they hold.
-template <class T>
-__device__ __forceinline__ void stage_rows(T* tile, int ld, const T* src, int64_t stride_t, int rows, int d, bool aligned, uint64_t* bar,
-                                           int lane) {
-    if (aligned) {
-        if (lane < rows) bulk_load(tile + lane * ld, src + lane * stride_t, d * (uint32_t)sizeof(T), bar);
-    } else {
-        for (int r = 0; r < rows; ++r)
-            for (int c = lane; c < d; c += 32) tile[r * ld + c] = src[r * stride_t + c];
+// One env and head's rows of a (t, n, h, d) tensor, 16 tokens at a time, into fetched tiles by one warp.  Where rows are
+// whole 16-byte chunks at 16-byte strides (`aligned`) one lane asks TMA for each panel, which also fills with zeros past the
+// sequence and past d; else the warp copies elements, and columns past d keep the zeros that the block put there.
+// (Alternatives on the way here, a block of 16 tokens x 3 x 64: 12 cp.async a lane 1,150 clocks of the helper's time,
+// 48 bulk copies of a row 3,550.)
+template <class T, int D>
+struct Fetch {
+    static constexpr int kWide = 128 / sizeof(T), kPanels = (D + kWide - 1) / kWide;
+    static constexpr int kElements = kPanels * kC * kWide;
+    static __device__ __forceinline__ void run(T* tile, const CUtensorMap* map, const T* rows, int64_t stride_t, int64_t n, int64_t h,
+                                               int col, int64_t t0, int count, int d, bool aligned, uint64_t* bar, int lane) {
+        if (aligned) {
+            if (lane == 0) {
+#pragma unroll
+                for (int i = 0; i < kPanels; ++i)
+                    tc::tma_load_4d(tile + i * kC * kWide, map, bar, col + i * kWide, (int)h, (int)n, (int)t0);
+            }
+        } else {
+            for (int r = 0; r < count; ++r)
+                for (int c = lane; c < d; c += 32) tile[panel_at<T>(r, c)] = rows[(t0 + r) * stride_t + col + c];
+        }
     }
-}
+};
 
 template <class T, int D>
-__device__ __forceinline__ void to_terms_warp(__nv_bfloat16* terms, int ld, const T* raw, int ld_raw, int lane) {
+__device__ __forceinline__ void to_terms_warp(__nv_bfloat16* terms, int ld, const T* raw, int lane) {
     constexpr int N = Terms<T>::n;
     for (int i = lane; i < kC * D / 2; i += 32) {
         const int r = i / (D / 2), c = i % (D / 2) * 2;
         uint32_t s[N];
-        split(to_f32(raw[r * ld_raw + c]), to_f32(raw[r * ld_raw + c + 1]), s);
+        const T* at = raw + panel_at<T>(r, c);
+        split(to_f32(at[0]), to_f32(at[1]), s);
 #pragma unroll
         for (int j = 0; j < N; ++j) *reinterpret_cast<uint32_t*>(terms + (j * kC + r) * ld + c) = s[j];
     }
@@ -416,25 +439,28 @@ constexpr int kForwardWarps = 4;  // state warps of a block: 64 columns
 template <class T, int DK>
 struct ForwardSmem {
     static constexpr int kWidth = kForwardWarps * 16;
-    static constexpr int kLd = DK + 16 / sizeof(T), kLdV = kWidth + 16 / sizeof(T);  // raw rows
-    static constexpr int kLdTerm = DK + 8;                                           // rows of terms; the same for bf16
+    static constexpr int kLdTerm = DK + 8;  // rows of terms
     static constexpr bool kInPlace = Terms<T>::n == 1;
     static constexpr int kBuffers = 4;  // state warps on one block, the helper on the next, two on their way
-    static constexpr size_t kRaw = (size_t)kC * (2 * kLd + kLdV) * sizeof(T);        // a buffer
+    static constexpr int kTileK = Fetch<T, DK>::kElements, kTileV = Fetch<T, kWidth>::kElements;
+    static constexpr size_t kRaw = (size_t)(2 * kTileK + kTileV) * sizeof(T);                        // a buffer
     static constexpr size_t kTerms = kInPlace ? 0 : (size_t)2 * 2 * Terms<T>::n * kC * kLdTerm * 2;  // of two blocks
     static constexpr int kLdS = 20;  // floats of a row of a warp's columns of the state on their way out
     static constexpr size_t kOut = (size_t)DK * kLdS * 4;  // of a warp: that, or its 16 x 16 outputs
-    static constexpr size_t kBytes = kBuffers * kRaw + kTerms + 2 * sizeof(Chunk) + sizeof(HelperScratch) + kForwardWarps * kOut + 8 * kBuffers;
-    static_assert(kRaw % 16 == 0 && kTerms % 16 == 0 && kOut % 16 == 0 && kOut >= kC * kLdOut * 2, "layout");
+    static constexpr size_t kBytes = 1024 + kBuffers * kRaw + kTerms + 2 * sizeof(Chunk) + sizeof(HelperScratch) + kForwardWarps * kOut + 8 * kBuffers;
+    static_assert(kRaw % 1024 == 0 && kTerms % 16 == 0 && kOut % 16 == 0 && kOut >= kC * kLdOut * 2, "layout");
 };
 
 template <class T, int DK>
-__global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) scan_forward_kernel(const Scan p) {
+__global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
+    scan_forward_kernel(const Scan p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q,
+                        const __grid_constant__ CUtensorMap map_v) {
     using L = ForwardSmem<T, DK>;
     constexpr int NT = Terms<T>::n, kTiles = DK / 8, kSteps = DK / 16;
     constexpr int NO = NT == 3 ? 3 : 2;  // terms that o needs: 16 bits and more against its own 8 or 11
-    extern __shared__ __align__(16) uint8_t smem[];
-    constexpr int warps = kForwardWarps, ldv = L::kLdV;
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + (1024 - (smem_at(smem_raw) & 1023) & 1023);
+    constexpr int warps = kForwardWarps;
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = lane / 4, quad = lane % 4;
     __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(smem + L::kBuffers * L::kRaw);
     Chunk* chunks = reinterpret_cast<Chunk*>(smem + L::kBuffers * L::kRaw + L::kTerms);
@@ -445,41 +471,46 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) s
     const int first_col = blockIdx.y * L::kWidth, cols = min(L::kWidth, p.dv - first_col);
     const int64_t blocks = (p.t + kC - 1) / kC;
     auto raw_tile = [&](int64_t b) { return reinterpret_cast<T*>(smem + b % L::kBuffers * L::kRaw); };
-    // K and Q of a block as operand tiles
-    auto k_tile = [&](int64_t b) -> const __nv_bfloat16* {
-        return L::kInPlace ? reinterpret_cast<const __nv_bfloat16*>(raw_tile(b)) : terms + (b & 1) * (L::kTerms / 4);
+    // term x of K (which = 0) or Q (1) of a block as an operand
+    auto operand = [&](int64_t b, int which, int x) {
+        if constexpr (L::kInPlace)
+            return Panels{reinterpret_cast<const __nv_bfloat16*>(raw_tile(b)) + which * L::kTileK};
+        else
+            return Rows{terms + ((b & 1) * 2 * NT + which * NT + x) * kC * L::kLdTerm, L::kLdTerm};
     };
-    auto q_tile = [&](int64_t b) -> const __nv_bfloat16* {
-        return k_tile(b) + (L::kInPlace ? kC * L::kLd : NT * kC * L::kLdTerm);
-    };
-    for (int i = threadIdx.x; i < (int)(L::kBuffers * L::kRaw / 16); i += blockDim.x)
-        reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);  // columns past dk and dv stay zero
+    if (!p.aligned)
+        for (int i = threadIdx.x; i < (int)(L::kBuffers * L::kRaw / 16); i += blockDim.x)
+            reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::kBuffers; ++i) tc::mbar_init(&arrived[i], 1);
+        for (int i = 0; i < L::kBuffers; ++i) tc::mbar_init(&arrived[i], 3);
         tc::mbar_init_fence();
+        tc::prefetch_map(&map_k);
+        tc::prefetch_map(&map_q);
+        tc::prefetch_map(&map_v);
     }
-    tc::fence_async_smem();
     __syncthreads();
 
+    // State warp 0 fetches K, 1 Q, 2 V.
+    auto fetch = [&](int64_t b) {
+        if (b >= blocks || warp > 2) return;
+        T* to = raw_tile(b) + warp * L::kTileK;
+        uint64_t* bar = &arrived[b % L::kBuffers];
+        const int count = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
+        if (warp == 2) {
+            if (p.aligned && lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(L::kTileV * sizeof(T)));
+            Fetch<T, L::kWidth>::run(to, &map_v, static_cast<const T*>(p.v) + n * p.sv.n + h * p.sv.h, p.sv.t, n, h, first_col, b * kC,
+                                     count, cols, p.aligned, bar, lane);
+        } else {
+            if (p.aligned && lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(L::kTileK * sizeof(T)));
+            const Strides& x = warp ? p.sq : p.sk;
+            Fetch<T, DK>::run(to, warp ? &map_q : &map_k, static_cast<const T*>(warp ? p.q : p.k) + n * x.n + h * x.h, x.t, n, h, 0,
+                              b * kC, count, p.dk, p.aligned, bar, lane);
+        }
+    };
+    for (int i = 0; i < 3; ++i) fetch(i);
+    if (!p.aligned) __syncthreads();
+
     if (warp == warps) {
-        const T* q = static_cast<const T*>(p.q) + n * p.sq.n + h * p.sq.h;
-        const T* k = static_cast<const T*>(p.k) + n * p.sk.n + h * p.sk.h;
-        const T* v = static_cast<const T*>(p.v) + n * p.sv.n + h * p.sv.h + first_col;
-        auto fetch = [&](int64_t b) {
-            if (b >= blocks) return;
-            T* to = raw_tile(b);
-            uint64_t* bar = &arrived[b % L::kBuffers];
-            const int rows = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
-            if (p.aligned) {
-                if (lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(rows * (2 * p.dk + cols) * sizeof(T)));
-                __syncwarp();
-            }
-            stage_rows(to, L::kLd, k + b * kC * p.sk.t, p.sk.t, rows, p.dk, p.aligned, bar, lane);
-            stage_rows(to + kC * L::kLd, L::kLd, q + b * kC * p.sq.t, p.sq.t, rows, p.dk, p.aligned, bar, lane);
-            stage_rows(to + 2 * kC * L::kLd, ldv, v + b * kC * p.sv.t, p.sv.t, rows, cols, p.aligned, bar, lane);
-        };
-        fetch(0);
-        fetch(1);
         const GatePointers get_gates(p, n, h, lane);
         Gates gates{}, next = get_gates.load(0, p.t, lane);
         float decay = 1.f;
@@ -509,12 +540,10 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) s
                     __syncthreads();
                     break;
                 }
-                __syncwarp();
-                fetch(b + 2);
                 if constexpr (!L::kInPlace) {
-                    __nv_bfloat16* to = terms + (b & 1) * (L::kTerms / 4);
-                    to_terms_warp<T, DK>(to, L::kLdTerm, raw_tile(b), L::kLd, lane);
-                    to_terms_warp<T, DK>(to + NT * kC * L::kLdTerm, L::kLdTerm, raw_tile(b) + kC * L::kLd, L::kLd, lane);
+                    __nv_bfloat16* to = terms + (b & 1) * 2 * NT * kC * L::kLdTerm;
+                    to_terms_warp<T, DK>(to, L::kLdTerm, raw_tile(b), lane);
+                    to_terms_warp<T, DK>(to + NT * kC * L::kLdTerm, L::kLdTerm, raw_tile(b) + L::kTileK, lane);
                     __syncwarp();
                 }
             }
@@ -523,7 +552,6 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) s
             const int r1 = later ? min(count, __ffs(later) - 1) : count;
             chunk_decays(hs.d, ch.gamma, ch.eta, ch.beta, ch.keep, within(lane, r0, r1) ? decay : 1.f, gates.beta, r0, r1, fresh, lane);
             if (lane == 0) ch.block = (int)b, ch.r0 = r0, ch.r1 = r1, ch.fresh = fresh;
-            const __nv_bfloat16 *kt = k_tile(b), *qt = q_tile(b);
             Acc kk[2], qk[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) kk[i].zero(), qk[i].zero();
@@ -532,8 +560,8 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) s
                 uint32_t ka[NT][4], qa[NT][4];
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
-                    load_rows(ka[x], kt + x * kC * L::kLdTerm, L::kLdTerm, st * 16, lane);
-                    load_rows(qa[x], qt + x * kC * L::kLdTerm, L::kLdTerm, st * 16, lane);
+                    load_rows(ka[x], operand(b, 0, x), st * 16, lane);
+                    load_rows(qa[x], operand(b, 1, x), st * 16, lane);
                 }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
@@ -619,7 +647,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) s
         if (b < 0) break;
         if (p.aligned) tc::mbar_wait_warp(&arrived[b % L::kBuffers], b / L::kBuffers & 1);  // long since; it makes the copies visible here
         const int r0 = ch.r0, r1 = ch.r1;
-        const __nv_bfloat16 *kt = k_tile(b), *qt = q_tile(b);
+        if (r0 == 0) fetch(b + 3);  // where block b - 1 was
         if (p.checkpoints && r0 == 0) put_state(p.checkpoints + (seq * blocks + b) * p.dk * p.dv);
         if (ch.fresh) {
 #pragma unroll
@@ -642,8 +670,8 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) s
             uint32_t ka[NT][4], qa[NT][4];
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
-                load_rows(ka[x], kt + x * kC * L::kLdTerm, L::kLdTerm, st * 16, lane);
-                load_rows(qa[x], qt + x * kC * L::kLdTerm, L::kLdTerm, st * 16, lane);
+                load_rows(ka[x], operand(b, 0, x), st * 16, lane);
+                load_rows(qa[x], operand(b, 1, x), st * 16, lane);
             }
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
@@ -660,9 +688,9 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) s
         // R^T; tokens outside the chunk are zero whatever their inputs hold
         uint32_t ra[3][4];
         {
-            const T* tv = raw_tile(b) + 2 * kC * L::kLd;
+            const T* tv = raw_tile(b) + 2 * L::kTileK;
             uint32_t vv[4];
-            if constexpr (L::kInPlace) load_columns(vv, reinterpret_cast<const __nv_bfloat16*>(tv), ldv, v0, lane);
+            if constexpr (L::kInPlace) load_columns(vv, Panels{reinterpret_cast<const __nv_bfloat16*>(tv)}, v0, lane);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 const int j = c * 8 + quad * 2;
@@ -675,8 +703,8 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) s
                         x0 = __uint_as_float(vv[c * 2 + half] << 16);
                         x1 = __uint_as_float(vv[c * 2 + half] & 0xFFFF0000u);
                     } else {
-                        x0 = to_f32(tv[j * ldv + v0 + row + half * 8]);
-                        x1 = to_f32(tv[(j + 1) * ldv + v0 + row + half * 8]);
+                        x0 = to_f32(tv[panel_at<T>(j, v0 + row + half * 8)]);
+                        x1 = to_f32(tv[panel_at<T>(j + 1, v0 + row + half * 8)]);
                     }
                     uint32_t tmp[3];
                     split(in0 ? fmaf(-ga.x, ks[c].v[half * 2], x0) : 0.f, in1 ? fmaf(-ga.y, ks[c].v[half * 2 + 1], x1) : 0.f, tmp);
@@ -760,7 +788,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3) s
         for (int st = 0; st < kSteps; ++st) {
             uint32_t kb[NT][4];
 #pragma unroll
-            for (int x = 0; x < NT; ++x) load_tokens(kb[x], kt + x * kC * L::kLdTerm, L::kLdTerm, st * 16, lane);
+            for (int x = 0; x < NT; ++x) load_tokens(kb[x], operand(b, 0, x), st * 16, lane);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
                 Acc& acc = s[2 * st + c];
@@ -922,8 +950,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
                 uint32_t ka[NT][4], qa[NT][4];
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
-                    load_rows(ka[x], kt + x * kC * L::kTk, L::kTk, st * 16, lane);
-                    load_rows(qa[x], qt + x * kC * L::kTk, L::kTk, st * 16, lane);
+                    load_rows(ka[x], Rows{kt + x * kC * L::kTk, L::kTk}, st * 16, lane);
+                    load_rows(qa[x], Rows{qt + x * kC * L::kTk, L::kTk}, st * 16, lane);
                 }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
@@ -968,7 +996,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
             if (has_v) {
                 uint32_t ob[NT][4];
 #pragma unroll
-                for (int x = 0; x < NT; ++x) load_tokens(ob[x], ot + x * kC * L::kTv, L::kTv, c0, lane);
+                for (int x = 0; x < NT; ++x) load_tokens(ob[x], Rows{ot + x * kC * L::kTv, L::kTv}, c0, lane);
                 const float e0 = ws.w.eta[row], e1 = ws.w.eta[row + 8];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
@@ -1041,9 +1069,9 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
                 // this slice's share of W = dO U^T and dL = -dR U^T
                 uint32_t uu[3][4], oa[NT][4], ra[3][4];
 #pragma unroll
-                for (int x = 0; x < 3; ++x) load_rows(uu[x], ut + x * kC * L::kTv, L::kTv, c0, lane);
+                for (int x = 0; x < 3; ++x) load_rows(uu[x], Rows{ut + x * kC * L::kTv, L::kTv}, c0, lane);
 #pragma unroll
-                for (int x = 0; x < NT; ++x) load_rows(oa[x], ot + x * kC * L::kTv, L::kTv, c0, lane);
+                for (int x = 0; x < NT; ++x) load_rows(oa[x], Rows{ot + x * kC * L::kTv, L::kTv}, c0, lane);
 #pragma unroll
                 for (int z = 0; z < 4; ++z) {
                     const float2 r = *reinterpret_cast<const float2*>(&ws.r[row + z % 2 * 8][quad * 2 + z / 2 * 8]);
@@ -1093,11 +1121,11 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
                 for (int st = 0; st < DV / 16; ++st) {
                     uint32_t oa[NT][4], ua[3][4], xa[3][4];
 #pragma unroll
-                    for (int x = 0; x < NT; ++x) load_rows(oa[x], ot + x * kC * L::kTv, L::kTv, st * 16, lane);
+                    for (int x = 0; x < NT; ++x) load_rows(oa[x], Rows{ot + x * kC * L::kTv, L::kTv}, st * 16, lane);
 #pragma unroll
                     for (int x = 0; x < 3; ++x) {
-                        load_rows(ua[x], ut + x * kC * L::kTv, L::kTv, st * 16, lane);
-                        load_rows(xa[x], xt + x * kC * L::kTv, L::kTv, st * 16, lane);
+                        load_rows(ua[x], Rows{ut + x * kC * L::kTv, L::kTv}, st * 16, lane);
+                        load_rows(xa[x], Rows{xt + x * kC * L::kTv, L::kTv}, st * 16, lane);
                     }
                     Acc s[2];
 #pragma unroll
@@ -1180,8 +1208,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
                 }
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
-                    load_tokens(kb[x], kt + x * kC * L::kTk, L::kTk, c0, lane);
-                    load_tokens(qb[x], qt + x * kC * L::kTk, L::kTk, c0, lane);
+                    load_tokens(kb[x], Rows{kt + x * kC * L::kTk, L::kTk}, c0, lane);
+                    load_tokens(qb[x], Rows{qt + x * kC * L::kTk, L::kTk}, c0, lane);
                 }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
@@ -1246,8 +1274,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
                     uint32_t qa[NT][4], ka[NT][4];  // rows = dk, k = tokens
 #pragma unroll
                     for (int x = 0; x < NT; ++x) {
-                        load_columns(qa[x], qt + x * kC * L::kTk, L::kTk, c0, lane);
-                        load_columns(ka[x], kt + x * kC * L::kTk, L::kTk, c0, lane);
+                        load_columns(qa[x], Rows{qt + x * kC * L::kTk, L::kTk}, c0, lane);
+                        load_columns(ka[x], Rows{kt + x * kC * L::kTk, L::kTk}, c0, lane);
 #pragma unroll
                         for (int z = 0; z < 4; ++z) {
                             qa[x][z] &= z < 2 ? m0 : m1;
@@ -1259,8 +1287,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
                         uint32_t xb[3][4], yb[3][4];
 #pragma unroll
                         for (int x = 0; x < 3; ++x) {
-                            load_tokens(xb[x], xt + x * kC * L::kTv, L::kTv, st * 16, lane);
-                            load_tokens(yb[x], yt + x * kC * L::kTv, L::kTv, st * 16, lane);
+                            load_tokens(xb[x], Rows{xt + x * kC * L::kTv, L::kTv}, st * 16, lane);
+                            load_tokens(yb[x], Rows{yt + x * kC * L::kTv, L::kTv}, st * 16, lane);
                         }
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
@@ -1282,16 +1310,16 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
                     uint32_t xa[3][4], ya[3][4];  // rows = dv, k = tokens
 #pragma unroll
                     for (int x = 0; x < 3; ++x) {
-                        load_columns(xa[x], xt + x * kC * L::kTv, L::kTv, c0, lane);
-                        load_columns(ya[x], yt + x * kC * L::kTv, L::kTv, c0, lane);
+                        load_columns(xa[x], Rows{xt + x * kC * L::kTv, L::kTv}, c0, lane);
+                        load_columns(ya[x], Rows{yt + x * kC * L::kTv, L::kTv}, c0, lane);
                     }
 #pragma unroll
                     for (int st = 0; st < DK / 16; ++st) {
                         uint32_t kb[NT][4], qb[NT][4];
 #pragma unroll
                         for (int x = 0; x < NT; ++x) {
-                            load_tokens(kb[x], kt + x * kC * L::kTk, L::kTk, st * 16, lane);
-                            load_tokens(qb[x], qt + x * kC * L::kTk, L::kTk, st * 16, lane);
+                            load_tokens(kb[x], Rows{kt + x * kC * L::kTk, L::kTk}, st * 16, lane);
+                            load_tokens(qb[x], Rows{qt + x * kC * L::kTk, L::kTk}, st * 16, lane);
                         }
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
@@ -1328,13 +1356,31 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(
 
 // ------------------------------------------------------------------- host
 
+// A (t, n, h, d) tensor for Fetch.  Dimensions of one element have no stride to speak of.
+template <class T>
+int map_rows(CUtensorMap* map, const void* base, const Strides& s, const Scan& p, int d) {
+    const uint64_t dims[4] = {(uint64_t)d, (uint64_t)p.h, (uint64_t)p.n, (uint64_t)p.t};
+    auto bytes = [](int64_t count, int64_t stride) { return count > 1 ? (uint64_t)stride * sizeof(T) : 16u; };
+    const uint64_t strides[3] = {bytes(p.h, s.h), bytes(p.n, s.n), bytes(p.t, s.t)};
+    const uint32_t box[4] = {128 / sizeof(T), 1, 1, kC};
+    const CUtensorMapDataType type = sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : Terms<T>::n == 1 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    return encode_map(map, type, 4, base, dims, strides, box);
+}
+
 template <class T, int DK>
 int launch_forward_dk(const Scan& p, cudaStream_t st) {
     using L = ForwardSmem<T, DK>;
     auto* kernel = scan_forward_kernel<T, DK>;
     if (int rc = cuda_status(allow_smem(kernel, (int)L::kBytes), "delta_scan")) return rc;
     const dim3 grid(static_cast<unsigned>(p.n * p.h), (p.dv + L::kWidth - 1) / L::kWidth);
-    kernel<<<grid, (kForwardWarps + 1) * 32, L::kBytes, st>>>(p);
+    CUtensorMap map_k{}, map_q{}, map_v{};
+    if (p.aligned && p.t) {
+        if (int rc = map_rows<T>(&map_k, p.k, p.sk, p, p.dk)) return rc;
+        if (int rc = map_rows<T>(&map_q, p.q, p.sq, p, p.dk)) return rc;
+        if (int rc = map_rows<T>(&map_v, p.v, p.sv, p, p.dv)) return rc;
+    }
+    kernel<<<grid, (kForwardWarps + 1) * 32, L::kBytes, st>>>(p, map_k, map_q, map_v);
     return cuda_status(cudaGetLastError(), "delta_scan");
 }
 
