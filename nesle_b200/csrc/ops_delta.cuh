@@ -482,7 +482,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
         for (int i = threadIdx.x; i < (int)(L::kBuffers * L::kRaw / 16); i += blockDim.x)
             reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
     if (threadIdx.x == 0) {
-        for (int i = 0; i < L::kBuffers; ++i) tc::mbar_init(&arrived[i], 3);
+        for (int i = 0; i < L::kBuffers; ++i) tc::mbar_init(&arrived[i], 1);
         tc::mbar_init_fence();
         tc::prefetch_map(&map_k);
         tc::prefetch_map(&map_q);
@@ -490,27 +490,22 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
     }
     __syncthreads();
 
-    // State warp 0 fetches K, 1 Q, 2 V.
-    auto fetch = [&](int64_t b) {
-        if (b >= blocks || warp > 2) return;
-        T* to = raw_tile(b) + warp * L::kTileK;
-        uint64_t* bar = &arrived[b % L::kBuffers];
-        const int count = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
-        if (warp == 2) {
-            if (p.aligned && lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(L::kTileV * sizeof(T)));
-            Fetch<T, L::kWidth>::run(to, &map_v, static_cast<const T*>(p.v) + n * p.sv.n + h * p.sv.h, p.sv.t, n, h, first_col, b * kC,
-                                     count, cols, p.aligned, bar, lane);
-        } else {
-            if (p.aligned && lane == 0) tc::mbar_expect_tx(bar, (uint32_t)(L::kTileK * sizeof(T)));
-            const Strides& x = warp ? p.sq : p.sk;
-            Fetch<T, DK>::run(to, warp ? &map_q : &map_k, static_cast<const T*>(warp ? p.q : p.k) + n * x.n + h * x.h, x.t, n, h, 0,
-                              b * kC, count, p.dk, p.aligned, bar, lane);
-        }
-    };
-    for (int i = 0; i < 3; ++i) fetch(i);
-    if (!p.aligned) __syncthreads();
-
     if (warp == warps) {
+        const T* q = static_cast<const T*>(p.q) + n * p.sq.n + h * p.sq.h;
+        const T* k = static_cast<const T*>(p.k) + n * p.sk.n + h * p.sk.h;
+        const T* v = static_cast<const T*>(p.v) + n * p.sv.n + h * p.sv.h;
+        auto fetch = [&](int64_t b) {
+            if (b >= blocks) return;
+            T* to = raw_tile(b);
+            uint64_t* bar = &arrived[b % L::kBuffers];
+            const int count = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
+            if (p.aligned && lane == 0) tc::mbar_expect_tx(bar, (uint32_t)L::kRaw);
+            Fetch<T, DK>::run(to, &map_k, k, p.sk.t, n, h, 0, b * kC, count, p.dk, p.aligned, bar, lane);
+            Fetch<T, DK>::run(to + L::kTileK, &map_q, q, p.sq.t, n, h, 0, b * kC, count, p.dk, p.aligned, bar, lane);
+            Fetch<T, L::kWidth>::run(to + 2 * L::kTileK, &map_v, v, p.sv.t, n, h, first_col, b * kC, count, cols, p.aligned, bar, lane);
+        };
+        fetch(0);
+        fetch(1);
         const GatePointers get_gates(p, n, h, lane);
         Gates gates{}, next = get_gates.load(0, p.t, lane);
         float decay = 1.f;
@@ -540,6 +535,8 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                     __syncthreads();
                     break;
                 }
+                __syncwarp();
+                fetch(b + 2);
                 if constexpr (!L::kInPlace) {
                     __nv_bfloat16* to = terms + (b & 1) * 2 * NT * kC * L::kLdTerm;
                     to_terms_warp<T, DK>(to, L::kLdTerm, raw_tile(b), lane);
@@ -647,7 +644,6 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
         if (b < 0) break;
         if (p.aligned) tc::mbar_wait_warp(&arrived[b % L::kBuffers], b / L::kBuffers & 1);  // long since; it makes the copies visible here
         const int r0 = ch.r0, r1 = ch.r1;
-        if (r0 == 0) fetch(b + 3);  // where block b - 1 was
         if (p.checkpoints && r0 == 0) put_state(p.checkpoints + (seq * blocks + b) * p.dk * p.dv);
         if (ch.fresh) {
 #pragma unroll
