@@ -119,8 +119,8 @@ typedef struct nesle_delta_args {
     float scale;
     void* o;               /* [t][n][h][dv], contiguous */
     float* final_state;    /* or NULL */
-    float* errors;         /* [t][n][h][dv] and nesle_delta_checkpoint_floats floats that the backward pass reads; both NULL */
-    float* checkpoints;    /* where no gradient is wanted */
+    float* errors;         /* nesle_delta_error_floats and nesle_delta_checkpoint_floats floats, 16-byte aligned, that the */
+    float* checkpoints;    /* backward pass reads; both NULL where no gradient is wanted */
     /* backward only; contiguous */
     const void* d_o;       /* like o */
     const float* d_final;  /* or NULL for zeros */
@@ -132,6 +132,7 @@ typedef struct nesle_delta_args {
 
 /* The same over t tokens; and its gradients, of all inputs, from those of o and of the final state.  The backward call
  * takes the forward call's inputs, errors and checkpoints.  The gradient of g is zero at tokens that start an episode. */
+uint64_t nesle_delta_error_floats(const nesle_delta_args* args);
 uint64_t nesle_delta_checkpoint_floats(const nesle_delta_args* args);
 int nesle_delta_scan(const nesle_delta_args* args, void* stream);
 int nesle_delta_scan_backward(const nesle_delta_args* args, void* stream);

@@ -137,6 +137,7 @@ SIGNATURES = {
     "nesle_delta_step": (ctypes.c_int, [ctypes.POINTER(DeltaStepArgs), ctypes.c_void_p]),
     "nesle_delta_scan": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), ctypes.c_void_p]),
     "nesle_delta_scan_backward": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), ctypes.c_void_p]),
+    "nesle_delta_error_floats": (ctypes.c_uint64, [ctypes.POINTER(DeltaArgs)]),
     "nesle_delta_checkpoint_floats": (ctypes.c_uint64, [ctypes.POINTER(DeltaArgs)]),
     "nesle_orthogonalize": (ctypes.c_int, [ctypes.POINTER(OrthArgs), ctypes.c_void_p]),
     "nesle_orth_workspace": (ctypes.c_uint64, [ctypes.POINTER(OrthArgs)]),

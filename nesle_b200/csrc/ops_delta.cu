@@ -217,6 +217,10 @@ uint64_t nesle_delta_checkpoint_floats(const nesle_delta_args* a) {
     return a ? a->n * a->h * ((a->t + delta::kC - 1) / delta::kC) * a->dk * a->dv : 0;
 }
 
+uint64_t nesle_delta_error_floats(const nesle_delta_args* a) {
+    return a ? a->n * a->h * ((a->t + delta::kC - 1) / delta::kC) * ((a->dv + 15) / 16) * 16 * delta::kC : 0;
+}
+
 int nesle_delta_scan(const nesle_delta_args* args, void* stream) {
     return guarded([&]() -> int {
         if (!args) return invalid("delta_scan: null argument");
@@ -226,6 +230,8 @@ int nesle_delta_scan(const nesle_delta_args* args, void* stream) {
         if (a.t && (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.o)) return invalid("delta_scan: null argument");
         OnDevice on(a.device);
         if (!on.ok) return invalid("delta_scan: device ordinal out of range");
+        if (!a.errors != !a.checkpoints) return invalid("delta_scan: errors and checkpoints go together");
+        if (reinterpret_cast<uintptr_t>(a.errors) % 16) return invalid("delta_scan: errors must be 16-byte aligned");
         delta::Scan p = delta::to_scan(a, false);
         if (int rc = stall_counter(a.device, &p.stalls)) return rc;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -247,7 +253,10 @@ int nesle_delta_scan_backward(const nesle_delta_args* args, void* stream) {
             return invalid("delta_scan_backward: null argument");
         OnDevice on(a.device);
         if (!on.ok) return invalid("delta_scan_backward: device ordinal out of range");
-        const delta::Scan p = delta::to_scan(a, true);
+        if (reinterpret_cast<uintptr_t>(a.errors) % 16 || reinterpret_cast<uintptr_t>(a.checkpoints) % 16)
+            return invalid("delta_scan_backward: errors and checkpoints must be 16-byte aligned");
+        delta::Scan p = delta::to_scan(a, true);
+        if (int rc = stall_counter(a.device, &p.stalls)) return rc;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         if (a.dtype == NESLE_F32) return delta::launch_backward<float>(p, st);
         if (a.dtype == NESLE_BF16) return delta::launch_backward<__nv_bfloat16>(p, st);

@@ -57,7 +57,7 @@ struct Scan {
     bool aligned;  // every row of q, k, v (and d_o) is whole 16-byte chunks and starts on 16 bytes
     void* o;
     float* final_state;
-    float* errors;       // [t][n][h][dv], NULL where no gradient is wanted
+    float* errors;       // as error_at() says, NULL where no gradient is wanted
     float* checkpoints;  // [n][h][ceil(t / 16)][dk][dv], the state before each chunk
     const void* d_o;     // contiguous
     const float* d_final;
@@ -160,82 +160,6 @@ __device__ __forceinline__ void load_tokens(uint32_t (&r)[4], const Tile& t, int
 template <class Tile>
 __device__ __forceinline__ void load_columns(uint32_t (&r)[4], const Tile& t, int c0, int lane) {
     ldmatrix4_t(r, t.at(lane % 8 + lane / 16 * 8, c0 + lane / 8 % 2 * 8));
-}
-
-// 16 bytes, or zeros where not `in`.  (A byte count in a register instead of the predicate took 180 clocks a copy.)
-__device__ __forceinline__ void cp_async16(void* dst, const void* src, bool in) {
-    asm volatile("{\n\t.reg .pred P;\n\tsetp.eq.u32 P, %2, 0;\n\tcp.async.cg.shared.global [%0], [%1], 16, P;\n\t}" ::"r"(smem_at(dst)),
-                 "l"(src), "r"((uint32_t)in)
-                 : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
-// Rows t0.. of a (tokens, d) tensor into a tile of 16 x D with rows `ld` apart; zeros past the sequence and past d.
-template <class T, int D>
-__device__ __forceinline__ void stage(T* tile, int ld, const T* src, int64_t stride_t, int64_t t0, int64_t t_end, int d, bool aligned) {
-    constexpr int kPer = 16 / sizeof(T), kRow = D / kPer;
-    for (int i = threadIdx.x; i < kC * kRow; i += blockDim.x) {
-        const int r = i / kRow, c = i % kRow * kPer;
-        const bool in = t0 + r < t_end && c < d;
-        T* to = tile + r * ld + c;
-        const T* from = src + (in ? (t0 + r) * stride_t + c : 0);
-        if (aligned) {
-            cp_async16(to, from, in);
-        } else {
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) to[j] = in && c + j < d ? from[j] : from_f32<T>(0.f);
-        }
-    }
-}
-
-// A raw tile as its bf16 terms (bf16 itself is used in place).
-template <class T, int D>
-__device__ __forceinline__ void to_terms(__nv_bfloat16* terms, int ld, const T* raw, int ld_raw) {
-    constexpr int N = Terms<T>::n;
-    for (int i = threadIdx.x; i < kC * D / 2; i += blockDim.x) {
-        const int r = i / (D / 2), c = i % (D / 2) * 2;
-        uint32_t s[N];
-        split(to_f32(raw[r * ld_raw + c]), to_f32(raw[r * ld_raw + c + 1]), s);
-#pragma unroll
-        for (int j = 0; j < N; ++j) *reinterpret_cast<uint32_t*>(terms + (j * kC + r) * ld + c) = s[j];
-    }
-}
-
-// What a warp keeps of a chunk's scalars.
-struct alignas(16) Decays {
-    float d[kC][kC];   // D_ij, zero above the diagonal and outside the chunk's tokens
-    float gamma[kC];   // zero outside, and all zero in a chunk that starts an episode
-    float eta[kC];
-    float beta[kC];    // zero outside
-    float keep;        // Gamma
-};
-
-// Tokens r0..r1-1; lane i < 16 holds a_i (1 outside) and beta_i.
-__device__ __forceinline__ void fill_decays(Decays& w, float a, float beta, int r0, int r1, bool fresh, int lane) {
-    float run = 0.f, last = 0.f;
-#pragma unroll
-    for (int i = 0; i < kC; ++i) {
-        const float ai = __shfl_sync(0xffffffffu, a, i);
-        const bool in = i >= r0 && i < r1;
-        if (lane == 16)
-            run = i == r0 ? (fresh ? 0.f : ai) : run * ai;
-        else
-            run = i == lane ? (in ? 1.f : 0.f) : run * ai;
-        if (lane < 16)
-            w.d[i][lane] = in ? run : 0.f;
-        else if (lane == 16)
-            w.gamma[i] = in ? run : 0.f;
-        if (i == r1 - 1) last = run;
-    }
-    if (lane < 16) {
-        w.eta[lane] = lane < r1 ? last : 0.f;
-        w.beta[lane] = lane >= r0 && lane < r1 ? beta : 0.f;
-    } else if (lane == 16) {
-        w.keep = last;
-    }
-    __syncwarp();
 }
 
 // Gate scalars of the 16 tokens of a block, lane i < 16 holding token i: loads only, so that they can be on their way
@@ -430,6 +354,12 @@ __device__ __forceinline__ void to_terms_warp(__nv_bfloat16* terms, int ld, cons
 #pragma unroll
         for (int j = 0; j < N; ++j) *reinterpret_cast<uint32_t*>(terms + (j * kC + r) * ld + c) = s[j];
     }
+}
+
+// Errors are kept as the accumulators hold them: for every 16 tokens and 16 columns two tiles, of 8 tokens each, a float4 a
+// lane.  The index of a lane's float4.
+__device__ __forceinline__ int64_t error_at(int64_t block, int slices, int slice, int tile, int lane) {
+    return ((block * slices + slice) * 2 + tile) * 32 + lane;
 }
 
 constexpr int kLdOut = 24;  // 16-bit elements of a row of a warp's 16 x 16 tile on its way out
@@ -636,6 +566,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
             });
         }
     };
+    const int slices = (p.dv + 15) / 16;
     const int64_t step_t = p.n * p.h * p.dv, first = (n * p.h + h) * p.dv + c0;
     for (int turn = 0;; ++turn) {
         __syncthreads();
@@ -723,11 +654,15 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                 e.zero();
                 mma_terms<3>(e, ra, bb);
                 const int j = c * 8 + quad * 2;
-                if (p.errors) {
-                    float* er = p.errors + (b * kC + j) * step_t + first + row;
+                if (p.errors && first_col / 16 + warp < slices) {
+                    float4* to = reinterpret_cast<float4*>(p.errors) + error_at(seq * blocks + b, slices, first_col / 16 + warp, c, lane);
+                    if (r0 == 0 && r1 == kC) {
+                        __stcs(to, make_float4(e.v[0], e.v[1], e.v[2], e.v[3]));
+                    } else {
 #pragma unroll
-                    for (int z = 0; z < 4; ++z)
-                        if (within(j + z % 2, r0, r1) && (whole || c0 + row + z / 2 * 8 < p.dv)) __stcs(er + z % 2 * step_t + z / 2 * 8, e.v[z]);
+                        for (int z = 0; z < 4; ++z)
+                            if (within(j + z % 2, r0, r1)) reinterpret_cast<float*>(to)[z] = e.v[z];
+                    }
                 }
                 const float2 be = *reinterpret_cast<const float2*>(&ch.beta[j]), et = *reinterpret_cast<const float2*>(&ch.eta[j]);
                 const float h0 = be.x * et.x, h1 = be.y * et.y;  // rounded once more than beta e, then eta: 2^-24
@@ -805,548 +740,732 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
 // Over the chunks from last to first, with dS the gradient of the state after
 // the chunk, E and the state S before it kept by the forward pass:
 //
-//   dU = scale (D o Q K^T)^T dO + eta K dS        (I + L)^T dR = dU,  L = beta D o K K^T (i > j)
-//   dV = beta dR    dbeta_i = dR_i . e_i    dL = -dR U^T    W = dO U^T
+//   dU = scale (D o Q K^T)^T dO + eta K dS        ubar = N^T dU,  N = (I + beta D o K K^T (i > j))^-1
+//   dV = beta ubar    dbeta_i = ubar_i . e_i    dL = -ubar U^T    W = dO U^T
 //   dA = scale D o W (i >= j)    dP = beta D o dL (i > j)
 //   dQ = scale gamma dO S^T + dA K
-//   dK = -beta gamma dR S^T + eta U dS^T + dA^T Q + (dP + dP^T) K
-//   dS <- Gamma dS + (scale gamma Q)^T dO - (beta gamma K)^T dR
-//   dg_l = sum_{i>=l>j} E_ij + sum_{i>=l} (q_i . dq_i^S + k_i . dk_i^S) + sum_{j<l} k_j . dk_j^{dS} + Gamma <dS, S>
+//   dK = -beta gamma ubar S^T + eta U dS^T + dA^T Q + (dP + dP^T) K
+//   dS <- Gamma dS + (scale gamma Q)^T dO - (beta gamma K)^T ubar
+//   dg_l = sum_{i>=l>j} E_ij + sum_{i>=l} (q_i . dq_i^S + k_i . dk_i^S) + sum_{j<l} u_j . (eta_j dS^T k_j) + Gamma <dS, S>
 //   E_ij = dA_ij q_i.k_j + dP_ij k_i.k_j
 //
-// (^S and ^{dS}: the parts of dq and dk that come through S and dS.)  A block
-// takes one (env, head).  A warp has two parts: 16 columns of dS, transposed,
-// for what sums over dk (dU), and 16 rows of dS for what sums over dv (dQ, dK);
-// both copies stay in registers.  X = -beta gamma dR, Y = scale gamma dO and U
-// go through shared memory as bf16 terms.
+// (^S: the parts of dq and dk that come through S.)  A block takes one (env,
+// head).  A warp has two parts.  For what sums over dk it owns 16 columns of dS,
+// transposed in registers as in the forward pass, and takes dU, ubar and the
+// update of dS without leaving them.  For what sums over dv (dQ, dK) it owns 16
+// rows: dS goes through shared memory in fp32, U and ubar as bf16 terms, S comes
+// from the checkpoint.  A helper prepares the next chunk (decays, Q K^T, K K^T,
+// N) and finishes dg and dbeta of the last.  Two barriers a chunk.
 
-constexpr int kRowPad = 20;  // floats of a row of a warp's 16 x 16 scratch
+struct alignas(16) BackChunk {
+    __nv_bfloat16 n[3][kC][kLdM];    // N, by terms
+    __nv_bfloat16 att[3][kC][kLdM];  // scale D_ij q_i.k_j (i >= j), by terms
+    float fa[kC][kC], fp[kC][kC];    // scale D_ij (i >= j), beta_i D_ij (i > j); zero outside the chunk
+    float qk[kC][kC], kk[kC][kC];
+    float gamma[kC], eta[kC], beta[kC];
+    float keep;
+    int block, r0, r1, fresh;
+    int state;                       // S counts: the chunk begins its block and no episode
+};
 
-template <class T, int DK, int DV>
-struct BackwardSmem {
-    static constexpr int kWarps = (DK > DV ? DK : DV) / 16, kWarpsV = DV / 16, kWarpsK = DK / 16;
-    static constexpr int kPad = 16 / sizeof(T);
-    static constexpr int kLdK = DK + kPad, kLdV = DV + kPad;   // raw rows
-    static constexpr int kTk = DK + 8, kTv = DV + 8;           // rows of terms; the same for bf16
-    static constexpr int NT = Terms<T>::n;
-    static constexpr bool kInPlace = NT == 1;
-    static constexpr int kLdE = DV + 4;
-    static constexpr size_t kRaw = (size_t)kC * (2 * kLdK + kLdV) * sizeof(T) + (size_t)kC * kLdE * 4;  // of one buffer
-    static constexpr size_t kTerms = kInPlace ? 0 : (size_t)NT * kC * (2 * kTk + kTv) * 2;
-    static constexpr size_t kTile3 = (size_t)3 * kC * kTv * 2;
-    struct alignas(16) Shared {
-        float part[kWarpsV][2][kC][kC];      // W and dL by slices of dv
-        float qk[kC][kC], kk[kC][kC];        // q_i.k_j, k_i.k_j
-        float da[kC][kC + 1], dp[kC][kC + 1], ee[kC][kC + 1];
-        float dot_i[kWarpsK][kC], dot_j[kWarpsK][kC], dot_s[kWarpsK], dbeta[kWarpsV][kC];
-    };
-    struct alignas(16) Warp {
-        Decays w;
-        float l[kC][kC];        // L_ij at [i][j]
-        float r[kC][kRowPad];   // dU, then dR
-    };
-    static_assert(offsetof(Warp, r) % 16 == 0 && kRaw % 16 == 0 && kTerms % 16 == 0 && kTile3 % 16 == 0, "alignment of vector accesses");
-    static constexpr size_t kBytes = 2 * kRaw + kTerms + 3 * kTile3 + sizeof(Shared) + kWarps * sizeof(Warp);
+// What warps add up for a chunk's scalars.
+template <int kWarpsK, int kWarpsV>
+struct alignas(16) BackSums {
+    float dot_i[kWarpsK][kC], dot_s[kWarpsK], dot_j[kWarpsV][kC], dbeta[kWarpsV][kC];
 };
 
 template <class T, int DK, int DV>
-__global__ void __launch_bounds__((DK > DV ? DK : DV) * 2) scan_backward_kernel(const Scan p) {
-    using L = BackwardSmem<T, DK, DV>;
-    constexpr int NT = Terms<T>::n;
-    extern __shared__ __align__(16) uint8_t smem[];
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = lane / 4, quad = lane % 4;
-    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(smem + 2 * L::kRaw);
-    __nv_bfloat16* ut = reinterpret_cast<__nv_bfloat16*>(smem + 2 * L::kRaw + L::kTerms);
-    __nv_bfloat16* xt = ut + 3 * kC * L::kTv;
-    __nv_bfloat16* yt = xt + 3 * kC * L::kTv;
-    typename L::Shared& sh = *reinterpret_cast<typename L::Shared*>(smem + 2 * L::kRaw + L::kTerms + 3 * L::kTile3);
-    typename L::Warp& ws = reinterpret_cast<typename L::Warp*>(&sh + 1)[warp];
-    const int64_t seq = blockIdx.x, n = seq / p.h, h = seq % p.h;
-    const T* q = static_cast<const T*>(p.q) + n * p.sq.n + h * p.sq.h;
-    const T* k = static_cast<const T*>(p.k) + n * p.sk.n + h * p.sk.h;
-    const int64_t out_t = p.n * p.h, out_0 = n * p.h + h;  // rows of contiguous (t, n, h, d) tensors
-    const T* d_o = static_cast<const T*>(p.d_o) + out_0 * p.dv;
-    const float* errors = p.errors + out_0 * p.dv;
-    const int64_t blocks = (p.t + kC - 1) / kC;
-    const bool has_v = warp < L::kWarpsV, has_k = warp < L::kWarpsK;
-    const int c0 = warp * 16;
-    const bool e_aligned = p.dv % 4 == 0;
-
-    auto fetch = [&](int64_t b, int buf) {
-        T* to = reinterpret_cast<T*>(smem + buf * L::kRaw);
-        stage<T, DK>(to, L::kLdK, k, p.sk.t, b * kC, p.t, p.dk, p.aligned);
-        stage<T, DK>(to + kC * L::kLdK, L::kLdK, q, p.sq.t, b * kC, p.t, p.dk, p.aligned);
-        stage<T, DV>(to + 2 * kC * L::kLdK, L::kLdV, d_o, out_t * p.dv, b * kC, p.t, p.dv, p.aligned);
-        stage<float, DV>(reinterpret_cast<float*>(to + kC * (2 * L::kLdK + L::kLdV)), L::kLdE, errors, out_t * p.dv, b * kC, p.t,
-                         p.dv, e_aligned);
-        cp_async_commit();
+struct BackwardSmem {
+    static constexpr int kWarpsK = DK / 16, kWarpsV = DV / 16, kWarps = DK > DV ? kWarpsK : kWarpsV;
+    static constexpr int NT = Terms<T>::n;
+    static constexpr bool kInPlace = NT == 1;
+    // bf16 is used as fetched: warps on one block, the helper on the next, one on its way.  Others are turned into terms on
+    // arrival, for two blocks, and one buffer is enough.
+    static constexpr int kBuffers = kInPlace ? 3 : 1;
+    static constexpr int kTileK = Fetch<T, DK>::kElements, kTileV = Fetch<T, DV>::kElements;
+    static constexpr size_t kRaw = (size_t)(2 * kTileK + kTileV) * sizeof(T);
+    static constexpr int kTk = DK + 8, kTv = DV + 8;  // rows of terms
+    static constexpr size_t kTermBlock = kInPlace ? 0 : (size_t)NT * kC * (2 * kTk + kTv) * 2;
+    static constexpr size_t kTile3 = (size_t)3 * kC * kTv * 2;    // U, ubar
+    static constexpr int kLdS = DV + 8;
+    static constexpr size_t kState = (size_t)DK * kLdS * 4;       // dS
+    static constexpr size_t kFetched = (size_t)Fetch<float, DV>::kPanels * DK * 128;  // S, panels of 32 columns
+    using Sums = BackSums<kWarpsK, kWarpsV>;
+    struct alignas(16) Shared {
+        BackChunk chunk[2];
+        Sums sums[2];
+        HelperScratch hs;
+        __nv_bfloat16 da[3][kC][kLdM], dp[3][kC][kLdM];
+        float ee[2][kC][kC + 1];  // E through dA, and through dP
+        uint64_t arrived[kBuffers], state_arrived;
     };
+    static constexpr size_t kOut = sizeof(T) == 2 ? (size_t)kC * kLdOut * 2 : 0;  // of a warp
+    static constexpr size_t kBase = 1024 + kBuffers * kRaw + 2 * kTermBlock + 2 * kTile3 + kState + sizeof(Shared) + kWarps * kOut;
+    // S is fetched a chunk ahead where it has room, else read from global memory when needed.
+    static constexpr bool kFetchState = kBase + kFetched <= 227 * 1024;
+    static constexpr size_t kBytes = kBase + (kFetchState ? kFetched : 0);
+    static_assert(kRaw % 1024 == 0 && kFetched % 1024 == 0 && kTermBlock % 16 == 0 && kTile3 % 16 == 0 && kState % 16 == 0, "layout");
+    static_assert(kBytes <= 227 * 1024, "shared memory");
+};
 
-    // dS twice: rows c0.. (dk) x dv, and columns c0.. (dv) x dk transposed.
-    Acc ds[DV / 8], dst[DK / 8];
-    const float* df = p.d_final ? p.d_final + seq * p.dk * p.dv : nullptr;
-#pragma unroll
-    for (int i = 0; i < DV / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int kk = c0 + row + e / 2 * 8, c = i * 8 + quad * 2 + e % 2;
-            ds[i].v[e] = df && kk < p.dk && c < p.dv ? df[(int64_t)kk * p.dv + c] : 0.f;
-        }
-#pragma unroll
-    for (int i = 0; i < DK / 8; ++i)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int kk = i * 8 + quad * 2 + e % 2, c = c0 + row + e / 2 * 8;
-            dst[i].v[e] = df && kk < p.dk && c < p.dv ? df[(int64_t)kk * p.dv + c] : 0.f;
-        }
+__device__ __forceinline__ void store_columns(__nv_bfloat16* tile, int ld, int c0, const uint32_t (&r)[4], int lane) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(
+                     smem_at(tile + (lane % 8 + lane / 16 * 8) * ld + c0 + lane / 8 % 2 * 8)),
+                 "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3])
+                 : "memory");
+}
 
-    if (blocks) fetch(blocks - 1, (blocks - 1) & 1);
-    const GatePointers get_gates(p, n, h, lane);
-    Gates next = get_gates.load((blocks - 1) * kC, p.t, lane);
-    for (int64_t b = blocks - 1; b >= 0; --b) {
-        const int buf = b & 1;
-        cp_async_wait<0>();
-        __syncthreads();
-        if (b > 0) fetch(b - 1, buf ^ 1);
-        const Gates gates = next;
-        if (b > 0) next = get_gates.load((b - 1) * kC, p.t, lane);
-        const uint32_t starts = gates.starts();
-        const T* rk = reinterpret_cast<const T*>(smem + buf * L::kRaw);
-        const T* rq = rk + kC * L::kLdK;
-        const T* ro = rq + kC * L::kLdK;
-        const float* er = reinterpret_cast<const float*>(ro + kC * L::kLdV);
-        const __nv_bfloat16 *kt, *qt, *ot;
-        if constexpr (L::kInPlace) {
-            kt = reinterpret_cast<const __nv_bfloat16*>(rk);
-            qt = reinterpret_cast<const __nv_bfloat16*>(rq);
-            ot = reinterpret_cast<const __nv_bfloat16*>(ro);
-        } else {
-            kt = terms;
-            qt = terms + NT * kC * L::kTk;
-            ot = terms + 2 * NT * kC * L::kTk;
-            to_terms<T, DK>(terms, L::kTk, rk, L::kLdK);
-            to_terms<T, DK>(terms + NT * kC * L::kTk, L::kTk, rq, L::kLdK);
-            to_terms<T, DV>(terms + 2 * NT * kC * L::kTk, L::kTv, ro, L::kLdV);
-            __syncthreads();
-        }
-        const int count = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
-        for (int r1 = count; r1 > 0;) {
+// Sums over a warp's rows of values that belong to columns (tokens 2 quad, 2 quad + 1 and those + 8).
+__device__ __forceinline__ void add_over_rows(float (&x)[4]) {
+#pragma unroll
+    for (int w = 4; w < 32; w *= 2)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], w);
+}
+
+template <class T, int DK, int DV>
+__global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : DV) <= 64 ? 2 : 1)
+    scan_backward_kernel(const Scan p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q,
+                         const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_s) {
+    using L = BackwardSmem<T, DK, DV>;
+    constexpr int NT = Terms<T>::n, ND = NT == 3 ? 3 : 2;  // ND: terms of dS and U for dk alone, which leaves as T
+    extern __shared__ __align__(16) uint8_t smem_raw[];
+    uint8_t* smem = smem_raw + (1024 - (smem_at(smem_raw) & 1023) & 1023);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, row = lane / 4, quad = lane % 4;
+    float* fetched = reinterpret_cast<float*>(smem + L::kBuffers * L::kRaw);
+    uint8_t* at = smem + L::kBuffers * L::kRaw + (L::kFetchState ? L::kFetched : 0);
+    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(at);
+    __nv_bfloat16* ut = reinterpret_cast<__nv_bfloat16*>(at + 2 * L::kTermBlock);  // U
+    __nv_bfloat16* bt = ut + L::kTile3 / 2;                                        // ubar
+    float* st = reinterpret_cast<float*>(bt + L::kTile3 / 2);                      // dS, rows = dk
+    typename L::Shared& sh = *reinterpret_cast<typename L::Shared*>(st + L::kState / 4);
+    const int64_t seq = blockIdx.x, n = seq / p.h, h = seq % p.h;
+    const int64_t out_t = p.n * p.h, out_0 = n * p.h + h;  // rows of contiguous (t, n, h, d) tensors
+    const int64_t blocks = (p.t + kC - 1) / kC;
+    const int slices = (p.dv + 15) / 16;
+    const bool fetch_state = L::kFetchState && p.dv % 4 == 0;
+    auto raw_tile = [&](int64_t b) { return reinterpret_cast<T*>(smem + b % L::kBuffers * L::kRaw); };
+    // term x of K (which = 0), Q (1) or dO (2) of a block as an operand
+    auto operand = [&](int64_t b, int which, int x) {
+        if constexpr (L::kInPlace)
+            return Panels{reinterpret_cast<const __nv_bfloat16*>(raw_tile(b)) + which * L::kTileK};
+        else
+            return Rows{terms + (b & 1) * (L::kTermBlock / 2) + which * NT * kC * L::kTk + x * kC * (which == 2 ? L::kTv : L::kTk),
+                        which == 2 ? L::kTv : L::kTk};
+    };
+    if (!p.aligned)
+        for (int i = threadIdx.x; i < (int)(L::kBuffers * L::kRaw / 16); i += blockDim.x)
+            reinterpret_cast<uint4*>(smem)[i] = make_uint4(0, 0, 0, 0);
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < L::kBuffers; ++i) tc::mbar_init(&sh.arrived[i], 1);
+        tc::mbar_init(&sh.state_arrived, 1);
+        tc::mbar_init_fence();
+        tc::prefetch_map(&map_k);
+        tc::prefetch_map(&map_q);
+        tc::prefetch_map(&map_o);
+    }
+    __syncthreads();
+
+    if (warp == L::kWarps) {
+        const T* q = static_cast<const T*>(p.q) + n * p.sq.n + h * p.sq.h;
+        const T* k = static_cast<const T*>(p.k) + n * p.sk.n + h * p.sk.h;
+        const T* d_o = static_cast<const T*>(p.d_o) + out_0 * p.dv;
+        auto fetch = [&](int64_t b) {
+            if (b < 0) return;
+            T* to = raw_tile(b);
+            uint64_t* bar = &sh.arrived[b % L::kBuffers];
+            const int count = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
+            if (p.aligned && lane == 0) tc::mbar_expect_tx(bar, (uint32_t)L::kRaw);
+            Fetch<T, DK>::run(to, &map_k, k, p.sk.t, n, h, 0, b * kC, count, p.dk, p.aligned, bar, lane);
+            Fetch<T, DK>::run(to + L::kTileK, &map_q, q, p.sq.t, n, h, 0, b * kC, count, p.dk, p.aligned, bar, lane);
+            Fetch<T, DV>::run(to + 2 * L::kTileK, &map_o, d_o, out_t * p.dv, n, h, 0, b * kC, count, p.dv, p.aligned, bar, lane);
+        };
+        const GatePointers get_gates(p, n, h, lane);
+        Gates gates{}, next = get_gates.load((blocks - 1) * kC, p.t, lane);
+        float decay = 1.f;
+        uint32_t starts = 0;
+        int64_t b = blocks, turn_of_block = -1;
+        int r1 = 0;
+        fetch(blocks - 1);
+        // the chunk before the last one prepared
+        auto prepare = [&](BackChunk& ch) {
+            if (r1 == 0) {
+                --b;
+                if (b < 0) {
+                    if (lane == 0) ch.block = -1;
+                    return;
+                }
+                ++turn_of_block;
+                r1 = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
+                gates = next;
+                if (b > 0) next = get_gates.load((b - 1) * kC, p.t, lane);
+                decay = gates.decay();
+                starts = gates.starts();
+                // phases of a buffer's barrier count the blocks that it has held
+                if (p.aligned && !tc::mbar_wait_warp(&sh.arrived[b % L::kBuffers], turn_of_block / L::kBuffers & 1)) {
+                    if (lane == 0) {
+                        atomicAdd(p.stalls, 1u);
+                        ch.block = -1;
+                    }
+                    b = 0, r1 = 0;
+                    return;
+                }
+                __syncwarp();
+                if constexpr (!L::kInPlace) {
+                    __nv_bfloat16* to = terms + (b & 1) * (L::kTermBlock / 2);
+                    to_terms_warp<T, DK>(to, L::kTk, raw_tile(b), lane);
+                    to_terms_warp<T, DK>(to + NT * kC * L::kTk, L::kTk, raw_tile(b) + L::kTileK, lane);
+                    to_terms_warp<T, DV>(to + 2 * NT * kC * L::kTk, L::kTv, raw_tile(b) + 2 * L::kTileK, lane);
+                    tc::fence_async_smem();
+                    __syncwarp();
+                }
+                fetch(b - 1);
+            }
             const uint32_t earlier = starts & ((1u << r1) - 1);
             const int r0 = earlier ? 31 - __clz(earlier) : 0;
             const bool fresh = starts >> r0 & 1;
-            fill_decays(ws.w, within(lane, r0, r1) ? gates.decay() : 1.f, gates.beta, r0, r1, fresh, lane);
-            const uint32_t m0 = pair_mask(quad * 2, r0, r1), m1 = pair_mask(quad * 2 + 8, r0, r1);
-
-            // k_i.k_j, and k_j.q_i with tokens j as rows; dU through dS
-            Acc kk[2], kq[2], du[2];
+            HelperScratch& hs = sh.hs;
+            chunk_decays(hs.d, ch.gamma, ch.eta, ch.beta, ch.keep, within(lane, r0, r1) ? decay : 1.f, gates.beta, r0, r1, fresh, lane);
+            if (lane == 0) ch.block = (int)b, ch.r0 = r0, ch.r1 = r1, ch.fresh = fresh, ch.state = !fresh;
+            Acc kk[2], qk[2];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) kk[c].zero(), kq[c].zero(), du[c].zero();
+            for (int i = 0; i < 2; ++i) kk[i].zero(), qk[i].zero();
 #pragma unroll
-            for (int st = 0; st < DK / 16; ++st) {
+            for (int s = 0; s < DK / 16; ++s) {
                 uint32_t ka[NT][4], qa[NT][4];
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
-                    load_rows(ka[x], Rows{kt + x * kC * L::kTk, L::kTk}, st * 16, lane);
-                    load_rows(qa[x], Rows{qt + x * kC * L::kTk, L::kTk}, st * 16, lane);
+                    load_rows(ka[x], operand(b, 0, x), s * 16, lane);
+                    load_rows(qa[x], operand(b, 1, x), s * 16, lane);
                 }
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    uint32_t kb[NT][2], qb[NT][2], sb[3][2], lo[3], hi[3];
+                    uint32_t kb[NT][2];
 #pragma unroll
-                    for (int x = 0; x < NT; ++x) {
-                        kb[x][0] = ka[x][c], kb[x][1] = ka[x][c + 2];
-                        qb[x][0] = qa[x][c], qb[x][1] = qa[x][c + 2];
-                    }
+                    for (int x = 0; x < NT; ++x) kb[x][0] = ka[x][c], kb[x][1] = ka[x][c + 2];
                     mma_terms<3>(kk[c], ka, kb);
-                    mma_terms<3>(kq[c], ka, qb);
-                    split(dst[2 * st].v[2 * c], dst[2 * st].v[2 * c + 1], lo);
-                    split(dst[2 * st + 1].v[2 * c], dst[2 * st + 1].v[2 * c + 1], hi);
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) sb[x][0] = lo[x], sb[x][1] = hi[x];
-                    mma_terms<3>(du[c], ka, sb);
+                    mma_terms<3>(qk[c], qa, kb);
                 }
             }
-            uint32_t att[3][4];  // scale (D o Q K^T)^T: rows j, k = i
+            __syncwarp();
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const int x = row + half * 8, y = c * 8 + quad * 2;
-                    float at[2];
+                    const int i = row + half * 8, j = c * 8 + quad * 2;
+                    const float2 d = *reinterpret_cast<const float2*>(&hs.d[i][j]);
+                    const float be = ch.beta[i];
+                    const bool in0 = within(i, r0, r1) && j >= r0, in1 = within(i, r0, r1) && j + 1 >= r0;
+                    const float2 fa = make_float2(in0 && i >= j ? p.scale * d.x : 0.f, in1 && i >= j + 1 ? p.scale * d.y : 0.f);
+                    const float2 fb = make_float2(in0 && i > j ? be * d.x : 0.f, in1 && i > j + 1 ? be * d.y : 0.f);
+                    const float2 vq = make_float2(fa.x != 0.f ? qk[c].v[half * 2] : 0.f, fa.y != 0.f ? qk[c].v[half * 2 + 1] : 0.f);
+                    // k_i.k_j counts where dP may, also at beta = 0, where dP is zero
+                    const float2 vk = make_float2(in0 && i > j ? kk[c].v[half * 2] : 0.f, in1 && i > j + 1 ? kk[c].v[half * 2 + 1] : 0.f);
+                    *reinterpret_cast<float2*>(&ch.fa[i][j]) = fa;
+                    *reinterpret_cast<float2*>(&ch.fp[i][j]) = fb;
+                    *reinterpret_cast<float2*>(&ch.qk[i][j]) = vq;
+                    *reinterpret_cast<float2*>(&ch.kk[i][j]) = vk;
+                    *reinterpret_cast<float2*>(&hs.b[i][j]) = make_float2(fb.x * vk.x, fb.y * vk.y);
+                    uint32_t s[3];
+                    split(fa.x * vq.x, fa.y * vq.y, s);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const bool in = within(x, r0, r1) && within(y + e, r0, r1);
-                        const float raw_kk = kk[c].v[half * 2 + e], raw_kq = kq[c].v[half * 2 + e];
-                        ws.l[x][y + e] = in && x > y + e ? ws.w.beta[x] * ws.w.d[x][y + e] * raw_kk : 0.f;
-                        at[e] = in && y + e >= x ? p.scale * ws.w.d[y + e][x] * raw_kq : 0.f;
-                        if (warp == 0) {
-                            sh.kk[x][y + e] = in ? raw_kk : 0.f;
-                            sh.qk[y + e][x] = in ? raw_kq : 0.f;
-                        }
-                    }
-                    uint32_t tmp[3];
-                    split(at[0], at[1], tmp);
-#pragma unroll
-                    for (int z = 0; z < 3; ++z) att[z][c * 2 + half] = tmp[z];
+                    for (int x = 0; x < 3; ++x) *reinterpret_cast<uint32_t*>(&ch.att[x][i][j]) = s[x];
                 }
-            if (has_v) {
-                uint32_t ob[NT][4];
-#pragma unroll
-                for (int x = 0; x < NT; ++x) load_tokens(ob[x], Rows{ot + x * kC * L::kTv, L::kTv}, c0, lane);
-                const float e0 = ws.w.eta[row], e1 = ws.w.eta[row + 8];
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    du[c].v[0] *= e0, du[c].v[1] *= e0, du[c].v[2] *= e1, du[c].v[3] *= e1;
-                    uint32_t bb[NT][2];
-#pragma unroll
-                    for (int x = 0; x < NT; ++x) bb[x][0] = ob[x][2 * c] & m0, bb[x][1] = ob[x][2 * c + 1] & m1;
-                    mma_terms<3>(du[c], att, bb);
-#pragma unroll
-                    for (int half = 0; half < 2; ++half)
-                        *reinterpret_cast<float2*>(&ws.r[row + half * 8][c * 8 + quad * 2]) =
-                            make_float2(du[c].v[half * 2], du[c].v[half * 2 + 1]);
-                }
-                __syncwarp();
-                float part[kC];
-#pragma unroll
-                for (int i = 0; i < kC; ++i) part[i] = 0.f;
-                if (lane < 16) {  // one column each: back substitution
-                    float x[kC];
-#pragma unroll
-                    for (int i = 0; i < kC; ++i) x[i] = ws.r[i][lane];
-                    T* dv = static_cast<T*>(p.dv_out) + (b * kC * out_t + out_0) * p.dv + c0 + lane;
-#pragma unroll
-                    for (int i = kC - 1; i >= 0; --i) {
-                        const bool in = within(i, r0, r1);
-                        const float r = in ? x[i] : 0.f;
-                        ws.r[i][lane] = r;
-                        if (in && c0 + lane < p.dv) dv[i * out_t * p.dv] = from_f32<T>(ws.w.beta[i] * r);
-                        part[i] = in ? r * er[i * L::kLdE + c0 + lane] : 0.f;
-#pragma unroll
-                        for (int j = 0; j < i; ++j) x[j] = fmaf(-ws.l[i][j], r, x[j]);
-                    }
-                }
-                // dbeta: 16 sums over 16 lanes, halving the sums that a lane carries at each exchange
-#pragma unroll
-                for (int bit = 3; bit >= 0; --bit) {
-                    const int w = 1 << bit;
-                    const bool up = lane & w;
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (i >= w) break;
-                        const float give = up ? part[i] : part[i + w], have = up ? part[i + w] : part[i];
-                        part[i] = have + __shfl_xor_sync(0xffffffffu, give, w);
-                    }
-                }
-                if (lane < 16) sh.dbeta[warp][lane] = part[0];
-                __syncwarp();
-                // U, X, Y of this warp's columns as terms
-#pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    const int i = z * 4 + lane / 8, c = lane % 8 * 2;
-                    const bool in = within(i, r0, r1);
-                    const float be = ws.w.beta[i], ga = ws.w.gamma[i];
-                    const float2 e = *reinterpret_cast<const float2*>(er + i * L::kLdE + c0 + c);
-                    const float2 r = *reinterpret_cast<const float2*>(&ws.r[i][c]);
-                    const float y0 = to_f32(ro[i * L::kLdV + c0 + c]), y1 = to_f32(ro[i * L::kLdV + c0 + c + 1]);
-                    uint32_t su[3], sx[3], sy[3];
-                    split(in ? be * e.x : 0.f, in ? be * e.y : 0.f, su);
-                    split(-be * ga * r.x, -be * ga * r.y, sx);
-                    split(in ? p.scale * ga * y0 : 0.f, in ? p.scale * ga * y1 : 0.f, sy);
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) {
-                        const int at = (x * kC + i) * L::kTv + c0 + c;
-                        *reinterpret_cast<uint32_t*>(ut + at) = su[x];
-                        *reinterpret_cast<uint32_t*>(xt + at) = sx[x];
-                        *reinterpret_cast<uint32_t*>(yt + at) = sy[x];
-                    }
-                }
-                __syncwarp();
-                // this slice's share of W = dO U^T and dL = -dR U^T
-                uint32_t uu[3][4], oa[NT][4], ra[3][4];
-#pragma unroll
-                for (int x = 0; x < 3; ++x) load_rows(uu[x], Rows{ut + x * kC * L::kTv, L::kTv}, c0, lane);
-#pragma unroll
-                for (int x = 0; x < NT; ++x) load_rows(oa[x], Rows{ot + x * kC * L::kTv, L::kTv}, c0, lane);
-#pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    const float2 r = *reinterpret_cast<const float2*>(&ws.r[row + z % 2 * 8][quad * 2 + z / 2 * 8]);
-                    uint32_t tmp[3];
-                    split(-r.x, -r.y, tmp);
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) ra[x][z] = tmp[x];
-                }
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t ub[3][2];
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) ub[x][0] = uu[x][c], ub[x][1] = uu[x][c + 2];
-                    Acc w, dl;
-                    w.zero(), dl.zero();
-                    mma_terms<3>(w, oa, ub);
-                    mma_terms<3>(dl, ra, ub);
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        *reinterpret_cast<float2*>(&sh.part[warp][0][row + half * 8][c * 8 + quad * 2]) = make_float2(w.v[half * 2], w.v[half * 2 + 1]);
-                        *reinterpret_cast<float2*>(&sh.part[warp][1][row + half * 8][c * 8 + quad * 2]) = make_float2(dl.v[half * 2], dl.v[half * 2 + 1]);
-                    }
-                }
-            }
-            __syncthreads();
-            for (int e = threadIdx.x; e < kC * kC; e += blockDim.x) {
-                const int i = e / kC, j = e % kC;
-                float w = 0.f, dl = 0.f;
-#pragma unroll
-                for (int x = 0; x < L::kWarpsV; ++x) w += sh.part[x][0][i][j], dl += sh.part[x][1][i][j];
-                const bool in = within(i, r0, r1) && within(j, r0, r1);
-                const float d = ws.w.d[i][j];
-                const float da = in && i >= j ? p.scale * d * w : 0.f, dp = in && i > j ? ws.w.beta[i] * d * dl : 0.f;
-                sh.da[i][j] = da;
-                sh.dp[i][j] = dp;
-                sh.ee[i][j] = i > j ? da * sh.qk[i][j] + dp * sh.kk[i][j] : 0.f;
-            }
-            Acc dq[2], dk[2], dku[2];
-#pragma unroll
-            for (int c = 0; c < 2; ++c) dq[c].zero(), dk[c].zero(), dku[c].zero();
-            if (has_k) {
-                const float* s0 = p.checkpoints + (seq * blocks + b) * p.dk * p.dv;
-                float dot = 0.f;
-                const int k0 = c0 + row, k1 = k0 + 8;
-                const bool in0 = !fresh && k0 < p.dk, in1 = !fresh && k1 < p.dk;
-#pragma unroll
-                for (int st = 0; st < DV / 16; ++st) {
-                    uint32_t oa[NT][4], ua[3][4], xa[3][4];
-#pragma unroll
-                    for (int x = 0; x < NT; ++x) load_rows(oa[x], Rows{ot + x * kC * L::kTv, L::kTv}, st * 16, lane);
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) {
-                        load_rows(ua[x], Rows{ut + x * kC * L::kTv, L::kTv}, st * 16, lane);
-                        load_rows(xa[x], Rows{xt + x * kC * L::kTv, L::kTv}, st * 16, lane);
-                    }
-                    Acc s[2];
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const int c = st * 16 + x * 8 + quad * 2 + e;
-                            s[x].v[e] = in0 && c < p.dv ? s0[(int64_t)k0 * p.dv + c] : 0.f;
-                            s[x].v[2 + e] = in1 && c < p.dv ? s0[(int64_t)k1 * p.dv + c] : 0.f;
-                        }
-#pragma unroll
-                    for (int x = 0; x < 2; ++x)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) dot = fmaf(s[x].v[e], ds[2 * st + x].v[e], dot);
-#pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t sb[3][2], db[3][2], lo[3], hi[3];
-                        split(s[0].v[2 * c], s[0].v[2 * c + 1], lo);
-                        split(s[1].v[2 * c], s[1].v[2 * c + 1], hi);
-#pragma unroll
-                        for (int x = 0; x < 3; ++x) sb[x][0] = lo[x], sb[x][1] = hi[x];
-                        split(ds[2 * st].v[2 * c], ds[2 * st].v[2 * c + 1], lo);
-                        split(ds[2 * st + 1].v[2 * c], ds[2 * st + 1].v[2 * c + 1], hi);
-#pragma unroll
-                        for (int x = 0; x < 3; ++x) db[x][0] = lo[x], db[x][1] = hi[x];
-                        mma_terms<3>(dq[c], oa, sb);
-                        mma_terms<3>(dk[c], xa, sb);
-                        mma_terms<3>(dku[c], ua, db);
-                    }
-                }
-                // the decays' gradients need q.dq and k.dk of these parts alone
-                const float g0 = p.scale * ws.w.gamma[row], g1 = p.scale * ws.w.gamma[row + 8], e0 = ws.w.eta[row], e1 = ws.w.eta[row + 8];
-                float di[2] = {0.f, 0.f}, dj[2] = {0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int half = e / 2, at = (row + half * 8) * L::kLdK + c0 + c * 8 + quad * 2 + e % 2;
-                        dq[c].v[e] *= half ? g1 : g0;
-                        dku[c].v[e] *= half ? e1 : e0;
-                        const float kv = to_f32(rk[at]);
-                        di[half] += to_f32(rq[at]) * dq[c].v[e] + kv * dk[c].v[e];
-                        dj[half] += kv * dku[c].v[e];
-                    }
-#pragma unroll
-                for (int w = 1; w < 4; w *= 2) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        di[half] += __shfl_xor_sync(0xffffffffu, di[half], w);
-                        dj[half] += __shfl_xor_sync(0xffffffffu, dj[half], w);
-                    }
-                }
-#pragma unroll
-                for (int w = 1; w < 32; w *= 2) dot += __shfl_xor_sync(0xffffffffu, dot, w);
-                if (quad == 0) {
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        sh.dot_i[warp][row + half * 8] = di[half];
-                        sh.dot_j[warp][row + half * 8] = dj[half];
-                    }
-                }
-                if (lane == 0) sh.dot_s[warp] = ws.w.keep * dot;
-            }
-            __syncthreads();
-            if (has_k) {
-                uint32_t da[3][4], dat[3][4], dp[3][4], kb[NT][4], qb[NT][4];
-#pragma unroll
-                for (int z = 0; z < 4; ++z) {
-                    const int x = row + z % 2 * 8, y = quad * 2 + z / 2 * 8;
-                    uint32_t tmp[3];
-                    split(sh.da[x][y], sh.da[x][y + 1], tmp);
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) da[i][z] = tmp[i];
-                    split(sh.da[y][x], sh.da[y + 1][x], tmp);
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) dat[i][z] = tmp[i];
-                    split(sh.dp[x][y] + sh.dp[y][x], sh.dp[x][y + 1] + sh.dp[y + 1][x], tmp);
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) dp[i][z] = tmp[i];
-                }
-#pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                    load_tokens(kb[x], Rows{kt + x * kC * L::kTk, L::kTk}, c0, lane);
-                    load_tokens(qb[x], Rows{qt + x * kC * L::kTk, L::kTk}, c0, lane);
-                }
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t k2[NT][2], q2[NT][2];
-#pragma unroll
-                    for (int x = 0; x < NT; ++x) {
-                        k2[x][0] = kb[x][2 * c] & m0, k2[x][1] = kb[x][2 * c + 1] & m1;
-                        q2[x][0] = qb[x][2 * c] & m0, q2[x][1] = qb[x][2 * c + 1] & m1;
-                    }
-                    mma_terms<3>(dq[c], da, k2);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) dk[c].v[e] += dku[c].v[e];
-                    mma_terms<3>(dk[c], dat, q2);
-                    mma_terms<3>(dk[c], dp, k2);
-#pragma unroll
-                    for (int half = 0; half < 2; ++half) {
-                        const int i = row + half * 8, col = c0 + c * 8 + quad * 2;
-                        if (within(i, r0, r1)) {
-                            const int64_t at = ((b * kC + i) * out_t + out_0) * p.dk + col;
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-                                if (col + e < p.dk) {
-                                    static_cast<T*>(p.dq)[at + e] = from_f32<T>(dq[c].v[half * 2 + e]);
-                                    static_cast<T*>(p.dk_out)[at + e] = from_f32<T>(dk[c].v[half * 2 + e]);
-                                }
-                        }
-                    }
-                }
-            }
-            if (warp == 0) {
-                // column j's sums of E from the last row up, then row l's first l columns
-                float tail = 0.f;
-                if (lane < 16)
-                    for (int i = kC - 1; i >= 0; --i) {
-                        tail += sh.ee[i][lane];
-                        sh.ee[i][lane] = tail;
-                    }
-                __syncwarp();
-                if (within(lane, r0, r1)) {
-                    float dg = 0.f;
-                    for (int j = 0; j < lane; ++j) dg += sh.ee[lane][j];
-                    for (int x = 0; x < L::kWarpsK; ++x) {
-                        for (int i = lane; i < r1; ++i) dg += sh.dot_i[x][i];
-                        for (int j = r0; j < lane; ++j) dg += sh.dot_j[x][j];
-                        dg += sh.dot_s[x];
-                    }
-                    float dbeta = 0.f;
-                    for (int x = 0; x < L::kWarpsV; ++x) dbeta += sh.dbeta[x][lane];
-                    const int64_t at = (b * kC + lane) * out_t + out_0;
-                    p.dg[at] = dg;
-                    p.dbeta[at] = dbeta;
-                }
-            }
-            if (fresh) {  // the state before was dropped
-#pragma unroll
-                for (int i = 0; i < DV / 8; ++i) ds[i].zero();
-#pragma unroll
-                for (int i = 0; i < DK / 8; ++i) dst[i].zero();
-            } else {
-                const float keep = ws.w.keep;
-                if (has_k) {
-                    uint32_t qa[NT][4], ka[NT][4];  // rows = dk, k = tokens
-#pragma unroll
-                    for (int x = 0; x < NT; ++x) {
-                        load_columns(qa[x], Rows{qt + x * kC * L::kTk, L::kTk}, c0, lane);
-                        load_columns(ka[x], Rows{kt + x * kC * L::kTk, L::kTk}, c0, lane);
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            qa[x][z] &= z < 2 ? m0 : m1;
-                            ka[x][z] &= z < 2 ? m0 : m1;
-                        }
-                    }
-#pragma unroll
-                    for (int st = 0; st < DV / 16; ++st) {
-                        uint32_t xb[3][4], yb[3][4];
-#pragma unroll
-                        for (int x = 0; x < 3; ++x) {
-                            load_tokens(xb[x], Rows{xt + x * kC * L::kTv, L::kTv}, st * 16, lane);
-                            load_tokens(yb[x], Rows{yt + x * kC * L::kTv, L::kTv}, st * 16, lane);
-                        }
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            Acc& acc = ds[2 * st + c];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc.v[e] *= keep;
-                            uint32_t x2[3][2], y2[3][2];
-#pragma unroll
-                            for (int x = 0; x < 3; ++x) {
-                                x2[x][0] = xb[x][2 * c], x2[x][1] = xb[x][2 * c + 1];
-                                y2[x][0] = yb[x][2 * c], y2[x][1] = yb[x][2 * c + 1];
-                            }
-                            mma_terms<3>(acc, qa, y2);
-                            mma_terms<3>(acc, ka, x2);
-                        }
-                    }
-                }
-                if (has_v) {
-                    uint32_t xa[3][4], ya[3][4];  // rows = dv, k = tokens
-#pragma unroll
-                    for (int x = 0; x < 3; ++x) {
-                        load_columns(xa[x], Rows{xt + x * kC * L::kTv, L::kTv}, c0, lane);
-                        load_columns(ya[x], Rows{yt + x * kC * L::kTv, L::kTv}, c0, lane);
-                    }
-#pragma unroll
-                    for (int st = 0; st < DK / 16; ++st) {
-                        uint32_t kb[NT][4], qb[NT][4];
-#pragma unroll
-                        for (int x = 0; x < NT; ++x) {
-                            load_tokens(kb[x], Rows{kt + x * kC * L::kTk, L::kTk}, st * 16, lane);
-                            load_tokens(qb[x], Rows{qt + x * kC * L::kTk, L::kTk}, st * 16, lane);
-                        }
-#pragma unroll
-                        for (int c = 0; c < 2; ++c) {
-                            Acc& acc = dst[2 * st + c];
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) acc.v[e] *= keep;
-                            uint32_t k2[NT][2], q2[NT][2];
-#pragma unroll
-                            for (int x = 0; x < NT; ++x) {
-                                k2[x][0] = kb[x][2 * c] & m0, k2[x][1] = kb[x][2 * c + 1] & m1;
-                                q2[x][0] = qb[x][2 * c] & m0, q2[x][1] = qb[x][2 * c + 1] & m1;
-                            }
-                            mma_terms<3>(acc, ya, q2);
-                            mma_terms<3>(acc, xa, k2);
-                        }
-                    }
-                }
-            }
-            __syncthreads();  // U, X, Y and the sums are free for the next chunk
+            __syncwarp();
+            invert_lower(hs, lane);
+            store_terms<3>(ch.n, hs.b, lane);
+            __syncwarp();
             r1 = r0;
-        }
-    }
-    if (p.dstate && has_k) {
-        float* to = p.dstate + seq * p.dk * p.dv;
+        };
+        // dg and dbeta of a chunk, from its sums
+        auto finish = [&](const BackChunk& ch, const typename L::Sums& sums) {
+            // column j's sums of E from the last row up, then row l's first l columns
+            float tail = 0.f;
+            if (lane < 16) {
 #pragma unroll
-        for (int i = 0; i < DV / 8; ++i)
+                for (int i = kC - 1; i >= 0; --i) {
+                    tail += sh.ee[0][i][lane] + sh.ee[1][i][lane];
+                    sh.ee[0][i][lane] = tail;
+                }
+            }
+            __syncwarp();
+            // lane l: the sums over i >= l and over j < l, from the warps' parts
+            const bool in = within(lane, ch.r0, ch.r1);
+            float di = 0.f, dj = 0.f, dot = 0.f, dbeta = 0.f;
+#pragma unroll
+            for (int x = 0; x < L::kWarpsK; ++x) {
+                di += in ? sums.dot_i[x][lane & 15] : 0.f;
+                dot += sums.dot_s[x];
+            }
+#pragma unroll
+            for (int x = 0; x < L::kWarpsV; ++x) {
+                dj += in ? sums.dot_j[x][lane & 15] : 0.f;
+                dbeta += sums.dbeta[x][lane & 15];
+            }
+#pragma unroll
+            for (int w = 1; w < 16; w *= 2) {
+                const float up = __shfl_down_sync(0xffffffffu, di, w, 16), down = __shfl_up_sync(0xffffffffu, dj, w, 16);
+                if ((lane & 15) + w < 16) di += up;
+                if ((lane & 15) >= w) dj += down;
+            }
+            const float before = __shfl_up_sync(0xffffffffu, dj, 1, 16);
+            if (in) {
+                float dg = di + ((lane & 15) ? before : 0.f) + dot;
+#pragma unroll
+                for (int j = 0; j < kC - 1; ++j)
+                    if (j < lane) dg += sh.ee[0][lane][j];
+                const int64_t to = (ch.block * (int64_t)kC + lane) * out_t + out_0;
+                p.dg[to] = dg;
+                p.dbeta[to] = dbeta;
+            }
+        };
+        prepare(sh.chunk[0]);
+        __syncthreads();
+        for (int turn = 0;; ++turn) {
+            const BackChunk& ch = sh.chunk[turn & 1];
+            if (ch.block >= 0 && ch.state && fetch_state && lane == 0) {
+                tc::mbar_expect_tx(&sh.state_arrived, (uint32_t)L::kFetched);
+#pragma unroll
+                for (int i = 0; i < Fetch<float, DV>::kPanels; ++i)
+                    tc::tma_load_3d(fetched + i * DK * 32, &map_s, &sh.state_arrived, i * 32, 0, (int)(seq * blocks + ch.block));
+            }
+            if (turn) finish(sh.chunk[(turn & 1) ^ 1], sh.sums[(turn & 1) ^ 1]);
+            if (ch.block < 0) break;
+            __syncwarp();
+            __syncthreads();  // after U, ubar and dS are in shared memory
+            prepare(sh.chunk[(turn & 1) ^ 1]);
+            __syncthreads();  // after dA and dP are
+        }
+        return;
+    }
+
+    const bool has_v = warp < L::kWarpsV, has_k = warp < L::kWarpsK;
+    const int c0 = warp * 16;
+    const bool whole_v = c0 + 16 <= p.dv, whole_k = c0 + 16 <= p.dk;
+    const bool v_aligned = sizeof(T) == 2 && p.dv % 8 == 0 && reinterpret_cast<uintptr_t>(p.dv_out) % 16 == 0;
+    const bool k_pairs = sizeof(T) == 2 && p.dk % 2 == 0 && (reinterpret_cast<uintptr_t>(p.dq) | reinterpret_cast<uintptr_t>(p.dk_out)) % 4 == 0;
+    T* out_tile = reinterpret_cast<T*>(reinterpret_cast<uint8_t*>(&sh + 1) + warp * L::kOut);
+    Acc ds[DK / 8];  // dS^T: rows = columns c0.. of the state, columns = dk
+    auto each_state = [&](auto&& f) {
+#pragma unroll
+        for (int i = 0; i < DK / 8; ++i)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int kk = c0 + row + e / 2 * 8, c = i * 8 + quad * 2 + e % 2;
-                if (kk < p.dk && c < p.dv) to[(int64_t)kk * p.dv + c] = ds[i].v[e];
+                const int kk = i * 8 + quad * 2 + e % 2, c = c0 + row + e / 2 * 8;
+                f(ds[i].v[e], kk, c, kk < p.dk && c < p.dv);
             }
+    };
+    {
+        const float* df = p.d_final ? p.d_final + seq * p.dk * p.dv : nullptr;
+        each_state([&](float& x, int kk, int c, bool in) { x = df && in ? df[kk * p.dv + c] : 0.f; });
+    }
+    uint32_t states = 0;  // fetched so far
+    __syncthreads();
+    for (int turn = 0;; ++turn) {
+        const BackChunk& ch = sh.chunk[turn & 1];
+        typename L::Sums& sums = sh.sums[turn & 1];
+        const int64_t b = ch.block;
+        if (b < 0) break;
+        const int r0 = ch.r0, r1 = ch.r1;
+        const bool state = ch.state;
+        const uint32_t m0 = pair_mask(quad * 2, r0, r1), m1 = pair_mask(quad * 2 + 8, r0, r1);
+        // the copies of this block were waited for by the helper; a wait that is over makes them visible here
+        if constexpr (L::kInPlace)
+            if (p.aligned) tc::mbar_wait_warp(&sh.arrived[b % L::kBuffers], (blocks - 1 - b) / L::kBuffers & 1);
+
+        uint32_t xa[3][4];  // (-beta gamma ubar)^T for the update of dS
+        if (has_v) {
+            Acc e[2];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                e[c].zero();
+                if (warp < slices) {
+                    const float4 x = __ldcs(reinterpret_cast<const float4*>(p.errors) + error_at(seq * blocks + b, slices, warp, c, lane));
+                    e[c].v[0] = x.x, e[c].v[1] = x.y, e[c].v[2] = x.z, e[c].v[3] = x.w;
+                }
+            }
+            // dS to shared memory, and (K dS)^T
+            Acc du[2];
+            du[0].zero(), du[1].zero();
+#pragma unroll
+            for (int s = 0; s < DK / 16; ++s) {
+                uint32_t sa[3][4], ka[NT][4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    uint32_t tmp[3];
+                    const Acc& t = ds[2 * s + z / 2];
+                    split(t.v[z % 2 * 2], t.v[z % 2 * 2 + 1], tmp);
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) sa[x][z] = tmp[x];
+                    float* to = st + (s * 16 + z / 2 * 8 + quad * 2) * L::kLdS + c0 + row + z % 2 * 8;
+                    to[0] = t.v[z % 2 * 2];
+                    to[L::kLdS] = t.v[z % 2 * 2 + 1];
+                }
+#pragma unroll
+                for (int x = 0; x < NT; ++x) load_rows(ka[x], operand(b, 0, x), s * 16, lane);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t kb[NT][2];
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) kb[x][0] = ka[x][c], kb[x][1] = ka[x][c + 2];
+                    mma_terms<3>(du[c], sa, kb);
+                }
+            }
+            // U, and what eta gets: u_j . (dS^T k_j)
+            uint32_t ua[3][4];
+            float zj[4], be[4];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                const int j = c * 8 + quad * 2;
+                const float2 b2 = *reinterpret_cast<const float2*>(&ch.beta[j]), et = *reinterpret_cast<const float2*>(&ch.eta[j]);
+                const bool in0 = within(j, r0, r1), in1 = within(j + 1, r0, r1);
+                float u[4];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    const bool in = z % 2 ? in1 : in0;
+                    e[c].v[z] = in ? e[c].v[z] : 0.f;
+                    du[c].v[z] = in ? du[c].v[z] * (z % 2 ? et.y : et.x) : 0.f;
+                    u[z] = e[c].v[z] * (z % 2 ? b2.y : b2.x);
+                }
+                zj[c * 2] = u[0] * du[c].v[0] + u[2] * du[c].v[2];
+                zj[c * 2 + 1] = u[1] * du[c].v[1] + u[3] * du[c].v[3];
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t tmp[3];
+                    split(u[half * 2], u[half * 2 + 1], tmp);
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) ua[x][c * 2 + half] = tmp[x];
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 3; ++x) store_columns(ut + x * kC * L::kTv, L::kTv, c0, ua[x], lane);
+            // dU += dO^T (scale D o Q K^T), ubar^T = dU^T N
+            uint32_t oa[NT][4], ab[3][4];
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                load_columns(oa[x], operand(b, 2, x), c0, lane);
+#pragma unroll
+                for (int z = 0; z < 4; ++z) oa[x][z] &= z < 2 ? m0 : m1;
+            }
+#pragma unroll
+            for (int x = 0; x < 3; ++x) load_tokens(ab[x], Rows{&ch.att[x][0][0], kLdM}, 0, lane);
+            uint32_t da[3][4];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t bb[3][2];
+#pragma unroll
+                for (int x = 0; x < 3; ++x) bb[x][0] = ab[x][2 * c], bb[x][1] = ab[x][2 * c + 1];
+                mma_terms<3>(du[c], oa, bb);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t tmp[3];
+                    split(du[c].v[half * 2], du[c].v[half * 2 + 1], tmp);
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) da[x][c * 2 + half] = tmp[x];
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 3; ++x) load_tokens(ab[x], Rows{&ch.n[x][0][0], kLdM}, 0, lane);
+            uint32_t ba[3][4];
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t bb[3][2];
+#pragma unroll
+                for (int x = 0; x < 3; ++x) bb[x][0] = ab[x][2 * c], bb[x][1] = ab[x][2 * c + 1];
+                Acc ub;
+                ub.zero();
+                mma_terms<3>(ub, da, bb);
+                const int j = c * 8 + quad * 2;
+                const float2 b2 = *reinterpret_cast<const float2*>(&ch.beta[j]), ga = *reinterpret_cast<const float2*>(&ch.gamma[j]);
+                const bool in0 = within(j, r0, r1), in1 = within(j + 1, r0, r1);
+#pragma unroll
+                for (int z = 0; z < 4; ++z)
+                    if (!(z % 2 ? in1 : in0)) ub.v[z] = 0.f;
+                be[c * 2] = ub.v[0] * e[c].v[0] + ub.v[2] * e[c].v[2];
+                be[c * 2 + 1] = ub.v[1] * e[c].v[1] + ub.v[3] * e[c].v[3];
+                const float x0 = -b2.x * ga.x, x1 = -b2.y * ga.y;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    uint32_t tmp[3], tmp2[3];
+                    split(ub.v[half * 2], ub.v[half * 2 + 1], tmp);
+                    split(x0 * ub.v[half * 2], x1 * ub.v[half * 2 + 1], tmp2);
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) ba[x][c * 2 + half] = tmp[x], xa[x][c * 2 + half] = tmp2[x];
+                }
+                // dv = beta ubar
+                if (v_aligned && whole_v) {
+#pragma unroll
+                    for (int z = 0; z < 4; ++z)
+                        out_tile[(j + z % 2) * kLdOut + row + z / 2 * 8] = from_f32<T>((z % 2 ? b2.y : b2.x) * ub.v[z]);
+                } else {
+                    T* dv = static_cast<T*>(p.dv_out) + ((b * kC + j) * out_t + out_0) * p.dv + c0 + row;
+#pragma unroll
+                    for (int z = 0; z < 4; ++z)
+                        if ((z % 2 ? in1 : in0) && c0 + row + z / 2 * 8 < p.dv)
+                            dv[z % 2 * out_t * p.dv + z / 2 * 8] = from_f32<T>((z % 2 ? b2.y : b2.x) * ub.v[z]);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 3; ++x) store_columns(bt + x * kC * L::kTv, L::kTv, c0, ba[x], lane);
+            if constexpr (sizeof(T) == 2) {
+                if (v_aligned && whole_v) {
+                    __syncwarp();
+                    const int i = lane / 2;
+                    if (within(i, r0, r1))
+                        *reinterpret_cast<uint4*>(static_cast<T*>(p.dv_out) + ((b * kC + i) * out_t + out_0) * p.dv + c0 + lane % 2 * 8) =
+                            *reinterpret_cast<const uint4*>(out_tile + i * kLdOut + lane % 2 * 8);
+                }
+            }
+            add_over_rows(zj);
+            add_over_rows(be);
+            if (row == 0) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const int j = x / 2 * 8 + quad * 2 + x % 2;
+                    sums.dot_j[warp][j] = zj[x];
+                    sums.dbeta[warp][j] = be[x];
+                }
+            }
+        }
+        __syncthreads();
+
+        // W = dO U^T and dL = -ubar U^T, a half of one for each of the first four warps, into dA and dP
+        for (int task = warp; task < 4; task += L::kWarps) {
+            const int c = task & 1;
+            const bool is_w = task < 2;
+            Acc acc;
+            acc.zero();
+#pragma unroll
+            for (int s = 0; s < DV / 16; ++s) {
+                uint32_t uu[3][4], ub[3][2];
+#pragma unroll
+                for (int x = 0; x < 3; ++x) {
+                    load_rows(uu[x], Rows{ut + x * kC * L::kTv, L::kTv}, s * 16, lane);
+                    ub[x][0] = c ? uu[x][1] : uu[x][0], ub[x][1] = c ? uu[x][3] : uu[x][2];
+                }
+                if (is_w) {
+                    uint32_t oa[NT][4];
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) load_rows(oa[x], operand(b, 2, x), s * 16, lane);
+                    mma_terms<3>(acc, oa, ub);
+                } else {
+                    uint32_t ra[3][4];
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) load_rows(ra[x], Rows{bt + x * kC * L::kTv, L::kTv}, s * 16, lane);
+                    mma_terms<3>(acc, ra, ub);
+                }
+            }
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int i = row + half * 8, j = c * 8 + quad * 2;
+                const float2 f = *reinterpret_cast<const float2*>(is_w ? &ch.fa[i][j] : &ch.fp[i][j]);
+                const float2 g = *reinterpret_cast<const float2*>(is_w ? &ch.qk[i][j] : &ch.kk[i][j]);
+                const float s = is_w ? 1.f : -1.f;
+                const float x = f.x != 0.f ? s * f.x * acc.v[half * 2] : 0.f, y = f.y != 0.f ? s * f.y * acc.v[half * 2 + 1] : 0.f;
+                uint32_t tmp[3];
+                split(x, y, tmp);
+#pragma unroll
+                for (int z = 0; z < 3; ++z) *reinterpret_cast<uint32_t*>(is_w ? &sh.da[z][i][j] : &sh.dp[z][i][j]) = tmp[z];
+                sh.ee[is_w ? 0 : 1][i][j] = i > j ? x * g.x : 0.f;
+                sh.ee[is_w ? 0 : 1][i][j + 1] = i > j + 1 ? y * g.y : 0.f;
+            }
+        }
+
+        Acc dq[2], dk[2], dku[2];
+#pragma unroll
+        for (int c = 0; c < 2; ++c) dq[c].zero(), dk[c].zero(), dku[c].zero();
+        if (has_k) {
+            const float* s0 = p.checkpoints + (seq * blocks + b) * p.dk * p.dv;
+            if (fetch_state && state) tc::mbar_wait_warp(&sh.state_arrived, states & 1);
+            float dot = 0.f;
+#pragma unroll
+            for (int s = 0; s < DV / 16; ++s) {
+                uint32_t oa[NT][4], ra[3][4], ua[ND][4];
+#pragma unroll
+                for (int x = 0; x < NT; ++x) load_rows(oa[x], operand(b, 2, x), s * 16, lane);
+#pragma unroll
+                for (int x = 0; x < 3; ++x) load_rows(ra[x], Rows{bt + x * kC * L::kTv, L::kTv}, s * 16, lane);
+#pragma unroll
+                for (int x = 0; x < ND; ++x) load_rows(ua[x], Rows{ut + x * kC * L::kTv, L::kTv}, s * 16, lane);
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {  // rows of the state c0 + 8 c + row
+                    uint32_t sb[3][2], db[ND][2];
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const int kk = c0 + c * 8 + row, col = s * 16 + half * 8 + quad * 2;
+                        float2 x = make_float2(0.f, 0.f);
+                        if (state) {
+                            if (fetch_state) {
+                                x = *reinterpret_cast<const float2*>(fetched + col / 32 * (DK * 32) + kk * 32 + ((col / 4 % 8) ^ (kk & 7)) * 4 + col % 4);
+                            } else if (kk < p.dk) {
+                                if (col < p.dv) x.x = s0[kk * p.dv + col];
+                                if (col + 1 < p.dv) x.y = s0[kk * p.dv + col + 1];
+                            }
+                        }
+                        const float2 y = *reinterpret_cast<const float2*>(st + kk * L::kLdS + col);
+                        if (state) dot = fmaf(x.x, y.x, fmaf(x.y, y.y, dot));
+                        uint32_t tmp[3], tmp2[ND];
+                        split(x.x, x.y, tmp);
+                        split(y.x, y.y, tmp2);
+#pragma unroll
+                        for (int z = 0; z < 3; ++z) sb[z][half] = tmp[z];
+#pragma unroll
+                        for (int z = 0; z < ND; ++z) db[z][half] = tmp2[z];
+                    }
+                    mma_terms<3>(dq[c], oa, sb);
+                    mma_terms<3>(dk[c], ra, sb);
+                    mma_terms<ND>(dku[c], ua, db);
+                }
+            }
+            // the decays' gradients need q.dq and k.dk of the parts through S alone
+            const float g0 = p.scale * ch.gamma[row], g1 = p.scale * ch.gamma[row + 8], e0 = ch.eta[row], e1 = ch.eta[row + 8];
+            const float x0 = -ch.beta[row] * ch.gamma[row], x1 = -ch.beta[row + 8] * ch.gamma[row + 8];
+            float di[2] = {0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const int half = e / 2;
+                    const T* qv = raw_tile(b) + L::kTileK;
+                    dq[c].v[e] *= half ? g1 : g0;
+                    dk[c].v[e] *= half ? x1 : x0;
+                    dku[c].v[e] *= half ? e1 : e0;
+                    float kx, qx;
+                    if constexpr (L::kInPlace) {
+                        const int px = panel_at<T>(row + half * 8, c0 + c * 8 + quad * 2 + e % 2);
+                        kx = to_f32(qv[px - L::kTileK]), qx = to_f32(qv[px]);
+                    } else {
+                        kx = qx = 0.f;
+#pragma unroll
+                        for (int x = NT - 1; x >= 0; --x) {
+                            kx += __bfloat162float(*operand(b, 0, x).at(row + half * 8, c0 + c * 8 + quad * 2 + e % 2));
+                            qx += __bfloat162float(*operand(b, 1, x).at(row + half * 8, c0 + c * 8 + quad * 2 + e % 2));
+                        }
+                    }
+                    di[half] += qx * dq[c].v[e] + kx * dk[c].v[e];
+                }
+#pragma unroll
+            for (int w = 1; w < 4; w *= 2)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) di[half] += __shfl_xor_sync(0xffffffffu, di[half], w);
+#pragma unroll
+            for (int w = 1; w < 32; w *= 2) dot += __shfl_xor_sync(0xffffffffu, dot, w);
+            if (quad == 0) sums.dot_i[warp][row] = di[0], sums.dot_i[warp][row + 8] = di[1];
+            if (lane == 0) sums.dot_s[warp] = ch.keep * dot;
+        }
+        if (state) ++states;
+        __syncthreads();
+
+        if (has_k) {
+            uint32_t da[3][4], dat[3][4], dp[3][4], dpt[3][4], kb[NT][4], qb[NT][4];
+#pragma unroll
+            for (int x = 0; x < 3; ++x) {
+                load_rows(da[x], Rows{&sh.da[x][0][0], kLdM}, 0, lane);
+                load_columns(dat[x], Rows{&sh.da[x][0][0], kLdM}, 0, lane);
+                load_rows(dp[x], Rows{&sh.dp[x][0][0], kLdM}, 0, lane);
+                load_columns(dpt[x], Rows{&sh.dp[x][0][0], kLdM}, 0, lane);
+            }
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                load_tokens(kb[x], operand(b, 0, x), c0, lane);
+                load_tokens(qb[x], operand(b, 1, x), c0, lane);
+            }
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t k2[NT][2], q2[NT][2];
+#pragma unroll
+                for (int x = 0; x < NT; ++x) {
+                    k2[x][0] = kb[x][2 * c] & m0, k2[x][1] = kb[x][2 * c + 1] & m1;
+                    q2[x][0] = qb[x][2 * c] & m0, q2[x][1] = qb[x][2 * c + 1] & m1;
+                }
+                mma_terms<ND>(dq[c], da, k2);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) dk[c].v[e] += dku[c].v[e];
+                mma_terms<ND>(dk[c], dat, q2);
+                mma_terms<ND>(dk[c], dp, k2);
+                mma_terms<ND>(dk[c], dpt, k2);
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int i = row + half * 8, col = c0 + c * 8 + quad * 2;
+                    if (!within(i, r0, r1)) continue;
+                    const int64_t to = ((b * kC + i) * out_t + out_0) * p.dk + col;
+                    if (k_pairs && whole_k) {
+                        if constexpr (sizeof(T) == 2) {
+                            union { T h[2]; uint32_t u; } x, y;
+                            x.h[0] = from_f32<T>(dq[c].v[half * 2]), x.h[1] = from_f32<T>(dq[c].v[half * 2 + 1]);
+                            y.h[0] = from_f32<T>(dk[c].v[half * 2]), y.h[1] = from_f32<T>(dk[c].v[half * 2 + 1]);
+                            *reinterpret_cast<uint32_t*>(static_cast<T*>(p.dq) + to) = x.u;
+                            *reinterpret_cast<uint32_t*>(static_cast<T*>(p.dk_out) + to) = y.u;
+                        }
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+                            if (col + e < p.dk) {
+                                static_cast<T*>(p.dq)[to + e] = from_f32<T>(dq[c].v[half * 2 + e]);
+                                static_cast<T*>(p.dk_out)[to + e] = from_f32<T>(dk[c].v[half * 2 + e]);
+                            }
+                    }
+                }
+            }
+        }
+        if (has_v) {
+            if (ch.fresh) {  // the state before was dropped
+#pragma unroll
+                for (int i = 0; i < DK / 8; ++i) ds[i].zero();
+            } else {
+                const float keep = ch.keep;
+                uint32_t ya[3][4];  // (scale gamma dO)^T
+                {
+                    uint32_t oa[NT][4];
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) load_columns(oa[x], operand(b, 2, x), c0, lane);
+#pragma unroll
+                    for (int z = 0; z < 4; ++z) {
+                        const int j = z / 2 * 8 + quad * 2;
+                        const float2 ga = *reinterpret_cast<const float2*>(&ch.gamma[j]);
+                        float o0 = 0.f, o1 = 0.f;
+#pragma unroll
+                        for (int x = NT - 1; x >= 0; --x) {
+                            o0 += __uint_as_float(oa[x][z] << 16);
+                            o1 += __uint_as_float(oa[x][z] & 0xFFFF0000u);
+                        }
+                        uint32_t tmp[3];
+                        split(within(j, r0, r1) ? p.scale * ga.x * o0 : 0.f, within(j + 1, r0, r1) ? p.scale * ga.y * o1 : 0.f, tmp);
+#pragma unroll
+                        for (int x = 0; x < 3; ++x) ya[x][z] = tmp[x];
+                    }
+                }
+#pragma unroll
+                for (int s = 0; s < DK / 16; ++s) {
+                    uint32_t kb[NT][4], qb[NT][4];
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                        load_tokens(kb[x], operand(b, 0, x), s * 16, lane);
+                        load_tokens(qb[x], operand(b, 1, x), s * 16, lane);
+                    }
+#pragma unroll
+                    for (int c = 0; c < 2; ++c) {
+                        Acc& acc = ds[2 * s + c];
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) acc.v[e] *= keep;
+                        uint32_t k2[NT][2], q2[NT][2];
+#pragma unroll
+                        for (int x = 0; x < NT; ++x) {
+                            k2[x][0] = kb[x][2 * c] & m0, k2[x][1] = kb[x][2 * c + 1] & m1;
+                            q2[x][0] = qb[x][2 * c] & m0, q2[x][1] = qb[x][2 * c + 1] & m1;
+                        }
+                        mma_terms<3>(acc, ya, q2);
+                        mma_terms<3>(acc, xa, k2);
+                    }
+                }
+            }
+        }
+    }
+    if (p.dstate && has_v) {
+        float* to = p.dstate + seq * p.dk * p.dv;
+        each_state([&](float& x, int kk, int c, bool in) {
+            if (in) to[kk * p.dv + c] = x;
+        });
     }
 }
 
@@ -1384,8 +1503,22 @@ template <class T, int DK, int DV>
 int launch_backward_dk_dv(const Scan& p, cudaStream_t st) {
     using L = BackwardSmem<T, DK, DV>;
     auto* kernel = scan_backward_kernel<T, DK, DV>;
+    CUtensorMap map_k{}, map_q{}, map_o{}, map_s{};
+    if (p.aligned) {
+        const Strides so{p.n * p.h * p.dv, p.h * p.dv, p.dv};
+        if (int rc = map_rows<T>(&map_k, p.k, p.sk, p, p.dk)) return rc;
+        if (int rc = map_rows<T>(&map_q, p.q, p.sq, p, p.dk)) return rc;
+        if (int rc = map_rows<T>(&map_o, p.d_o, so, p, p.dv)) return rc;
+    }
+    if (L::kFetchState && p.dv % 4 == 0) {
+        const uint64_t dims[3] = {(uint64_t)p.dv, (uint64_t)p.dk, (uint64_t)(p.n * p.h * ((p.t + kC - 1) / kC))};
+        const uint64_t strides[2] = {p.dv * 4ull, (uint64_t)p.dk * p.dv * 4};
+        const uint32_t box[3] = {32, DK, 1};
+        if (dims[2] > 0x7FFFFFFFull) return invalid("delta_scan_backward: more than 2^31 states");
+        if (int rc = encode_map(&map_s, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, p.checkpoints, dims, strides, box)) return rc;
+    }
     if (int rc = cuda_status(allow_smem(kernel, (int)L::kBytes), "delta_scan_backward")) return rc;
-    kernel<<<static_cast<unsigned>(p.n * p.h), L::kWarps * 32, L::kBytes, st>>>(p);
+    kernel<<<static_cast<unsigned>(p.n * p.h), (L::kWarps + 1) * 32, L::kBytes, st>>>(p, map_k, map_q, map_o, map_s);
     return cuda_status(cudaGetLastError(), "delta_scan_backward");
 }
 

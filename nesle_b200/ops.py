@@ -295,7 +295,7 @@ class _DeltaScan(torch.autograd.Function):
         a.o, a.final_state = o.data_ptr(), final.data_ptr()
         lib = _lib.load()
         if grad:
-            errors = torch.empty((t, n, h, dv), dtype=torch.float32, device=dev)
+            errors = torch.empty(lib.nesle_delta_error_floats(ctypes.byref(a)), dtype=torch.float32, device=dev)
             checkpoints = torch.empty(lib.nesle_delta_checkpoint_floats(ctypes.byref(a)), dtype=torch.float32, device=dev)
             a.errors, a.checkpoints = errors.data_ptr(), checkpoints.data_ptr()
             ctx.save_for_backward(q, k, v, g, beta, reset, errors, checkpoints)
