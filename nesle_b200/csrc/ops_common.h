@@ -39,13 +39,12 @@ int guarded(F&& body) noexcept {
     }
 }
 
-// Makes `device` current for the scope.
+// Makes `device` current for the scope.  cudaSetDevice is called even where it already is: a thread that has made no CUDA
+// call yet (the autograd engine's, for one) has no context bound, and encoding a tensor map needs one.
 struct OnDevice {
     int prev = -1;
     bool ok = true;
-    explicit OnDevice(int device) {
-        ok = cudaGetDevice(&prev) == cudaSuccess && (prev == device || cudaSetDevice(device) == cudaSuccess);
-    }
+    explicit OnDevice(int device) { ok = cudaGetDevice(&prev) == cudaSuccess && cudaSetDevice(device) == cudaSuccess; }
     ~OnDevice() {
         int cur = -1;
         if (prev >= 0 && cudaGetDevice(&cur) == cudaSuccess && cur != prev) cudaSetDevice(prev);

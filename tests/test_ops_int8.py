@@ -5,6 +5,8 @@ rounding of the epilogue alone: the sum to fp32 and three fp32 operations (at
 most 4 * 2^-24 of the largest term) and one rounding to the output type."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -179,6 +181,19 @@ def test_on_another_stream_and_in_a_graph():
     graph.replay()
     assert torch.equal(out, ops.int8_linear(x, w, 0.25))
 
+
+@pytest.mark.gpu
+def test_in_a_thread_that_has_made_no_cuda_call():
+    x = torch.randint(0, 256, (200, 64), generator=_gen(2), device="cuda", dtype=torch.uint8)
+    q, ws = _weight(96, 64, 4)
+    w, out = ops.Int8Weight(q, ws), torch.empty((200, 96), device="cuda", dtype=torch.bfloat16)
+    want = ops.int8_linear(x, w, 0.25)
+    torch.cuda.synchronize()
+    thread = threading.Thread(target=lambda: ops.int8_linear(x, w, 0.25, out=out))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
 
 @pytest.mark.gpu
 def test_refusals():
