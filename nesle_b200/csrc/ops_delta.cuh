@@ -30,6 +30,8 @@
 #pragma once
 #include <stddef.h>
 
+#include <type_traits>
+
 #include "ops_common.h"
 #include "tc05.cuh"
 
@@ -98,21 +100,96 @@ struct Acc {  // 16 x 8 of a result: rows lane/4 and lane/4 + 8, columns 2 (lane
     __device__ __forceinline__ void zero() { v[0] = v[1] = v[2] = v[3] = 0.f; }
 };
 
-__device__ __forceinline__ void mma(Acc& c, const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void mma(Acc& c, const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c.v[0]), "+f"(c.v[1]), "+f"(c.v[2]), "+f"(c.v[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
 }
 
-// c += A B with A in NA terms and B in NB; pairs of terms i + j < kMost, the smallest first.
+// The pairs of terms (i, j), i < NA, j < NB, i + j < kMost, the smallest products first.
 template <int kMost, int NA, int NB>
-__device__ __forceinline__ void mma_terms(Acc& c, const uint32_t (&a)[NA][4], const uint32_t (&b)[NB][2]) {
-#pragma unroll
-    for (int s = kMost - 1; s >= 0; --s)
-#pragma unroll
+struct Pairs {
+    __host__ __device__ static constexpr int count() {
+        int n = 0;
         for (int i = 0; i < NA; ++i)
-            if (s - i >= 0 && s - i < NB) mma(c, a[i], b[s - i][0], b[s - i][1]);
+            for (int j = 0; j < NB; ++j) n += i + j < kMost;
+        return n;
+    }
+    __host__ __device__ static constexpr int at(int k) {  // 8 i + j of the k-th
+        for (int s = kMost - 1; s >= 0; --s)
+            for (int i = 0; i < NA; ++i)
+                if (s - i >= 0 && s - i < NB && k-- == 0) return 8 * i + s - i;
+        return 0;
+    }
+    static constexpr int n = count();
+};
+
+// One product after another into one accumulator waits for it 30-odd clocks each time, and a product takes 8 to issue: so
+// products go round four accumulators or so.  Each call of a step adds pair k of one product to the accumulators of two
+// neighbouring column tiles.
+template <class P, int k, int NA, int NB>
+__device__ __forceinline__ void step2(Acc& c0, Acc& c1, const uint32_t (&a)[NA][4], const uint32_t (&b0)[NB][2], const uint32_t (&b1)[NB][2]) {
+    if constexpr (k < P::n) {
+        constexpr int i = P::at(k) / 8, j = P::at(k) % 8;
+        mma(c0, a[i], b0[j]);
+        mma(c1, a[i], b1[j]);
+    }
+}
+template <int k, int n, class F>
+__device__ __forceinline__ void each_step(F&& f) {
+    if constexpr (k < n) {
+        f(std::integral_constant<int, k>{});
+        each_step<k + 1, n>(f);
+    }
+}
+// c += A b for two column tiles.
+template <int kMost, int NA, int NB>
+__device__ __forceinline__ void mma2(Acc (&c)[2], const uint32_t (&a)[NA][4], const uint32_t (&b)[2][NB][2]) {
+    using P = Pairs<kMost, NA, NB>;
+    each_step<0, P::n>([&](auto k) { step2<P, k.value>(c[0], c[1], a, b[0], b[1]); });
+}
+// Two products into accumulators of their own, in turn.
+template <int kMostX, int kMostY, int NXA, int NXB, int NYA, int NYB>
+__device__ __forceinline__ void mma2_zip(Acc (&x)[2], const uint32_t (&xa)[NXA][4], const uint32_t (&xb)[2][NXB][2], Acc (&y)[2],
+                                         const uint32_t (&ya)[NYA][4], const uint32_t (&yb)[2][NYB][2]) {
+    using X = Pairs<kMostX, NXA, NXB>;
+    using Y = Pairs<kMostY, NYA, NYB>;
+    each_step<0, (X::n > Y::n ? X::n : Y::n)>([&](auto k) {
+        step2<X, k.value>(x[0], x[1], xa, xb[0], xb[1]);
+        step2<Y, k.value>(y[0], y[1], ya, yb[0], yb[1]);
+    });
+}
+// The same product over two pairs of accumulators, which are then added: for a product that stands alone.
+template <int kMost, int NA, int NB>
+__device__ __forceinline__ void mma2_split(Acc (&c)[2], const uint32_t (&a)[NA][4], const uint32_t (&b)[2][NB][2]) {
+    using P = Pairs<kMost, NA, NB>;
+    Acc d[2];
+    d[0].zero(), d[1].zero();
+    each_step<0, (P::n + 1) / 2>([&](auto k) {
+        step2<P, 2 * k.value>(d[0], d[1], a, b[0], b[1]);
+        step2<P, 2 * k.value + 1>(c[0], c[1], a, b[0], b[1]);
+    });
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[i].v[e] += d[i].v[e];
+}
+
+// Registers of load_rows as a B operand whose columns are the tile's rows, of load_tokens as one whose columns are the
+// tile's columns; tokens outside the chunk masked.
+template <int N>
+__device__ __forceinline__ void as_rows(uint32_t (&b)[2][N][2], const uint32_t (&r)[N][4]) {
+#pragma unroll
+    for (int x = 0; x < N; ++x)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) b[c][x][0] = r[x][c], b[c][x][1] = r[x][c + 2];
+}
+template <int N>
+__device__ __forceinline__ void as_columns(uint32_t (&b)[2][N][2], const uint32_t (&r)[N][4], uint32_t m0 = ~0u, uint32_t m1 = ~0u) {
+#pragma unroll
+    for (int x = 0; x < N; ++x)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) b[c][x][0] = r[x][2 * c] & m0, b[c][x][1] = r[x][2 * c + 1] & m1;
 }
 
 __device__ __forceinline__ uint32_t smem_at(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
@@ -490,14 +567,9 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                     load_rows(ka[x], operand(b, 0, x), st * 16, lane);
                     load_rows(qa[x], operand(b, 1, x), st * 16, lane);
                 }
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t kb[NT][2];
-#pragma unroll
-                    for (int x = 0; x < NT; ++x) kb[x][0] = ka[x][c], kb[x][1] = ka[x][c + 2];
-                    mma_terms<3>(kk[c], ka, kb);
-                    mma_terms<NO>(qk[c], qa, kb);
-                }
+                uint32_t kb[2][NT][2];
+                as_rows(kb, ka);
+                mma2_zip<3, NO>(kk, ka, kb, qk, qa, kb);
             }
             __syncwarp();
 #pragma unroll
@@ -600,17 +672,10 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                 load_rows(ka[x], operand(b, 0, x), st * 16, lane);
                 load_rows(qa[x], operand(b, 1, x), st * 16, lane);
             }
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t kb[NT][2], qb[NT][2];
-#pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                    kb[x][0] = ka[x][c], kb[x][1] = ka[x][c + 2];
-                    qb[x][0] = qa[x][c], qb[x][1] = qa[x][c + 2];
-                }
-                mma_terms<3>(ks[c], sa, kb);
-                mma_terms<NO>(qs[c], sa, qb);
-            }
+            uint32_t kb[2][NT][2], qb[2][NT][2];
+            as_rows(kb, ka);
+            as_rows(qb, qa);
+            mma2_zip<3, NO>(ks, sa, kb, qs, sa, qb);
         }
         // R^T; tokens outside the chunk are zero whatever their inputs hold
         uint32_t ra[3][4];
@@ -643,16 +708,15 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
         }
         uint32_t uo[NO][4], ue[3][4];  // U^T and (eta U)^T
         {
-            uint32_t mb[3][4];
+            uint32_t mb[3][4], bb[2][3][2];
             load_operand(mb, ch.m, lane);
+            as_rows(bb, mb);
+            Acc ee[2];
+            ee[0].zero(), ee[1].zero();
+            mma2_split<3>(ee, ra, bb);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t bb[3][2];
-#pragma unroll
-                for (int x = 0; x < 3; ++x) bb[x][0] = mb[x][c], bb[x][1] = mb[x][c + 2];
-                Acc e;
-                e.zero();
-                mma_terms<3>(e, ra, bb);
+                const Acc& e = ee[c];
                 const int j = c * 8 + quad * 2;
                 if (p.errors && first_col / 16 + warp < slices) {
                     float4* to = reinterpret_cast<float4*>(p.errors) + error_at(seq * blocks + b, slices, first_col / 16 + warp, c, lane);
@@ -679,15 +743,10 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
             }
         }
         {
-            uint32_t ab[NO][4];
+            uint32_t ab[NO][4], bb[2][NO][2];
             load_operand(ab, ch.att, lane);
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t bb[NO][2];
-#pragma unroll
-                for (int x = 0; x < NO; ++x) bb[x][0] = ab[x][c], bb[x][1] = ab[x][c + 2];
-                mma_terms<NO>(qs[c], uo, bb);
-            }
+            as_rows(bb, ab);
+            mma2_split<NO>(qs, uo, bb);
         }
         if (o_aligned && whole) {  // by a transposed tile in shared memory, 16 bytes a lane
             if constexpr (sizeof(T) == 2) {
@@ -716,20 +775,23 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
         const float keep = ch.keep;
         const uint32_t m0 = pair_mask(quad * 2, r0, r1), m1 = pair_mask(quad * 2 + 8, r0, r1);
 #pragma unroll
-        for (int st = 0; st < kSteps; ++st) {
-            uint32_t kb[NT][4];
+        for (int i = 0; i < kTiles; ++i)
 #pragma unroll
-            for (int x = 0; x < NT; ++x) load_tokens(kb[x], operand(b, 0, x), st * 16, lane);
+            for (int e = 0; e < 4; ++e) s[i].v[e] *= keep;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                Acc& acc = s[2 * st + c];
+        for (int st = 0; st < kSteps; st += 2) {
+            uint32_t kb[2][NT][4], bb[2][2][NT][2];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) acc.v[e] *= keep;
-                uint32_t bb[NT][2];
+            for (int half = 0; half < 2; ++half) {
 #pragma unroll
-                for (int x = 0; x < NT; ++x) bb[x][0] = kb[x][2 * c] & m0, bb[x][1] = kb[x][2 * c + 1] & m1;
-                mma_terms<3>(acc, ue, bb);
+                for (int x = 0; x < NT; ++x) load_tokens(kb[half][x], operand(b, 0, x), (st + half) * 16, lane);
+                as_columns(bb[half], kb[half], m0, m1);
             }
+            using P = Pairs<3, 3, NT>;
+            each_step<0, P::n>([&](auto k) {
+                step2<P, k.value>(s[2 * st], s[2 * st + 1], ue, bb[0][0], bb[0][1]);
+                step2<P, k.value>(s[2 * st + 2], s[2 * st + 3], ue, bb[1][0], bb[1][1]);
+            });
         }
     }
     if (p.final_state) put_state(p.final_state + seq * p.dk * p.dv);
@@ -938,14 +1000,9 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                     load_rows(ka[x], operand(b, 0, x), s * 16, lane);
                     load_rows(qa[x], operand(b, 1, x), s * 16, lane);
                 }
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t kb[NT][2];
-#pragma unroll
-                    for (int x = 0; x < NT; ++x) kb[x][0] = ka[x][c], kb[x][1] = ka[x][c + 2];
-                    mma_terms<3>(kk[c], ka, kb);
-                    mma_terms<3>(qk[c], qa, kb);
-                }
+                uint32_t kb[2][NT][2];
+                as_rows(kb, ka);
+                mma2_zip<3, 3>(kk, ka, kb, qk, qa, kb);
             }
             __syncwarp();
 #pragma unroll
@@ -1085,8 +1142,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                 }
             }
             // dS to shared memory, and (K dS)^T
-            Acc du[2];
-            du[0].zero(), du[1].zero();
+            Acc du[2], du2[2];
+            du[0].zero(), du[1].zero(), du2[0].zero(), du2[1].zero();
 #pragma unroll
             for (int s = 0; s < DK / 16; ++s) {
                 uint32_t sa[3][4], ka[NT][4];
@@ -1103,14 +1160,14 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                 }
 #pragma unroll
                 for (int x = 0; x < NT; ++x) load_rows(ka[x], operand(b, 0, x), s * 16, lane);
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t kb[NT][2];
-#pragma unroll
-                    for (int x = 0; x < NT; ++x) kb[x][0] = ka[x][c], kb[x][1] = ka[x][c + 2];
-                    mma_terms<3>(du[c], sa, kb);
-                }
+                uint32_t kb[2][NT][2];
+                as_rows(kb, ka);
+                mma2<3>(s % 2 ? du2 : du, sa, kb);
             }
+#pragma unroll
+            for (int c = 0; c < 2; ++c)
+#pragma unroll
+                for (int z = 0; z < 4; ++z) du[c].v[z] += du2[c].v[z];
             // U, and what eta gets: u_j . (dS^T k_j)
             uint32_t ua[3][4];
             float zj[4], be[4];
@@ -1149,13 +1206,11 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
             }
 #pragma unroll
             for (int x = 0; x < 3; ++x) load_tokens(ab[x], Rows{&ch.att[x][0][0], kLdM}, 0, lane);
-            uint32_t da[3][4];
+            uint32_t da[3][4], bb[2][3][2];
+            as_columns(bb, ab);
+            mma2_split<3>(du, oa, bb);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t bb[3][2];
-#pragma unroll
-                for (int x = 0; x < 3; ++x) bb[x][0] = ab[x][2 * c], bb[x][1] = ab[x][2 * c + 1];
-                mma_terms<3>(du[c], oa, bb);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t tmp[3];
@@ -1167,14 +1222,13 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
 #pragma unroll
             for (int x = 0; x < 3; ++x) load_tokens(ab[x], Rows{&ch.n[x][0][0], kLdM}, 0, lane);
             uint32_t ba[3][4];
+            as_columns(bb, ab);
+            Acc ubar[2];
+            ubar[0].zero(), ubar[1].zero();
+            mma2_split<3>(ubar, da, bb);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t bb[3][2];
-#pragma unroll
-                for (int x = 0; x < 3; ++x) bb[x][0] = ab[x][2 * c], bb[x][1] = ab[x][2 * c + 1];
-                Acc ub;
-                ub.zero();
-                mma_terms<3>(ub, da, bb);
+                Acc& ub = ubar[c];
                 const int j = c * 8 + quad * 2;
                 const float2 b2 = *reinterpret_cast<const float2*>(&ch.beta[j]), ga = *reinterpret_cast<const float2*>(&ch.gamma[j]);
                 const bool in0 = within(j, r0, r1), in1 = within(j + 1, r0, r1);
@@ -1233,8 +1287,9 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
         for (int task = warp; task < 4; task += L::kWarps) {
             const int c = task & 1;
             const bool is_w = task < 2;
-            Acc acc;
-            acc.zero();
+            Acc parts[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) parts[i].zero();
 #pragma unroll
             for (int s = 0; s < DV / 16; ++s) {
                 uint32_t uu[3][4], ub[3][2];
@@ -1247,14 +1302,19 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                     uint32_t oa[NT][4];
 #pragma unroll
                     for (int x = 0; x < NT; ++x) load_rows(oa[x], operand(b, 2, x), s * 16, lane);
-                    mma_terms<3>(acc, oa, ub);
+                    using P = Pairs<3, NT, 3>;
+                    each_step<0, P::n>([&](auto k) { mma(parts[(k.value + s) % 4], oa[P::at(k.value) / 8], ub[P::at(k.value) % 8]); });
                 } else {
                     uint32_t ra[3][4];
 #pragma unroll
                     for (int x = 0; x < 3; ++x) load_rows(ra[x], Rows{bt + x * kC * L::kTv, L::kTv}, s * 16, lane);
-                    mma_terms<3>(acc, ra, ub);
+                    using P = Pairs<3, 3, 3>;
+                    each_step<0, P::n>([&](auto k) { mma(parts[(k.value + s) % 4], ra[P::at(k.value) / 8], ub[P::at(k.value) % 8]); });
                 }
             }
+            Acc acc;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc.v[e] = (parts[0].v[e] + parts[1].v[e]) + (parts[2].v[e] + parts[3].v[e]);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
                 const int i = row + half * 8, j = c * 8 + quad * 2;
@@ -1287,9 +1347,9 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                 for (int x = 0; x < 3; ++x) load_rows(ra[x], Rows{bt + x * kC * L::kTv, L::kTv}, s * 16, lane);
 #pragma unroll
                 for (int x = 0; x < ND; ++x) load_rows(ua[x], Rows{ut + x * kC * L::kTv, L::kTv}, s * 16, lane);
+                uint32_t sb[2][3][2], db[2][ND][2];
 #pragma unroll
                 for (int c = 0; c < 2; ++c) {  // rows of the state c0 + 8 c + row
-                    uint32_t sb[3][2], db[ND][2];
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
                         const int kk = c0 + c * 8 + row, col = s * 16 + half * 8 + quad * 2;
@@ -1308,14 +1368,21 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                         split(x.x, x.y, tmp);
                         split(y.x, y.y, tmp2);
 #pragma unroll
-                        for (int z = 0; z < 3; ++z) sb[z][half] = tmp[z];
+                        for (int z = 0; z < 3; ++z) sb[c][z][half] = tmp[z];
 #pragma unroll
-                        for (int z = 0; z < ND; ++z) db[z][half] = tmp2[z];
+                        for (int z = 0; z < ND; ++z) db[c][z][half] = tmp2[z];
                     }
-                    mma_terms<3>(dq[c], oa, sb);
-                    mma_terms<3>(dk[c], ra, sb);
-                    mma_terms<ND>(dku[c], ua, db);
                 }
+                using X = Pairs<3, 3, 3>;    // dk: 6
+                using Y = Pairs<3, NT, 3>;   // dq: 3 (5, 6), then
+                using Z = Pairs<ND, ND, ND>; // U dS^T: 3 (3, 6)
+                each_step<0, Y::n + Z::n>([&](auto k) {
+                    step2<X, k.value>(dk[0], dk[1], ra, sb[0], sb[1]);
+                    if constexpr (k.value < Y::n)
+                        step2<Y, k.value>(dq[0], dq[1], oa, sb[0], sb[1]);
+                    else
+                        step2<Z, k.value - Y::n>(dku[0], dku[1], ua, db[0], db[1]);
+                });
             }
             // the decays' gradients need q.dq and k.dk of the parts through S alone
             const float g0 = p.scale * ch.gamma[row], g1 = p.scale * ch.gamma[row + 8], e0 = ch.eta[row], e1 = ch.eta[row + 8];
@@ -1370,20 +1437,15 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                 load_tokens(kb[x], operand(b, 0, x), c0, lane);
                 load_tokens(qb[x], operand(b, 1, x), c0, lane);
             }
+            uint32_t k2[2][NT][2], q2[2][NT][2];
+            as_columns(k2, kb, m0, m1);
+            as_columns(q2, qb, m0, m1);
+            mma2_zip<ND, ND>(dq, da, k2, dk, dat, q2);
+            mma2_zip<ND, ND>(dku, dp, k2, dk, dpt, k2);
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                uint32_t k2[NT][2], q2[NT][2];
-#pragma unroll
-                for (int x = 0; x < NT; ++x) {
-                    k2[x][0] = kb[x][2 * c] & m0, k2[x][1] = kb[x][2 * c + 1] & m1;
-                    q2[x][0] = qb[x][2 * c] & m0, q2[x][1] = qb[x][2 * c + 1] & m1;
-                }
-                mma_terms<ND>(dq[c], da, k2);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) dk[c].v[e] += dku[c].v[e];
-                mma_terms<ND>(dk[c], dat, q2);
-                mma_terms<ND>(dk[c], dp, k2);
-                mma_terms<ND>(dk[c], dpt, k2);
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     const int i = row + half * 8, col = c0 + c * 8 + quad * 2;
@@ -1436,26 +1498,25 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                     }
                 }
 #pragma unroll
-                for (int s = 0; s < DK / 16; ++s) {
-                    uint32_t kb[NT][4], qb[NT][4];
+                for (int i = 0; i < DK / 8; ++i)
 #pragma unroll
-                    for (int x = 0; x < NT; ++x) {
-                        load_tokens(kb[x], operand(b, 0, x), s * 16, lane);
-                        load_tokens(qb[x], operand(b, 1, x), s * 16, lane);
-                    }
+                    for (int e = 0; e < 4; ++e) ds[i].v[e] *= keep;
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        Acc& acc = ds[2 * s + c];
+                for (int s = 0; s < DK / 16; s += 2) {
+                    using P = Pairs<3, 3, NT>;
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) acc.v[e] *= keep;
-                        uint32_t k2[NT][2], q2[NT][2];
+                    for (int which = 0; which < 2; ++which) {
+                        uint32_t kb[2][NT][4], bb[2][2][NT][2];
 #pragma unroll
-                        for (int x = 0; x < NT; ++x) {
-                            k2[x][0] = kb[x][2 * c] & m0, k2[x][1] = kb[x][2 * c + 1] & m1;
-                            q2[x][0] = qb[x][2 * c] & m0, q2[x][1] = qb[x][2 * c + 1] & m1;
+                        for (int half = 0; half < 2; ++half) {
+#pragma unroll
+                            for (int x = 0; x < NT; ++x) load_tokens(kb[half][x], operand(b, which, x), (s + half) * 16, lane);
+                            as_columns(bb[half], kb[half], m0, m1);
                         }
-                        mma_terms<3>(acc, ya, q2);
-                        mma_terms<3>(acc, xa, k2);
+                        each_step<0, P::n>([&](auto k) {
+                            step2<P, k.value>(ds[2 * s], ds[2 * s + 1], which ? ya : xa, bb[0][0], bb[0][1]);
+                            step2<P, k.value>(ds[2 * s + 2], ds[2 * s + 3], which ? ya : xa, bb[1][0], bb[1][1]);
+                        });
                     }
                 }
             }
