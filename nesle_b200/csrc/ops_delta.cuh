@@ -82,16 +82,33 @@ __device__ __forceinline__ uint32_t pack(float lo, float hi) {
     asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// x, y as sums of N bf16 each, packed pairwise.
-template <int N>
+// Two fp32 in one instruction (fma.rn.f32x2): a * b + c.
+__device__ __forceinline__ void fma2(float& x, float& y, float a0, float a1, float b0, float b1) {
+    asm("{\n\t.reg .b64 A, B, C;\n\tmov.b64 A, {%2, %3};\n\tmov.b64 B, {%4, %5};\n\tmov.b64 C, {%0, %1};\n\t"
+        "fma.rn.f32x2 C, A, B, C;\n\tmov.b64 {%0, %1}, C;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(a0), "f"(a1), "f"(b0), "f"(b1));
+}
+__device__ __forceinline__ void mul2(float& x, float& y, float b) {
+    asm("{\n\t.reg .b64 B, C;\n\tmov.b64 B, {%2, %2};\n\tmov.b64 C, {%0, %1};\n\tmul.rn.f32x2 C, C, B;\n\tmov.b64 {%0, %1}, C;\n\t}"
+        : "+f"(x), "+f"(y)
+        : "f"(b));
+}
+
+// x, y as sums of N bf16 each, packed pairwise.  kPaired takes both remainders in one instruction, which saves two of
+// eleven and wants its registers in pairs: 2 to 4% of the forward pass's time, and 11% slower in the backward pass,
+// whose registers are full.
+template <bool kPaired = false, int N>
 __device__ __forceinline__ void split(float x, float y, uint32_t (&out)[N]) {
 #pragma unroll
     for (int i = 0; i < N; ++i) {
         out[i] = pack(x, y);
-        if (i + 1 < N) {
-            x -= __uint_as_float(out[i] << 16);
-            y -= __uint_as_float(out[i] & 0xFFFF0000u);
-        }
+        if (i + 1 == N) break;
+        const float hx = __uint_as_float(out[i] << 16), hy = __uint_as_float(out[i] & 0xFFFF0000u);
+        if constexpr (kPaired)
+            fma2(x, y, hx, hy, -1.f, -1.f);
+        else
+            x -= hx, y -= hy;
     }
 }
 
@@ -583,7 +600,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                     *reinterpret_cast<float2*>(&hs.b[i][j]) = make_float2(in0 && i > j ? d.x * be.x * kk[c].v[half * 2] : 0.f,
                                                                           in1 && i > j + 1 ? d.y * be.y * kk[c].v[half * 2 + 1] : 0.f);
                     uint32_t s[NO];
-                    split(in0 && i >= j ? d.x * qk[c].v[half * 2] : 0.f, in1 && i >= j + 1 ? d.y * qk[c].v[half * 2 + 1] : 0.f, s);
+                    split<true>(in0 && i >= j ? d.x * qk[c].v[half * 2] : 0.f, in1 && i >= j + 1 ? d.y * qk[c].v[half * 2 + 1] : 0.f, s);
 #pragma unroll
                     for (int x = 0; x < NO; ++x) *reinterpret_cast<uint32_t*>(&ch.att[x][i][j]) = s[x];
                 }
@@ -662,7 +679,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
             for (int z = 0; z < 4; ++z) {
                 uint32_t tmp[3];
                 const Acc& t = s[2 * st + z / 2];
-                split(t.v[z % 2 * 2], t.v[z % 2 * 2 + 1], tmp);
+                split<true>(t.v[z % 2 * 2], t.v[z % 2 * 2 + 1], tmp);
 #pragma unroll
                 for (int x = 0; x < 3; ++x) sa[x][z] = tmp[x];
             }
@@ -699,7 +716,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                         x1 = to_f32(tv[panel_at<T>(j + 1, v0 + row + half * 8)]);
                     }
                     uint32_t tmp[3];
-                    split(in0 ? fmaf(-ga.x, ks[c].v[half * 2], x0) : 0.f, in1 ? fmaf(-ga.y, ks[c].v[half * 2 + 1], x1) : 0.f, tmp);
+                    split<true>(in0 ? fmaf(-ga.x, ks[c].v[half * 2], x0) : 0.f, in1 ? fmaf(-ga.y, ks[c].v[half * 2 + 1], x1) : 0.f, tmp);
 #pragma unroll
                     for (int x = 0; x < 3; ++x) ra[x][c * 2 + half] = tmp[x];
                 }
@@ -733,8 +750,8 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t t2[NO], t3[3];
-                    split(be.x * e.v[half * 2], be.y * e.v[half * 2 + 1], t2);
-                    split(h0 * e.v[half * 2], h1 * e.v[half * 2 + 1], t3);
+                    split<true>(be.x * e.v[half * 2], be.y * e.v[half * 2 + 1], t2);
+                    split<true>(h0 * e.v[half * 2], h1 * e.v[half * 2 + 1], t3);
 #pragma unroll
                     for (int x = 0; x < NO; ++x) uo[x][c * 2 + half] = t2[x];
 #pragma unroll
@@ -775,9 +792,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
         const float keep = ch.keep;
         const uint32_t m0 = pair_mask(quad * 2, r0, r1), m1 = pair_mask(quad * 2 + 8, r0, r1);
 #pragma unroll
-        for (int i = 0; i < kTiles; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s[i].v[e] *= keep;
+        for (int i = 0; i < kTiles; ++i) mul2(s[i].v[0], s[i].v[1], keep), mul2(s[i].v[2], s[i].v[3], keep);
 #pragma unroll
         for (int st = 0; st < kSteps; st += 2) {
             uint32_t kb[2][NT][4], bb[2][2][NT][2];
