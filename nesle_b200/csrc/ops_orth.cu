@@ -14,7 +14,7 @@
 // 2^12 keeps both parts well inside fp16's range; it leaves as an exact power
 // of two.
 //
-// Each step is three launches over tiles of 128 x 128, A and P only on and
+// Each step is three launches over tiles of 128 rows, A and P only on and
 // above the diagonal (both are symmetric; a tile is written to both sides).
 // tcgen05 reads both operands K-major: X for X X^T, and its transpose for P X,
 // so the last product's epilogue writes both.
@@ -39,26 +39,35 @@ __device__ __forceinline__ void split(float v, __half& hi, __half& lo) {
 // ----------------------------------------------------- norm, scaling, layout
 
 constexpr int kNormThreads = 256;
+constexpr int kNormRuns = 8;  // loads in flight a thread
 
-// Partial sums of squares: block (i, b) takes every gridDim.x-th run of elements of matrix b.  In 64 bits: no update is
-// too small or too large to be squared, and the partials are added in a fixed order.
+// Partial sums of squares: block (i, b) takes every gridDim.x-th run of 2,048 elements of matrix b, row after row.  In 64
+// bits: no update is too small or too large to be squared, and the partials are added in a fixed order.
 template <class T>
 __global__ void __launch_bounds__(kNormThreads) square_sums_kernel(const T* __restrict__ x, int64_t stride_b, int64_t stride_r,
                                                                   int64_t stride_c, uint32_t rows, uint32_t cols,
                                                                   double* __restrict__ partial) {
+    grid_launch_next();
     const T* m = x + blockIdx.y * stride_b;
     double sum = 0;
-    // Along the denser dimension, so that a warp's loads lie together.
+    // Along the denser dimension, so that a warp's loads lie together; one long row where rows follow one another.
     const bool by_row = stride_c <= stride_r;
-    const uint32_t outer = by_row ? rows : cols, inner = by_row ? cols : rows;
     const int64_t so = by_row ? stride_r : stride_c, si = by_row ? stride_c : stride_r;
-    const uint32_t runs = (inner + kNormThreads - 1) / kNormThreads;
-    for (uint64_t i = blockIdx.x; i < static_cast<uint64_t>(outer) * runs; i += gridDim.x) {
-        const uint32_t o = static_cast<uint32_t>(i / runs), at = static_cast<uint32_t>(i % runs) * kNormThreads + threadIdx.x;
-        if (at < inner) {
-            const double v = to_f32(m[o * so + at * si]);
-            sum += v * v;
+    uint64_t outer = by_row ? rows : cols, inner = by_row ? cols : rows;
+    if (so == static_cast<int64_t>(inner) * si) inner *= outer, outer = 1;
+    constexpr uint32_t kRun = kNormThreads * kNormRuns;
+    const uint64_t runs = (inner + kRun - 1) / kRun;
+    for (uint64_t i = blockIdx.x; i < outer * runs; i += gridDim.x) {
+        const uint64_t o = outer == 1 ? 0 : i / runs, at = (outer == 1 ? i : i % runs) * kRun + threadIdx.x;
+        const T* from = m + static_cast<int64_t>(o) * so;
+        float v[kNormRuns];
+#pragma unroll
+        for (int k = 0; k < kNormRuns; ++k) {
+            const uint64_t e = at + k * kNormThreads;
+            v[k] = e < inner ? to_f32(from[static_cast<int64_t>(e) * si]) : 0.f;
         }
+#pragma unroll
+        for (int k = 0; k < kNormRuns; ++k) sum += static_cast<double>(v[k]) * v[k];
     }
     __shared__ double part[kNormThreads / 32];
 #pragma unroll
@@ -69,48 +78,64 @@ __global__ void __launch_bounds__(kNormThreads) square_sums_kernel(const T* __re
         for (int i = 1; i < kNormThreads / 32; ++i) sum += part[i];
         partial[blockIdx.y * gridDim.x + blockIdx.x] = sum;
     }
-    grid_launch_next();
 }
 
-// X = kScale M / (|M| + eps) as fp16 pairs, and its transpose, by tiles of 64 x 64 of X.  `planes` of a pair: high part,
-// then low part, each rows x ld.
+// X = kScale M / (|M| + eps) as fp16 pairs, and its transpose, by tiles of 64 x 64 of X: high part, then low part, each
+// rows x ld.
+constexpr int kMostPartials = 256;  // one a thread
+
 template <class T>
 __global__ void __launch_bounds__(256) scale_kernel(const T* __restrict__ x, int64_t stride_b, int64_t stride_r, int64_t stride_c,
                                                     uint32_t m, uint32_t n, const double* __restrict__ partial, uint32_t partials,
                                                     double eps, __half* __restrict__ out, uint32_t ld, __half* __restrict__ out_t,
                                                     uint32_t ld_t) {
     __shared__ float tile[64][65];
-    grid_wait();
+    __shared__ double part[8];
     grid_launch_next();
-    double sum = 0;
-    for (uint32_t i = 0; i < partials; ++i) sum += partial[blockIdx.z * partials + i];
-    const double factor = static_cast<double>(kScale) / (sqrt(sum) + eps);
     const T* mat = x + blockIdx.z * stride_b;
     const uint32_t r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
     const bool by_row = stride_c <= stride_r;
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const int r = by_row ? i / 64 : i % 64, c = by_row ? i % 64 : i / 64;
-        tile[r][c] = r0 + r < m && c0 + c < n
-                         ? static_cast<float>(to_f32(mat[(r0 + r) * stride_r + (c0 + c) * stride_c]) * factor)
-                         : 0.f;
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {  // the caller's matrix: nothing before this launch writes it
+        const int i = threadIdx.x + k * 256, r = by_row ? i / 64 : i % 64, c = by_row ? i % 64 : i / 64;
+        v[k] = r0 + r < m && c0 + c < n ? to_f32(mat[static_cast<int64_t>(r0 + r) * stride_r + static_cast<int64_t>(c0 + c) * stride_c]) : 0.f;
+    }
+    grid_wait();
+    double sum = threadIdx.x < partials ? partial[blockIdx.z * partials + threadIdx.x] : 0.0;
+#pragma unroll
+    for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
+    __syncthreads();
+    sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += part[i];
+    const double factor = static_cast<double>(kScale) / (sqrt(sum) + eps);
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+        const int i = threadIdx.x + k * 256, r = by_row ? i / 64 : i % 64, c = by_row ? i % 64 : i / 64;
+        tile[r][c] = static_cast<float>(v[k] * factor);
     }
     __syncthreads();
     __half* hi = out + static_cast<uint64_t>(blockIdx.z) * 2 * m * ld;
     __half* hi_t = out_t + static_cast<uint64_t>(blockIdx.z) * 2 * n * ld_t;
-    for (int i = threadIdx.x; i < 64 * 64; i += 256) {
-        const uint32_t a = i / 64, b = i % 64;
-        __half h, l;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
+        const uint32_t a = i / 32, b = i % 32 * 2;  // ld is a multiple of 8: a pair is inside or outside
+        __half2 h, l;
         if (r0 + a < m && c0 + b < ld) {
-            split(tile[a][b], h, l);
+            split(tile[a][b], h.x, l.x);
+            split(tile[a][b + 1], h.y, l.y);
             const uint64_t at = static_cast<uint64_t>(r0 + a) * ld + c0 + b;
-            hi[at] = h;
-            hi[static_cast<uint64_t>(m) * ld + at] = l;
+            *reinterpret_cast<__half2*>(hi + at) = h;
+            *reinterpret_cast<__half2*>(hi + static_cast<uint64_t>(m) * ld + at) = l;
         }
         if (c0 + a < n && r0 + b < ld_t) {
-            split(tile[b][a], h, l);
+            split(tile[b][a], h.x, l.x);
+            split(tile[b + 1][a], h.y, l.y);
             const uint64_t at = static_cast<uint64_t>(c0 + a) * ld_t + r0 + b;
-            hi_t[at] = h;
-            hi_t[static_cast<uint64_t>(n) * ld_t + at] = l;
+            *reinterpret_cast<__half2*>(hi_t + at) = h;
+            *reinterpret_cast<__half2*>(hi_t + static_cast<uint64_t>(n) * ld_t + at) = l;
         }
     }
 }
@@ -131,13 +156,18 @@ struct Job {
     int last_t;
 };
 
-constexpr int kTile = 128, kSlice = 64, kStages = 3;
-constexpr int kOperand = kTile * kSlice * 2;   // one fp16 part of one operand: 16 KB
-constexpr int kStageBytes = 4 * kOperand;      // A high, A low, B high, B low
-constexpr int kRow = kTile + 4;                // floats of a row of partial sums in shared memory
+constexpr int kTile = 128, kSlice = 64;  // rows of a tile, k of a stage
 constexpr int kThreads = 256;
-constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
-static_assert(kTile * kRow * 4 <= kStages * kStageBytes, "partial sums take the place of the operands");
+
+template <int kBN>  // columns of a tile
+struct Shape {
+    static constexpr int kStages = kBN == 128 ? 3 : 4;
+    static constexpr int kA = kTile * kSlice * 2, kB = kBN * kSlice * 2;  // one fp16 part of an operand
+    static constexpr int kStageBytes = 2 * (kA + kB);                     // A high, A low, B high, B low
+    static constexpr int kRow = kBN + 4;                                  // floats of a row of partial sums
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
+    static_assert(kTile * kRow * 4 <= kStages * kStageBytes, "partial sums take the place of the operands");
+};
 
 __device__ __forceinline__ uint32_t cluster_rank() {
     uint32_t r;
@@ -155,23 +185,23 @@ __device__ __forceinline__ float4 peer_load(const float* p, uint32_t rank) {
     return v;
 }
 
-union Half4 {
-    __half h[4];
-    uint2 u;
-};
 union Half8 {
     __half h[8];
     uint4 u;
 };
 
-// One 128 x 128 tile by a cluster of kSplit blocks, each over its share of k; their fp32 partial sums meet in shared
-// memory, block r adding rows r * 128 / kSplit and on, over the ranks in order.
-template <int kProduct, int kSplit>
+// One tile by a cluster of kSplit blocks, each over its share of k; their fp32 partial sums meet in shared memory, block
+// r adding columns r kBN / kSplit and on, over the ranks in order.  In the epilogue a thread has one row and runs of 8
+// columns: its row's stores are 16 bytes, and of a column a warp stores 32 neighbouring rows.
+template <int kProduct, int kBN, int kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, Job job, unsigned int* stalls) {
+    using S = Shape<kBN>;
+    constexpr int kStages = S::kStages;
+    constexpr bool kSymmetric = kProduct == kGram || kProduct == kPoly;
     extern __shared__ uint8_t raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(base + kStages * kStageBytes);
+    uint64_t* full = reinterpret_cast<uint64_t*>(base + kStages * S::kStageBytes);
     uint64_t* empty = full + kStages;
     uint64_t* done = empty + kStages;
     uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
@@ -182,10 +212,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint32_t ti, tj;
     {
         uint32_t t = blockIdx.x / kSplit;
-        if constexpr (kProduct == kGram || kProduct == kPoly) {  // row ti holds the tiles ti..tiles_n-1
+        if constexpr (kSymmetric) {  // row ti holds the tiles from its diagonal block on
             ti = 0;
-            for (uint32_t row = job.tiles_n; t >= row; --row, ++ti) t -= row;
-            tj = ti + t;
+            for (uint32_t left = job.tiles_n; t >= left; left -= kTile / kBN, ++ti) t -= left;
+            tj = ti * (kTile / kBN) + t;
         } else {
             ti = t % job.tiles_m;  // neighbours share X's columns
             tj = t / job.tiles_m;
@@ -204,13 +234,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::prefetch_map(&map_a);
         tc::prefetch_map(&map_b);
     }
-    if (warp == 1) tc::tmem_alloc(slot, kTile);
+    if (warp == 1) tc::tmem_alloc(slot, kBN);
     tc::fence_before();
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = *slot;
-    grid_wait();  // what the launches before this one wrote
     grid_launch_next();
+    grid_wait();  // what the launches before this one wrote
     bool ok = true;
 
     if (warp == 0 && tc::elect_one()) {
@@ -218,25 +248,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t s = first; s < last; ++s, ++it) {
             const uint32_t i = it % kStages;
             if (!(ok = tc::mbar_wait(&empty[i], (it / kStages & 1) ^ 1))) break;
-            uint8_t* st = base + i * kStageBytes;
-            tc::mbar_expect_tx(&full[i], kStageBytes);
+            uint8_t* st = base + i * S::kStageBytes;
+            tc::mbar_expect_tx(&full[i], S::kStageBytes);
             tc::tma_load_3d(st, &map_a, &full[i], s * kSlice, ti * kTile, batch * 2);
-            tc::tma_load_3d(st + kOperand, &map_a, &full[i], s * kSlice, ti * kTile, batch * 2 + 1);
-            tc::tma_load_3d(st + 2 * kOperand, &map_b, &full[i], s * kSlice, tj * kTile, batch * 2);
-            tc::tma_load_3d(st + 3 * kOperand, &map_b, &full[i], s * kSlice, tj * kTile, batch * 2 + 1);
+            tc::tma_load_3d(st + 2 * S::kA, &map_b, &full[i], s * kSlice, tj * kBN, batch * 2);
+            tc::tma_load_3d(st + S::kA, &map_a, &full[i], s * kSlice, ti * kTile, batch * 2 + 1);
+            tc::tma_load_3d(st + 2 * S::kA + S::kB, &map_b, &full[i], s * kSlice, tj * kBN, batch * 2 + 1);
         }
         for (uint32_t s = it < kStages ? 0 : it - kStages; s < it; ++s)  // a load in flight lands before the block goes on
             ok = tc::mbar_wait(&full[s % kStages], s / kStages & 1) && ok;
     } else if (warp == 1 && tc::elect_one()) {
-        constexpr uint32_t idesc = tc::idesc_f16(kTile);
+        constexpr uint32_t idesc = tc::idesc_f16(kBN);
         uint32_t it = 0;
         for (uint32_t s = first; s < last; ++s, ++it) {
             const uint32_t i = it % kStages;
             if (!(ok = tc::mbar_wait(&full[i], it / kStages & 1))) break;
             tc::fence_after();
-            const uint8_t* st = base + i * kStageBytes;
-            const uint64_t ah = tc::tile_desc(st), al = tc::tile_desc(st + kOperand), bh = tc::tile_desc(st + 2 * kOperand),
-                           bl = tc::tile_desc(st + 3 * kOperand);
+            const uint8_t* st = base + i * S::kStageBytes;
+            const uint64_t ah = tc::tile_desc(st), al = tc::tile_desc(st + S::kA), bh = tc::tile_desc(st + 2 * S::kA),
+                           bl = tc::tile_desc(st + 2 * S::kA + S::kB);
 #pragma unroll
             for (int kk = 0; kk < kSlice / 16; ++kk) {
                 tc::mma_f16(tmem, al + 2 * kk, bh + 2 * kk, idesc, it > 0 || kk > 0);
@@ -250,122 +280,114 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncwarp();
     ok = tc::mbar_wait_warp(done, 0) && ok;
     tc::fence_after();
-    __syncthreads();  // nobody reads the operands any more
-    {
-        // warp w reads lanes (w % 4) * 32 and on, columns (w / 4) * 64 and on
-        const int r = (warp % 4) * 32 + lane;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int c = (warp / 4) * 64 + h * 32;
-            uint32_t v[32];
-            tc::tmem_ld32(tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16) + c, v);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                *reinterpret_cast<uint4*>(sums + r * kRow + c + 4 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-        }
-    }
-    tc::fence_before();
-    if constexpr (kSplit > 1)
-        cluster_sync();
-    else
-        __syncthreads();
-    tc::fence_after();
-    if (warp == 1) tc::tmem_free(tmem, kTile);
 
-    constexpr int kRows = kTile / kSplit;
-    const int row0 = rank * kRows;
-    const uint64_t plane = static_cast<uint64_t>(job.m) * job.ld;
-    __half* out = job.out + batch * 2 * plane;
-#pragma unroll 4
-    for (int e = threadIdx.x; e < kRows * (kTile / 4); e += kThreads) {
-        const int r = row0 + e / (kTile / 4), c = e % (kTile / 4) * 4;
-        float* mine = sums + r * kRow + c;
-        float4 v;
-        if constexpr (kSplit > 1) {
-            v = peer_load(mine, 0);
-#pragma unroll
-            for (int p = 1; p < kSplit; ++p) {
-                const float4 w = peer_load(mine, p);
-                v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
-            }
-        } else {
-            v = *reinterpret_cast<const float4*>(mine);
-        }
-        const uint32_t i = ti * kTile + r, j = tj * kTile + c;
-        float f[4] = {v.x, v.y, v.z, v.w};
-        const bool inside = i < job.m && j < job.n;
+    // This thread's row, and its columns: of its half of the tile, the rank's share.
+    const int r = (warp % 4) * 32 + lane, half = warp / 4;
+    constexpr int kHalf = kBN / 2, kMine = kHalf / kSplit;
+    const uint32_t i = ti * kTile + r;
+    const uint32_t at_tmem = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16) + half * kHalf;
+    const uint64_t plane = static_cast<uint64_t>(job.m) * job.ld, plane_t = static_cast<uint64_t>(job.n) * job.ld_t;
+    const bool mirror = kProduct == kLast ? job.last_t : kProduct == kApply || (tj * kBN) / kTile != ti;
+
+    auto emit = [&](int c, const float (&acc)[8]) {  // columns c..c+7 of the tile
+        const uint32_t j = tj * kBN + c;
+        if (i >= job.m || j >= job.n) return;
+        float f[8];
         const uint64_t at = static_cast<uint64_t>(i) * job.ld + j;
         if constexpr (kProduct == kPoly) {
-            Half4 gh, gl;
-            gh.u = gl.u = make_uint2(0, 0);
-            if (inside) {
-                const __half* g = job.gram + batch * 2 * plane;
-                gh.u = *reinterpret_cast<const uint2*>(g + at);
-                gl.u = *reinterpret_cast<const uint2*>(g + plane + at);
-            }
+            const __half* g = job.gram + batch * 2 * plane + at;
+            Half8 gh, gl;
+            gh.u = *reinterpret_cast<const uint4*>(g);
+            gl.u = *reinterpret_cast<const uint4*>(g + plane);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                f[q] = fmaf(kB, __half2float(gh.h[q]) + __half2float(gl.h[q]),
-                            fmaf(kC / kScale, f[q], i == j + q ? kA * kScale : 0.f));
-        } else if constexpr (kProduct == kLast) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q) f[q] *= 1.f / (kScale * kScale);
+            for (int q = 0; q < 8; ++q)
+                f[q] = fmaf(kB, __half2float(gh.h[q]) + __half2float(gl.h[q]), fmaf(kC / kScale, acc[q], i == j + q ? kA * kScale : 0.f));
         } else {
+            constexpr float kBack = kProduct == kLast ? 1.f / (kScale * kScale) : 1.f / kScale;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) f[q] *= 1.f / kScale;
+            for (int q = 0; q < 8; ++q) f[q] = acc[q] * kBack;
         }
         if constexpr (kProduct == kLast) {
-            if (!job.last_t && inside) {
-                __nv_bfloat16* o = job.last + (static_cast<uint64_t>(batch) * job.m + i) * job.n + j;
-                if (job.n % 4 == 0) {
-                    union { __nv_bfloat16 h[4]; uint2 u; } b;
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) b.h[q] = __float2bfloat16_rn(f[q]);
-                    *reinterpret_cast<uint2*>(o) = b.u;
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 4; ++q)
-                        if (j + q < job.n) o[q] = __float2bfloat16_rn(f[q]);
-                }
-            }
-        } else if (inside) {
-            Half4 h, l;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) split(f[q], h.h[q], l.h[q]);
-            *reinterpret_cast<uint2*>(out + at) = h.u;
-            *reinterpret_cast<uint2*>(out + plane + at) = l.u;
-        }
-        *reinterpret_cast<float4*>(mine) = make_float4(f[0], f[1], f[2], f[3]);  // only this block reads its rows
-    }
-    __syncthreads();
-    // The transpose: a thread takes one column's run of 8 rows, neighbours take neighbouring columns.
-    if (kProduct == kLast ? job.last_t : (kProduct == kApply || ti != tj)) {
-        for (int e = threadIdx.x; e < kTile * (kRows / 8); e += kThreads) {
-            const int c = e % kTile, r = row0 + e / kTile * 8;
-            const uint32_t j = tj * kTile + c, i = ti * kTile + r;
-            if (j >= job.n || i >= job.m) continue;
-            if constexpr (kProduct == kLast) {
+            if (job.last_t) {
                 __nv_bfloat16* o = job.last + (static_cast<uint64_t>(batch) * job.n + j) * job.m + i;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (j + q < job.n) o[static_cast<uint64_t>(q) * job.m] = __float2bfloat16_rn(f[q]);
+            } else {
+                __nv_bfloat16* o = job.last + (static_cast<uint64_t>(batch) * job.m + i) * job.n + j;
                 union { __nv_bfloat16 h[8]; uint4 u; } b;
 #pragma unroll
-                for (int q = 0; q < 8; ++q) b.h[q] = __float2bfloat16_rn(sums[(r + q) * kRow + c]);
-                if (job.m % 8 == 0) {
+                for (int q = 0; q < 8; ++q) b.h[q] = __float2bfloat16_rn(f[q]);
+                if (job.n % 8 == 0) {
                     *reinterpret_cast<uint4*>(o) = b.u;
                 } else {
 #pragma unroll
                     for (int q = 0; q < 8; ++q)
-                        if (i + q < job.m) o[q] = b.h[q];
+                        if (j + q < job.n) o[q] = b.h[q];
                 }
-            } else {
-                const uint64_t plane_t = static_cast<uint64_t>(job.n) * job.ld_t, at = static_cast<uint64_t>(j) * job.ld_t + i;
-                __half* o = job.out_t + batch * 2 * plane_t;
-                Half8 h, l;
-#pragma unroll
-                for (int q = 0; q < 8; ++q) split(sums[(r + q) * kRow + c], h.h[q], l.h[q]);
-                *reinterpret_cast<uint4*>(o + at) = h.u;
-                *reinterpret_cast<uint4*>(o + plane_t + at) = l.u;
             }
+        } else {
+            Half8 h, l;
+#pragma unroll
+            for (int q = 0; q < 8; ++q) split(f[q], h.h[q], l.h[q]);
+            __half* o = job.out + batch * 2 * plane + at;
+            *reinterpret_cast<uint4*>(o) = h.u;
+            *reinterpret_cast<uint4*>(o + plane) = l.u;
+            if (mirror) {
+                __half* t = job.out_t + batch * 2 * plane_t + static_cast<uint64_t>(j) * job.ld_t + i;
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (j + q < job.n) {
+                        t[static_cast<uint64_t>(q) * job.ld_t] = h.h[q];
+                        t[plane_t + static_cast<uint64_t>(q) * job.ld_t] = l.h[q];
+                    }
+            }
+        }
+    };
+    if constexpr (kSplit == 1) {
+#pragma unroll
+        for (int c = 0; c < kHalf; c += 32) {
+            uint32_t v[32];
+            tc::tmem_ld32(at_tmem + c, v);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int q = 0; q < 32; q += 8) {
+                float acc[8];
+#pragma unroll
+                for (int x = 0; x < 8; ++x) acc[x] = __uint_as_float(v[q + x]);
+                emit(half * kHalf + c + q, acc);
+            }
+        }
+        tc::fence_before();
+        __syncthreads();
+        tc::fence_after();
+        if (warp == 1) tc::tmem_free(tmem, kBN);
+    } else {
+        __syncthreads();  // nobody reads the operands any more
+#pragma unroll
+        for (int c = 0; c < kHalf; c += 32) {
+            uint32_t v[32];
+            tc::tmem_ld32(at_tmem + c, v);
+            tc::tmem_wait_ld();
+#pragma unroll
+            for (int x = 0; x < 32; x += 4)
+                *reinterpret_cast<uint4*>(sums + r * S::kRow + half * kHalf + c + x) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+        }
+        tc::fence_before();
+        cluster_sync();
+        tc::fence_after();
+        if (warp == 1) tc::tmem_free(tmem, kBN);
+#pragma unroll
+        for (int c = 0; c < kMine; c += 8) {
+            const int col = half * kHalf + rank * kMine + c;
+            float acc[8] = {};
+#pragma unroll
+            for (int p = 0; p < kSplit; ++p) {
+                const float4 x = peer_load(sums + r * S::kRow + col, p), y = peer_load(sums + r * S::kRow + col + 4, p);
+                acc[0] += x.x, acc[1] += x.y, acc[2] += x.z, acc[3] += x.w;
+                acc[4] += y.x, acc[5] += y.y, acc[6] += y.z, acc[7] += y.w;
+            }
+            emit(col, acc);
         }
     }
     if (!ok) atomicAdd(stalls, 1u);
@@ -376,7 +398,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 uint32_t up8(uint32_t v) { return (v + 7) / 8 * 8; }
 uint64_t up256(uint64_t v) { return (v + 255) / 256 * 256; }
-constexpr uint32_t kNormBlocks = 64;
+constexpr uint32_t kNormBlocks = kMostPartials;
+
+uint32_t norm_blocks(uint64_t elements) {  // one run each while that is fewer
+    const uint64_t runs = (elements + kNormThreads * kNormRuns - 1) / (kNormThreads * kNormRuns);
+    return static_cast<uint32_t>(runs < kNormBlocks ? runs : kNormBlocks);
+}
 
 struct Layout {  // byte offsets of the workspace's parts
     uint32_t m, n, ld_n, ld_m;
@@ -398,21 +425,21 @@ struct Layout {  // byte offsets of the workspace's parts
     }
 };
 
-int map_pair(CUtensorMap* map, const void* p, uint32_t rows, uint32_t cols, uint32_t ld, uint64_t batch) {
+int map_pair(CUtensorMap* map, const void* p, uint32_t rows, uint32_t cols, uint32_t ld, uint64_t batch, uint32_t box_rows) {
     const uint64_t dims[3] = {cols, rows, batch * 2}, strides[2] = {ld * 2ull, static_cast<uint64_t>(rows) * ld * 2};
-    const uint32_t box[3] = {kSlice, kTile, 1};
+    const uint32_t box[3] = {kSlice, box_rows, 1};
     return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p, dims, strides, box);
 }
 
-template <int kProduct, int kSplit>
+template <int kProduct, int kBN, int kSplit>
 int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const Job& job, uint32_t tiles, uint32_t batch, unsigned int* stalls,
                    cudaStream_t st) {
-    auto* kernel = product_kernel<kProduct, kSplit>;
-    if (int rc = cuda_status(allow_smem(kernel, kSmem), "orthogonalize")) return rc;
+    auto* kernel = product_kernel<kProduct, kBN, kSplit>;
+    if (int rc = cuda_status(allow_smem(kernel, Shape<kBN>::kSmem), "orthogonalize")) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(tiles * kSplit, batch);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = kSmem;
+    cfg.dynamicSmemBytes = Shape<kBN>::kSmem;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -425,29 +452,47 @@ int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const Job& job,
     return cuda_status(cudaLaunchKernelEx(&cfg, kernel, ma, mb, job, stalls), "orthogonalize");
 }
 
-// k is split over a cluster while that leaves every block two slices and all blocks run at once.
-template <int kProduct>
-int launch_split(const CUtensorMap& ma, const CUtensorMap& mb, Job job, uint32_t batch, int sms, unsigned int* stalls, cudaStream_t st) {
-    job.tiles_m = (job.m + kTile - 1) / kTile;
-    job.tiles_n = (job.n + kTile - 1) / kTile;
-    const bool symmetric = kProduct == kGram || kProduct == kPoly;
-    const uint32_t tiles = symmetric ? job.tiles_n * (job.tiles_n + 1) / 2 : job.tiles_m * job.tiles_n;
-    const uint32_t slices = (job.k + kSlice - 1) / kSlice;
-    uint32_t s = 8;
-    while (s > 1 && (static_cast<uint64_t>(tiles) * batch * s > static_cast<uint32_t>(sms) || slices < 2 * s)) s /= 2;
-    switch (s) {
-        case 8: return launch_product<kProduct, 8>(ma, mb, job, tiles, batch, stalls, st);
-        case 4: return launch_product<kProduct, 4>(ma, mb, job, tiles, batch, stalls, st);
-        case 2: return launch_product<kProduct, 2>(ma, mb, job, tiles, batch, stalls, st);
-        default: return launch_product<kProduct, 1>(ma, mb, job, tiles, batch, stalls, st);
+struct Operand {  // a stored pair as either side of a product
+    CUtensorMap rows128, rows64;
+    int encode(const void* p, uint32_t rows, uint32_t cols, uint32_t ld, uint64_t batch) {
+        if (int rc = map_pair(&rows128, p, rows, cols, ld, batch, 128)) return rc;
+        return map_pair(&rows64, p, rows, cols, ld, batch, 64);
     }
+};
+
+uint32_t count_tiles(bool symmetric, Job& job, uint32_t bn) {
+    job.tiles_m = (job.m + kTile - 1) / kTile;
+    job.tiles_n = (job.n + bn - 1) / bn;
+    if (!symmetric) return job.tiles_m * job.tiles_n;
+    uint32_t tiles = 0;
+    for (uint32_t i = 0; i < job.tiles_m; ++i) tiles += job.tiles_n - i * (kTile / bn);
+    return tiles;
+}
+
+// Narrow tiles, and k split over a cluster (while every block has two slices), as long as all blocks run at once; wide
+// tiles, which read their operands less often, where there are more than that.
+template <int kProduct>
+int launch_sized(const Operand& a, const Operand& b, Job job, uint32_t batch, int sms, unsigned int* stalls, cudaStream_t st) {
+    const bool symmetric = kProduct == kGram || kProduct == kPoly;
+    const uint64_t narrow = static_cast<uint64_t>(count_tiles(symmetric, job, 64)) * batch;
+    if (narrow > static_cast<uint32_t>(sms)) {
+        const uint32_t tiles = count_tiles(symmetric, job, 128);
+        return launch_product<kProduct, 128, 1>(a.rows128, b.rows128, job, tiles, batch, stalls, st);
+    }
+    const uint32_t tiles = static_cast<uint32_t>(narrow / batch), slices = (job.k + kSlice - 1) / kSlice;
+    if (narrow * 4 <= static_cast<uint32_t>(sms) && slices >= 8)
+        return launch_product<kProduct, 64, 4>(a.rows128, b.rows64, job, tiles, batch, stalls, st);
+    if (narrow * 2 <= static_cast<uint32_t>(sms) && slices >= 4)
+        return launch_product<kProduct, 64, 2>(a.rows128, b.rows64, job, tiles, batch, stalls, st);
+    return launch_product<kProduct, 64, 1>(a.rows128, b.rows64, job, tiles, batch, stalls, st);
 }
 
 template <class T>
 int launch_scaling(const nesle_orth_args& a, const Layout& lay, uint8_t* ws, int64_t sr, int64_t sc, cudaStream_t st) {
     const T* x = static_cast<const T*>(a.x);
     double* partial = reinterpret_cast<double*>(ws + lay.partial);
-    square_sums_kernel<T><<<dim3(kNormBlocks, static_cast<unsigned>(a.batch)), kNormThreads, 0, st>>>(x, a.stride_b, sr, sc, lay.m, lay.n, partial);
+    const uint32_t partials = norm_blocks(static_cast<uint64_t>(lay.m) * lay.n);
+    square_sums_kernel<T><<<dim3(partials, static_cast<unsigned>(a.batch)), kNormThreads, 0, st>>>(x, a.stride_b, sr, sc, lay.m, lay.n, partial);
     if (int rc = cuda_status(cudaGetLastError(), "orthogonalize")) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((lay.n + 63) / 64, (lay.m + 63) / 64, static_cast<unsigned>(a.batch));
@@ -459,7 +504,7 @@ int launch_scaling(const nesle_orth_args& a, const Layout& lay, uint8_t* ws, int
     cfg.attrs = at;
     cfg.numAttrs = 1;
     return cuda_status(cudaLaunchKernelEx(&cfg, scale_kernel<T>, x, a.stride_b, sr, sc, lay.m, lay.n, static_cast<const double*>(partial),
-                                          kNormBlocks, a.eps, reinterpret_cast<__half*>(ws + lay.x[0]), lay.ld_n,
+                                          partials, a.eps, reinterpret_cast<__half*>(ws + lay.x[0]), lay.ld_n,
                                           reinterpret_cast<__half*>(ws + lay.xt[0]), lay.ld_m),
                        "orthogonalize");
 }
@@ -481,25 +526,25 @@ int run(const nesle_orth_args& a, cudaStream_t st) {
     if ((rc = stall_counter(a.device, &stalls))) return rc;
     const int sms = sm_count(a.device);
     __half *gram = reinterpret_cast<__half*>(ws + lay.gram), *poly = reinterpret_cast<__half*>(ws + lay.poly);
-    CUtensorMap map_x[2], map_xt[2], map_g, map_p;
+    Operand op_x[2], op_xt[2], op_g, op_p;
     for (int i = 0; i < 2; ++i) {
-        if ((rc = map_pair(&map_x[i], ws + lay.x[i], m, n, lay.ld_n, batch))) return rc;
-        if ((rc = map_pair(&map_xt[i], ws + lay.xt[i], n, m, lay.ld_m, batch))) return rc;
+        if ((rc = op_x[i].encode(ws + lay.x[i], m, n, lay.ld_n, batch))) return rc;
+        if ((rc = op_xt[i].encode(ws + lay.xt[i], n, m, lay.ld_m, batch))) return rc;
     }
-    if ((rc = map_pair(&map_g, gram, m, m, lay.ld_m, batch))) return rc;
-    if ((rc = map_pair(&map_p, poly, m, m, lay.ld_m, batch))) return rc;
+    if ((rc = op_g.encode(gram, m, m, lay.ld_m, batch))) return rc;
+    if ((rc = op_p.encode(poly, m, m, lay.ld_m, batch))) return rc;
     for (int step = 0; step < a.steps; ++step) {
         const int from = step & 1, to = from ^ 1;
         Job g{};
         g.m = g.n = m, g.k = n;
         g.out = g.out_t = gram;
         g.ld = g.ld_t = lay.ld_m;
-        if ((rc = launch_split<kGram>(map_x[from], map_x[from], g, batch, sms, stalls, st))) return rc;
+        if ((rc = launch_sized<kGram>(op_x[from], op_x[from], g, batch, sms, stalls, st))) return rc;
         Job p = g;
         p.k = m;
         p.gram = gram;
         p.out = p.out_t = poly;
-        if ((rc = launch_split<kPoly>(map_g, map_g, p, batch, sms, stalls, st))) return rc;
+        if ((rc = launch_sized<kPoly>(op_g, op_g, p, batch, sms, stalls, st))) return rc;
         Job x{};
         x.m = m, x.n = n, x.k = m;
         x.out = reinterpret_cast<__half*>(ws + lay.x[to]);
@@ -508,8 +553,8 @@ int run(const nesle_orth_args& a, cudaStream_t st) {
         x.ld_t = lay.ld_m;
         x.last = static_cast<__nv_bfloat16*>(a.out);
         x.last_t = tall;
-        rc = step + 1 < a.steps ? launch_split<kApply>(map_p, map_xt[from], x, batch, sms, stalls, st)
-                                : launch_split<kLast>(map_p, map_xt[from], x, batch, sms, stalls, st);
+        rc = step + 1 < a.steps ? launch_sized<kApply>(op_p, op_xt[from], x, batch, sms, stalls, st)
+                                : launch_sized<kLast>(op_p, op_xt[from], x, batch, sms, stalls, st);
         if (rc) return rc;
     }
     return NESLE_OK;

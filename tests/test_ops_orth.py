@@ -9,6 +9,8 @@ later step multiplies what is there by at most a = 3.4445 (the derivative of
 the quintic on [0, 1.21]).  Then one rounding to bf16."""
 from __future__ import annotations
 
+import threading
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -154,3 +156,16 @@ def test_empty_and_refusals():
     ):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.gpu
+def test_in_a_thread_that_has_made_no_cuda_call():
+    x = momentum(130, 260, seed=11)
+    want = ops.orthogonalize(x)
+    out = torch.empty_like(want)
+    torch.cuda.synchronize()
+    thread = threading.Thread(target=lambda: ops.orthogonalize(x, out=out))
+    thread.start()
+    thread.join()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
