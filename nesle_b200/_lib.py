@@ -6,6 +6,7 @@ by ``python -m nesle_b200.build`` (``__graft_entry__.build()``).
 from __future__ import annotations
 
 import ctypes
+import struct
 from pathlib import Path
 
 import numpy as np
@@ -56,43 +57,12 @@ class FcsState(ctypes.Structure):
                 ("oam", ctypes.c_uint8 * 256)]
 
 
-class Int8Args(ctypes.Structure):
-    _fields_ = [("x", ctypes.c_void_p), ("x_unsigned", ctypes.c_int), ("ld_x", ctypes.c_int64),
-                ("x_scale", ctypes.c_void_p), ("x_scale_value", ctypes.c_float), ("w", ctypes.c_void_p),
-                ("w_biased", ctypes.c_void_p), ("ld_w", ctypes.c_int64), ("w_scale", ctypes.c_void_p),
-                ("bias", ctypes.c_void_p), ("y", ctypes.c_void_p), ("y_dtype", ctypes.c_int), ("ld_y", ctypes.c_int64),
-                ("m", ctypes.c_uint64), ("k", ctypes.c_uint64), ("n", ctypes.c_uint64), ("relu", ctypes.c_int),
-                ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64), ("device", ctypes.c_int)]
-
-
-class OrthArgs(ctypes.Structure):
-    _fields_ = [("x", ctypes.c_void_p), ("dtype", ctypes.c_int), ("stride_b", ctypes.c_int64),
-                ("stride_r", ctypes.c_int64), ("stride_c", ctypes.c_int64), ("batch", ctypes.c_uint64),
-                ("rows", ctypes.c_uint64), ("cols", ctypes.c_uint64), ("steps", ctypes.c_int), ("eps", ctypes.c_double),
-                ("out", ctypes.c_void_p), ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_uint64),
-                ("device", ctypes.c_int)]
-
-
-_void, _i64, _u64 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_uint64
-
-
-class DeltaStepArgs(ctypes.Structure):
-    _fields_ = [*((x, _void) for x in ("q", "k", "v")), *((x, _i64) for x in ("q_n", "q_h", "k_n", "k_h", "v_n", "v_h")),
-                ("dtype", ctypes.c_int), ("g", _void), ("beta", _void),
-                *((x, _i64) for x in ("g_n", "g_h", "beta_n", "beta_h")), ("reset", _void), ("reset_n", _i64),
-                ("state", _void), ("state_n", _i64), ("state_h", _i64), ("o", _void),
-                *((x, _u64) for x in ("n", "h", "dk", "dv")), ("scale", ctypes.c_float), ("device", ctypes.c_int)]
-
-
-class DeltaArgs(ctypes.Structure):
-    _fields_ = [*((x, _void) for x in ("q", "k", "v")),
-                *((x, _i64) for x in ("q_t", "q_n", "q_h", "k_t", "k_n", "k_h", "v_t", "v_n", "v_h")),
-                ("dtype", ctypes.c_int), ("g", _void), ("beta", _void),
-                *((x, _i64) for x in ("g_t", "g_n", "g_h", "beta_t", "beta_n", "beta_h")), ("reset", _void),
-                ("reset_t", _i64), ("reset_n", _i64), ("state", _void),
-                *((x, _u64) for x in ("t", "n", "h", "dk", "dv")), ("scale", ctypes.c_float),
-                *((x, _void) for x in ("o", "final_state", "errors", "checkpoints", "d_o", "d_final", "dq", "d_k", "d_v",
-                                       "dg", "dbeta", "dstate")), ("device", ctypes.c_int)]
+# Argument blocks of include/nesle_ops.h, packed by the struct module in C layout ("@": native sizes and alignment): a
+# third of the time of building a ctypes.Structure, and these calls are short.  One letter a member, in order.
+INT8_ARGS = struct.Struct("@PiqPfPPqPPPiqQQQiPQi")
+ORTH_ARGS = struct.Struct("@PiqqqQQQidPPQi")
+DELTA_STEP_ARGS = struct.Struct("@PPPqqqqqqiPPqqqqPqPqqPQQQQfi")
+DELTA_ARGS = struct.Struct("@PPPqqqqqqqqqiPPqqqqqqPqqPQQQQQf" + "P" * 12 + "i")
 
 
 # Exported symbols and their ctypes signatures (every function include/*.h declares).
@@ -132,15 +102,15 @@ SIGNATURES = {
     "nesle_quantize_rows": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64, ctypes.c_uint64,
                                            ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p,
                                            ctypes.c_int, ctypes.c_void_p]),
-    "nesle_int8_linear": (ctypes.c_int, [ctypes.POINTER(Int8Args), ctypes.c_void_p]),
-    "nesle_int8_workspace": (ctypes.c_uint64, [ctypes.POINTER(Int8Args)]),
-    "nesle_delta_step": (ctypes.c_int, [ctypes.POINTER(DeltaStepArgs), ctypes.c_void_p]),
-    "nesle_delta_scan": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), ctypes.c_void_p]),
-    "nesle_delta_scan_backward": (ctypes.c_int, [ctypes.POINTER(DeltaArgs), ctypes.c_void_p]),
-    "nesle_delta_error_floats": (ctypes.c_uint64, [ctypes.POINTER(DeltaArgs)]),
-    "nesle_delta_checkpoint_floats": (ctypes.c_uint64, [ctypes.POINTER(DeltaArgs)]),
-    "nesle_orthogonalize": (ctypes.c_int, [ctypes.POINTER(OrthArgs), ctypes.c_void_p]),
-    "nesle_orth_workspace": (ctypes.c_uint64, [ctypes.POINTER(OrthArgs)]),
+    "nesle_int8_linear": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "nesle_int8_workspace": (ctypes.c_uint64, [ctypes.c_void_p]),
+    "nesle_delta_step": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "nesle_delta_scan": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "nesle_delta_scan_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "nesle_delta_error_floats": (ctypes.c_uint64, [ctypes.c_void_p]),
+    "nesle_delta_checkpoint_floats": (ctypes.c_uint64, [ctypes.c_void_p]),
+    "nesle_orthogonalize": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "nesle_orth_workspace": (ctypes.c_uint64, [ctypes.c_void_p]),
 }
 
 # EnvRecord (csrc/nesle_state.h), the first 128 bytes of a saved state blob.

@@ -7,6 +7,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <exception>
 #include <string>
 
@@ -61,10 +62,16 @@ int stall_counter(int device, unsigned int** out);
 int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
                const uint64_t* strides, const uint32_t* box);
 
-// Allows a kernel its dynamic shared memory (an attribute of the function on the current device).
-template <class K>
-cudaError_t allow_smem(K* kernel, int bytes) {
-    return cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+// Allows a kernel its dynamic shared memory on the current device, `device`: once for each.
+template <auto* kKernel>
+int allow_smem(int bytes, int device, const char* where) {
+    static std::atomic<uint64_t> done{0};
+    const uint64_t bit = device >= 0 && device < 64 ? uint64_t(1) << device : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return NESLE_OK;
+    const int rc = cuda_status(
+        cudaFuncSetAttribute(reinterpret_cast<const void*>(kKernel), cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), where);
+    if (!rc) done.fetch_or(bit, std::memory_order_relaxed);
+    return rc;
 }
 
 template <class T>

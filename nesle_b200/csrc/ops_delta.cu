@@ -176,6 +176,7 @@ Scan to_scan(const nesle_delta_args& a, bool backward) {
     p.o = a.o, p.final_state = a.final_state, p.errors = a.errors, p.checkpoints = a.checkpoints;
     p.d_o = a.d_o, p.d_final = a.d_final, p.dq = a.dq, p.dk_out = a.d_k, p.dv_out = a.d_v, p.dg = a.dg, p.dbeta = a.dbeta;
     p.dstate = a.dstate;
+    p.device = a.device;
     return p;
 }
 

@@ -66,6 +66,7 @@ struct Scan {
     void *dq, *dk_out, *dv_out;
     float *dg, *dbeta, *dstate;
     unsigned int* stalls;
+    int device;
 };
 
 template <class T>
@@ -1562,8 +1563,8 @@ int map_rows(CUtensorMap* map, const void* base, const Strides& s, const Scan& p
 template <class T, int DK>
 int launch_forward_dk(const Scan& p, cudaStream_t st) {
     using L = ForwardSmem<T, DK>;
-    auto* kernel = scan_forward_kernel<T, DK>;
-    if (int rc = cuda_status(allow_smem(kernel, (int)L::kBytes), "delta_scan")) return rc;
+    constexpr auto* kernel = scan_forward_kernel<T, DK>;
+    if (int rc = allow_smem<kernel>((int)L::kBytes, p.device, "delta_scan")) return rc;
     const dim3 grid(static_cast<unsigned>(p.n * p.h), (p.dv + L::kWidth - 1) / L::kWidth);
     CUtensorMap map_k{}, map_q{}, map_v{};
     if (p.aligned && p.t) {
@@ -1578,7 +1579,7 @@ int launch_forward_dk(const Scan& p, cudaStream_t st) {
 template <class T, int DK, int DV>
 int launch_backward_dk_dv(const Scan& p, cudaStream_t st) {
     using L = BackwardSmem<T, DK, DV>;
-    auto* kernel = scan_backward_kernel<T, DK, DV>;
+    constexpr auto* kernel = scan_backward_kernel<T, DK, DV>;
     CUtensorMap map_k{}, map_q{}, map_o{}, map_s{};
     if (p.aligned) {
         const Strides so{p.n * p.h * p.dv, p.h * p.dv, p.dv};
@@ -1593,7 +1594,7 @@ int launch_backward_dk_dv(const Scan& p, cudaStream_t st) {
         if (dims[2] > 0x7FFFFFFFull) return invalid("delta_scan_backward: more than 2^31 states");
         if (int rc = encode_map(&map_s, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, p.checkpoints, dims, strides, box)) return rc;
     }
-    if (int rc = cuda_status(allow_smem(kernel, (int)L::kBytes), "delta_scan_backward")) return rc;
+    if (int rc = allow_smem<kernel>((int)L::kBytes, p.device, "delta_scan_backward")) return rc;
     kernel<<<static_cast<unsigned>(p.n * p.h), (L::kWarps + 1) * 32, L::kBytes, st>>>(p, map_k, map_q, map_o, map_s);
     return cuda_status(cudaGetLastError(), "delta_scan_backward");
 }

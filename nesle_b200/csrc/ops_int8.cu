@@ -1,5 +1,7 @@
 // ops_int8.cu -- quantisation of rows to 8 bits, and the product of 8-bit
 // integers with a scale for each token and each channel.
+#include <type_traits>
+
 #include "ops_common.h"
 #include "tc05.cuh"
 
@@ -467,12 +469,13 @@ int launch_tiles(const nesle_int8_args& a, const uint8_t* x, int64_t ld_x, const
     if (tiles > 0x7FFFFFFFull) return invalid("int8_linear: too many tiles");
     const unsigned grid = static_cast<unsigned>(tiles < (uint64_t)sm_count(a.device) ? tiles : sm_count(a.device));
     const int threads = kUnsigned ? 320 : 192;
-    auto go = [&](auto kernel) -> int {
-        if (int rc = cuda_status(allow_smem(kernel, T::kSmem), "int8_linear")) return rc;
+    auto go = [&](auto tma) -> int {
+        constexpr auto* kernel = int8_tile_kernel<kUnsigned, Out, kBN, decltype(tma)::value>;
+        if (int rc = allow_smem<kernel>(T::kSmem, a.device, "int8_linear")) return rc;
         kernel<<<grid, threads, T::kSmem, st>>>(mx, mw, my, ep, stalls);
         return cuda_status(cudaGetLastError(), "int8_linear");
     };
-    return tma_out ? go(int8_tile_kernel<kUnsigned, Out, kBN, true>) : go(int8_tile_kernel<kUnsigned, Out, kBN, false>);
+    return tma_out ? go(std::true_type{}) : go(std::false_type{});
 }
 
 template <bool kUnsigned, class Out>

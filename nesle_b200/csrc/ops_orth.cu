@@ -41,14 +41,11 @@ __device__ __forceinline__ void split(float v, __half& hi, __half& lo) {
 constexpr int kNormThreads = 256;
 constexpr int kNormRuns = 8;  // loads in flight a thread
 
-// Partial sums of squares: block (i, b) takes every gridDim.x-th run of 2,048 elements of matrix b, row after row.  In 64
-// bits: no update is too small or too large to be squared, and the partials are added in a fixed order.
+// The block's part of a matrix's sum of squares (in thread 0): every `blocks`-th run of 2,048 elements, row after row.  In
+// 64 bits: no update is too small or too large to be squared, and the parts are added in a fixed order.
 template <class T>
-__global__ void __launch_bounds__(kNormThreads) square_sums_kernel(const T* __restrict__ x, int64_t stride_b, int64_t stride_r,
-                                                                  int64_t stride_c, uint32_t rows, uint32_t cols,
-                                                                  double* __restrict__ partial) {
-    grid_launch_next();
-    const T* m = x + blockIdx.y * stride_b;
+__device__ __forceinline__ double square_sum(const T* __restrict__ m, int64_t stride_r, int64_t stride_c, uint32_t rows, uint32_t cols,
+                                             uint32_t block, uint32_t blocks) {
     double sum = 0;
     // Along the denser dimension, so that a warp's loads lie together; one long row where rows follow one another.
     const bool by_row = stride_c <= stride_r;
@@ -57,7 +54,7 @@ __global__ void __launch_bounds__(kNormThreads) square_sums_kernel(const T* __re
     if (so == static_cast<int64_t>(inner) * si) inner *= outer, outer = 1;
     constexpr uint32_t kRun = kNormThreads * kNormRuns;
     const uint64_t runs = (inner + kRun - 1) / kRun;
-    for (uint64_t i = blockIdx.x; i < outer * runs; i += gridDim.x) {
+    for (uint64_t i = block; i < outer * runs; i += blocks) {
         const uint64_t o = outer == 1 ? 0 : i / runs, at = (outer == 1 ? i : i % runs) * kRun + threadIdx.x;
         const T* from = m + static_cast<int64_t>(o) * so;
         float v[kNormRuns];
@@ -72,12 +69,21 @@ __global__ void __launch_bounds__(kNormThreads) square_sums_kernel(const T* __re
     __shared__ double part[kNormThreads / 32];
 #pragma unroll
     for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    __syncthreads();
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) {
+    if (threadIdx.x == 0)
         for (int i = 1; i < kNormThreads / 32; ++i) sum += part[i];
-        partial[blockIdx.y * gridDim.x + blockIdx.x] = sum;
-    }
+    return sum;
+}
+
+template <class T>
+__global__ void __launch_bounds__(kNormThreads) square_sums_kernel(const T* __restrict__ x, int64_t stride_b, int64_t stride_r,
+                                                                  int64_t stride_c, uint32_t rows, uint32_t cols,
+                                                                  double* __restrict__ partial) {
+    grid_launch_next();
+    const double sum = square_sum(x + blockIdx.y * stride_b, stride_r, stride_c, rows, cols, blockIdx.x, gridDim.x);
+    if (threadIdx.x == 0) partial[blockIdx.y * gridDim.x + blockIdx.x] = sum;
 }
 
 // X = kScale M / (|M| + eps) as fp16 pairs, and its transpose, by tiles of 64 x 64 of X: high part, then low part, each
@@ -85,26 +91,25 @@ __global__ void __launch_bounds__(kNormThreads) square_sums_kernel(const T* __re
 constexpr int kMostPartials = 256;  // one a thread
 
 template <class T>
-__global__ void __launch_bounds__(256) scale_kernel(const T* __restrict__ x, int64_t stride_b, int64_t stride_r, int64_t stride_c,
-                                                    uint32_t m, uint32_t n, const double* __restrict__ partial, uint32_t partials,
-                                                    double eps, __half* __restrict__ out, uint32_t ld, __half* __restrict__ out_t,
-                                                    uint32_t ld_t) {
-    __shared__ float tile[64][65];
-    __shared__ double part[8];
-    grid_launch_next();
-    const T* mat = x + blockIdx.z * stride_b;
-    const uint32_t r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+__device__ __forceinline__ void load_tile(float (&v)[16], const T* mat, int64_t stride_r, int64_t stride_c, uint32_t m, uint32_t n,
+                                          uint32_t r0, uint32_t c0) {
     const bool by_row = stride_c <= stride_r;
-    float v[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {  // the caller's matrix: nothing before this launch writes it
+    for (int k = 0; k < 16; ++k) {
         const int i = threadIdx.x + k * 256, r = by_row ? i / 64 : i % 64, c = by_row ? i % 64 : i / 64;
         v[k] = r0 + r < m && c0 + c < n ? to_f32(mat[static_cast<int64_t>(r0 + r) * stride_r + static_cast<int64_t>(c0 + c) * stride_c]) : 0.f;
     }
-    grid_wait();
-    double sum = threadIdx.x < partials ? partial[blockIdx.z * partials + threadIdx.x] : 0.0;
+}
+
+__device__ __forceinline__ void scale_tile(const float (&v)[16], const double* partial, uint32_t partials, double eps, bool by_row,
+                                           uint32_t m, uint32_t n, uint32_t r0, uint32_t c0, __half* hi, uint32_t ld, __half* hi_t,
+                                           uint32_t ld_t) {
+    __shared__ float tile[64][65];
+    __shared__ double part[8];
+    double sum = threadIdx.x < partials ? partial[threadIdx.x] : 0.0;
 #pragma unroll
     for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+    __syncthreads();
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
     __syncthreads();
     sum = 0;
@@ -117,8 +122,6 @@ __global__ void __launch_bounds__(256) scale_kernel(const T* __restrict__ x, int
         tile[r][c] = static_cast<float>(v[k] * factor);
     }
     __syncthreads();
-    __half* hi = out + static_cast<uint64_t>(blockIdx.z) * 2 * m * ld;
-    __half* hi_t = out_t + static_cast<uint64_t>(blockIdx.z) * 2 * n * ld_t;
 #pragma unroll 4
     for (int i = threadIdx.x; i < 64 * 32; i += 256) {
         const uint32_t a = i / 32, b = i % 32 * 2;  // ld is a multiple of 8: a pair is inside or outside
@@ -138,6 +141,19 @@ __global__ void __launch_bounds__(256) scale_kernel(const T* __restrict__ x, int
             *reinterpret_cast<__half2*>(hi_t + static_cast<uint64_t>(n) * ld_t + at) = l;
         }
     }
+}
+
+template <class T>
+__global__ void __launch_bounds__(256) scale_kernel(const T* __restrict__ x, int64_t stride_b, int64_t stride_r, int64_t stride_c,
+                                                    uint32_t m, uint32_t n, const double* __restrict__ partial, uint32_t partials,
+                                                    double eps, __half* __restrict__ out, uint32_t ld, __half* __restrict__ out_t,
+                                                    uint32_t ld_t) {
+    grid_launch_next();
+    float v[16];
+    load_tile(v, x + blockIdx.z * stride_b, stride_r, stride_c, m, n, blockIdx.y * 64, blockIdx.x * 64);  // the caller's matrix
+    grid_wait();
+    scale_tile(v, partial + blockIdx.z * partials, partials, eps, stride_c <= stride_r, m, n, blockIdx.y * 64, blockIdx.x * 64,
+               out + static_cast<uint64_t>(blockIdx.z) * 2 * m * ld, ld, out_t + static_cast<uint64_t>(blockIdx.z) * 2 * n * ld_t, ld_t);
 }
 
 // ------------------------------------------------------------------ products
@@ -167,6 +183,7 @@ struct Shape {
     static constexpr int kRow = kBN + 4;                                  // floats of a row of partial sums
     static constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
     static_assert(kTile * kRow * 4 <= kStages * kStageBytes, "partial sums take the place of the operands");
+    static_assert(8 * 4 * 32 * 40 * 2 <= kStages * kStageBytes, "and so do the warps' blocks of results");
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -190,9 +207,219 @@ union Half8 {
     uint4 u;
 };
 
+// A warp's 8 columns on their way to transposed storage: 32 rows of each, high and low parts.
+struct alignas(16) WarpTile {
+    __half h[2][8][40];  // 80 bytes a column: 16-byte reads of 8 columns fall on all banks
+};
+
+// Columns j..j+7 of row i0 + lane of a product, from its accumulators, by a whole warp; `mirror`: and transposed, which
+// goes through shared memory so that a store is 8 rows of a column.
+template <int kProduct>
+__device__ __forceinline__ void emit_run(const Job& job, uint32_t batch, uint32_t i0, uint32_t j, bool mirror, const float (&acc)[8],
+                                         WarpTile& wt, int lane) {
+    const uint64_t plane = static_cast<uint64_t>(job.m) * job.ld, plane_t = static_cast<uint64_t>(job.n) * job.ld_t;
+    if (i0 >= job.m || j >= job.n) return;  // the same for the warp
+    const uint32_t i = i0 + lane;
+    const bool inside = i < job.m;
+    float f[8];
+    const uint64_t at = static_cast<uint64_t>(i) * job.ld + j;
+    if constexpr (kProduct == kPoly) {
+        Half8 gh, gl;
+        gh.u = gl.u = make_uint4(0, 0, 0, 0);
+        if (inside) {
+            const __half* g = job.gram + batch * 2 * plane + at;
+            gh.u = *reinterpret_cast<const uint4*>(g);
+            gl.u = *reinterpret_cast<const uint4*>(g + plane);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+            f[q] = fmaf(kB, __half2float(gh.h[q]) + __half2float(gl.h[q]), fmaf(kC / kScale, acc[q], i == j + q ? kA * kScale : 0.f));
+    } else {
+        constexpr float kBack = kProduct == kLast ? 1.f / (kScale * kScale) : 1.f / kScale;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) f[q] = acc[q] * kBack;
+    }
+    // what a lane stores of the transpose: 8 rows of column lane / 4
+    const uint32_t tj = j + lane / 4, ti = i0 + lane % 4 * 8;
+    const bool t_inside = tj < job.n && ti < job.m;
+    if constexpr (kProduct == kLast) {
+        union Bf8 {
+            __nv_bfloat16 h[8];
+            uint4 u;
+        } b;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) b.h[q] = __float2bfloat16_rn(f[q]);
+        if (!job.last_t) {
+            if (!inside) return;
+            __nv_bfloat16* o = job.last + (static_cast<uint64_t>(batch) * job.m + i) * job.n + j;
+            if (job.n % 8 == 0) {
+                *reinterpret_cast<uint4*>(o) = b.u;
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (j + q < job.n) o[q] = b.h[q];
+            }
+            return;
+        }
+        __nv_bfloat16(*tile)[40] = reinterpret_cast<__nv_bfloat16(*)[40]>(wt.h[0]);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) tile[q][lane] = b.h[q];
+        __syncwarp();
+        if (t_inside) {
+            b.u = *reinterpret_cast<const uint4*>(&tile[lane / 4][lane % 4 * 8]);
+            __nv_bfloat16* o = job.last + (static_cast<uint64_t>(batch) * job.n + tj) * job.m + ti;
+            if (job.m % 8 == 0) {
+                *reinterpret_cast<uint4*>(o) = b.u;
+            } else {
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (ti + q < job.m) o[q] = b.h[q];
+            }
+        }
+        __syncwarp();
+    } else {
+        Half8 h, l;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) split(f[q], h.h[q], l.h[q]);
+        if (inside) {
+            __half* o = job.out + batch * 2 * plane + at;
+            *reinterpret_cast<uint4*>(o) = h.u;
+            *reinterpret_cast<uint4*>(o + plane) = l.u;
+        }
+        if (!mirror) return;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) wt.h[0][q][lane] = h.h[q], wt.h[1][q][lane] = l.h[q];
+        __syncwarp();
+        if (t_inside) {
+            __half* t = job.out_t + batch * 2 * plane_t + static_cast<uint64_t>(tj) * job.ld_t + ti;
+            *reinterpret_cast<uint4*>(t) = *reinterpret_cast<const uint4*>(&wt.h[0][lane / 4][lane % 4 * 8]);
+            *reinterpret_cast<uint4*>(t + plane_t) = *reinterpret_cast<const uint4*>(&wt.h[1][lane / 4][lane % 4 * 8]);
+        }
+        __syncwarp();
+    }
+}
+
+// 32 columns at once: a warp's 32 x 32 values of both parts and of their transposes, so that every access to global
+// memory is 16 bytes a lane and 64 of a row (a lane a row, as emit_run stores, takes the memory pipe four times as long).
+constexpr int kPitch = 40;  // 80 bytes a row: any 8 rows' 16-byte chunks fall on all banks
+struct alignas(16) WarpBlock {
+    __half h[2][32][kPitch], t[2][32][kPitch];
+};
+
+// h to t, transposed, by 8 x 8 blocks.
+__device__ __forceinline__ void transpose_block(const __half (&h)[32][kPitch], __half (&t)[32][kPitch], int lane) {
+#pragma unroll
+    for (int c = 0; c < 32; c += 8) {
+        uint32_t r[4];
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                     : "r"(tc::smem_u32(&h[lane][c]))
+                     : "memory");
+        asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(tc::smem_u32(&t[c + lane % 8][lane / 8 * 8])), "r"(r[0]),
+                     "r"(r[1]), "r"(r[2]), "r"(r[3])
+                     : "memory");
+    }
+}
+
+// Rows of a warp's block to a row-major matrix of rows x cols, `ld` apart.
+template <class T>
+__device__ __forceinline__ void store_block(T* out, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t r0, uint32_t c0, const __half (&h)[32][kPitch],
+                                            bool vector, int lane) {
+    const uint32_t c = c0 + lane % 4 * 8;
+#pragma unroll
+    for (int k = 0; k < 32; k += 8) {
+        const uint32_t r = r0 + k + lane / 4;
+        if (r >= rows || c >= cols) continue;
+        const uint4 x = *reinterpret_cast<const uint4*>(&h[k + lane / 4][lane % 4 * 8]);
+        T* to = out + r * ld + c;
+        if (vector) {
+            *reinterpret_cast<uint4*>(to) = x;
+        } else {
+            const T* v = reinterpret_cast<const T*>(&x);
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (c + q < cols) to[q] = v[q];
+        }
+    }
+}
+
+template <int kProduct>
+__device__ __forceinline__ void emit_block(const Job& job, uint32_t batch, uint32_t i0, uint32_t j0, bool mirror, const uint32_t (&acc)[32],
+                                           WarpBlock& wb, int lane) {
+    if (i0 >= job.m || j0 >= job.n) return;  // the same for the warp
+    const uint64_t plane = static_cast<uint64_t>(job.m) * job.ld, plane_t = static_cast<uint64_t>(job.n) * job.ld_t;
+    if constexpr (kProduct == kPoly) {
+        const __half* g = job.gram + batch * 2 * plane;
+        const uint32_t c = j0 + lane % 4 * 8;
+        uint4 x[2][4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t r = i0 + k * 8 + lane / 4;
+            const bool in = r < job.m && c < job.n;
+            x[0][k] = in ? *reinterpret_cast<const uint4*>(g + static_cast<uint64_t>(r) * job.ld + c) : make_uint4(0, 0, 0, 0);
+            x[1][k] = in ? *reinterpret_cast<const uint4*>(g + plane + static_cast<uint64_t>(r) * job.ld + c) : make_uint4(0, 0, 0, 0);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            *reinterpret_cast<uint4*>(&wb.t[0][k * 8 + lane / 4][lane % 4 * 8]) = x[0][k];
+            *reinterpret_cast<uint4*>(&wb.t[1][k * 8 + lane / 4][lane % 4 * 8]) = x[1][k];
+        }
+        __syncwarp();
+    }
+    const uint32_t i = i0 + lane;
+#pragma unroll
+    for (int q8 = 0; q8 < 32; q8 += 8) {
+        Half8 h, l, gh, gl;
+        if constexpr (kProduct == kPoly) {
+            gh.u = *reinterpret_cast<const uint4*>(&wb.t[0][lane][q8]);
+            gl.u = *reinterpret_cast<const uint4*>(&wb.t[1][lane][q8]);
+        }
+#pragma unroll
+        for (int q = 0; q < 8; ++q) {
+            float f = __uint_as_float(acc[q8 + q]);
+            if constexpr (kProduct == kPoly)
+                f = fmaf(kB, __half2float(gh.h[q]) + __half2float(gl.h[q]), fmaf(kC / kScale, f, i == j0 + q8 + q ? kA * kScale : 0.f));
+            else
+                f *= kProduct == kLast ? 1.f / (kScale * kScale) : 1.f / kScale;
+            if constexpr (kProduct == kLast) {
+                const __nv_bfloat16 b = __float2bfloat16_rn(f);
+                h.h[q] = reinterpret_cast<const __half&>(b);  // 16 bits to be moved
+            } else {
+                split(f, h.h[q], l.h[q]);
+            }
+        }
+        *reinterpret_cast<uint4*>(&wb.h[0][lane][q8]) = h.u;
+        if constexpr (kProduct != kLast) *reinterpret_cast<uint4*>(&wb.h[1][lane][q8]) = l.u;
+    }
+    __syncwarp();
+    if constexpr (kProduct == kLast) {
+        __nv_bfloat16* out = job.last + static_cast<uint64_t>(batch) * job.m * job.n;
+        if (job.last_t) {
+            transpose_block(wb.h[0], wb.t[0], lane);
+            __syncwarp();
+            store_block(out, job.m, job.n, job.m, j0, i0, wb.t[0], job.m % 8 == 0, lane);
+        } else {
+            store_block(out, job.n, job.m, job.n, i0, j0, wb.h[0], job.n % 8 == 0, lane);
+        }
+    } else {
+        __half* out = job.out + batch * 2 * plane;
+        store_block(out, job.ld, job.m, job.n, i0, j0, wb.h[0], true, lane);
+        store_block(out + plane, job.ld, job.m, job.n, i0, j0, wb.h[1], true, lane);
+        if (mirror) {
+            transpose_block(wb.h[0], wb.t[0], lane);
+            transpose_block(wb.h[1], wb.t[1], lane);
+            __syncwarp();
+            __half* out_t = job.out_t + batch * 2 * plane_t;
+            store_block(out_t, job.ld_t, job.n, job.m, j0, i0, wb.t[0], true, lane);
+            store_block(out_t + plane_t, job.ld_t, job.n, job.m, j0, i0, wb.t[1], true, lane);
+        }
+    }
+    __syncwarp();
+}
+
 // One tile by a cluster of kSplit blocks, each over its share of k; their fp32 partial sums meet in shared memory, block
 // r adding columns r kBN / kSplit and on, over the ranks in order.  In the epilogue a thread has one row and runs of 8
-// columns: its row's stores are 16 bytes, and of a column a warp stores 32 neighbouring rows.
+// columns.
 template <int kProduct, int kBN, int kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, Job job, unsigned int* stalls) {
@@ -284,79 +511,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     // This thread's row, and its columns: of its half of the tile, the rank's share.
     const int r = (warp % 4) * 32 + lane, half = warp / 4;
     constexpr int kHalf = kBN / 2, kMine = kHalf / kSplit;
-    const uint32_t i = ti * kTile + r;
     const uint32_t at_tmem = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16) + half * kHalf;
-    const uint64_t plane = static_cast<uint64_t>(job.m) * job.ld, plane_t = static_cast<uint64_t>(job.n) * job.ld_t;
     const bool mirror = kProduct == kLast ? job.last_t : kProduct == kApply || (tj * kBN) / kTile != ti;
 
-    auto emit = [&](int c, const float (&acc)[8]) {  // columns c..c+7 of the tile
-        const uint32_t j = tj * kBN + c;
-        if (i >= job.m || j >= job.n) return;
-        float f[8];
-        const uint64_t at = static_cast<uint64_t>(i) * job.ld + j;
-        if constexpr (kProduct == kPoly) {
-            const __half* g = job.gram + batch * 2 * plane + at;
-            Half8 gh, gl;
-            gh.u = *reinterpret_cast<const uint4*>(g);
-            gl.u = *reinterpret_cast<const uint4*>(g + plane);
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-                f[q] = fmaf(kB, __half2float(gh.h[q]) + __half2float(gl.h[q]), fmaf(kC / kScale, acc[q], i == j + q ? kA * kScale : 0.f));
-        } else {
-            constexpr float kBack = kProduct == kLast ? 1.f / (kScale * kScale) : 1.f / kScale;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) f[q] = acc[q] * kBack;
-        }
-        if constexpr (kProduct == kLast) {
-            if (job.last_t) {
-                __nv_bfloat16* o = job.last + (static_cast<uint64_t>(batch) * job.n + j) * job.m + i;
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (j + q < job.n) o[static_cast<uint64_t>(q) * job.m] = __float2bfloat16_rn(f[q]);
-            } else {
-                __nv_bfloat16* o = job.last + (static_cast<uint64_t>(batch) * job.m + i) * job.n + j;
-                union { __nv_bfloat16 h[8]; uint4 u; } b;
-#pragma unroll
-                for (int q = 0; q < 8; ++q) b.h[q] = __float2bfloat16_rn(f[q]);
-                if (job.n % 8 == 0) {
-                    *reinterpret_cast<uint4*>(o) = b.u;
-                } else {
-#pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        if (j + q < job.n) o[q] = b.h[q];
-                }
-            }
-        } else {
-            Half8 h, l;
-#pragma unroll
-            for (int q = 0; q < 8; ++q) split(f[q], h.h[q], l.h[q]);
-            __half* o = job.out + batch * 2 * plane + at;
-            *reinterpret_cast<uint4*>(o) = h.u;
-            *reinterpret_cast<uint4*>(o + plane) = l.u;
-            if (mirror) {
-                __half* t = job.out_t + batch * 2 * plane_t + static_cast<uint64_t>(j) * job.ld_t + i;
-#pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (j + q < job.n) {
-                        t[static_cast<uint64_t>(q) * job.ld_t] = h.h[q];
-                        t[plane_t + static_cast<uint64_t>(q) * job.ld_t] = l.h[q];
-                    }
-            }
-        }
+    __shared__ WarpTile warp_tiles[kThreads / 32];
+    auto emit = [&](int c, const float (&acc)[8]) {
+        emit_run<kProduct>(job, batch, ti * kTile + (warp % 4) * 32, tj * kBN + c, mirror, acc, warp_tiles[warp], lane);
     };
     if constexpr (kSplit == 1) {
+        __syncthreads();  // nobody reads the operands any more
+        WarpBlock* blocks = reinterpret_cast<WarpBlock*>(base);
 #pragma unroll
         for (int c = 0; c < kHalf; c += 32) {
             uint32_t v[32];
             tc::tmem_ld32(at_tmem + c, v);
             tc::tmem_wait_ld();
-#pragma unroll
-            for (int q = 0; q < 32; q += 8) {
-                float acc[8];
-#pragma unroll
-                for (int x = 0; x < 8; ++x) acc[x] = __uint_as_float(v[q + x]);
-                emit(half * kHalf + c + q, acc);
-            }
+            emit_block<kProduct>(job, batch, ti * kTile + (warp % 4) * 32, tj * kBN + half * kHalf + c, mirror, v, blocks[warp], lane);
         }
         tc::fence_before();
         __syncthreads();
@@ -432,10 +602,10 @@ int map_pair(CUtensorMap* map, const void* p, uint32_t rows, uint32_t cols, uint
 }
 
 template <int kProduct, int kBN, int kSplit>
-int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const Job& job, uint32_t tiles, uint32_t batch, unsigned int* stalls,
-                   cudaStream_t st) {
-    auto* kernel = product_kernel<kProduct, kBN, kSplit>;
-    if (int rc = cuda_status(allow_smem(kernel, Shape<kBN>::kSmem), "orthogonalize")) return rc;
+int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const Job& job, uint32_t tiles, uint32_t batch, int device,
+                   unsigned int* stalls, cudaStream_t st) {
+    constexpr auto* kernel = product_kernel<kProduct, kBN, kSplit>;
+    if (int rc = allow_smem<kernel>(Shape<kBN>::kSmem, device, "orthogonalize")) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(tiles * kSplit, batch);
     cfg.blockDim = dim3(kThreads);
@@ -472,19 +642,20 @@ uint32_t count_tiles(bool symmetric, Job& job, uint32_t bn) {
 // Narrow tiles, and k split over a cluster (while every block has two slices), as long as all blocks run at once; wide
 // tiles, which read their operands less often, where there are more than that.
 template <int kProduct>
-int launch_sized(const Operand& a, const Operand& b, Job job, uint32_t batch, int sms, unsigned int* stalls, cudaStream_t st) {
+int launch_sized(const Operand& a, const Operand& b, Job job, uint32_t batch, int device, unsigned int* stalls, cudaStream_t st) {
+    const int sms = sm_count(device);
     const bool symmetric = kProduct == kGram || kProduct == kPoly;
     const uint64_t narrow = static_cast<uint64_t>(count_tiles(symmetric, job, 64)) * batch;
     if (narrow > static_cast<uint32_t>(sms)) {
         const uint32_t tiles = count_tiles(symmetric, job, 128);
-        return launch_product<kProduct, 128, 1>(a.rows128, b.rows128, job, tiles, batch, stalls, st);
+        return launch_product<kProduct, 128, 1>(a.rows128, b.rows128, job, tiles, batch, device, stalls, st);
     }
     const uint32_t tiles = static_cast<uint32_t>(narrow / batch), slices = (job.k + kSlice - 1) / kSlice;
     if (narrow * 4 <= static_cast<uint32_t>(sms) && slices >= 8)
-        return launch_product<kProduct, 64, 4>(a.rows128, b.rows64, job, tiles, batch, stalls, st);
+        return launch_product<kProduct, 64, 4>(a.rows128, b.rows64, job, tiles, batch, device, stalls, st);
     if (narrow * 2 <= static_cast<uint32_t>(sms) && slices >= 4)
-        return launch_product<kProduct, 64, 2>(a.rows128, b.rows64, job, tiles, batch, stalls, st);
-    return launch_product<kProduct, 64, 1>(a.rows128, b.rows64, job, tiles, batch, stalls, st);
+        return launch_product<kProduct, 64, 2>(a.rows128, b.rows64, job, tiles, batch, device, stalls, st);
+    return launch_product<kProduct, 64, 1>(a.rows128, b.rows64, job, tiles, batch, device, stalls, st);
 }
 
 template <class T>
@@ -516,15 +687,14 @@ int run(const nesle_orth_args& a, cudaStream_t st) {
     const int64_t sr = tall ? a.stride_c : a.stride_r, sc = tall ? a.stride_r : a.stride_c;
     const uint32_t batch = static_cast<uint32_t>(a.batch), m = lay.m, n = lay.n;
     int rc;
+    unsigned int* stalls = nullptr;
+    if ((rc = stall_counter(a.device, &stalls))) return rc;
     switch (a.dtype) {
         case NESLE_F32: rc = launch_scaling<float>(a, lay, ws, sr, sc, st); break;
         case NESLE_BF16: rc = launch_scaling<__nv_bfloat16>(a, lay, ws, sr, sc, st); break;
         default: rc = launch_scaling<__half>(a, lay, ws, sr, sc, st); break;
     }
     if (rc) return rc;
-    unsigned int* stalls = nullptr;
-    if ((rc = stall_counter(a.device, &stalls))) return rc;
-    const int sms = sm_count(a.device);
     __half *gram = reinterpret_cast<__half*>(ws + lay.gram), *poly = reinterpret_cast<__half*>(ws + lay.poly);
     Operand op_x[2], op_xt[2], op_g, op_p;
     for (int i = 0; i < 2; ++i) {
@@ -539,12 +709,12 @@ int run(const nesle_orth_args& a, cudaStream_t st) {
         g.m = g.n = m, g.k = n;
         g.out = g.out_t = gram;
         g.ld = g.ld_t = lay.ld_m;
-        if ((rc = launch_sized<kGram>(op_x[from], op_x[from], g, batch, sms, stalls, st))) return rc;
+        if ((rc = launch_sized<kGram>(op_x[from], op_x[from], g, batch, a.device, stalls, st))) return rc;
         Job p = g;
         p.k = m;
         p.gram = gram;
         p.out = p.out_t = poly;
-        if ((rc = launch_sized<kPoly>(op_g, op_g, p, batch, sms, stalls, st))) return rc;
+        if ((rc = launch_sized<kPoly>(op_g, op_g, p, batch, a.device, stalls, st))) return rc;
         Job x{};
         x.m = m, x.n = n, x.k = m;
         x.out = reinterpret_cast<__half*>(ws + lay.x[to]);
@@ -553,8 +723,8 @@ int run(const nesle_orth_args& a, cudaStream_t st) {
         x.ld_t = lay.ld_m;
         x.last = static_cast<__nv_bfloat16*>(a.out);
         x.last_t = tall;
-        rc = step + 1 < a.steps ? launch_sized<kApply>(op_p, op_xt[from], x, batch, sms, stalls, st)
-                                : launch_sized<kLast>(op_p, op_xt[from], x, batch, sms, stalls, st);
+        rc = step + 1 < a.steps ? launch_sized<kApply>(op_p, op_xt[from], x, batch, a.device, stalls, st)
+                                : launch_sized<kLast>(op_p, op_xt[from], x, batch, a.device, stalls, st);
         if (rc) return rc;
     }
     return NESLE_OK;

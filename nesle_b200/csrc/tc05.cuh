@@ -1,7 +1,7 @@
 // tc05.cuh -- the PTX that the tensor-core kernels use: mbarriers, TMA tiles,
 // tensor memory and tcgen05.mma on K-major operands in 128-byte swizzled tiles.
 //
-// Every wait ends: after kWaitLimitNs a wait gives up, the role that gave up
+// Every wait ends: after kWaitClocks a wait gives up, the role that gave up
 // leaves its loop, and the kernel counts a stall (nesle_ops_stalls) and exits
 // with its tensor memory freed.
 #pragma once
@@ -11,7 +11,7 @@
 namespace nesle {
 namespace tc {
 
-constexpr unsigned long long kWaitLimitNs = 1000000000ull;
+constexpr long long kWaitClocks = 2000000000ll;  // about a second
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -42,17 +42,12 @@ __device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-__device__ __forceinline__ unsigned long long now_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-// Waits for the phase with `parity` to end; false after kWaitLimitNs.
+// Waits for the phase with `parity` to end; false after kWaitClocks.
 __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity) {
     if (mbar_try(b, parity)) return true;
-    const unsigned long long t0 = now_ns();
+    const long long t0 = clock64();
     while (!mbar_try(b, parity))
-        if (now_ns() - t0 > kWaitLimitNs) return false;
+        if (clock64() - t0 > kWaitClocks) return false;
     return true;
 }
 // The same for a whole warp: all lanes go on, or none.

@@ -26,6 +26,7 @@ from . import _lib
 __all__ = ["Int8Weight", "delta_scan", "delta_step", "int8_linear", "orthogonalize", "quantize_rows", "stalls"]
 
 _DTYPE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_stream = torch._C._cuda_getCurrentRawStream
 
 
 def _require(ok: bool, message: str) -> None:
@@ -33,22 +34,29 @@ def _require(ok: bool, message: str) -> None:
         raise ValueError(message)
 
 
-def _on(x: torch.Tensor, device: torch.device, name: str) -> None:
-    _require(isinstance(x, torch.Tensor) and x.device == device, f"{name} must be a tensor on {device}")
+def _on(x: torch.Tensor, index: int, name: str) -> None:
+    if not isinstance(x, torch.Tensor) or x.get_device() != index:
+        raise ValueError(f"{name} must be a tensor on cuda:{index}")
 
 
-def _cuda_device(x, name: str) -> torch.device:
-    _require(isinstance(x, torch.Tensor) and x.is_cuda, f"{name} must be a CUDA tensor")
-    return x.device
-
-
-def _stream(device: torch.device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+def _cuda_device(x, name: str) -> int:
+    if not isinstance(x, torch.Tensor) or not x.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor")
+    return x.get_device()
 
 
 def _no_grad_path(name: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError(f"{name} has no gradient; call it under torch.no_grad() or on detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError(f"{name} has no gradient; call it under torch.no_grad() or on detached tensors")
+
+
+def _call(name: str, args: bytes, stream: int) -> None:
+    lib = _lib.load()
+    rc = getattr(lib, name)(args, stream)
+    if rc:
+        _lib.check(rc, lib)
 
 
 def stalls(device: int = 0) -> int:
@@ -60,15 +68,16 @@ def stalls(device: int = 0) -> int:
 
 # ------------------------------------------------------------------ 8-bit product
 
-def _rows(x: torch.Tensor) -> torch.Tensor:
-    """(..., cols) as (rows, cols) with unit column stride; copies only where the layout has to change."""
-    x = x.reshape(-1, x.shape[-1]) if x.dim() != 2 else x
-    return x if x.stride(1) == 1 or x.shape[1] <= 1 else x.contiguous()
-
-
-def _ld(x: torch.Tensor) -> int:
-    """Row stride of a 2-D tensor; where a stride carries no meaning (one row, or none) the row length."""
-    return x.stride(0) if x.shape[0] > 1 else max(x.shape[1], 1)
+def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
+    """(..., cols) as (rows, cols) with unit column stride and rows that do not overlap, and the rows' distance; copies
+    only where the layout has to change.  Where a stride carries no meaning (one row, or none) it is the row length."""
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1])
+    rows, cols = x.shape
+    ld, unit = x.stride()
+    if (unit != 1 and cols > 1) or (ld < cols and rows > 1):
+        x, ld = x.contiguous(), cols
+    return x, ld if rows > 1 else max(cols, 1)
 
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -77,22 +86,26 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     0.  A NaN or an infinity in a row becomes the row's scale.  ``q``'s rows lie a multiple of 16 bytes apart, as
     :func:`int8_linear` reads them best."""
     dev = _cuda_device(x, "x")
-    _require(x.dtype in _DTYPE, "x must be float32, bfloat16 or float16")
+    dtype = _DTYPE.get(x.dtype)
+    _require(dtype is not None, "x must be float32, bfloat16 or float16")
     _require(x.dim() >= 1, "x needs at least one dimension")
     _no_grad_path("quantize_rows", x)
-    shape, x = x.shape, x if x.dim() > 1 else x[None]
+    shape = x.shape
     cols = shape[-1]
     if cols == 0:
         return x.new_empty(shape, dtype=torch.int8), x.new_zeros(shape[:-1], dtype=torch.float32)
-    x2 = _rows(x)
-    if x2.stride(0) < cols and x2.shape[0] > 1:  # rows that overlap or repeat (an expanded tensor)
-        x2 = x2.contiguous()
-    ld = -(-cols // 16) * 16
-    q = torch.empty((x2.shape[0], ld), dtype=torch.int8, device=dev)[:, :cols]
-    scale = torch.empty(x2.shape[0], dtype=torch.float32, device=dev)
-    _lib.check(_lib.load().nesle_quantize_rows(x2.data_ptr(), _DTYPE[x2.dtype], x2.shape[0], cols, _ld(x2), q.data_ptr(),
-                                               ld, scale.data_ptr(), dev.index, _stream(dev)))
-    return (q if len(shape) == 2 else q.unflatten(0, shape[:-1]) if len(shape) > 2 else q[0]), scale.view(shape[:-1])
+    x, ld = _rows(x)
+    rows = x.shape[0]
+    ld_q = -(-cols // 16) * 16
+    q = torch.empty((rows, ld_q), dtype=torch.int8, device=x.device)
+    scale = torch.empty(shape[:-1], dtype=torch.float32, device=x.device)
+    lib = _lib.load()
+    rc = lib.nesle_quantize_rows(x.data_ptr(), dtype, rows, cols, ld, q.data_ptr(), ld_q, scale.data_ptr(), dev, _stream(dev))
+    if rc:
+        _lib.check(rc, lib)
+    if ld_q != cols:
+        q = q[:, :cols]
+    return (q if len(shape) == 2 else q.unflatten(0, shape[:-1]) if len(shape) > 2 else q[0]), scale
 
 
 class Int8Weight:
@@ -106,11 +119,14 @@ class Int8Weight:
         _require(scale.dtype == torch.float32 and scale.shape == q.shape[:1], "scale must be float32 of shape (n,)")
         self.n, self.k = q.shape
         self.ld = max(16, -(-self.k // 16) * 16)
-        self.q = torch.zeros((self.n, self.ld), dtype=torch.int8, device=dev)
-        self.q[:, :self.k] = q
+        if self.ld == self.k:
+            self.q = q.detach().clone(memory_format=torch.contiguous_format)
+        else:
+            self.q = torch.nn.functional.pad(q.detach(), (0, self.ld - self.k))
         self.biased = self.q.view(torch.uint8) ^ 128  # two's complement: flipping the top bit adds 128
-        self.scale = scale.detach().contiguous().clone()
-        self.device = dev
+        self.scale = scale.detach().clone(memory_format=torch.contiguous_format)
+        self.device = q.device
+        self._index = dev
 
     @classmethod
     def from_float(cls, weight: torch.Tensor) -> "Int8Weight":
@@ -131,52 +147,52 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
     floating, which is quantised per token first (:func:`quantize_rows`; ``x_scale`` stays None).  ``bias`` is float32
     ``(n,)``.  The result is ``(..., n)`` in ``out_dtype`` (bfloat16, float16 or float32), or written to ``out``."""
     dev = _cuda_device(x, "x")
-    _require(isinstance(weight, Int8Weight) and weight.device == dev, f"weight must be an Int8Weight on {dev}")
-    _require(x.dim() >= 1 and x.shape[-1] == weight.k, f"x must have {weight.k} columns, has shape {tuple(x.shape)}")
+    _require(isinstance(weight, Int8Weight) and weight._index == dev, f"weight must be an Int8Weight on cuda:{dev}")
+    n, k = weight.n, weight.k
+    shape = x.shape
+    _require(len(shape) >= 1 and shape[-1] == k, f"x must have {k} columns, has shape {tuple(shape)}")
     _no_grad_path("int8_linear", x, bias)
     if x.dtype in _DTYPE:
         _require(x_scale is None, "x_scale is computed where x is floating")
         x, x_scale = quantize_rows(x)
-    _require(x.dtype in (torch.uint8, torch.int8), "x must be uint8, int8 or floating")
-    shape = x.shape[:-1]
-    x2 = _rows(x if x.dim() > 1 else x[None])
-    if x2.stride(0) < x2.shape[1] and x2.shape[0] > 1:
-        x2 = x2.contiguous()
-    m, k = x2.shape
-    a = _lib.Int8Args()
+    unsigned = x.dtype == torch.uint8
+    _require(unsigned or x.dtype == torch.int8, "x must be uint8, int8 or floating")
+    shape = shape[:-1]
+    x, ld_x = _rows(x)
+    m = x.shape[0]
+    scale_ptr, scale_value, bias_ptr = 0, 0.0, 0
     if isinstance(x_scale, torch.Tensor):
         _on(x_scale, dev, "x_scale")
         _require(x_scale.dtype == torch.float32 and x_scale.shape == shape, f"x_scale must be float32 of shape {tuple(shape)}")
         x_scale = x_scale.contiguous()
-        a.x_scale = x_scale.data_ptr()
+        scale_ptr = x_scale.data_ptr()
     else:
         _require(x_scale is not None, "x_scale is needed where x is integer")
-        a.x_scale_value = float(x_scale)
+        scale_value = float(x_scale)
     if bias is not None:
         _on(bias, dev, "bias")
-        _require(bias.dtype == torch.float32 and bias.shape == (weight.n,), f"bias must be float32 of shape ({weight.n},)")
+        _require(bias.dtype == torch.float32 and bias.shape == (n,), f"bias must be float32 of shape ({n},)")
         bias = bias.detach().contiguous()
-        a.bias = bias.data_ptr()
+        bias_ptr = bias.data_ptr()
     if out is None:
         _require(out_dtype in _DTYPE, "out_dtype must be float32, bfloat16 or float16")
-        out = torch.empty((*shape, weight.n), dtype=out_dtype, device=dev)
+        out = torch.empty((*shape, n), dtype=out_dtype, device=x.device)
+        ld_y = max(n, 1)
     else:
         _on(out, dev, "out")
-        _require(out.dtype in _DTYPE and out.shape == (*shape, weight.n), f"out must be floating of shape {(*shape, weight.n)}")
-        _require(out.dim() < 3 or out.is_contiguous(), "out of more than two dimensions must be contiguous")
-    y = out.view(-1, weight.n) if out.dim() != 2 else out
-    _require(y.stride(1) == 1 or y.shape[1] <= 1, "out must have unit column stride")
-    _require(y.shape[0] <= 1 or y.stride(0) >= weight.n, "out's rows must not overlap")
-    a.x, a.x_unsigned, a.ld_x = x2.data_ptr(), x2.dtype == torch.uint8, _ld(x2)
-    a.w, a.w_biased, a.ld_w, a.w_scale = weight.q.data_ptr(), weight.biased.data_ptr(), weight.ld, weight.scale.data_ptr()
-    a.y, a.y_dtype, a.ld_y = y.data_ptr(), _DTYPE[y.dtype], _ld(y)
-    a.m, a.k, a.n, a.relu, a.device = m, k, weight.n, relu, dev.index
-    lib = _lib.load()
-    need = lib.nesle_int8_workspace(ctypes.byref(a))
-    if need:
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = scratch.data_ptr(), need
-    _lib.check(lib.nesle_int8_linear(ctypes.byref(a), _stream(dev)))
+        _require(out.dtype in _DTYPE and out.shape == (*shape, n), f"out must be floating of shape {(*shape, n)}")
+        _require(out.dim() == 2 or out.is_contiguous(), "out of other than two dimensions must be contiguous")
+        ld_y = out.stride(0) if out.dim() == 2 and m > 1 else max(n, 1)
+        _require(out.dim() != 2 or out.stride(1) == 1 or n <= 1, "out must have unit column stride")
+        _require(ld_y >= n, "out's rows must not overlap")
+    x_ptr = x.data_ptr()
+    # rows that do not lie on 16 bytes are laid out again in scratch memory
+    need = m * (-(-k // 16) * 16) if x_ptr % 16 or ld_x % 16 else 0
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+    _call("nesle_int8_linear",
+          _lib.INT8_ARGS.pack(x_ptr, unsigned, ld_x, scale_ptr, scale_value, weight.q.data_ptr(), weight.biased.data_ptr(),
+                              weight.ld, weight.scale.data_ptr(), bias_ptr, out.data_ptr(), _DTYPE[out.dtype], ld_y, m, k, n,
+                              relu, scratch.data_ptr() if need else 0, need, dev), _stream(dev))
     return out
 
 
@@ -195,42 +211,48 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, eps: float = 1e-7,
     _no_grad_path("orthogonalize", update)
     rows, cols = update.shape[-2:]
     if out is None:
-        out = torch.empty(update.shape, dtype=torch.bfloat16, device=dev)
+        out = torch.empty(update.shape, dtype=torch.bfloat16, device=update.device)
     else:
         _on(out, dev, "out")
         _require(out.dtype == torch.bfloat16 and out.shape == update.shape and out.is_contiguous(),
                  f"out must be contiguous bfloat16 of shape {tuple(update.shape)}")
     x = update if update.dim() == 3 else update.reshape(-1, rows, cols) if out.numel() else update.new_empty((0, rows, cols))
-    a = _lib.OrthArgs(x.data_ptr(), _DTYPE[x.dtype], *x.stride(), *x.shape, steps, eps, out.data_ptr(), None, 0, dev.index)
-    lib = _lib.load()
-    need = lib.nesle_orth_workspace(ctypes.byref(a))
-    if need:
-        scratch = torch.empty(need, dtype=torch.uint8, device=dev)
-        a.workspace, a.workspace_bytes = scratch.data_ptr(), need
-    _lib.check(lib.nesle_orthogonalize(ctypes.byref(a), _stream(dev)))
+
+    def args(scratch=0, size=0):
+        return _lib.ORTH_ARGS.pack(x.data_ptr(), _DTYPE[x.dtype], *x.stride(), *x.shape, steps, eps, out.data_ptr(), scratch,
+                                   size, dev)
+
+    need = _lib.load().nesle_orth_workspace(args())
+    scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
+    _call("nesle_orthogonalize", args(scratch.data_ptr(), need), _stream(dev))
     return out
 
 
 # ------------------------------------------------------------------ gated delta rule
 
-def _delta_inputs(q, k, v, g, beta, reset, lead: str):
+def _delta_inputs(q, k, v, g, beta, reset, lead: str) -> int:
     """Checks what delta_step and delta_scan share; ``lead`` names the dimensions before the head size."""
     dev = _cuda_device(q, "q")
+    shape, dtype = q.shape, q.dtype
     dims = len(lead) + 1
-    _require(q.dtype in _DTYPE, "q must be float32, bfloat16 or float16")
-    _require(q.dim() == dims, f"q must have shape ({', '.join(lead)}, dk)")
+    _require(dtype in _DTYPE, "q must be float32, bfloat16 or float16")
+    _require(len(shape) == dims, f"q must have shape ({', '.join(lead)}, dk)")
+    heads = shape[:-1]
     for name, x in (("k", k), ("v", v), ("g", g), ("beta", beta)):
         _on(x, dev, name)
-    _require(k.shape == q.shape and k.dtype == q.dtype, f"k must be {q.dtype} of shape {tuple(q.shape)}")
-    _require(v.dim() == dims and v.shape[:-1] == q.shape[:-1] and v.dtype == q.dtype,
-             f"v must be {q.dtype} of shape {tuple(q.shape[:-1])} + (dv,)")
-    for name, x in (("g", g), ("beta", beta)):
-        _require(x.dtype == torch.float32 and x.shape == q.shape[:-1], f"{name} must be float32 of shape {tuple(q.shape[:-1])}")
-    _require(1 <= q.shape[-1] <= 128 and 1 <= v.shape[-1] <= 128, "head sizes must be 1 to 128")
+    if k.shape != shape or k.dtype != dtype:
+        raise ValueError(f"k must be {dtype} of shape {tuple(shape)}")
+    if v.dim() != dims or v.shape[:-1] != heads or v.dtype != dtype:
+        raise ValueError(f"v must be {dtype} of shape {tuple(heads)} + (dv,)")
+    if g.dtype != torch.float32 or g.shape != heads:
+        raise ValueError(f"g must be float32 of shape {tuple(heads)}")
+    if beta.dtype != torch.float32 or beta.shape != heads:
+        raise ValueError(f"beta must be float32 of shape {tuple(heads)}")
+    _require(1 <= shape[-1] <= 128 and 1 <= v.shape[-1] <= 128, "head sizes must be 1 to 128")
     if reset is not None:
         _on(reset, dev, "reset")
-        _require(reset.dtype in (torch.bool, torch.uint8) and reset.shape == q.shape[:-2],
-                 f"reset must be bool or uint8 of shape {tuple(q.shape[:-2])}")
+        if reset.dtype not in (torch.bool, torch.uint8) or reset.shape != shape[:-2]:
+            raise ValueError(f"reset must be bool or uint8 of shape {tuple(shape[:-2])}")
     return dev
 
 
@@ -254,80 +276,78 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     n, h, dk = q.shape
     dv = v.shape[-1]
     _on(state, dev, "state")
-    _require(state.dtype == torch.float32 and state.shape == (n, h, dk, dv), f"state must be float32 of shape {(n, h, dk, dv)}")
-    _require((state.stride(3) == 1 or dv == 1) and (state.stride(2) == dv or dk == 1), "state's matrices must be contiguous")
-    _require((n <= 1 or state.stride(0) >= dk * dv) and (h <= 1 or state.stride(1) >= dk * dv), "state's matrices must not overlap")
+    if state.dtype != torch.float32 or state.shape != (n, h, dk, dv):
+        raise ValueError(f"state must be float32 of shape {(n, h, dk, dv)}")
+    s_n, s_h, s_k, s_v = state.stride()
+    _require((s_v == 1 or dv == 1) and (s_k == dv or dk == 1), "state's matrices must be contiguous")
+    _require((n <= 1 or s_n >= dk * dv) and (h <= 1 or s_h >= dk * dv), "state's matrices must not overlap")
     if out is None:
-        out = torch.empty((n, h, dv), dtype=q.dtype, device=dev)
+        out = torch.empty((n, h, dv), dtype=q.dtype, device=q.device)
     else:
         _on(out, dev, "out")
         _require(out.dtype == q.dtype and out.shape == (n, h, dv) and out.is_contiguous(),
                  f"out must be contiguous {q.dtype} of shape {(n, h, dv)}")
     q, k, v = _unit(q), _unit(k), _unit(v)
-    a = _lib.DeltaStepArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-                           v.stride(0), v.stride(1), _DTYPE[q.dtype], g.data_ptr(), beta.data_ptr(), g.stride(0), g.stride(1),
-                           beta.stride(0), beta.stride(1), None if reset is None else reset.data_ptr(),
-                           0 if reset is None else reset.stride(0), state.data_ptr(), state.stride(0), state.stride(1),
-                           out.data_ptr(), n, h, dk, dv, dk ** -0.5 if scale is None else scale, dev.index)
-    _lib.check(_lib.load().nesle_delta_step(ctypes.byref(a), _stream(dev)))
+    reset_ptr, reset_n = (0, 0) if reset is None else (reset.data_ptr(), reset.stride(0))
+    _call("nesle_delta_step",
+          _lib.DELTA_STEP_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
+                                    _DTYPE[q.dtype], g.data_ptr(), beta.data_ptr(), *g.stride(), *beta.stride(), reset_ptr,
+                                    reset_n, state.data_ptr(), s_n, s_h, out.data_ptr(), n, h, dk, dv,
+                                    dk ** -0.5 if scale is None else scale, dev), _stream(dev))
     return out
 
 
-def _scan_args(q, k, v, g, beta, reset, state, scale, dev):
-    t, n, h, dk = q.shape
-    return _lib.DeltaArgs(q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), q_t=q.stride(0), q_n=q.stride(1), q_h=q.stride(2),
-                          k_t=k.stride(0), k_n=k.stride(1), k_h=k.stride(2), v_t=v.stride(0), v_n=v.stride(1),
-                          v_h=v.stride(2), dtype=_DTYPE[q.dtype], g=g.data_ptr(), beta=beta.data_ptr(), g_t=g.stride(0),
-                          g_n=g.stride(1), g_h=g.stride(2), beta_t=beta.stride(0), beta_n=beta.stride(1),
-                          beta_h=beta.stride(2), reset=None if reset is None else reset.data_ptr(),
-                          reset_t=0 if reset is None else reset.stride(0), reset_n=0 if reset is None else reset.stride(1),
-                          state=None if state is None else state.data_ptr(), t=t, n=n, h=h, dk=dk, dv=v.shape[-1],
-                          scale=scale, device=dev.index)
+def _scan_args(q, k, v, g, beta, reset, state, scale, dev, *rest: int) -> bytes:
+    """``rest``: o, final_state, errors, checkpoints, d_o, d_final, dq, d_k, d_v, dg, dbeta, dstate as far as given."""
+    reset_ptr, reset_t, reset_n = (0, 0, 0) if reset is None else (reset.data_ptr(), *reset.stride())
+    return _lib.DELTA_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:3], *k.stride()[:3], *v.stride()[:3],
+                                _DTYPE[q.dtype], g.data_ptr(), beta.data_ptr(), *g.stride(), *beta.stride(), reset_ptr,
+                                reset_t, reset_n, 0 if state is None else state.data_ptr(), *q.shape, v.shape[-1], scale,
+                                *rest, *(0,) * (12 - len(rest)), dev)
 
 
 class _DeltaScan(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, g, beta, state, reset, scale, grad):
-        dev, (t, n, h, dk), dv = q.device, q.shape, v.shape[-1]
-        o = torch.empty((t, n, h, dv), dtype=q.dtype, device=dev)
-        final = torch.empty((n, h, dk, dv), dtype=torch.float32, device=dev)
-        a = _scan_args(q, k, v, g, beta, reset, state, scale, dev)
-        a.o, a.final_state = o.data_ptr(), final.data_ptr()
-        lib = _lib.load()
+    def forward(ctx, q, k, v, g, beta, state, reset, scale, grad, dev):
+        (t, n, h, dk), dv, device = q.shape, v.shape[-1], q.device
+        o = torch.empty((t, n, h, dv), dtype=q.dtype, device=device)
+        final = torch.empty((n, h, dk, dv), dtype=torch.float32, device=device)
+        kept = (0, 0)
         if grad:
-            errors = torch.empty(lib.nesle_delta_error_floats(ctypes.byref(a)), dtype=torch.float32, device=dev)
-            checkpoints = torch.empty(lib.nesle_delta_checkpoint_floats(ctypes.byref(a)), dtype=torch.float32, device=dev)
-            a.errors, a.checkpoints = errors.data_ptr(), checkpoints.data_ptr()
+            lib, sizes = _lib.load(), _scan_args(q, k, v, g, beta, reset, state, scale, dev)
+            errors = torch.empty(lib.nesle_delta_error_floats(sizes), dtype=torch.float32, device=device)
+            checkpoints = torch.empty(lib.nesle_delta_checkpoint_floats(sizes), dtype=torch.float32, device=device)
+            kept = errors.data_ptr(), checkpoints.data_ptr()
             ctx.save_for_backward(q, k, v, g, beta, reset, errors, checkpoints)
-            ctx.scale, ctx.has_state = scale, state is not None
+            ctx.scale, ctx.has_state, ctx.dev = scale, state is not None, dev
             ctx.set_materialize_grads(False)
-        _lib.check(lib.nesle_delta_scan(ctypes.byref(a), _stream(dev)))
+        _call("nesle_delta_scan", _scan_args(q, k, v, g, beta, reset, state, scale, dev, o.data_ptr(), final.data_ptr(), *kept),
+              _stream(dev))
         return o, final
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_final):
         q, k, v, g, beta, reset, errors, checkpoints = ctx.saved_tensors
-        dev, (t, n, h, dk) = q.device, q.shape
+        dev, device, (t, n, h, dk) = ctx.dev, q.device, q.shape
         d_o = torch.zeros_like(v, memory_format=torch.contiguous_format) if d_o is None else d_o.contiguous()
         if d_final is not None:
             d_final = d_final.contiguous()
-        dq, dk_, dv_ = (torch.empty(x.shape, dtype=x.dtype, device=dev) for x in (q, k, v))
-        dg, dbeta = (torch.empty(x.shape, dtype=torch.float32, device=dev) for x in (g, beta))
+        dq, dk_, dv_ = (torch.empty(x.shape, dtype=x.dtype, device=device) for x in (q, k, v))
+        dg, dbeta = (torch.empty(x.shape, dtype=torch.float32, device=device) for x in (g, beta))
         dstate = None
         if ctx.has_state and ctx.needs_input_grad[5]:
-            dstate = torch.empty((n, h, dk, v.shape[-1]), dtype=torch.float32, device=dev)
+            dstate = torch.empty((n, h, dk, v.shape[-1]), dtype=torch.float32, device=device)
         if t == 0:
             if dstate is not None:
                 dstate = torch.zeros_like(dstate) if d_final is None else d_final.clone()
-            return dq, dk_, dv_, dg, dbeta, dstate, None, None, None
-        a = _scan_args(q, k, v, g, beta, reset, None, ctx.scale, dev)
-        a.errors, a.checkpoints, a.d_o = errors.data_ptr(), checkpoints.data_ptr(), d_o.data_ptr()
-        a.d_final = None if d_final is None else d_final.data_ptr()
-        a.dq, a.d_k, a.d_v, a.dg, a.dbeta = (x.data_ptr() for x in (dq, dk_, dv_, dg, dbeta))
-        a.dstate = None if dstate is None else dstate.data_ptr()
-        _lib.check(_lib.load().nesle_delta_scan_backward(ctypes.byref(a), _stream(dev)))
-        return dq, dk_, dv_, dg, dbeta, dstate, None, None, None
+        else:
+            _call("nesle_delta_scan_backward",
+                  _scan_args(q, k, v, g, beta, reset, None, ctx.scale, dev, 0, 0, errors.data_ptr(), checkpoints.data_ptr(),
+                             d_o.data_ptr(), 0 if d_final is None else d_final.data_ptr(), dq.data_ptr(), dk_.data_ptr(),
+                             dv_.data_ptr(), dg.data_ptr(), dbeta.data_ptr(), 0 if dstate is None else dstate.data_ptr()),
+                  _stream(dev))
+        return dq, dk_, dv_, dg, dbeta, dstate, None, None, None, None
 
 
 def delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -345,9 +365,9 @@ def delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     t, n, h, dk = q.shape
     if state is not None:
         _on(state, dev, "state")
-        _require(state.dtype == torch.float32 and state.shape == (n, h, dk, v.shape[-1]),
-                 f"state must be float32 of shape {(n, h, dk, v.shape[-1])}")
+        if state.dtype != torch.float32 or state.shape != (n, h, dk, v.shape[-1]):
+            raise ValueError(f"state must be float32 of shape {(n, h, dk, v.shape[-1])}")
         state = state.contiguous()
     grad = torch.is_grad_enabled() and any(x is not None and x.requires_grad for x in (q, k, v, g, beta, state))
     return _DeltaScan.apply(_unit(q), _unit(k), _unit(v), g, beta, state, reset, dk ** -0.5 if scale is None else float(scale),
-                            grad)
+                            grad, dev)
