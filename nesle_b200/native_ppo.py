@@ -153,7 +153,7 @@ class PPOTrainer:
                                env_offset=offset)
         self.batch.reset_device()
         self.mask_table = torch.tensor(w.SIMPLE_MOVEMENT_MASKS, dtype=torch.uint8, device=self.dev)
-        self.model = make_model(2048, len(w.SIMPLE_MOVEMENT_MASKS), config.hidden_sizes, self.dev)
+        self.model = self._make_model()
         if world > 1:  # identical initial weights on every rank
             import torch.distributed as dist
 
@@ -167,8 +167,7 @@ class PPOTrainer:
         self._split_graphs = world > 1
         self._graph = None
         self._eager_steps = 0
-        self.opt = torch.optim.Adam(self.model.parameters(), lr=config.learning_rate, eps=1e-5,
-                                    capturable=self.use_graphs)
+        self.opt = self._make_optimizer()
         T, N = config.n_steps, config.num_envs
         self.obs_buf = torch.empty((T, N, 2048), dtype=torch.uint8, device=self.dev)
         self.act_buf = torch.empty((T, N), dtype=torch.long, device=self.dev)
@@ -181,6 +180,14 @@ class PPOTrainer:
         self.rewards = torch.utils.dlpack.from_dlpack(self.batch.rewards_device())
         self.dones = torch.utils.dlpack.from_dlpack(self.batch.last_done_device())
         self.global_step = 0
+
+    def _make_model(self):
+        return make_model(2048, len(w.SIMPLE_MOVEMENT_MASKS), self.cfg.hidden_sizes, self.dev)
+
+    def _make_optimizer(self):
+        import torch
+
+        return torch.optim.Adam(self.model.parameters(), lr=self.cfg.learning_rate, eps=1e-5, capturable=self.use_graphs)
 
     def rollout(self) -> None:
         """n_steps env-steps of every env; no host synchronisation."""
@@ -205,10 +212,13 @@ class PPOTrainer:
 
     def _minibatch_loss(self, obs, act, logp, adv, ret):
         """Clipped-surrogate PPO loss of one minibatch (native_ppo.py:545-563)."""
+        logits, newvalue = self.model(obs)
+        return self._surrogate_loss(logits, newvalue, act, logp, adv, ret)
+
+    def _surrogate_loss(self, logits, newvalue, act, logp, adv, ret):
         import torch
 
         cfg = self.cfg
-        logits, newvalue = self.model(obs)
         logp_all = torch.log_softmax(logits, dim=-1)
         newlogp = logp_all.gather(1, act[:, None]).squeeze(1)
         entropy = -(logp_all.exp() * logp_all).sum(-1).mean()

@@ -18,6 +18,7 @@ No counterpart in the reference.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -306,6 +307,14 @@ def _scan_args(q, k, v, g, beta, reset, state, scale, dev, *rest: int) -> bytes:
                                 *rest, *(0,) * (12 - len(rest)), dev)
 
 
+@functools.lru_cache(maxsize=256)
+def _scan_sizes(t: int, n: int, h: int, dk: int, dv: int) -> tuple[int, int]:
+    """Floats of the errors and the states that a scan keeps for its gradients."""
+    sizes = _lib.DELTA_ARGS.pack(*(0,) * 25, t, n, h, dk, dv, 0.0, *(0,) * 12, 0)
+    lib = _lib.load()
+    return lib.nesle_delta_error_floats(sizes), lib.nesle_delta_checkpoint_floats(sizes)
+
+
 class _DeltaScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, reset, scale, grad, dev):
@@ -314,9 +323,9 @@ class _DeltaScan(torch.autograd.Function):
         final = torch.empty((n, h, dk, dv), dtype=torch.float32, device=device)
         kept = (0, 0)
         if grad:
-            lib, sizes = _lib.load(), _scan_args(q, k, v, g, beta, reset, state, scale, dev)
-            errors = torch.empty(lib.nesle_delta_error_floats(sizes), dtype=torch.float32, device=device)
-            checkpoints = torch.empty(lib.nesle_delta_checkpoint_floats(sizes), dtype=torch.float32, device=device)
+            sizes = _scan_sizes(t, n, h, dk, dv)
+            errors = torch.empty(sizes[0], dtype=torch.float32, device=device)
+            checkpoints = torch.empty(sizes[1], dtype=torch.float32, device=device)
             kept = errors.data_ptr(), checkpoints.data_ptr()
             ctx.save_for_backward(q, k, v, g, beta, reset, errors, checkpoints)
             ctx.scale, ctx.has_state, ctx.dev = scale, state is not None, dev
@@ -326,8 +335,9 @@ class _DeltaScan(torch.autograd.Function):
         return o, final
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, d_o, d_final):
+        if torch.is_grad_enabled():  # create_graph=True
+            raise RuntimeError("delta_scan has first derivatives only")
         q, k, v, g, beta, reset, errors, checkpoints = ctx.saved_tensors
         dev, device, (t, n, h, dk) = ctx.dev, q.device, q.shape
         d_o = torch.zeros_like(v, memory_format=torch.contiguous_format) if d_o is None else d_o.contiguous()

@@ -1,0 +1,107 @@
+"""The operators' C boundary (include/nesle_ops.h) without a GPU: the packed
+argument blocks have the C layout, and every entry checks its arguments before
+it touches a device."""
+from __future__ import annotations
+
+import ctypes
+import re
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+from nesle_b200 import _lib
+
+ROOT = Path(__file__).resolve().parents[1]
+BLOCKS = {"nesle_int8_args": _lib.INT8_ARGS, "nesle_orth_args": _lib.ORTH_ARGS,
+          "nesle_delta_step_args": _lib.DELTA_STEP_ARGS, "nesle_delta_args": _lib.DELTA_ARGS}
+
+
+@pytest.fixture(scope="module")
+def lib():
+    from nesle_b200 import build
+
+    build.build()
+    return _lib.load()
+
+
+def members(name: str) -> list[str]:
+    text = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "nesle_ops.h").read_text(), flags=re.S)
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), text, flags=re.S).group(1)
+    out = []
+    for declaration in body.split(";"):
+        out += [x.strip().lstrip("*").split()[-1].lstrip("*") for x in declaration.split(",") if x.strip()]
+    return out
+
+
+@pytest.mark.parametrize("name", BLOCKS)
+def test_argument_blocks_have_the_c_layout(name, tmp_path):
+    """Every member at the offset that the struct format gives it."""
+    if not shutil.which("gcc"):
+        pytest.skip("gcc is not available")
+    names = members(name)
+    source = '#include <stdio.h>\n#include "nesle_ops.h"\nint main(void) {\n' + "".join(
+        f'printf("%zu %zu\\n", offsetof({name}, {m}), sizeof((({name}*)0)->{m}));\n' for m in names) + "return 0; }\n"
+    (tmp_path / "a.c").write_text(source)
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), "-o", str(tmp_path / "a"), str(tmp_path / "a.c")], check=True)
+    want = [tuple(map(int, x.split())) for x in subprocess.run([str(tmp_path / "a")], capture_output=True, text=True,
+                                                               check=True).stdout.splitlines()]
+    letters = re.sub(r"\s", "", BLOCKS[name].format.lstrip("@"))
+    assert len(letters) == len(names)
+    import struct
+
+    got = []
+    for i, letter in enumerate(letters):
+        size = struct.calcsize("@" + letter)
+        got.append((struct.calcsize("@" + letters[:i + 1]) - size, size))
+    assert got == want
+
+
+def test_null_and_bad_arguments_are_refused(lib):
+    invalid = _lib.NESLE_ERR_INVALID
+    for name in ("nesle_int8_linear", "nesle_orthogonalize", "nesle_delta_step", "nesle_delta_scan",
+                 "nesle_delta_scan_backward"):
+        assert getattr(lib, name)(None, None) == invalid, name
+        assert lib.nesle_last_error()
+    assert lib.nesle_quantize_rows(None, 0, 4, 4, 4, None, 16, None, 0, None) == invalid
+    assert lib.nesle_quantize_rows(1, 0, 4, 8, 4, 1, 16, 1, 0, None) == invalid  # rows overlap
+    assert lib.nesle_ops_stalls(0, None) == invalid
+
+    def delta(t=4, n=1, h=1, dk=16, dv=16, dtype=0):
+        return _lib.DELTA_ARGS.pack(16, 16, 16, *(16,) * 9, dtype, 16, 16, *(1,) * 6, 0, 0, 0, 0, t, n, h, dk, dv, 1.0,
+                                    *(0,) * 12, 0)
+
+    assert lib.nesle_delta_scan(delta(dk=129), None) == invalid
+    assert lib.nesle_delta_scan(delta(dv=0), None) == invalid
+    assert lib.nesle_delta_scan(delta(dtype=9), None) == invalid
+    assert lib.nesle_delta_scan(delta(), None) == invalid  # no output
+    assert lib.nesle_delta_scan_backward(delta(t=0), None) == invalid
+    assert lib.nesle_delta_scan(delta(n=0), None) == _lib.NESLE_OK  # nothing to do
+    orth = _lib.ORTH_ARGS.pack(16, 0, 16, 4, 1, 1, 4, 4, 0, 1e-7, 16, 0, 0, 0)
+    assert lib.nesle_orthogonalize(orth, None) == invalid  # no steps
+    assert b"steps" in lib.nesle_last_error()
+
+
+def test_sizes_of_what_a_scan_keeps(lib):
+    args = _lib.DELTA_ARGS.pack(*(0,) * 25, 33, 5, 3, 40, 72, 0.0, *(0,) * 12, 0)
+    assert lib.nesle_delta_checkpoint_floats(args) == 5 * 3 * 3 * 40 * 72  # a state for every 16 tokens begun
+    assert lib.nesle_delta_error_floats(args) == 5 * 3 * 3 * 5 * 256       # 16 x 16 tiles
+    assert lib.nesle_delta_error_floats(None) == 0
+
+
+def test_tensors_that_are_not_on_a_gpu_are_refused():
+    torch = pytest.importorskip("torch")
+    from nesle_b200 import ops
+
+    x = torch.zeros((2, 3, 16))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.quantize_rows(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.orthogonalize(x)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.delta_step(x, x, x, x[..., 0], x[..., 0], torch.zeros((2, 3, 16, 16)))
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.int8_linear(x, None)
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.Int8Weight(torch.zeros((4, 4), dtype=torch.int8), torch.zeros(4))

@@ -327,6 +327,15 @@ def test_only_what_is_asked_for_has_a_gradient():
 
 
 @pytest.mark.gpu
+def test_second_derivatives_are_refused():
+    x = inputs(5, 1, 1, 16, 16, seed=17)
+    q = x["q"].clone().requires_grad_()
+    o, _ = ops.delta_scan(q, x["k"], x["v"], x["g"], x["beta"], x["state"])
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(o.square().sum(), q, create_graph=True)
+
+
+@pytest.mark.gpu
 def test_refusals():
     x = inputs(3, 2, 2, 16, 16)
     args = [x[i] for i in NAMES]
