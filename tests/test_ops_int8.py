@@ -55,7 +55,8 @@ def _quantized(x):
 
 
 SIZES = [(1, 2048, 512), (1, 1, 1), (2, 17, 3), (16, 64, 8), (17, 100, 9), (64, 256, 130), (65, 128, 16), (128, 128, 64),
-         (129, 127, 65), (200, 130, 129), (257, 2048, 512), (1000, 300, 257), (300, 96, 2048), (20000, 64, 33)]
+         (129, 127, 65), (200, 130, 129), (257, 2048, 512), (1000, 300, 257), (300, 96, 2048), (20000, 64, 33),
+         (19001, 200, 300), (9500, 130, 513), (20000, 16, 129), (6400, 1000, 700)]
 
 
 @pytest.mark.gpu
