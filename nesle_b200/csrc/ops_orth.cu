@@ -177,13 +177,13 @@ constexpr int kThreads = 256;
 
 template <int kBN>  // columns of a tile
 struct Shape {
-    static constexpr int kStages = kBN == 128 ? 3 : 4;
+    static constexpr int kStages = 3;
     static constexpr int kA = kTile * kSlice * 2, kB = kBN * kSlice * 2;  // one fp16 part of an operand
     static constexpr int kStageBytes = 2 * (kA + kB);                     // A high, A low, B high, B low
-    static constexpr int kRow = kBN + 4;                                  // floats of a row of partial sums
-    static constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
-    static_assert(kTile * kRow * 4 <= kStages * kStageBytes, "partial sums take the place of the operands");
-    static_assert(8 * 4 * 32 * 40 * 2 <= kStages * kStageBytes, "and so do the warps' blocks of results");
+    // A block's columns of a tile from every block of its cluster: rows of kBN / split floats, padded by 4.
+    static constexpr int kShares = kBN == 64 ? 4 * kTile * (kBN / 4 + 4) * 4 : 0;
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + kShares + 256;
+    static_assert(8 * 4 * 32 * 40 * 2 <= kStages * kStageBytes, "the warps' blocks of results take the place of the operands");
 };
 
 __device__ __forceinline__ uint32_t cluster_rank() {
@@ -194,12 +194,10 @@ __device__ __forceinline__ uint32_t cluster_rank() {
 __device__ __forceinline__ void cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-__device__ __forceinline__ float4 peer_load(const float* p, uint32_t rank) {
+__device__ __forceinline__ uint32_t peer_address(const void* p, uint32_t rank) {
     uint32_t at;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(tc::smem_u32(p)), "r"(rank));
-    float4 v;
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
-    return v;
+    return at;
 }
 
 union Half8 {
@@ -417,9 +415,9 @@ __device__ __forceinline__ void emit_block(const Job& job, uint32_t batch, uint3
     __syncwarp();
 }
 
-// One tile by a cluster of kSplit blocks, each over its share of k; their fp32 partial sums meet in shared memory, block
-// r adding columns r kBN / kSplit and on, over the ranks in order.  In the epilogue a thread has one row and runs of 8
-// columns.
+// One tile by a cluster of kSplit blocks, each over its share of k; every block sends the others their columns of its
+// fp32 sums and adds up its own from all, in the order of the ranks.  (Fetching them from the others' shared memory took
+// 4,000 to 6,000 clocks, sending them takes 1,400.)
 template <int kProduct, int kBN, int kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, Job job, unsigned int* stalls) {
@@ -428,11 +426,11 @@ __global__ void __launch_bounds__(kThreads, 1)
     constexpr bool kSymmetric = kProduct == kGram || kProduct == kPoly;
     extern __shared__ uint8_t raw[];
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    uint64_t* full = reinterpret_cast<uint64_t*>(base + kStages * S::kStageBytes);
+    float* shares = reinterpret_cast<float*>(base + kStages * S::kStageBytes);
+    uint64_t* full = reinterpret_cast<uint64_t*>(base + kStages * S::kStageBytes + S::kShares);
     uint64_t* empty = full + kStages;
     uint64_t* done = empty + kStages;
     uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
-    float* sums = reinterpret_cast<float*>(base);
 
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     const uint32_t rank = kSplit > 1 ? cluster_rank() : 0, batch = blockIdx.y;
@@ -463,7 +461,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (warp == 1) tc::tmem_alloc(slot, kBN);
     tc::fence_before();
-    __syncthreads();
+    if constexpr (kSplit > 1)
+        cluster_sync();  // the others' shared memory is there
+    else
+        __syncthreads();
     tc::fence_after();
     const uint32_t tmem = *slot;
     grid_launch_next();
@@ -533,15 +534,16 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc::fence_after();
         if (warp == 1) tc::tmem_free(tmem, kBN);
     } else {
-        __syncthreads();  // nobody reads the operands any more
+        static_assert(kHalf == 32, "one load of tensor memory");
+        constexpr int kPitch = kBN / kSplit + 4;
+        uint32_t v[32];
+        tc::tmem_ld32(at_tmem, v);
+        tc::tmem_wait_ld();
 #pragma unroll
-        for (int c = 0; c < kHalf; c += 32) {
-            uint32_t v[32];
-            tc::tmem_ld32(at_tmem + c, v);
-            tc::tmem_wait_ld();
-#pragma unroll
-            for (int x = 0; x < 32; x += 4)
-                *reinterpret_cast<uint4*>(sums + r * S::kRow + half * kHalf + c + x) = make_uint4(v[x], v[x + 1], v[x + 2], v[x + 3]);
+        for (int x = 0; x < 32; x += 4) {
+            const uint32_t at = peer_address(shares + (rank * kTile + r) * kPitch + half * kMine + x % kMine, x / kMine);
+            asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(v[x]), "r"(v[x + 1]), "r"(v[x + 2]), "r"(v[x + 3])
+                         : "memory");
         }
         tc::fence_before();
         cluster_sync();
@@ -549,19 +551,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (warp == 1) tc::tmem_free(tmem, kBN);
 #pragma unroll
         for (int c = 0; c < kMine; c += 8) {
-            const int col = half * kHalf + rank * kMine + c;
             float acc[8] = {};
 #pragma unroll
             for (int p = 0; p < kSplit; ++p) {
-                const float4 x = peer_load(sums + r * S::kRow + col, p), y = peer_load(sums + r * S::kRow + col + 4, p);
+                const float* from = shares + (p * kTile + r) * kPitch + half * kMine + c;
+                const float4 x = *reinterpret_cast<const float4*>(from), y = *reinterpret_cast<const float4*>(from + 4);
                 acc[0] += x.x, acc[1] += x.y, acc[2] += x.z, acc[3] += x.w;
                 acc[4] += y.x, acc[5] += y.y, acc[6] += y.z, acc[7] += y.w;
             }
-            emit(col, acc);
+            emit(half * kHalf + rank * kMine + c, acc);
         }
     }
     if (!ok) atomicAdd(stalls, 1u);
-    if constexpr (kSplit > 1) cluster_sync();  // a peer may still read this block's sums
 }
 
 // ----------------------------------------------------------------------- host
@@ -639,7 +640,7 @@ uint32_t count_tiles(bool symmetric, Job& job, uint32_t bn) {
     return tiles;
 }
 
-// Narrow tiles, and k split over a cluster (while every block has two slices), as long as all blocks run at once; wide
+// Narrow tiles, and k split over a cluster where it is long enough to pay for that, as long as all blocks run at once; wide
 // tiles, which read their operands less often, where there are more than that.
 template <int kProduct>
 int launch_sized(const Operand& a, const Operand& b, Job job, uint32_t batch, int device, unsigned int* stalls, cudaStream_t st) {
@@ -651,9 +652,10 @@ int launch_sized(const Operand& a, const Operand& b, Job job, uint32_t batch, in
         return launch_product<kProduct, 128, 1>(a.rows128, b.rows128, job, tiles, batch, device, stalls, st);
     }
     const uint32_t tiles = static_cast<uint32_t>(narrow / batch), slices = (job.k + kSlice - 1) / kSlice;
+    // A slice takes 1,000 clocks, joining a cluster's shares 3,500.
     if (narrow * 4 <= static_cast<uint32_t>(sms) && slices >= 8)
         return launch_product<kProduct, 64, 4>(a.rows128, b.rows64, job, tiles, batch, device, stalls, st);
-    if (narrow * 2 <= static_cast<uint32_t>(sms) && slices >= 4)
+    if (narrow * 2 <= static_cast<uint32_t>(sms) && slices >= 8)
         return launch_product<kProduct, 64, 2>(a.rows128, b.rows64, job, tiles, batch, device, stalls, st);
     return launch_product<kProduct, 64, 1>(a.rows128, b.rows64, job, tiles, batch, device, stalls, st);
 }
