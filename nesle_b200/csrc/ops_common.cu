@@ -37,7 +37,7 @@ int sm_count(int device) {
 }
 
 int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
-               const uint64_t* strides, const uint32_t* box) {
+               const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -59,7 +59,7 @@ int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void*
         if (i) s[i - 1] = strides[i - 1];
     }
     const CUresult r = encode(map, type, static_cast<cuuint32_t>(rank), const_cast<void*>(base), d, s, b, e,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return set_error(NESLE_ERR_CUDA, ("cuTensorMapEncodeTiled: error " + std::to_string((int)r)).c_str());
     return NESLE_OK;

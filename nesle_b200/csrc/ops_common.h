@@ -58,9 +58,9 @@ int sm_count(int device);
 int stall_counter(int device, unsigned int** out);
 
 // A tiled tensor map over `rank` dimensions, innermost first; `strides` are the
-// byte strides of dimensions 1..rank-1.  128-byte swizzle, zero fill.
+// byte strides of dimensions 1..rank-1.  Zero fill.
 int encode_map(CUtensorMap* map, CUtensorMapDataType type, int rank, const void* base, const uint64_t* dims,
-               const uint64_t* strides, const uint32_t* box);
+               const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B);
 
 // Allows a kernel its dynamic shared memory on the current device, `device`: once for each.
 template <auto* kKernel>

@@ -36,54 +36,72 @@ __device__ __forceinline__ void split(float v, __half& hi, __half& lo) {
     lo = __float2half_rn(v - __half2float(hi));
 }
 
+union Half8 {
+    __half h[8];
+    uint4 u;
+};
+
 // ----------------------------------------------------- norm, scaling, layout
 
 constexpr int kNormThreads = 256;
 constexpr int kNormRuns = 8;  // loads in flight a thread
 
-// The block's part of a matrix's sum of squares (in thread 0): every `blocks`-th run of 2,048 elements, row after row.  In
-// 64 bits: no update is too small or too large to be squared, and the parts are added in a fixed order.
+// Partial sums of squares: block (i, b) takes every gridDim.x-th run of 2,048 loads of matrix b, row after row.  In 64
+// bits: no update is too small or too large to be squared, and the partials are added in a fixed order.
 template <class T>
-__device__ __forceinline__ double square_sum(const T* __restrict__ m, int64_t stride_r, int64_t stride_c, uint32_t rows, uint32_t cols,
-                                             uint32_t block, uint32_t blocks) {
+__global__ void __launch_bounds__(kNormThreads) square_sums_kernel(const T* __restrict__ x, int64_t stride_b, int64_t stride_r,
+                                                                  int64_t stride_c, uint32_t rows, uint32_t cols,
+                                                                  double* __restrict__ partial) {
+    grid_launch_next();
+    const T* m = x + blockIdx.y * stride_b;
     double sum = 0;
     // Along the denser dimension, so that a warp's loads lie together; one long row where rows follow one another.
     const bool by_row = stride_c <= stride_r;
     const int64_t so = by_row ? stride_r : stride_c, si = by_row ? stride_c : stride_r;
     uint64_t outer = by_row ? rows : cols, inner = by_row ? cols : rows;
     if (so == static_cast<int64_t>(inner) * si) inner *= outer, outer = 1;
-    constexpr uint32_t kRun = kNormThreads * kNormRuns;
-    const uint64_t runs = (inner + kRun - 1) / kRun;
-    for (uint64_t i = block; i < outer * runs; i += blocks) {
-        const uint64_t o = outer == 1 ? 0 : i / runs, at = (outer == 1 ? i : i % runs) * kRun + threadIdx.x;
+    // 16 bytes a load where every row is whole chunks on 16 bytes.
+    constexpr uint32_t kPer = 16 / sizeof(T);
+    const bool vector = si == 1 && inner % kPer == 0 && (outer == 1 || so % kPer == 0) && reinterpret_cast<uintptr_t>(m) % 16 == 0;
+    const uint32_t run = kNormThreads * kNormRuns * (vector ? kPer : 1);
+    const uint64_t runs = (inner + run - 1) / run;
+    for (uint64_t i = blockIdx.x; i < outer * runs; i += gridDim.x) {
+        const uint64_t o = outer == 1 ? 0 : i / runs, first = (outer == 1 ? i : i % runs) * run;
         const T* from = m + static_cast<int64_t>(o) * so;
-        float v[kNormRuns];
+        if (vector) {
+            uint4 v[kNormRuns];
 #pragma unroll
-        for (int k = 0; k < kNormRuns; ++k) {
-            const uint64_t e = at + k * kNormThreads;
-            v[k] = e < inner ? to_f32(from[static_cast<int64_t>(e) * si]) : 0.f;
+            for (int k = 0; k < kNormRuns; ++k) {
+                const uint64_t e = first + (k * kNormThreads + threadIdx.x) * kPer;
+                v[k] = e < inner ? __ldg(reinterpret_cast<const uint4*>(from + e)) : make_uint4(0, 0, 0, 0);
+            }
+#pragma unroll
+            for (int k = 0; k < kNormRuns; ++k)
+#pragma unroll
+                for (uint32_t j = 0; j < kPer; ++j) {
+                    const double e = to_f32(reinterpret_cast<const T*>(&v[k])[j]);
+                    sum += e * e;
+                }
+        } else {
+            float v[kNormRuns];
+#pragma unroll
+            for (int k = 0; k < kNormRuns; ++k) {
+                const uint64_t e = first + k * kNormThreads + threadIdx.x;
+                v[k] = e < inner ? to_f32(from[static_cast<int64_t>(e) * si]) : 0.f;
+            }
+#pragma unroll
+            for (int k = 0; k < kNormRuns; ++k) sum += static_cast<double>(v[k]) * v[k];
         }
-#pragma unroll
-        for (int k = 0; k < kNormRuns; ++k) sum += static_cast<double>(v[k]) * v[k];
     }
     __shared__ double part[kNormThreads / 32];
 #pragma unroll
     for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    __syncthreads();
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
     __syncthreads();
-    if (threadIdx.x == 0)
+    if (threadIdx.x == 0) {
         for (int i = 1; i < kNormThreads / 32; ++i) sum += part[i];
-    return sum;
-}
-
-template <class T>
-__global__ void __launch_bounds__(kNormThreads) square_sums_kernel(const T* __restrict__ x, int64_t stride_b, int64_t stride_r,
-                                                                  int64_t stride_c, uint32_t rows, uint32_t cols,
-                                                                  double* __restrict__ partial) {
-    grid_launch_next();
-    const double sum = square_sum(x + blockIdx.y * stride_b, stride_r, stride_c, rows, cols, blockIdx.x, gridDim.x);
-    if (threadIdx.x == 0) partial[blockIdx.y * gridDim.x + blockIdx.x] = sum;
+        partial[blockIdx.y * gridDim.x + blockIdx.x] = sum;
+    }
 }
 
 // X = kScale M / (|M| + eps) as fp16 pairs, and its transpose, by tiles of 64 x 64 of X: high part, then low part, each
@@ -91,25 +109,26 @@ __global__ void __launch_bounds__(kNormThreads) square_sums_kernel(const T* __re
 constexpr int kMostPartials = 256;  // one a thread
 
 template <class T>
-__device__ __forceinline__ void load_tile(float (&v)[16], const T* mat, int64_t stride_r, int64_t stride_c, uint32_t m, uint32_t n,
-                                          uint32_t r0, uint32_t c0) {
+__global__ void __launch_bounds__(256) scale_kernel(const T* __restrict__ x, int64_t stride_b, int64_t stride_r, int64_t stride_c,
+                                                    uint32_t m, uint32_t n, const double* __restrict__ partial, uint32_t partials,
+                                                    double eps, __half* __restrict__ out, uint32_t ld, __half* __restrict__ out_t,
+                                                    uint32_t ld_t) {
+    __shared__ float tile[64][65];
+    __shared__ double part[8];
+    grid_launch_next();
+    const T* mat = x + blockIdx.z * stride_b;
+    const uint32_t r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
     const bool by_row = stride_c <= stride_r;
+    float v[16];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
+    for (int k = 0; k < 16; ++k) {  // the caller's matrix: nothing before this launch writes it
         const int i = threadIdx.x + k * 256, r = by_row ? i / 64 : i % 64, c = by_row ? i % 64 : i / 64;
         v[k] = r0 + r < m && c0 + c < n ? to_f32(mat[static_cast<int64_t>(r0 + r) * stride_r + static_cast<int64_t>(c0 + c) * stride_c]) : 0.f;
     }
-}
-
-__device__ __forceinline__ void scale_tile(const float (&v)[16], const double* partial, uint32_t partials, double eps, bool by_row,
-                                           uint32_t m, uint32_t n, uint32_t r0, uint32_t c0, __half* hi, uint32_t ld, __half* hi_t,
-                                           uint32_t ld_t) {
-    __shared__ float tile[64][65];
-    __shared__ double part[8];
-    double sum = threadIdx.x < partials ? partial[threadIdx.x] : 0.0;
+    grid_wait();
+    double sum = threadIdx.x < partials ? partial[blockIdx.z * partials + threadIdx.x] : 0.0;
 #pragma unroll
     for (int d = 16; d; d /= 2) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-    __syncthreads();
     if (threadIdx.x % 32 == 0) part[threadIdx.x / 32] = sum;
     __syncthreads();
     sum = 0;
@@ -122,38 +141,27 @@ __device__ __forceinline__ void scale_tile(const float (&v)[16], const double* p
         tile[r][c] = static_cast<float>(v[k] * factor);
     }
     __syncthreads();
-#pragma unroll 4
-    for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-        const uint32_t a = i / 32, b = i % 32 * 2;  // ld is a multiple of 8: a pair is inside or outside
-        __half2 h, l;
-        if (r0 + a < m && c0 + b < ld) {
-            split(tile[a][b], h.x, l.x);
-            split(tile[a][b + 1], h.y, l.y);
+    __half* hi = out + static_cast<uint64_t>(blockIdx.z) * 2 * m * ld;
+    __half* hi_t = out_t + static_cast<uint64_t>(blockIdx.z) * 2 * n * ld_t;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {  // 8 values a store; ld and ld_t are multiples of 8
+        const uint32_t i = threadIdx.x + k * 256, a = i / 8, b = i % 8 * 8;
+        Half8 h, l;
+        if (r0 + a < m && c0 + b < n) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) split(tile[a][b + q], h.h[q], l.h[q]);
             const uint64_t at = static_cast<uint64_t>(r0 + a) * ld + c0 + b;
-            *reinterpret_cast<__half2*>(hi + at) = h;
-            *reinterpret_cast<__half2*>(hi + static_cast<uint64_t>(m) * ld + at) = l;
+            *reinterpret_cast<uint4*>(hi + at) = h.u;
+            *reinterpret_cast<uint4*>(hi + static_cast<uint64_t>(m) * ld + at) = l.u;
         }
-        if (c0 + a < n && r0 + b < ld_t) {
-            split(tile[b][a], h.x, l.x);
-            split(tile[b + 1][a], h.y, l.y);
+        if (c0 + a < n && r0 + b < m) {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) split(tile[b + q][a], h.h[q], l.h[q]);
             const uint64_t at = static_cast<uint64_t>(c0 + a) * ld_t + r0 + b;
-            *reinterpret_cast<__half2*>(hi_t + at) = h;
-            *reinterpret_cast<__half2*>(hi_t + static_cast<uint64_t>(n) * ld_t + at) = l;
+            *reinterpret_cast<uint4*>(hi_t + at) = h.u;
+            *reinterpret_cast<uint4*>(hi_t + static_cast<uint64_t>(n) * ld_t + at) = l.u;
         }
     }
-}
-
-template <class T>
-__global__ void __launch_bounds__(256) scale_kernel(const T* __restrict__ x, int64_t stride_b, int64_t stride_r, int64_t stride_c,
-                                                    uint32_t m, uint32_t n, const double* __restrict__ partial, uint32_t partials,
-                                                    double eps, __half* __restrict__ out, uint32_t ld, __half* __restrict__ out_t,
-                                                    uint32_t ld_t) {
-    grid_launch_next();
-    float v[16];
-    load_tile(v, x + blockIdx.z * stride_b, stride_r, stride_c, m, n, blockIdx.y * 64, blockIdx.x * 64);  // the caller's matrix
-    grid_wait();
-    scale_tile(v, partial + blockIdx.z * partials, partials, eps, stride_c <= stride_r, m, n, blockIdx.y * 64, blockIdx.x * 64,
-               out + static_cast<uint64_t>(blockIdx.z) * 2 * m * ld, ld, out_t + static_cast<uint64_t>(blockIdx.z) * 2 * n * ld_t, ld_t);
 }
 
 // ------------------------------------------------------------------ products
@@ -172,7 +180,7 @@ struct Job {
     int last_t;
 };
 
-constexpr int kTile = 128, kSlice = 64;  // rows of a tile, k of a stage
+constexpr uint32_t kTile = 128, kSlice = 64;  // rows of a tile, k of a stage
 constexpr int kThreads = 256;
 
 template <int kBN>  // columns of a tile
@@ -199,11 +207,6 @@ __device__ __forceinline__ uint32_t peer_address(const void* p, uint32_t rank) {
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(tc::smem_u32(p)), "r"(rank));
     return at;
 }
-
-union Half8 {
-    __half h[8];
-    uint4 u;
-};
 
 // A warp's 8 columns on their way to transposed storage: 32 rows of each, high and low parts.
 struct alignas(16) WarpTile {
@@ -565,6 +568,119 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (!ok) atomicAdd(stalls, 1u);
 }
 
+// Large matrices: tiles of 256 x 256, one a block, two accumulators of 128 x 256 that fill tensor memory.  What bounds
+// the 128 x 128 tiles is their operands' way from L2 (48 bytes a clock and SM when all SMs read): 64 KB for 768 clocks of
+// products.  Here 64 KB, a slice of 32, feed 1,536 clocks.
+struct Wide {
+    static constexpr uint32_t kSide = 256, kSlice = 32;
+    static constexpr int kStages = 3;
+    static constexpr int kPart = kSide * kSlice * 2, kStageBytes = 4 * kPart;  // A high, A low, B high, B low
+    static constexpr int kSmem = 1024 + kStages * kStageBytes + 256;
+    static_assert(8 * sizeof(WarpBlock) <= kStages * kStageBytes, "the warps' blocks of results take the place of the operands");
+};
+
+template <int kProduct>
+__global__ void __launch_bounds__(kThreads, 1)
+    wide_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, Job job, unsigned int* stalls) {
+    constexpr int kStages = Wide::kStages;
+    constexpr uint32_t kSide = Wide::kSide;
+    extern __shared__ uint8_t raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    uint64_t* full = reinterpret_cast<uint64_t*>(base + kStages * Wide::kStageBytes);
+    uint64_t* empty = full + kStages;
+    uint64_t* done = empty + kStages;
+    uint32_t* slot = reinterpret_cast<uint32_t*>(done + 1);
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const uint32_t batch = blockIdx.y;
+    uint32_t ti, tj;
+    {
+        uint32_t t = blockIdx.x;
+        if constexpr (kProduct == kGram || kProduct == kPoly) {
+            ti = 0;
+            for (uint32_t left = job.tiles_n; t >= left; --left, ++ti) t -= left;
+            tj = ti + t;
+        } else {
+            ti = t % job.tiles_m;
+            tj = t / job.tiles_m;
+        }
+    }
+    const uint32_t slices = (job.k + Wide::kSlice - 1) / Wide::kSlice;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < kStages; ++i) {
+            tc::mbar_init(&full[i], 1);
+            tc::mbar_init(&empty[i], 1);
+        }
+        tc::mbar_init(done, 1);
+        tc::mbar_init_fence();
+        tc::prefetch_map(&map_a);
+        tc::prefetch_map(&map_b);
+    }
+    if (warp == 1) tc::tmem_alloc(slot, 512);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = *slot;
+    grid_launch_next();
+    grid_wait();
+    bool ok = true;
+    if (warp == 0 && tc::elect_one()) {
+        uint32_t it = 0;
+        for (uint32_t s = 0; s < slices; ++s, ++it) {
+            const uint32_t i = it % kStages;
+            if (!(ok = tc::mbar_wait(&empty[i], (it / kStages & 1) ^ 1))) break;
+            uint8_t* st = base + i * Wide::kStageBytes;
+            tc::mbar_expect_tx(&full[i], Wide::kStageBytes);
+            for (int part = 0; part < 2; ++part) {
+                tc::tma_load_3d(st + part * Wide::kPart, &map_a, &full[i], s * Wide::kSlice, ti * kSide, batch * 2 + part);
+                tc::tma_load_3d(st + (2 + part) * Wide::kPart, &map_b, &full[i], s * Wide::kSlice, tj * kSide, batch * 2 + part);
+            }
+        }
+        for (uint32_t s = it < kStages ? 0 : it - kStages; s < it; ++s)  // a load in flight lands before the block goes on
+            ok = tc::mbar_wait(&full[s % kStages], s / kStages & 1) && ok;
+    } else if (warp == 1 && tc::elect_one()) {
+        constexpr uint32_t idesc = tc::idesc_f16(kSide);
+        uint32_t it = 0;
+        for (uint32_t s = 0; s < slices; ++s, ++it) {
+            const uint32_t i = it % kStages;
+            if (!(ok = tc::mbar_wait(&full[i], it / kStages & 1))) break;
+            tc::fence_after();
+            const uint8_t* st = base + i * Wide::kStageBytes;
+            const uint64_t bh = tc::tile_desc64(st + 2 * Wide::kPart), bl = tc::tile_desc64(st + 3 * Wide::kPart);
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {  // rows 128 h and on
+                const uint64_t ah = tc::tile_desc64(st + h * (Wide::kPart / 2)), al = tc::tile_desc64(st + Wide::kPart + h * (Wide::kPart / 2));
+#pragma unroll
+                for (int kk = 0; kk < Wide::kSlice / 16; ++kk) {
+                    tc::mma_f16(tmem + h * kSide, al + 2 * kk, bh + 2 * kk, idesc, it > 0 || kk > 0);
+                    tc::mma_f16(tmem + h * kSide, ah + 2 * kk, bl + 2 * kk, idesc, true);
+                    tc::mma_f16(tmem + h * kSide, ah + 2 * kk, bh + 2 * kk, idesc, true);
+                }
+            }
+            tc::mma_commit(&empty[i]);
+        }
+        tc::mma_commit(done);
+    }
+    __syncwarp();
+    ok = tc::mbar_wait_warp(done, 0) && ok;
+    tc::fence_after();
+    __syncthreads();  // nobody reads the operands any more
+    const bool mirror = kProduct == kLast ? job.last_t : kProduct == kApply || tj != ti;
+    WarpBlock& mine = reinterpret_cast<WarpBlock*>(base)[warp];
+    const uint32_t at = tmem + (static_cast<uint32_t>((warp % 4) * 32) << 16) + warp / 4 * kSide;
+#pragma unroll 1
+    for (uint32_t c = 0; c < kSide; c += 32) {
+        uint32_t v[32];
+        tc::tmem_ld32(at + c, v);
+        tc::tmem_wait_ld();
+        emit_block<kProduct>(job, batch, ti * kSide + warp / 4 * kTile + (warp % 4) * 32, tj * kSide + c, mirror, v, mine, lane);
+    }
+    if (!ok) atomicAdd(stalls, 1u);
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    if (warp == 1) tc::tmem_free(tmem, 512);
+}
+
 // ----------------------------------------------------------------------- host
 
 uint32_t up8(uint32_t v) { return (v + 7) / 8 * 8; }
@@ -597,20 +713,32 @@ struct Layout {  // byte offsets of the workspace's parts
 };
 
 int map_pair(CUtensorMap* map, const void* p, uint32_t rows, uint32_t cols, uint32_t ld, uint64_t batch, uint32_t box_rows) {
+    const bool wide = box_rows == Wide::kSide;
     const uint64_t dims[3] = {cols, rows, batch * 2}, strides[2] = {ld * 2ull, static_cast<uint64_t>(rows) * ld * 2};
-    const uint32_t box[3] = {kSlice, box_rows, 1};
-    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p, dims, strides, box);
+    const uint32_t box[3] = {wide ? Wide::kSlice : kSlice, box_rows, 1};
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, p, dims, strides, box, wide ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
 }
 
 template <int kProduct, int kBN, int kSplit>
 int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const Job& job, uint32_t tiles, uint32_t batch, int device,
                    unsigned int* stalls, cudaStream_t st) {
-    constexpr auto* kernel = product_kernel<kProduct, kBN, kSplit>;
-    if (int rc = allow_smem<kernel>(Shape<kBN>::kSmem, device, "orthogonalize")) return rc;
+    constexpr auto* kernel = [] {
+        if constexpr (kBN == Wide::kSide)
+            return wide_kernel<kProduct>;
+        else
+            return product_kernel<kProduct, kBN, kSplit>;
+    }();
+    constexpr int kBytes = [] {
+        if constexpr (kBN == Wide::kSide)
+            return Wide::kSmem;
+        else
+            return Shape<kBN>::kSmem;
+    }();
+    if (int rc = allow_smem<kernel>(kBytes, device, "orthogonalize")) return rc;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(tiles * kSplit, batch);
     cfg.blockDim = dim3(kThreads);
-    cfg.dynamicSmemBytes = Shape<kBN>::kSmem;
+    cfg.dynamicSmemBytes = kBytes;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
     at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -624,40 +752,50 @@ int launch_product(const CUtensorMap& ma, const CUtensorMap& mb, const Job& job,
 }
 
 struct Operand {  // a stored pair as either side of a product
-    CUtensorMap rows128, rows64;
-    int encode(const void* p, uint32_t rows, uint32_t cols, uint32_t ld, uint64_t batch) {
-        if (int rc = map_pair(&rows128, p, rows, cols, ld, batch, 128)) return rc;
-        return map_pair(&rows64, p, rows, cols, ld, batch, 64);
-    }
+    const void* p;
+    uint32_t rows, cols, ld;
+    uint64_t batch;
+    int map(CUtensorMap* m, uint32_t box_rows) const { return map_pair(m, p, rows, cols, ld, batch, box_rows); }
 };
 
-uint32_t count_tiles(bool symmetric, Job& job, uint32_t bn) {
-    job.tiles_m = (job.m + kTile - 1) / kTile;
+uint32_t count_tiles(bool symmetric, Job& job, uint32_t bm, uint32_t bn) {
+    job.tiles_m = (job.m + bm - 1) / bm;
     job.tiles_n = (job.n + bn - 1) / bn;
     if (!symmetric) return job.tiles_m * job.tiles_n;
     uint32_t tiles = 0;
-    for (uint32_t i = 0; i < job.tiles_m; ++i) tiles += job.tiles_n - i * (kTile / bn);
+    for (uint32_t i = 0; i < job.tiles_m; ++i) tiles += job.tiles_n - i * (bm / bn);
     return tiles;
 }
 
-// Narrow tiles, and k split over a cluster where it is long enough to pay for that, as long as all blocks run at once; wide
-// tiles, which read their operands less often, where there are more than that.
+// Narrow tiles, and k split over a cluster where it is long enough to pay for that, as long as all blocks run at once; else
+// wide ones, which read their operands less often: 256 x 256 where they fill two thirds of the SMs (a product of 2,048 x
+// 4,096: 128 tiles 57 us, 512 of 128 x 128 101 us; a Gram matrix of 2,048: 36 and 136 tiles, 46 us with the latter).
 template <int kProduct>
 int launch_sized(const Operand& a, const Operand& b, Job job, uint32_t batch, int device, unsigned int* stalls, cudaStream_t st) {
-    const int sms = sm_count(device);
+    const uint64_t sms = sm_count(device);
     const bool symmetric = kProduct == kGram || kProduct == kPoly;
-    const uint64_t narrow = static_cast<uint64_t>(count_tiles(symmetric, job, 64)) * batch;
-    if (narrow > static_cast<uint32_t>(sms)) {
-        const uint32_t tiles = count_tiles(symmetric, job, 128);
-        return launch_product<kProduct, 128, 1>(a.rows128, b.rows128, job, tiles, batch, device, stalls, st);
+    CUtensorMap ma, mb;
+    auto maps = [&](uint32_t rows_a, uint32_t rows_b) {
+        const int rc = a.map(&ma, rows_a);
+        return rc ? rc : b.map(&mb, rows_b);
+    };
+    const uint64_t narrow = static_cast<uint64_t>(count_tiles(symmetric, job, kTile, 64)) * batch;
+    if (narrow <= sms) {
+        if (int rc = maps(kTile, 64)) return rc;
+        const uint32_t tiles = static_cast<uint32_t>(narrow / batch), slices = (job.k + kSlice - 1) / kSlice;
+        // A slice takes 1,000 clocks, joining a cluster's shares 3,500.
+        if (narrow * 4 <= sms && slices >= 8) return launch_product<kProduct, 64, 4>(ma, mb, job, tiles, batch, device, stalls, st);
+        if (narrow * 2 <= sms && slices >= 8) return launch_product<kProduct, 64, 2>(ma, mb, job, tiles, batch, device, stalls, st);
+        return launch_product<kProduct, 64, 1>(ma, mb, job, tiles, batch, device, stalls, st);
     }
-    const uint32_t tiles = static_cast<uint32_t>(narrow / batch), slices = (job.k + kSlice - 1) / kSlice;
-    // A slice takes 1,000 clocks, joining a cluster's shares 3,500.
-    if (narrow * 4 <= static_cast<uint32_t>(sms) && slices >= 8)
-        return launch_product<kProduct, 64, 4>(a.rows128, b.rows64, job, tiles, batch, device, stalls, st);
-    if (narrow * 2 <= static_cast<uint32_t>(sms) && slices >= 8)
-        return launch_product<kProduct, 64, 2>(a.rows128, b.rows64, job, tiles, batch, device, stalls, st);
-    return launch_product<kProduct, 64, 1>(a.rows128, b.rows64, job, tiles, batch, device, stalls, st);
+    const uint32_t wide = count_tiles(symmetric, job, Wide::kSide, Wide::kSide);
+    if (static_cast<uint64_t>(wide) * batch * 3 >= sms * 2) {
+        if (int rc = maps(Wide::kSide, Wide::kSide)) return rc;
+        return launch_product<kProduct, Wide::kSide, 1>(ma, mb, job, wide, batch, device, stalls, st);
+    }
+    if (int rc = maps(kTile, kTile)) return rc;
+    const uint32_t tiles = count_tiles(symmetric, job, kTile, kTile);
+    return launch_product<kProduct, kTile, 1>(ma, mb, job, tiles, batch, device, stalls, st);
 }
 
 template <class T>
@@ -698,13 +836,9 @@ int run(const nesle_orth_args& a, cudaStream_t st) {
     }
     if (rc) return rc;
     __half *gram = reinterpret_cast<__half*>(ws + lay.gram), *poly = reinterpret_cast<__half*>(ws + lay.poly);
-    Operand op_x[2], op_xt[2], op_g, op_p;
-    for (int i = 0; i < 2; ++i) {
-        if ((rc = op_x[i].encode(ws + lay.x[i], m, n, lay.ld_n, batch))) return rc;
-        if ((rc = op_xt[i].encode(ws + lay.xt[i], n, m, lay.ld_m, batch))) return rc;
-    }
-    if ((rc = op_g.encode(gram, m, m, lay.ld_m, batch))) return rc;
-    if ((rc = op_p.encode(poly, m, m, lay.ld_m, batch))) return rc;
+    const Operand op_x[2] = {{ws + lay.x[0], m, n, lay.ld_n, batch}, {ws + lay.x[1], m, n, lay.ld_n, batch}};
+    const Operand op_xt[2] = {{ws + lay.xt[0], n, m, lay.ld_m, batch}, {ws + lay.xt[1], n, m, lay.ld_m, batch}};
+    const Operand op_g{gram, m, m, lay.ld_m, batch}, op_p{poly, m, m, lay.ld_m, batch};
     for (int step = 0; step < a.steps; ++step) {
         const int from = step & 1, to = from ^ 1;
         Job g{};

@@ -121,6 +121,11 @@ __device__ __forceinline__ uint64_t tile_desc(const void* tile) {
     return static_cast<uint64_t>((smem_u32(tile) >> 4) & 0x3FFF) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
+// The same for rows of 64 bytes, 64-byte swizzle: groups of 8 rows are 512 bytes apart.
+__device__ __forceinline__ uint64_t tile_desc64(const void* tile) {
+    return static_cast<uint64_t>((smem_u32(tile) >> 4) & 0x3FFF) | (1ull << 16) | (32ull << 32) | (1ull << 46) | (4ull << 61);
+}
+
 constexpr uint32_t kTypeF16 = 0, kTypeU8 = 0, kTypeS8 = 1;
 // Instruction descriptors: M = 128, both operands K-major.
 __host__ __device__ constexpr uint32_t idesc_f16(uint32_t n) { return (1u << 4) | (kTypeF16 << 7) | (kTypeF16 << 10) | ((n >> 3) << 17) | (8u << 24); }

@@ -61,7 +61,7 @@ def momentum(*shape, seed=0, dtype=torch.float32, scale=1e-3):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows,cols", [(1, 1), (1, 50), (50, 1), (3, 5), (7, 256), (64, 64), (127, 129), (128, 128), (129, 127),
-                                       (130, 64), (200, 1000), (256, 512), (512, 256), (512, 2048), (1000, 300), (333, 2049)])
+                                       (130, 64), (200, 1000), (256, 512), (512, 256), (512, 2048), (1000, 300), (333, 2049), (1100, 6500), (3700, 3600)])
 def test_matches_64_bits(rows, cols):
     x = momentum(rows, cols, seed=rows + cols)
     check(ops.orthogonalize(x), x)
