@@ -306,6 +306,11 @@ __device__ __forceinline__ uint32_t pair_mask(int i, int r0, int r1) {
 // loads (TMA, two blocks of 16 tokens ahead), the decays, Q K^T and K K^T,
 // and M = (I + (D o K K^T) beta)^-1 by substitution, so that the triangular
 // solve is a product too.  One barrier a chunk.
+//
+// 1,024 envs x 4 heads x 128 tokens of 64 x 64, keeping states and errors for
+// the gradients: 307 us, 3.5 TB/s; instruction issue bounds it (44% of the slots
+// at 13 warps an SM).  4 envs x 4 heads x 4,096 tokens of 128 x 128: 551 us,
+// 2.2 us a chunk, a chain of products as long as the helper's work.
 
 constexpr int kLdM = kC + 8;  // bf16 of a row of a 16 x 16 operand tile
 
@@ -834,6 +839,10 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
 // rows: dS goes through shared memory in fp32, U and ubar as bf16 terms, S comes
 // from the checkpoint.  A helper prepares the next chunk (decays, Q K^T, K K^T,
 // N) and finishes dg and dbeta of the last.  Two barriers a chunk.
+//
+// 1,024 envs x 4 heads x 128 tokens of 64 x 64: 815 us, bounded by instruction
+// latency at 10 warps an SM (168 registers a thread, 100 KB of shared memory a
+// block): 36% of the issue slots, tensor cores 20% busy.
 
 struct alignas(16) BackChunk {
     __nv_bfloat16 n[3][kC][kLdM];    // N, by terms
