@@ -848,7 +848,7 @@ struct alignas(16) BackChunk {
     __nv_bfloat16 n[3][kC][kLdM];    // N, by terms
     __nv_bfloat16 att[3][kC][kLdM];  // scale D_ij q_i.k_j (i >= j), by terms
     float fa[kC][kC], fp[kC][kC];    // scale D_ij (i >= j), beta_i D_ij (i > j); zero outside the chunk
-    float qk[kC][kC], kk[kC][kC];
+    float qk[kC][kC], kk[kC][kC];    // q_i.k_j, k_i.k_j
     float gamma[kC], eta[kC], beta[kC];
     float keep;
     int block, r0, r1, fresh;
@@ -866,9 +866,9 @@ struct BackwardSmem {
     static constexpr int kWarpsK = DK / 16, kWarpsV = DV / 16, kWarps = DK > DV ? kWarpsK : kWarpsV;
     static constexpr int NT = Terms<T>::n;
     static constexpr bool kInPlace = NT == 1;
-    // bf16 is used as fetched: warps on one block, the helper on the next, one on its way.  Others are turned into terms on
-    // arrival, for two blocks, and one buffer is enough.
-    static constexpr int kBuffers = kInPlace ? 3 : 1;
+    // bf16 is used as fetched: warps on one block, the helper on the next, one on its way, for which heads of 128 have no
+    // room.  Others are turned into terms on arrival, for two blocks, and one buffer is enough.
+    static constexpr int kBuffers = kInPlace ? (DK + DV > 192 ? 2 : 3) : 1;
     static constexpr int kTileK = Fetch<T, DK>::kElements, kTileV = Fetch<T, DV>::kElements;
     static constexpr size_t kRaw = (size_t)(2 * kTileK + kTileV) * sizeof(T);
     static constexpr int kTk = DK + 8, kTv = DV + 8;  // rows of terms
@@ -888,7 +888,8 @@ struct BackwardSmem {
     };
     static constexpr size_t kOut = sizeof(T) == 2 ? (size_t)kC * kLdOut * 2 : 0;  // of a warp
     static constexpr size_t kBase = 1024 + kBuffers * kRaw + 2 * kTermBlock + 2 * kTile3 + kState + sizeof(Shared) + kWarps * kOut;
-    // S is fetched a chunk ahead where it has room, else read from global memory when needed.
+    // S is fetched a chunk ahead where it has room, else read from global memory when needed (1,024 envs of 64 x 64: 1,250 us
+    // against 815, although that leaves room for a third block on an SM).
     static constexpr bool kFetchState = kBase + kFetched <= 227 * 1024;
     static constexpr size_t kBytes = kBase + (kFetchState ? kFetched : 0);
     static_assert(kRaw % 1024 == 0 && kFetched % 1024 == 0 && kTermBlock % 16 == 0 && kTile3 % 16 == 0 && kState % 16 == 0, "layout");
@@ -911,7 +912,7 @@ __device__ __forceinline__ void add_over_rows(float (&x)[4]) {
 }
 
 template <class T, int DK, int DV>
-__global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : DV) <= 64 ? 2 : 1)
+__global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <= 64 ? 2 : 1)
     scan_backward_kernel(const Scan p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q,
                          const __grid_constant__ CUtensorMap map_o, const __grid_constant__ CUtensorMap map_s) {
     using L = BackwardSmem<T, DK, DV>;
@@ -973,7 +974,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
         uint32_t starts = 0;
         int64_t b = blocks, turn_of_block = -1;
         int r1 = 0;
-        fetch(blocks - 1);
+        if (L::kBuffers == 3) fetch(blocks - 1);
         // the chunk before the last one prepared
         auto prepare = [&](BackChunk& ch) {
             if (r1 == 0) {
@@ -984,6 +985,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                 }
                 ++turn_of_block;
                 r1 = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
+                fetch(L::kBuffers == 3 ? b - 1 : b);  // the warps are on b + 1
                 gates = next;
                 if (b > 0) next = get_gates.load((b - 1) * kC, p.t, lane);
                 decay = gates.decay();
@@ -1006,7 +1008,6 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                     tc::fence_async_smem();
                     __syncwarp();
                 }
-                fetch(b - 1);
             }
             const uint32_t earlier = starts & ((1u << r1) - 1);
             const int r0 = earlier ? 31 - __clz(earlier) : 0;
@@ -1382,6 +1383,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                         if (state) {
                             if (fetch_state) {
                                 x = *reinterpret_cast<const float2*>(fetched + col / 32 * (DK * 32) + kk * 32 + ((col / 4 % 8) ^ (kk & 7)) * 4 + col % 4);
+                            } else if (!L::kFetchState && p.dv % 2 == 0) {
+                                if (kk < p.dk && col < p.dv) x = __ldcs(reinterpret_cast<const float2*>(s0 + kk * p.dv + col));
                             } else if (kk < p.dk) {
                                 if (col < p.dv) x.x = s0[kk * p.dv + col];
                                 if (col + 1 < p.dv) x.y = s0[kk * p.dv + col + 1];
@@ -1522,10 +1525,14 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, (DK > DV ? DK : 
                         for (int x = 0; x < 3; ++x) ya[x][z] = tmp[x];
                     }
                 }
+                // Of large heads dS comes back from shared memory: its registers are the others' in between (128 x 128: 364
+                // bytes of spills without, 196 with; 64 x 64 has few and is 8% faster without).
+                constexpr bool kBack = DK > 64 || DV > 64;
 #pragma unroll
                 for (int i = 0; i < DK / 8; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) ds[i].v[e] *= keep;
+                    for (int e = 0; e < 4; ++e)
+                        ds[i].v[e] = keep * (kBack ? st[(i * 8 + quad * 2 + e % 2) * L::kLdS + c0 + row + e / 2 * 8] : ds[i].v[e]);
 #pragma unroll
                 for (int s = 0; s < DK / 16; s += 2) {
                     using P = Pairs<3, 3, NT>;
