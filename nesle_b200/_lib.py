@@ -106,6 +106,8 @@ SIGNATURES = {
     "nesle_int8_workspace": (ctypes.c_uint64, [ctypes.c_void_p]),
     "nesle_delta_step": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "nesle_delta_scan": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
+    "nesle_delta_scan_split": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    "nesle_delta_split_floats": (ctypes.c_uint64, [ctypes.c_void_p]),
     "nesle_delta_scan_backward": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p]),
     "nesle_delta_error_floats": (ctypes.c_uint64, [ctypes.c_void_p]),
     "nesle_delta_checkpoint_floats": (ctypes.c_uint64, [ctypes.c_void_p]),

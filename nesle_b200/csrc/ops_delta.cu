@@ -178,6 +178,7 @@ Scan to_scan(const nesle_delta_args& a, bool backward) {
     p.d_o = a.d_o, p.d_final = a.d_final, p.dq = a.dq, p.dk_out = a.d_k, p.dv_out = a.d_v, p.dg = a.dg, p.dbeta = a.dbeta;
     p.dstate = a.dstate;
     p.device = a.device;
+    p.segments = 1, p.per = (p.t + kC - 1) / kC;
     return p;
 }
 
@@ -223,7 +224,15 @@ uint64_t nesle_delta_error_floats(const nesle_delta_args* a) {
     return a ? a->n * a->h * ((a->t + delta::kC - 1) / delta::kC) * ((a->dv + 15) / 16) * 16 * delta::kC : 0;
 }
 
-int nesle_delta_scan(const nesle_delta_args* args, void* stream) {
+uint64_t nesle_delta_split_floats(const nesle_delta_args* a) {
+    if (!a || delta::check_common(a->dtype, a->n, a->h, a->dk, a->dv) || !a->t || a->t > 0x7FFFFFFFull || !a->n || !a->h) return 0;
+    const int segments = delta::count_segments((int64_t)a->t, (int64_t)(a->n * a->h), (int)a->dk, (int)a->dv, sm_count(a->device));
+    return a->n * a->h * (uint64_t)(segments - 1) * (a->dk * (a->dk + a->dv) + 1);
+}
+
+int nesle_delta_scan(const nesle_delta_args* args, void* stream) { return nesle_delta_scan_split(args, nullptr, stream); }
+
+int nesle_delta_scan_split(const nesle_delta_args* args, float* workspace, void* stream) {
     return guarded([&]() -> int {
         if (!args) return invalid("delta_scan: null argument");
         const nesle_delta_args& a = *args;
@@ -234,7 +243,15 @@ int nesle_delta_scan(const nesle_delta_args* args, void* stream) {
         if (!on.ok) return invalid("delta_scan: device ordinal out of range");
         if (!a.errors != !a.checkpoints) return invalid("delta_scan: errors and checkpoints go together");
         if (reinterpret_cast<uintptr_t>(a.errors) % 16) return invalid("delta_scan: errors must be 16-byte aligned");
+        if (reinterpret_cast<uintptr_t>(workspace) % 4) return invalid("delta_scan: workspace must be aligned");
         delta::Scan p = delta::to_scan(a, false);
+        if (workspace && a.t && a.t <= 0x7FFFFFFFull) {
+            p.segments = delta::count_segments(p.t, p.n * p.h, p.dk, p.dv, sm_count(a.device));
+            const int64_t all = (p.t + delta::kC - 1) / delta::kC;
+            p.per = (all + p.segments - 1) / p.segments;
+            p.ends = workspace;
+            p.restarts = reinterpret_cast<int*>(workspace + p.n * p.h * (p.segments - 1) * p.dk * (p.dk + p.dv));
+        }
         if (int rc = stall_counter(a.device, &p.stalls)) return rc;
         cudaStream_t st = static_cast<cudaStream_t>(stream);
         if (a.dtype == NESLE_F32) return delta::launch_forward<float>(p, st);

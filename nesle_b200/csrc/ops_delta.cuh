@@ -65,6 +65,10 @@ struct Scan {
     const float* d_final;
     void *dq, *dk_out, *dv_out;
     float *dg, *dbeta, *dstate;
+    int segments;        // 1, or what a sequence is cut into (launch_split)
+    int64_t per;         // blocks of 16 tokens of a segment
+    float* ends;         // [n][h][segments - 1]: the end of a segment (dk x dv), and what it makes of a state (dk x dk)
+    int* restarts;       // [n][h][segments - 1]: an episode starts in the segment
     unsigned int* stalls;
     int device;
 };
@@ -309,8 +313,9 @@ __device__ __forceinline__ uint32_t pair_mask(int i, int r0, int r1) {
 //
 // 1,024 envs x 4 heads x 128 tokens of 64 x 64, keeping states and errors for
 // the gradients: 298 us, 3.6 TB/s; instruction issue bounds it (44% of the slots
-// at 13 warps an SM).  4 envs x 4 heads x 4,096 tokens of 128 x 128: 546 us,
-// 2.2 us a chunk, a chain of products as long as the helper's work.
+// at 13 warps an SM).  4 envs x 4 heads x 4,096 tokens of 128 x 128: 250 us in
+// 6 segments (count_segments), 525 in one: 2.05 us a chunk where a block has an SM
+// to itself, a chain of products as long as the helper's work.
 
 constexpr int kLdM = kC + 8;  // bf16 of a row of a 16 x 16 operand tile
 
@@ -481,7 +486,7 @@ struct ForwardSmem {
     static_assert(kRaw % 1024 == 0 && kTerms % 16 == 0 && kOut % 16 == 0 && kOut >= kC * kLdOut * 2, "layout");
 };
 
-template <class T, int DK, bool kRegular>
+template <class T, int DK, bool kRegular, bool kEnds>
 __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
     scan_forward_kernel(const Scan p, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_q,
                         const __grid_constant__ CUtensorMap map_v) {
@@ -500,8 +505,16 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
     float* out_tiles = reinterpret_cast<float*>(&hs + 1);
     uint64_t* arrived = reinterpret_cast<uint64_t*>(out_tiles + warps * L::kOut / 4);  // a buffer's rows are there
     const int64_t seq = blockIdx.x, n = seq / p.h, h = seq % p.h;
-    const int first_col = blockIdx.y * L::kWidth, cols = kRegular ? L::kWidth : min(L::kWidth, dv - first_col);
-    const int64_t blocks = (p.t + kC - 1) / kC;
+    const int value_blocks = (dv + L::kWidth - 1) / L::kWidth;
+    const bool unit = kEnds && (int)blockIdx.y >= value_blocks;  // from a unit matrix, with no values: what the segment makes of a state
+    const int wide = unit ? dk : dv, first_col = ((int)blockIdx.y - (unit ? value_blocks : 0)) * L::kWidth;
+    const int cols = kRegular ? L::kWidth : min(L::kWidth, wide - first_col);
+    const int segment = (int)blockIdx.z;
+    if (unit && segment == 0) return;  // the state before the first token is known
+    const int64_t all = (p.t + kC - 1) / kC, b0 = segment * p.per;  // blocks are counted from the segment's first
+    const int64_t blocks = all - b0 < p.per ? all - b0 : p.per, t0 = b0 * kC;
+    const int64_t slot = seq * (p.segments - 1) + segment;
+    auto end_of = [&](int64_t at) { return p.ends + at * dk * (dk + dv); };
     auto raw_tile = [&](int64_t b) { return reinterpret_cast<T*>(smem + b % L::kBuffers * L::kRaw); };
     // term x of K (which = 0) or Q (1) of a block as an operand
     auto operand = [&](int64_t b, int which, int x) {
@@ -530,20 +543,21 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
             if (b >= blocks) return;
             T* to = raw_tile(b);
             uint64_t* bar = &arrived[b % L::kBuffers];
-            const int count = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
-            if (aligned && lane == 0) tc::mbar_expect_tx(bar, (uint32_t)L::kRaw);
-            Fetch<T, DK>::run(to, &map_k, k, p.sk.t, n, h, 0, b * kC, count, dk, aligned, bar, lane);
-            Fetch<T, DK>::run(to + L::kTileK, &map_q, q, p.sq.t, n, h, 0, b * kC, count, dk, aligned, bar, lane);
-            Fetch<T, L::kWidth>::run(to + 2 * L::kTileK, &map_v, v, p.sv.t, n, h, first_col, b * kC, count, cols, aligned, bar, lane);
+            const int64_t t = t0 + b * kC;
+            const int count = (int)(p.t - t < kC ? p.t - t : kC);
+            if (aligned && lane == 0) tc::mbar_expect_tx(bar, (uint32_t)((kEnds ? L::kTileK : 2 * L::kTileK) + (unit ? 0 : L::kTileV)) * sizeof(T));
+            Fetch<T, DK>::run(to, &map_k, k, p.sk.t, n, h, 0, t, count, dk, aligned, bar, lane);
+            if constexpr (!kEnds) Fetch<T, DK>::run(to + L::kTileK, &map_q, q, p.sq.t, n, h, 0, t, count, dk, aligned, bar, lane);
+            if (!unit) Fetch<T, L::kWidth>::run(to + 2 * L::kTileK, &map_v, v, p.sv.t, n, h, first_col, t, count, cols, aligned, bar, lane);
         };
         fetch(0);
         fetch(1);
         const GatePointers get_gates(p, n, h, lane);
-        Gates gates{}, next = get_gates.load(0, p.t, lane);
+        Gates gates{}, next = get_gates.load(t0, p.t, lane);
         float decay = 1.f;
         uint32_t starts = 0;
         int64_t b = -1;
-        int r0 = 0, count = 0;
+        int r0 = 0, count = 0, restarts = 0;
         for (int turn = 0;; ++turn) {
             Chunk& ch = chunks[turn & 1];
             if (r0 >= count) {  // the next block of 16 tokens
@@ -554,9 +568,9 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                     __syncthreads();
                     break;
                 }
-                count = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
+                count = (int)(p.t - t0 - b * kC < kC ? p.t - t0 - b * kC : kC);
                 gates = next;
-                next = get_gates.load((b + 1) * kC, p.t, lane);
+                next = get_gates.load(t0 + (b + 1) * kC, p.t, lane);
                 decay = gates.decay();
                 starts = gates.starts();
                 if (aligned && !tc::mbar_wait_warp(&arrived[b % L::kBuffers], b / L::kBuffers & 1)) {
@@ -572,11 +586,12 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                 if constexpr (!L::kInPlace) {
                     __nv_bfloat16* to = terms + (b & 1) * 2 * NT * kC * L::kLdTerm;
                     to_terms_warp<T, DK>(to, L::kLdTerm, raw_tile(b), lane);
-                    to_terms_warp<T, DK>(to + NT * kC * L::kLdTerm, L::kLdTerm, raw_tile(b) + L::kTileK, lane);
+                    if constexpr (!kEnds) to_terms_warp<T, DK>(to + NT * kC * L::kLdTerm, L::kLdTerm, raw_tile(b) + L::kTileK, lane);
                     __syncwarp();
                 }
             }
             const bool fresh = starts >> r0 & 1;
+            restarts |= fresh;
             const uint32_t later = starts & ~((2u << r0) - 1);
             const int r1 = later ? min(count, __ffs(later) - 1) : count;
             chunk_decays(hs.d, ch.gamma, ch.eta, ch.beta, ch.keep, within(lane, r0, r1) ? decay : 1.f, gates.beta, r0, r1, fresh, lane);
@@ -590,11 +605,14 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
                     load_rows(ka[x], operand(b, 0, x), st * 16, lane);
-                    load_rows(qa[x], operand(b, 1, x), st * 16, lane);
+                    if constexpr (!kEnds) load_rows(qa[x], operand(b, 1, x), st * 16, lane);
                 }
                 uint32_t kb[2][NT][2];
                 as_rows(kb, ka);
-                mma2_zip<3, NO>(kk, ka, kb, qk, qa, kb);
+                if constexpr (kEnds)
+                    mma2<3>(kk, ka, kb);
+                else
+                    mma2_zip<3, NO>(kk, ka, kb, qk, qa, kb);
             }
             __syncwarp();
 #pragma unroll
@@ -607,6 +625,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                     const bool in0 = within(i, r0, r1) && j >= r0, in1 = within(i, r0, r1) && j + 1 >= r0;  // and j <= i
                     *reinterpret_cast<float2*>(&hs.b[i][j]) = make_float2(in0 && i > j ? d.x * be.x * kk[c].v[half * 2] : 0.f,
                                                                           in1 && i > j + 1 ? d.y * be.y * kk[c].v[half * 2 + 1] : 0.f);
+                    if constexpr (kEnds) continue;
                     uint32_t s[NO];
                     split<true>(in0 && i >= j ? d.x * qk[c].v[half * 2] : 0.f, in1 && i >= j + 1 ? d.y * qk[c].v[half * 2 + 1] : 0.f, s);
 #pragma unroll
@@ -619,15 +638,17 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
             r0 = r1;
             __syncthreads();
         }
+        if (kEnds && lane == 0 && blockIdx.y == 0) p.restarts[slot] = restarts;
         return;
     }
 
     const int v0 = warp * 16, c0 = first_col + v0;  // this warp's columns of the state
-    const bool whole = kRegular || (dk == DK && c0 + 16 <= dv);
+    const bool whole = kEnds ? dk == DK && c0 + 16 <= wide : kRegular || (dk == DK && c0 + 16 <= dv);
     float* state_tile = out_tiles + warp * L::kOut / 4;
     __nv_bfloat16* out_tile = reinterpret_cast<__nv_bfloat16*>(state_tile);
-    const bool s_aligned = kRegular || (dv % 4 == 0 && reinterpret_cast<uintptr_t>(p.checkpoints) % 16 == 0 &&
-                           reinterpret_cast<uintptr_t>(p.final_state) % 16 == 0);
+    const bool s_aligned = kRegular || (dv % 4 == 0 && (kEnds ? dk % 4 == 0 && reinterpret_cast<uintptr_t>(p.ends) % 16 == 0
+                                                              : reinterpret_cast<uintptr_t>(p.checkpoints) % 16 == 0 &&
+                                                                    reinterpret_cast<uintptr_t>(p.final_state) % 16 == 0));
     const bool o_aligned = sizeof(T) == 2 && (kRegular || (dv % 8 == 0 && reinterpret_cast<uintptr_t>(p.o) % 16 == 0));
     Acc s[kTiles];  // S^T: rows = columns c0.. of the state, columns = dk
     // where this thread's values of a (dk, dv) matrix lie: value e of tile i at i * 8 * dv + at(e)
@@ -637,12 +658,15 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int kk = i * 8 + quad * 2 + e % 2, c = c0 + row + e / 2 * 8;
-                f(s[i].v[e], kk * dv + c, whole || (kk < dk && c < dv));
+                f(s[i].v[e], kk * wide + c, whole || (kk < dk && c < wide));
             }
     };
     {
-        const float* s0 = p.state ? p.state + seq * dk * dv : nullptr;
-        each_state([&](float& x, int at, bool in) { x = s0 && in ? s0[at] : 0.f; });
+        const float* s0 = segment ? (kEnds ? nullptr : end_of(slot - 1)) : p.state ? p.state + seq * dk * dv : nullptr;
+        if (unit)
+            each_state([&](float& x, int at, bool in) { x = in && at % (dk + 1) == 0 ? 1.f : 0.f; });
+        else
+            each_state([&](float& x, int at, bool in) { x = s0 && in ? s0[at] : 0.f; });
     }
     // The state to a (dk, dv) matrix: through shared memory, 16 columns of a row at a time, so that stores are 16 bytes.
     auto put_state = [&](float* to) {
@@ -652,10 +676,10 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) state_tile[(i * 8 + quad * 2 + e % 2) * L::kLdS + row + e / 2 * 8] = s[i].v[e];
             __syncwarp();
-            float4* out = reinterpret_cast<float4*>(to + (lane / 4) * dv + c0 + lane % 4 * 4);
+            float4* out = reinterpret_cast<float4*>(to + (lane / 4) * wide + c0 + lane % 4 * 4);
 #pragma unroll
             for (int i = 0; i < DK / 8; ++i)
-                __stcs(out + i * 2 * dv, *reinterpret_cast<const float4*>(state_tile + (i * 8 + lane / 4) * L::kLdS + lane % 4 * 4));
+                __stcs(out + i * 2 * wide, *reinterpret_cast<const float4*>(state_tile + (i * 8 + lane / 4) * L::kLdS + lane % 4 * 4));
             __syncwarp();
         } else {
             each_state([&](float& x, int at, bool in) {
@@ -672,7 +696,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
         if (b < 0) break;
         if (aligned) tc::mbar_wait_warp(&arrived[b % L::kBuffers], b / L::kBuffers & 1);  // long since; it makes the copies visible here
         const int r0 = ch.r0, r1 = ch.r1;
-        if (p.checkpoints && r0 == 0) put_state(p.checkpoints + (seq * blocks + b) * dk * dv);
+        if (!kEnds && p.checkpoints && r0 == 0) put_state(p.checkpoints + (seq * all + b0 + b) * dk * dv);
         if (ch.fresh) {
 #pragma unroll
             for (int i = 0; i < kTiles; ++i) s[i].zero();
@@ -695,12 +719,16 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
                 load_rows(ka[x], operand(b, 0, x), st * 16, lane);
-                load_rows(qa[x], operand(b, 1, x), st * 16, lane);
+                if constexpr (!kEnds) load_rows(qa[x], operand(b, 1, x), st * 16, lane);
             }
             uint32_t kb[2][NT][2], qb[2][NT][2];
             as_rows(kb, ka);
-            as_rows(qb, qa);
-            mma2_zip<3, NO>(ks, sa, kb, qs, sa, qb);
+            if constexpr (kEnds) {
+                mma2<3>(ks, sa, kb);
+            } else {
+                as_rows(qb, qa);
+                mma2_zip<3, NO>(ks, sa, kb, qs, sa, qb);
+            }
         }
         // R^T; tokens outside the chunk are zero whatever their inputs hold
         uint32_t ra[3][4];
@@ -723,6 +751,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                         x0 = to_f32(tv[panel_at<T>(j, v0 + row + half * 8)]);
                         x1 = to_f32(tv[panel_at<T>(j + 1, v0 + row + half * 8)]);
                     }
+                    if (unit) x0 = x1 = 0.f;
                     uint32_t tmp[3];
                     split<true>(in0 ? fmaf(-ga.x, ks[c].v[half * 2], x0) : 0.f, in1 ? fmaf(-ga.y, ks[c].v[half * 2 + 1], x1) : 0.f, tmp);
 #pragma unroll
@@ -743,8 +772,8 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
             for (int c = 0; c < 2; ++c) {
                 const Acc& e = ee[c];
                 const int j = c * 8 + quad * 2;
-                if (p.errors && first_col / 16 + warp < slices) {
-                    float4* to = reinterpret_cast<float4*>(p.errors) + error_at(seq * blocks + b, slices, first_col / 16 + warp, c, lane);
+                if (!kEnds && p.errors && first_col / 16 + warp < slices) {
+                    float4* to = reinterpret_cast<float4*>(p.errors) + error_at(seq * all + b0 + b, slices, first_col / 16 + warp, c, lane);
                     if (r0 == 0 && r1 == kC) {
                         __stcs(to, make_float4(e.v[0], e.v[1], e.v[2], e.v[3]));
                     } else {
@@ -758,22 +787,23 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
                     uint32_t t2[NO], t3[3];
-                    split<true>(be.x * e.v[half * 2], be.y * e.v[half * 2 + 1], t2);
+                    if constexpr (!kEnds) split<true>(be.x * e.v[half * 2], be.y * e.v[half * 2 + 1], t2);
                     split<true>(h0 * e.v[half * 2], h1 * e.v[half * 2 + 1], t3);
 #pragma unroll
-                    for (int x = 0; x < NO; ++x) uo[x][c * 2 + half] = t2[x];
+                    for (int x = 0; x < NO && !kEnds; ++x) uo[x][c * 2 + half] = t2[x];
 #pragma unroll
                     for (int x = 0; x < 3; ++x) ue[x][c * 2 + half] = t3[x];
                 }
             }
         }
-        {
+        if constexpr (!kEnds) {
             uint32_t ab[NO][4], bb[2][NO][2];
             load_operand(ab, ch.att, lane);
             as_rows(bb, ab);
             mma2_split<NO>(qs, uo, bb);
         }
-        if (o_aligned && whole) {  // by a transposed tile in shared memory, 16 bytes a lane
+        if constexpr (kEnds) {
+        } else if (o_aligned && whole) {  // by a transposed tile in shared memory, 16 bytes a lane
             if constexpr (sizeof(T) == 2) {
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
@@ -783,12 +813,12 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                 __syncwarp();
                 const int i = lane / 2;
                 if (within(i, r0, r1))
-                    *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + (b * kC + i) * step_t + first + lane % 2 * 8) =
+                    *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + (t0 + b * kC + i) * step_t + first + lane % 2 * 8) =
                         *reinterpret_cast<const uint4*>(out_tile + i * kLdOut + lane % 2 * 8);
                 __syncwarp();
             }
         } else {
-            T* o = static_cast<T*>(p.o) + b * kC * step_t + first + row;
+            T* o = static_cast<T*>(p.o) + (t0 + b * kC) * step_t + first + row;
 #pragma unroll
             for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -817,7 +847,146 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
             });
         }
     }
-    if (p.final_state) put_state(p.final_state + seq * dk * dv);
+    if constexpr (kEnds) {
+        put_state(end_of(slot) + (unit ? dk * dv : 0));
+    } else if (p.final_state && segment == p.segments - 1) {
+        put_state(p.final_state + seq * dk * dv);
+    }
+}
+
+// From segments' ends from zero (B) and what they make of a state (A) to their ends, in place and in order:
+// S <- A S + B, or B where an episode starts in the segment.  A block has kJoinCols columns of one sequence's state, a
+// warp 16 rows of them; products are of bf16 terms, as in the scan (by fused multiply-adds a segment of 128 x 128 took
+// 2.8 to 4.4 us, bound by reads of shared memory; this 2.5).  The A and B of two segments come while the product of
+// one is taken.
+constexpr int kJoinCols = 16, kJoinThreads = 256, kMostSegments = 512;
+
+template <int DK>
+struct JoinSmem {
+    static constexpr int kLd = DK + 8, kLdTerm = DK + 8;  // floats of a row of A; bf16 of a column of S
+    static constexpr size_t kA = (size_t)DK * kLd * 4, kTerms = (size_t)3 * kJoinCols * kLdTerm * 2;
+    static constexpr size_t kBytes = 3 * kA + kTerms + kMostSegments * 4;
+};
+
+template <int kBytes>
+__device__ __forceinline__ void copy_async(float* to, const float* from) {
+    if constexpr (kBytes == 16)  // not through L1, which this much shared memory leaves too small
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_at(to)), "l"(from) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_at(to)), "l"(from) : "memory");
+}
+
+template <int DK>
+__global__ void __launch_bounds__(kJoinThreads) scan_join_kernel(const Scan p) {
+    using L = JoinSmem<DK>;
+    extern __shared__ __align__(16) uint8_t join_shared[];
+    float* a = reinterpret_cast<float*>(join_shared);                                     // three of [DK][kLd]
+    __nv_bfloat16* terms = reinterpret_cast<__nv_bfloat16*>(join_shared + 3 * L::kA);     // S, by terms: [3][kJoinCols][kLdTerm]
+    int* joined = reinterpret_cast<int*>(join_shared + 3 * L::kA + L::kTerms);            // no episode starts in the segment
+    const int dk = p.dk, dv = p.dv, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int r0 = warp * 16 + lane / 4, c0 = blockIdx.y * kJoinCols + lane % 4 * 2;
+    const int64_t first = (int64_t)blockIdx.x * (p.segments - 1), size = (int64_t)dk * (dk + dv);
+    const bool vec = dk % 4 == 0 && dv % 4 == 0 && reinterpret_cast<uintptr_t>(p.ends) % 16 == 0;
+    for (int i = threadIdx.x; i < (int)((3 * L::kA + L::kTerms) / 16); i += kJoinThreads)  // rows and columns past dk stay zero
+        reinterpret_cast<uint4*>(join_shared)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = threadIdx.x; i < p.segments; i += kJoinThreads) joined[i] = i > 0 && i + 1 < p.segments && !p.restarts[first + i];
+    __syncthreads();
+    auto fetch = [&](int i) {  // A of segment i, where it is needed
+        if (i < p.segments && joined[i]) {
+            const float* from = p.ends + (first + i) * size + dk * dv;
+            float* to = a + i % 3 * DK * L::kLd;
+            constexpr int kPer = DK / 4, kStep = kJoinThreads / kPer;
+            const int row = threadIdx.x / kPer, c = threadIdx.x % kPer * 4;
+            if (vec && dk == DK) {
+#pragma unroll
+                for (int j = 0; j < DK; j += kStep) copy_async<16>(to + (row + j) * L::kLd + c, from + (row + j) * DK + c);
+            } else if (vec) {
+                for (int j = row; j < dk; j += kStep)
+                    if (c < dk) copy_async<16>(to + j * L::kLd + c, from + j * dk + c);
+            } else {
+                for (int j = warp; j < dk; j += kJoinThreads / 32)
+                    for (int e = lane; e < dk; e += 32) copy_async<4>(to + j * L::kLd + e, from + j * dk + e);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto each_pair = [&](int i, auto&& f) {  // this thread's values of segment i's end, two neighbours at a time
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int r = r0 + half * 8, c = c0 + t * 8;
+                if (i + 1 < p.segments && r < dk) f(t, half, p.ends + (first + i) * size + r * dv + c, c < dv, c + 1 < dv);
+            }
+    };
+    auto load = [&](Acc (&x)[2], int i) {
+        x[0].zero(), x[1].zero();
+        each_pair(i, [&](int t, int half, const float* from, bool in0, bool in1) {
+            if (vec && in1) {
+                const float2 y = *reinterpret_cast<const float2*>(from);
+                x[t].v[half * 2] = y.x, x[t].v[half * 2 + 1] = y.y;
+            } else {
+                if (in0) x[t].v[half * 2] = from[0];
+                if (in1) x[t].v[half * 2 + 1] = from[1];
+            }
+        });
+    };
+    Acc end[2], next[2], after[2];
+    load(end, 0);
+    load(next, 1);
+    fetch(1);
+    for (int i = 0;; ++i) {
+        fetch(i + 2);
+        load(after, i + 2);
+        if (joined[i] && warp * 16 < dk) {
+            const float* row = a + i % 3 * DK * L::kLd + r0 * L::kLd + lane % 4 * 2;
+#pragma unroll
+            for (int k = 0; k < DK; k += 16) {
+                uint32_t ta[3][4], tb[3][4], bb[2][3][2];
+#pragma unroll
+                for (int z = 0; z < 4; ++z) {
+                    const float2 x = *reinterpret_cast<const float2*>(row + z % 2 * 8 * L::kLd + k + z / 2 * 8);
+                    uint32_t t[3];
+                    split(x.x, x.y, t);
+#pragma unroll
+                    for (int y = 0; y < 3; ++y) ta[y][z] = t[y];
+                }
+#pragma unroll
+                for (int y = 0; y < 3; ++y) load_rows(tb[y], Rows{terms + y * kJoinCols * L::kLdTerm, L::kLdTerm}, k, lane);
+                as_rows(bb, tb);
+                mma2<3>(end, ta, bb);
+            }
+            each_pair(i, [&](int t, int half, float* to, bool in0, bool in1) {
+                if (vec && in1) {
+                    *reinterpret_cast<float2*>(to) = make_float2(end[t].v[half * 2], end[t].v[half * 2 + 1]);
+                } else {
+                    if (in0) to[0] = end[t].v[half * 2];
+                    if (in1) to[1] = end[t].v[half * 2 + 1];
+                }
+            });
+        }
+        if (i + 2 >= p.segments) break;
+        __syncthreads();  // S has been read
+        if (warp * 16 < DK) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t s[3];
+                    split(end[t].v[e], end[t].v[2 + e], s);
+#pragma unroll
+                    for (int x = 0; x < 3; ++x) {
+                        __nv_bfloat16* to = terms + (x * kJoinCols + t * 8 + lane % 4 * 2 + e) * L::kLdTerm + r0;
+                        to[0] = __ushort_as_bfloat16((unsigned short)s[x]);
+                        to[8] = __ushort_as_bfloat16((unsigned short)(s[x] >> 16));
+                    }
+                }
+        }
+        asm volatile("cp.async.wait_group 1;" ::: "memory");  // A of segment i + 1
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < 2; ++t) end[t] = next[t], next[t] = after[t];
+    }
 }
 
 // --------------------------------------------------------------- backward
@@ -1575,6 +1744,31 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
 // x 2 heads of 128 backwards 322 and 411.
 inline bool on_16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// How many segments a few long sequences are cut into; 1 where that gains nothing.
+//
+// A sequence's chunks follow one another, so a few long ones leave most SMs idle.  The state after a segment is linear
+// in the state before it, S' = A S + B: so first every segment's A and B at once, as scans from a unit matrix without
+// values and from zero (outputs left out), then the ends in order, one small product each, then every segment's outputs
+// at once from the state before it.  That is two scans of 1 / G of the chunks and G joins, of a chunk's time each, in
+// place of one scan, as long as a pass's blocks are all on the GPU together.  bfloat16, cut and whole: 4 envs x 4 heads
+// x 4,096 tokens of 128 in 6 segments 250 and 525 us, of 64 in 14 107 and 420; 1 x 2 x 4,096 of 128 in 21 about 115 and
+// 521; 4 x 4 x 512 of 128 in 5 57 and 70, of 64 in 8 37 and 57; 8 x 4 x 1,024 of 64 in 8 57 and 109.  More segments than
+// the GPU holds at once are slower again: 306 us for 7 in the first.
+constexpr int kSplitCost = 10;  // of the two more launches, in chunks
+
+inline int count_segments(int64_t t, int64_t heads, int dk, int dv, int sms) {
+    const int64_t all = (t + kC - 1) / kC, blocks = (int64_t)sms * (dk > 64 ? 2 : 3);
+    const int64_t value_blocks = (dv + 63) / 64, key_blocks = (dk + 63) / 64;
+    int64_t best = 1, best_cost = all;
+    for (int64_t g = 3; g <= all && g <= kMostSegments; ++g) {
+        if (heads * ((g - 1) * value_blocks + (g - 2) * key_blocks) > blocks || heads * g * value_blocks > blocks) break;
+        const int64_t cost = 2 * ((all + g - 1) / g) + g + kSplitCost;
+        if (cost < best_cost) best = g, best_cost = cost;
+    }
+    const int64_t per = (all + best - 1) / best;
+    return all ? (int)((all + per - 1) / per) : 1;
+}
+
 // A (t, n, h, d) tensor for Fetch.  Dimensions of one element have no stride to speak of.
 template <class T>
 int map_rows(CUtensorMap* map, const void* base, const Strides& s, const Scan& p, int d) {
@@ -1590,21 +1784,33 @@ int map_rows(CUtensorMap* map, const void* base, const Strides& s, const Scan& p
 template <class T, int DK>
 int launch_forward_dk(const Scan& p, cudaStream_t st) {
     using L = ForwardSmem<T, DK>;
-    const dim3 grid(static_cast<unsigned>(p.n * p.h), (p.dv + L::kWidth - 1) / L::kWidth);
+    const unsigned heads = static_cast<unsigned>(p.n * p.h), segments = p.segments;
+    const unsigned value_blocks = (p.dv + L::kWidth - 1) / L::kWidth, key_blocks = (p.dk + L::kWidth - 1) / L::kWidth;
     CUtensorMap map_k{}, map_q{}, map_v{};
     if (p.aligned && p.t) {
         if (int rc = map_rows<T>(&map_k, p.k, p.sk, p, p.dk)) return rc;
         if (int rc = map_rows<T>(&map_q, p.q, p.sq, p, p.dk)) return rc;
         if (int rc = map_rows<T>(&map_v, p.v, p.sv, p, p.dv)) return rc;
     }
-    auto go = [&](auto regular) -> int {
-        constexpr auto* kernel = scan_forward_kernel<T, DK, decltype(regular)::value>;
+    auto go = [&](auto regular, auto ends, dim3 grid) -> int {
+        constexpr auto* kernel = scan_forward_kernel<T, DK, decltype(regular)::value, decltype(ends)::value>;
         if (int rc = allow_smem<kernel>((int)L::kBytes, p.device, "delta_scan")) return rc;
         kernel<<<grid, (kForwardWarps + 1) * 32, L::kBytes, st>>>(p, map_k, map_q, map_v);
         return cuda_status(cudaGetLastError(), "delta_scan");
     };
-    const bool regular = p.aligned && p.dk == DK && p.dv % L::kWidth == 0 && on_16(p.o) && on_16(p.final_state) && on_16(p.checkpoints);
-    return regular ? go(std::true_type{}) : go(std::false_type{});
+    auto run = [&](auto regular) -> int {
+        if (segments > 1) {
+            if (int rc = go(regular, std::true_type{}, dim3(heads, value_blocks + key_blocks, segments - 1))) return rc;
+            using J = JoinSmem<DK>;
+            if (int rc = allow_smem<scan_join_kernel<DK>>((int)J::kBytes, p.device, "delta_scan")) return rc;
+            scan_join_kernel<DK><<<dim3(heads, (p.dv + kJoinCols - 1) / kJoinCols), kJoinThreads, J::kBytes, st>>>(p);
+            if (int rc = cuda_status(cudaGetLastError(), "delta_scan")) return rc;
+        }
+        return go(regular, std::false_type{}, dim3(heads, value_blocks, segments));
+    };
+    const bool regular = p.aligned && p.dk == DK && p.dv % L::kWidth == 0 && on_16(p.o) && on_16(p.final_state) &&
+                         on_16(p.checkpoints) && on_16(p.ends);
+    return regular ? run(std::true_type{}) : run(std::false_type{});
 }
 
 template <class T, int DK, int DV>

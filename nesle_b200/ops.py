@@ -53,9 +53,9 @@ def _no_grad_path(name: str, *tensors) -> None:
                 raise ValueError(f"{name} has no gradient; call it under torch.no_grad() or on detached tensors")
 
 
-def _call(name: str, args: bytes, stream: int) -> None:
+def _call(name: str, args: bytes, *rest: int) -> None:
     lib = _lib.load()
-    rc = getattr(lib, name)(args, stream)
+    rc = getattr(lib, name)(args, *rest)
     if rc:
         _lib.check(rc, lib)
 
@@ -315,6 +315,12 @@ def _scan_sizes(t: int, n: int, h: int, dk: int, dv: int) -> tuple[int, int]:
     return lib.nesle_delta_error_floats(sizes), lib.nesle_delta_checkpoint_floats(sizes)
 
 
+@functools.lru_cache(maxsize=256)
+def _scan_split(t: int, n: int, h: int, dk: int, dv: int, dev: int) -> int:
+    """Floats of the workspace with which a scan cuts its sequences into segments; 0 where it does not."""
+    return _lib.load().nesle_delta_split_floats(_lib.DELTA_ARGS.pack(*(0,) * 25, t, n, h, dk, dv, 0.0, *(0,) * 12, dev))
+
+
 class _DeltaScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, g, beta, state, reset, scale, grad, dev):
@@ -330,8 +336,11 @@ class _DeltaScan(torch.autograd.Function):
             ctx.save_for_backward(q, k, v, g, beta, reset, errors, checkpoints)
             ctx.scale, ctx.has_state, ctx.dev = scale, state is not None, dev
             ctx.set_materialize_grads(False)
-        _call("nesle_delta_scan", _scan_args(q, k, v, g, beta, reset, state, scale, dev, o.data_ptr(), final.data_ptr(), *kept),
-              _stream(dev))
+        split = _scan_split(t, n, h, dk, dv, dev)
+        ends = torch.empty(split, dtype=torch.float32, device=device) if split else None
+        _call("nesle_delta_scan_split",
+              _scan_args(q, k, v, g, beta, reset, state, scale, dev, o.data_ptr(), final.data_ptr(), *kept),
+              ends.data_ptr() if split else 0, _stream(dev))
         return o, final
 
     @staticmethod

@@ -224,6 +224,82 @@ def test_long_sequence_and_many_heads():
     check(inputs(5, 300, 3, 32, 32, torch.bfloat16, 0.05, seed=13), train=True)
 
 
+def is_cut(t, n, h, dk, dv):
+    return ops._scan_split(t, n, h, dk, dv, torch.cuda.current_device()) > 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("t,n,h,dk,dv", [(640, 1, 1, 64, 64), (801, 2, 2, 128, 128), (655, 1, 2, 32, 32), (999, 1, 1, 40, 72),
+                                         (641, 2, 1, 33, 65), (700, 1, 1, 128, 16), (700, 1, 2, 16, 128), (650, 1, 1, 1, 3)])
+def test_cut_sequences(t, n, h, dk, dv, dtype):
+    """A few long sequences run as segments side by side, joined by one more product: S <- A S + B."""
+    assert is_cut(t, n, h, dk, dv)
+    check(inputs(t, n, h, dk, dv, dtype, 0.003, seed=t + dk), train=dtype == torch.float32)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("decay", [-8.0, 3.0])
+@pytest.mark.parametrize("p_reset", [0.0, 0.4])
+def test_cut_sequences_of_weak_decays_and_many_episodes(decay, p_reset):
+    assert is_cut(1030, 2, 1, 64, 64) and not is_cut(1030, 1024, 4, 64, 64) and not is_cut(64, 2, 1, 64, 64)
+    check(inputs(1030, 2, 1, 64, 64, torch.float32, p_reset, seed=20, decay=decay), train=False)
+
+
+@pytest.mark.gpu
+def test_repeated_keys_in_cut_sequences():
+    x = inputs(640, 1, 2, 64, 64, torch.float32, 0.0, seed=21)
+    x["k"] = x["k"][:1].expand(640, -1, -1, -1).contiguous()
+    x["beta"] = torch.ones_like(x["beta"])
+    x["g"] = torch.zeros_like(x["g"])
+    check(x, train=False)
+
+
+@pytest.mark.gpu
+def test_nothing_passes_a_reset_in_cut_sequences():
+    """NaN of a state and of tokens stay in their episode, whatever segments it spans."""
+    t = 900
+    assert is_cut(t, 2, 1, 64, 64)
+    x = inputs(t, 2, 1, 64, 64, torch.bfloat16, 0.0, seed=22)
+    x["reset"][700] = True
+    bad = {i: y.clone() for i, y in x.items()}
+    bad["state"][:] = float("nan")
+    bad["k"][300], bad["v"][690], bad["g"][400], bad["q"][699] = float("nan"), float("inf"), float("nan"), float("inf")
+    for a, b in zip(*(ops.delta_scan(*(y[i] for i in NAMES), y["reset"]) for y in (x, bad))):
+        a, b = (a[700:], b[700:]) if len(a) == t else (a, b)
+        assert bool(torch.isfinite(b).all()) and torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_cut_sequences_strides_streams_graphs_and_workspaces():
+    t, n, h, d = 645, 2, 1, 32
+    x = inputs(t, n, h, d, d, torch.bfloat16, 0.004, seed=23)
+    odd = torch.cat([torch.zeros((t, n, h, 3), device="cuda", dtype=torch.bfloat16), x["q"], x["k"], x["v"]], -1)
+    check(dict(x, q=odd[..., 3:d + 3], k=odd[..., d + 3:2 * d + 3], v=odd[..., 2 * d + 3:]), train=False)
+    want = ops.delta_scan(*(x[i] for i in NAMES), x["reset"])
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        again = [ops.delta_scan(*(x[i] for i in NAMES), x["reset"]) for _ in range(3)]
+    side.synchronize()
+    assert all(torch.equal(a, b) for r in again for a, b in zip(want, r))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = ops.delta_scan(*(x[i] for i in NAMES), x["reset"])
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    # the C entry: without a workspace one scan, with one that is not aligned a refusal
+    o, s = torch.empty_like(want[0]), torch.empty_like(want[1])
+    dev = torch.cuda.current_device()
+    args = ops._scan_args(x["q"], x["k"], x["v"], x["g"], x["beta"], x["reset"], x["state"], d ** -0.5, dev, o.data_ptr(), s.data_ptr())
+    ops._call("nesle_delta_scan_split", args, 0, torch.cuda.current_stream().cuda_stream)
+    wide = {i: (y if i == "reset" else y.double()) for i, y in x.items()}
+    for got, ref, name in zip((o, s), reference(wide), ("o", "state")):
+        close(got, ref, d, d, name)
+    with pytest.raises(ValueError, match="workspace"):
+        ops._call("nesle_delta_scan_split", args, s.data_ptr() + 2, torch.cuda.current_stream().cuda_stream)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("n,h,dk,dv", [(1, 1, 64, 64), (5, 3, 64, 64), (33, 2, 128, 128), (4, 1, 1, 1), (7, 2, 40, 72), (3, 2, 33, 65),
