@@ -458,7 +458,8 @@ int launch_tiles(const nesle_int8_args& a, const uint8_t* x, int64_t ld_x, const
     if (int rc = encode_map(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, x, dx, sx, bx)) return rc;
     if (int rc = encode_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, dw, sw, bw)) return rc;
     // Results leave by TMA where their rows start on 16 bytes; else a thread stores its row's columns.
-    const bool tma_out = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.ld_y * sizeof(Out) % 16 == 0;
+    // A tiled store ends on 16 bytes, past n where n does not: such rows may have neighbours.
+    const bool tma_out = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.ld_y * sizeof(Out) % 16 == 0 && a.n * sizeof(Out) % 16 == 0;
     if (tma_out) {
         const uint64_t dy[2] = {a.n, a.m}, sy[1] = {a.ld_y * sizeof(Out)};
         const uint32_t by[2] = {128 / sizeof(Out), 32};

@@ -140,6 +140,21 @@ def test_quantize_rows_is_exact(dtype, rows, cols):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("start", range(17))
+def test_rows_that_start_anywhere(start):
+    """Every offset from 16 bytes, of tokens whose rows are an odd number of bytes apart, and rows of results likewise."""
+    ram = torch.randint(0, 256, (301, 407), generator=_gen(start), device="cuda", dtype=torch.uint8)
+    k = 390 - 3 * start
+    x = ram[:, start:start + k]
+    q, ws = _weight(131, k, start)
+    for dtype in (torch.bfloat16, torch.float32):
+        out = torch.full((301, 200), 7.0, device="cuda", dtype=dtype)
+        ops.int8_linear(x, ops.Int8Weight(q, ws), 0.5, out=out[:, start:start + 131])
+        _check(out[:, start:start + 131], x, 0.5, q, ws, None, False)
+        assert bool((out[:, :start] == 7).all()) and bool((out[:, start + 131:] == 7).all())
+
+
+@pytest.mark.gpu
 def test_quantize_rows_with_infinities_and_nan():
     x = torch.randn((4, 33), generator=_gen(0), device="cuda")
     x[1, 5], x[2, 6] = float("inf"), float("nan")
