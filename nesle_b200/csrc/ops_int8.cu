@@ -12,10 +12,13 @@ namespace {
 // ------------------------------------------------------------- quantize_rows
 //
 // One pass: a row's 16-byte chunks stay in registers between the maximum and
-// the division (4 chunks a thread; longer rows are read again, from L2).
-// Memory bound; small calls are a launch (2,048 x 512 bf16: 6.8 us).  The maximum is taken on the bit patterns of |x|, where a NaN
-// is above infinity and infinity above every number, so that a row with
-// either says so in its scale.
+// the rounding (4 chunks a thread; longer rows are read again, from L2).
+// Memory bound: 65,536 x 1,024 bf16 64 us, 3.1 TB/s; small calls are a launch
+// (2,048 x 512 bf16: 6.8 us).  Rows that are not aligned come element by
+// element (65,536 x 1,021: 122 us; 32 elements a thread and a warp a row, to
+// do without the block's barrier, took 135).  The maximum is taken on the bit
+// patterns of |x|, where a NaN is above infinity and infinity above every
+// number, so that a row with either says so in its scale.
 
 constexpr int kQuantThreads = 256;
 constexpr int kHeld = 4;
@@ -32,9 +35,41 @@ struct Chunk {
     }
 };
 
-__device__ __forceinline__ int8_t quantize(float x, float divisor) {
-    const float q = __fdiv_rn(x, divisor);
-    return q == q ? static_cast<int8_t>(fminf(fmaxf(rintf(q), -127.f), 127.f)) : int8_t(0);
+// rint(x / s), the quotient rounded to fp32 first, of a row whose largest magnitude is 127 s.  x times the reciprocal of s is
+// within 3 roundings of the quotient, 127 * 3 * 2^-24 < 2^-14, so that only a chunk with a product this near to half an integer
+// is divided (and all where s is below the normal numbers, whose reciprocal may be infinite); and a sum with 1.5 * 2^23
+// has the nearest integer in its low bits.  65,536 x 1,024 bf16: 76 us by divisions and conversions, 64 so.
+struct Divisor {
+    float value, reciprocal;
+    __device__ __forceinline__ explicit Divisor(float s) : value(s), reciprocal(s >= 0x1p-120f ? 1.f / s : __builtin_nanf("")) {}
+};
+
+template <int N>
+__device__ __forceinline__ void quantize(const float (&x)[N], const Divisor& d, int8_t (&out)[N]) {
+    constexpr float kRound = 12582912.f;
+    uint32_t bits[N];
+    bool sure = true;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float q = x[i] * d.reciprocal, r = q + kRound;
+        bits[i] = __float_as_uint(r);
+        sure = sure && fabsf(q - (r - kRound)) < 0.5f - 0x1p-14f;  // not with a NaN
+    }
+    if (!sure) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float q = __fdiv_rn(x[i], d.value);
+            bits[i] = __float_as_uint((q == q ? q : 0.f) + kRound);
+        }
+    }
+    if constexpr (N % 4 == 0) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            reinterpret_cast<uint32_t*>(out)[i / 4] = __byte_perm(__byte_perm(bits[i], bits[i + 1], 0x0040), __byte_perm(bits[i + 2], bits[i + 3], 0x0040), 0x5410);
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) out[i] = static_cast<int8_t>(bits[i]);
+    }
 }
 
 template <class T, bool kVec, int kPerRow>
@@ -77,20 +112,20 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* _
     }
     const float s = __fdiv_rn(__uint_as_float(most), 127.f);
     if (lane == 0) scale[row] = s;
-    const float divisor = s > 0.f || s != s ? s : 1.f;
+    const Divisor divisor(s > 0.f || s != s ? s : 1.f);
     int8_t* qr = q + static_cast<int64_t>(row) * ld_q;
     auto put = [&](const C& c, uint64_t at) {
-        if constexpr (kVec) {
-            alignas(8) int8_t b[kN];
+        float x[kN];
+        alignas(8) int8_t b[kN];
 #pragma unroll
-            for (int i = 0; i < kN; ++i) b[i] = quantize(to_f32(c.v[i]), divisor);
-            if constexpr (kN == 8)
-                *reinterpret_cast<uint2*>(qr + at * kN) = *reinterpret_cast<const uint2*>(b);
-            else
-                *reinterpret_cast<uint32_t*>(qr + at * kN) = *reinterpret_cast<const uint32_t*>(b);
-        } else {
-            qr[at] = quantize(to_f32(c.v[0]), divisor);
-        }
+        for (int i = 0; i < kN; ++i) x[i] = to_f32(c.v[i]);
+        quantize(x, divisor, b);
+        if constexpr (kN == 8)
+            *reinterpret_cast<uint2*>(qr + at * kN) = *reinterpret_cast<const uint2*>(b);
+        else if constexpr (kN == 4)
+            *reinterpret_cast<uint32_t*>(qr + at * kN) = *reinterpret_cast<const uint32_t*>(b);
+        else
+            qr[at] = b[0];
     };
 #pragma unroll
     for (int h = 0; h < kHeld; ++h) {
@@ -146,7 +181,8 @@ __device__ __forceinline__ float finish(int acc, float xs, float ws, float bias,
     return relu && y < 0.f ? 0.f : y;  // a NaN passes
 }
 
-// Rows of x copied to 16-byte aligned rows (unaligned x only): zeros from k to ld.
+// Rows of x copied to 16-byte aligned rows (unaligned x only): zeros from k to ld.  Bytes come as aligned words, which lie
+// in one page with the bytes of theirs that belong to the row (65,536 x 2,047: 46 us, byte by byte 82).
 __global__ void pad_rows_kernel(const uint8_t* __restrict__ x, int64_t ld_x, uint64_t rows, uint32_t k, uint8_t* __restrict__ out,
                                 uint32_t ld) {
     const uint32_t per = ld / 16;
@@ -156,9 +192,18 @@ __global__ void pad_rows_kernel(const uint8_t* __restrict__ x, int64_t ld_x, uin
         const uint64_t r = i / per;
         const uint32_t c = static_cast<uint32_t>(i % per) * 16;
         const uint8_t* p = x + static_cast<int64_t>(r) * ld_x + c;
-        alignas(16) uint8_t b[16];
+        const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 3);
+        const uint32_t* words = reinterpret_cast<const uint32_t*>(p - shift);
+        const uint32_t bytes = k - c < 16 ? k - c : 16;  // of this chunk, from the shift on
+        uint32_t w[5];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) b[j] = c + j < k ? p[j] : uint8_t(0);
+        for (uint32_t j = 0; j < 5; ++j) w[j] = j * 4 < shift + bytes ? __ldg(words + j) : 0u;  // words that hold a byte of the row
+        alignas(16) uint32_t b[4];
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t left = bytes > j * 4 ? bytes - j * 4 : 0;  // of this word
+            b[j] = __funnelshift_r(w[j], w[j + 1], shift * 8) & (left >= 4 ? ~0u : (1u << left * 8) - 1);
+        }
         *reinterpret_cast<uint4*>(out + r * ld + c) = *reinterpret_cast<const uint4*>(b);
     }
 }
@@ -236,9 +281,14 @@ __global__ void __launch_bounds__(256) int8_few_kernel(const uint8_t* __restrict
 // channels; TMA brings 128-byte slices of k of both operands, one thread issues
 // tcgen05.mma (kind::i8), accumulators alternate between two halves of tensor
 // memory so that a tile's epilogue runs under the next tile's products.
-// 65,536 x 2,048 to 512: 63 us, 2.2 PFLOP/s, 3.2 TB/s of what HBM has to give
+// 65,536 x 2,048 to 512: 62 us, 2.2 PFLOP/s, 3.2 TB/s of what HBM has to give
 // and take.  The operands' way from L2 bounds it: 48 KB a slice at 48 bytes a
 // clock and SM, 1,000 clocks for 512 clocks of products.
+//
+// Results leave by TMA where their rows start and end on 16 bytes, else from
+// the same tile in shared memory a row at a time, neighbouring lanes at
+// neighbouring columns (65,536 x 2,047 to 500: 92 us; a thread storing its own
+// row 385).
 //
 // Unsigned tokens multiply the weights + 128, which are unsigned too, and
 // sum_k x w = sum_k x (w + 128) - 128 sum_k x: four warps take the row sums of
@@ -253,7 +303,8 @@ struct Tile {
     static constexpr int kStage = kA + kB;
     static constexpr int kStaging = 4 * 32 * 128;  // 4 warps x 32 rows x 128 bytes on their way out
     static constexpr int kBars = 2 * kStages + 4;
-    static constexpr int kSmem = 1024 + kStages * kStage + kStaging + kBars * 8 + 16 + 2 * kBM * 4;
+    static constexpr int kChannels = 4 * 2 * 64 * 4;  // 4 warps' scales and biases of the columns at hand
+    static constexpr int kSmem = 1024 + kStages * kStage + kStaging + kBars * 8 + 16 + 2 * kBM * 4 + kChannels;
     static constexpr uint32_t kCols = 2 * kBN < 32 ? 32 : 2 * kBN;
 };
 
@@ -338,6 +389,8 @@ __global__ void __launch_bounds__(kUnsigned ? 320 : 192, 1)
         const int quarter = warp % 4;  // the lanes of tensor memory that this warp may read
         uint8_t* out = staging + (warp - 2) * 32 * 128;
         constexpr int kWide = 128 / sizeof(Out);  // columns of a 128-byte row on its way out
+        float* scales = reinterpret_cast<float*>(sums + 2 * kBM) + (warp - 2) * 128;
+        float* biases = scales + 64;
         uint32_t n = 0;
         for (uint32_t tile = blockIdx.x; tile < tiles && ok; tile += gridDim.x, ++n) {
             const uint32_t half = n & 1;
@@ -350,10 +403,15 @@ __global__ void __launch_bounds__(kUnsigned ? 320 : 192, 1)
 #pragma unroll 1
             for (int c = 0; c < kBN; c += kWide) {
                 if (col + c >= ep.n) break;  // the same for the whole warp
-                if constexpr (kTmaOut) {
+                if constexpr (kTmaOut)
                     if (lane == 0) tc::bulk_wait_read();
-                    __syncwarp();
+#pragma unroll
+                for (int j = lane; j < kWide; j += 32) {
+                    const uint32_t cn = col + c + j;
+                    scales[j] = cn < ep.n ? __ldg(ep.w_scale + cn) : 0.f;
+                    biases[j] = ep.bias && cn < ep.n ? __ldg(ep.bias + cn) : 0.f;
                 }
+                __syncwarp();
 #pragma unroll
                 for (int p = 0; p < kWide; p += 32) {
                     uint32_t acc[32];
@@ -361,25 +419,32 @@ __global__ void __launch_bounds__(kUnsigned ? 320 : 192, 1)
                     tc::tmem_wait_ld();
                     alignas(16) Out v[32];
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) {
-                        const uint32_t cn = col + c + p + j;
-                        const float ws = cn < ep.n ? __ldg(ep.w_scale + cn) : 0.f;
-                        const float bias = ep.bias && cn < ep.n ? __ldg(ep.bias + cn) : 0.f;
-                        v[j] = from_f32<Out>(finish(static_cast<int>(acc[j]) - less, xs, ws, bias, ep.relu));
+                    for (int j = 0; j < 32; j += 4) {
+                        const float4 ws = *reinterpret_cast<const float4*>(scales + p + j), be = *reinterpret_cast<const float4*>(biases + p + j);
+                        v[j] = from_f32<Out>(finish(static_cast<int>(acc[j]) - less, xs, ws.x, be.x, ep.relu));
+                        v[j + 1] = from_f32<Out>(finish(static_cast<int>(acc[j + 1]) - less, xs, ws.y, be.y, ep.relu));
+                        v[j + 2] = from_f32<Out>(finish(static_cast<int>(acc[j + 2]) - less, xs, ws.z, be.z, ep.relu));
+                        v[j + 3] = from_f32<Out>(finish(static_cast<int>(acc[j + 3]) - less, xs, ws.w, be.w, ep.relu));
                     }
-                    if constexpr (kTmaOut) {
-                        constexpr int kChunks = 32 * sizeof(Out) / 16;
+                    constexpr int kChunks = 32 * sizeof(Out) / 16;
 #pragma unroll
-                        for (int j = 0; j < kChunks; ++j) {
-                            const int chunk = (p * (int)sizeof(Out) / 16 + j) ^ (lane & 7);
-                            *reinterpret_cast<uint4*>(out + lane * 128 + chunk * 16) = reinterpret_cast<const uint4*>(v)[j];
-                        }
-                    } else if (row < ep.m) {
-                        Out* y = static_cast<Out*>(ep.y) + static_cast<int64_t>(row) * ep.ld_y + col + c + p;
-#pragma unroll
-                        for (int j = 0; j < 32; ++j)
-                            if (col + c + p + j < ep.n) y[j] = v[j];
+                    for (int j = 0; j < kChunks; ++j) {
+                        const int chunk = (p * (int)sizeof(Out) / 16 + j) ^ (lane & 7);
+                        *reinterpret_cast<uint4*>(out + lane * 128 + chunk * 16) = reinterpret_cast<const uint4*>(v)[j];
                     }
+                }
+                if constexpr (!kTmaOut) {  // a row at a time, neighbouring lanes neighbouring columns
+                    constexpr int kPer = 16 / sizeof(Out);
+                    __syncwarp();
+                    const uint32_t row0 = row - lane, rows = ep.m > row0 ? ep.m - row0 : 0;
+                    Out* y = static_cast<Out*>(ep.y) + static_cast<int64_t>(row0) * ep.ld_y + col + c;
+#pragma unroll 8
+                    for (uint32_t r = 0; r < 32; ++r)
+#pragma unroll
+                        for (int j = lane; j < kWide; j += 32)
+                            if (r < rows && col + c + j < ep.n)
+                                y[r * ep.ld_y + j] = reinterpret_cast<const Out*>(out + r * 128 + (j / kPer ^ (r & 7)) * 16)[j % kPer];
+                    __syncwarp();
                 }
                 if constexpr (kTmaOut) {
                     tc::fence_async_smem();
@@ -457,7 +522,6 @@ int launch_tiles(const nesle_int8_args& a, const uint8_t* x, int64_t ld_x, const
     const void* w = kUnsigned ? static_cast<const void*>(a.w_biased) : static_cast<const void*>(a.w);
     if (int rc = encode_map(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, x, dx, sx, bx)) return rc;
     if (int rc = encode_map(&mw, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, w, dw, sw, bw)) return rc;
-    // Results leave by TMA where their rows start on 16 bytes; else a thread stores its row's columns.
     // A tiled store ends on 16 bytes, past n where n does not: such rows may have neighbours.
     const bool tma_out = reinterpret_cast<uintptr_t>(a.y) % 16 == 0 && a.ld_y * sizeof(Out) % 16 == 0 && a.n * sizeof(Out) % 16 == 0;
     if (tma_out) {

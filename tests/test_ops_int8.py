@@ -140,6 +140,25 @@ def test_quantize_rows_is_exact(dtype, rows, cols):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("cols", [2048, 2047])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_quantize_rows_near_half_integers(cols, dtype):
+    """Quotients at, and within a few units in the last place of, half integers, in rows of every magnitude that fp32 has."""
+    exponents = torch.arange(-149, 122, device="cuda", dtype=torch.float64)[:, None]
+    g = _gen(17)
+    halves = torch.randint(-127, 127, (len(exponents), cols), generator=g, device="cuda").double() + 0.5
+    near = halves * (1 + torch.randint(-4, 5, halves.shape, generator=g, device="cuda").double() * 2.0 ** -24)
+    factor = 1 + torch.rand((len(exponents), 1), generator=g, device="cuda", dtype=torch.float64)
+    near[:, 0] = 127
+    x = (near * factor * 2.0 ** exponents).to(dtype)
+    q, s = ops.quantize_rows(x)
+    want_q, want_s = _quantized(x)
+    finite = torch.isfinite(want_s)
+    assert int(finite.sum()) > 250
+    assert torch.equal(s[finite], want_s[finite]) and torch.equal(q[finite], want_q[finite])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("start", range(17))
 def test_rows_that_start_anywhere(start):
     """Every offset from 16 bytes, of tokens whose rows are an odd number of bytes apart, and rows of results likewise."""
