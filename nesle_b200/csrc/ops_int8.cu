@@ -181,8 +181,23 @@ __device__ __forceinline__ float finish(int acc, float xs, float ws, float bias,
     return relu && y < 0.f ? 0.f : y;  // a NaN passes
 }
 
-// Rows of x copied to 16-byte aligned rows (unaligned x only): zeros from k to ld.  Bytes come as aligned words, which lie
-// in one page with the bytes of theirs that belong to the row (65,536 x 2,047: 46 us, byte by byte 82).
+// Up to 16 bytes from anywhere, zeros after them.  They come as aligned words, each of which lies in one page with the byte
+// of its that is asked for (rows of 65,536 x 2,047 laid out again: 46 us, byte by byte 82).
+__device__ __forceinline__ uint4 load_any(const uint8_t* p, uint32_t bytes) {
+    const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 3);
+    const uint32_t* words = reinterpret_cast<const uint32_t*>(p - shift);
+    uint32_t w[5], b[4];
+#pragma unroll
+    for (uint32_t j = 0; j < 5; ++j) w[j] = j * 4 < shift + bytes ? __ldg(words + j) : 0u;
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+        const uint32_t left = bytes > j * 4 ? bytes - j * 4 : 0;  // of this word
+        b[j] = __funnelshift_r(w[j], w[j + 1], shift * 8) & (left >= 4 ? ~0u : (1u << left * 8) - 1);
+    }
+    return make_uint4(b[0], b[1], b[2], b[3]);
+}
+
+// Rows of x copied to 16-byte aligned rows (many tokens of unaligned x only): zeros from k to ld.
 __global__ void pad_rows_kernel(const uint8_t* __restrict__ x, int64_t ld_x, uint64_t rows, uint32_t k, uint8_t* __restrict__ out,
                                 uint32_t ld) {
     const uint32_t per = ld / 16;
@@ -191,20 +206,7 @@ __global__ void pad_rows_kernel(const uint8_t* __restrict__ x, int64_t ld_x, uin
          i += static_cast<uint64_t>(gridDim.x) * blockDim.x) {
         const uint64_t r = i / per;
         const uint32_t c = static_cast<uint32_t>(i % per) * 16;
-        const uint8_t* p = x + static_cast<int64_t>(r) * ld_x + c;
-        const uint32_t shift = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 3);
-        const uint32_t* words = reinterpret_cast<const uint32_t*>(p - shift);
-        const uint32_t bytes = k - c < 16 ? k - c : 16;  // of this chunk, from the shift on
-        uint32_t w[5];
-#pragma unroll
-        for (uint32_t j = 0; j < 5; ++j) w[j] = j * 4 < shift + bytes ? __ldg(words + j) : 0u;  // words that hold a byte of the row
-        alignas(16) uint32_t b[4];
-#pragma unroll
-        for (uint32_t j = 0; j < 4; ++j) {
-            const uint32_t left = bytes > j * 4 ? bytes - j * 4 : 0;  // of this word
-            b[j] = __funnelshift_r(w[j], w[j + 1], shift * 8) & (left >= 4 ? ~0u : (1u << left * 8) - 1);
-        }
-        *reinterpret_cast<uint4*>(out + r * ld + c) = *reinterpret_cast<const uint4*>(b);
+        *reinterpret_cast<uint4*>(out + r * ld + c) = load_any(x + static_cast<int64_t>(r) * ld_x + c, min(k - c, 16u));
     }
 }
 
@@ -213,8 +215,9 @@ __global__ void pad_rows_kernel(const uint8_t* __restrict__ x, int64_t ld_x, uin
 // exact integer sums meet in shared memory.  A lane's 16-byte chunk feeds two
 // m16n8k32 products: any order of k is right as long as both operands have
 // it, so a chunk's words 0, 1 and 2, 3 are the low and high halves of one
-// product each.  The instruction takes uint8 by int8 as it is.  16 x 2,048 to
-// 512 channels: 6.0 us, most of it the launch and one trip to HBM.
+// product each.  The instruction takes uint8 by int8 as it is.  Tokens that are
+// not aligned are read as they are.  16 x 2,048 to 512 channels: 6.0 us, most
+// of it the launch and one trip to HBM.
 constexpr uint32_t kFewTokens = 64;
 
 __device__ __forceinline__ uint4 load16(const uint8_t* p, uint32_t at, uint32_t k) {
@@ -240,7 +243,7 @@ __device__ __forceinline__ void mma_16832(int (&c)[4], uint32_t a0, uint32_t a1,
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-template <bool kUnsigned, class Out>
+template <bool kUnsigned, class Out, bool kAligned>
 __global__ void __launch_bounds__(256) int8_few_kernel(const uint8_t* __restrict__ x, int64_t ld_x, const uint8_t* __restrict__ w,
                                                       int64_t ld_w, Epilogue ep) {
     __shared__ int part[8][16][8];
@@ -252,11 +255,17 @@ __global__ void __launch_bounds__(256) int8_few_kernel(const uint8_t* __restrict
     const uint8_t* wn = w + static_cast<int64_t>(hasn ? n0 + r : 0) * ld_w;
     int c[4] = {};
     const uint4 zero = make_uint4(0, 0, 0, 0);
+    auto token = [&](const uint8_t* row, uint32_t at) {
+        if constexpr (kAligned)
+            return load16(row, at, ep.k);
+        else
+            return load_any(row + at, min(ep.k - at, 16u));
+    };
 #pragma unroll 4
     for (uint32_t k0 = warp * 64; k0 < ep.k; k0 += 8 * 64) {
         const uint32_t at = k0 + quad * 16;
-        const uint4 a = has0 && at < ep.k ? load16(x0, at, ep.k) : zero;
-        const uint4 b = has1 && at < ep.k ? load16(x1, at, ep.k) : zero;
+        const uint4 a = has0 && at < ep.k ? token(x0, at) : zero;
+        const uint4 b = has1 && at < ep.k ? token(x1, at) : zero;
         const uint4 v = hasn && at < ep.k ? load16(wn, at, ep.k) : zero;
         mma_16832<kUnsigned>(c, a.x, b.x, a.y, b.y, v.x, v.y);
         mma_16832<kUnsigned>(c, a.z, b.z, a.w, b.w, v.z, v.w);
@@ -552,7 +561,20 @@ int run(const nesle_int8_args& a, cudaStream_t st) {
     Epilogue ep{a.x_scale, a.x_scale_value, a.w_scale, a.bias, a.y, a.ld_y, (uint32_t)a.m, (uint32_t)a.k, (uint32_t)a.n, a.relu};
     const uint8_t* x = static_cast<const uint8_t*>(a.x);
     int64_t ld_x = a.ld_x;
-    if (a.k && !aligned_x(a)) {
+    if (a.m <= kFewTokens || !a.k) {  // k = 0 is the bias alone
+        const uint64_t gy = (a.m + 15) / 16;
+        if (gy > 65535) {  // only with k = 0
+            return invalid("int8_linear: k = 0 with more than a million tokens");
+        }
+        const dim3 grid(static_cast<unsigned>((a.n + 7) / 8), static_cast<unsigned>(gy));
+        const uint8_t* w = reinterpret_cast<const uint8_t*>(a.w);
+        if (aligned_x(a))
+            int8_few_kernel<kUnsigned, Out, true><<<grid, 256, 0, st>>>(x, a.ld_x, w, a.ld_w, ep);
+        else
+            int8_few_kernel<kUnsigned, Out, false><<<grid, 256, 0, st>>>(x, a.ld_x, w, a.ld_w, ep);
+        return cuda_status(cudaGetLastError(), "int8_linear");
+    }
+    if (!aligned_x(a)) {
         ld_x = static_cast<int64_t>(padded(a.k));
         const uint64_t chunks = a.m * (ld_x / 16);
         const uint64_t most = 16ull * sm_count(a.device), want = (chunks + 255) / 256;
@@ -560,15 +582,6 @@ int run(const nesle_int8_args& a, cudaStream_t st) {
             x, a.ld_x, a.m, static_cast<uint32_t>(a.k), static_cast<uint8_t*>(a.workspace), static_cast<uint32_t>(ld_x));
         if (int rc = cuda_status(cudaGetLastError(), "int8_linear")) return rc;
         x = static_cast<const uint8_t*>(a.workspace);
-    }
-    if (a.m <= kFewTokens || !a.k) {  // k = 0 is the bias alone
-        const uint64_t gy = (a.m + 15) / 16;
-        if (gy > 65535) {  // only with k = 0
-            return invalid("int8_linear: k = 0 with more than a million tokens");
-        }
-        const dim3 grid(static_cast<unsigned>((a.n + 7) / 8), static_cast<unsigned>(gy));
-        int8_few_kernel<kUnsigned, Out><<<grid, 256, 0, st>>>(x, ld_x, reinterpret_cast<const uint8_t*>(a.w), a.ld_w, ep);
-        return cuda_status(cudaGetLastError(), "int8_linear");
     }
     // The widest tile that n fills, whose operands are read least often from L2, where its tiles occupy half of the SMs; else
     // narrower ones (2,048 tokens of 512 to 256 channels: 16 blocks of 256 channels 11.5 us, 64 of 64 6.4 us).
@@ -611,7 +624,7 @@ int nesle_quantize_rows(const void* x, int dtype, uint64_t rows, uint64_t cols, 
 }
 
 uint64_t nesle_int8_workspace(const nesle_int8_args* a) {
-    return a && a->k && !ops::aligned_x(*a) ? a->m * ops::padded(a->k) : 0;
+    return a && a->k && a->m > ops::kFewTokens && !ops::aligned_x(*a) ? a->m * ops::padded(a->k) : 0;
 }
 
 int nesle_int8_linear(const nesle_int8_args* args, void* stream) {

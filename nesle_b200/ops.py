@@ -187,8 +187,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
         _require(out.dim() != 2 or out.stride(1) == 1 or n <= 1, "out must have unit column stride")
         _require(ld_y >= n, "out's rows must not overlap")
     x_ptr = x.data_ptr()
-    # rows that do not lie on 16 bytes are laid out again in scratch memory
-    need = m * (-(-k // 16) * 16) if x_ptr % 16 or ld_x % 16 else 0
+    # many rows that do not lie on 16 bytes are laid out again in scratch memory (as much as nesle_int8_workspace says)
+    need = m * (-(-k // 16) * 16) if m > 64 and (x_ptr % 16 or ld_x % 16) else 0
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
     _call("nesle_int8_linear",
           _lib.INT8_ARGS.pack(x_ptr, unsigned, ld_x, scale_ptr, scale_value, weight.q.data_ptr(), weight.biased.data_ptr(),

@@ -256,3 +256,14 @@ def test_refusals():
     ):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("start", range(17))
+@pytest.mark.parametrize("m", [1, 33, 64])
+def test_few_rows_that_start_anywhere(m, start):
+    ram = torch.randint(0, 256, (m, 1031), generator=_gen(start), device="cuda", dtype=torch.uint8)
+    for k in (1 + start, 900 - start):
+        for x in (ram[:, start:start + k], ram.view(torch.int8)[:, start:start + k]):
+            q, ws = _weight(21, k, start)
+            _check(ops.int8_linear(x, ops.Int8Weight(q, ws), 0.5, out_dtype=torch.float32), x, 0.5, q, ws, None, False)
