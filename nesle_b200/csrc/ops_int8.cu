@@ -296,8 +296,9 @@ __global__ void __launch_bounds__(256) int8_few_kernel(const uint8_t* __restrict
 //
 // Results leave by TMA where their rows start and end on 16 bytes, else from
 // the same tile in shared memory a row at a time, neighbouring lanes at
-// neighbouring columns (65,536 x 2,047 to 500: 92 us; a thread storing its own
-// row 385).
+// neighbouring columns, two a store where rows start on 4 bytes and are even
+// (65,536 x 2,047 to 500: 79 us, one a store 92; a thread storing its own row
+// 385).
 //
 // Unsigned tokens multiply the weights + 128, which are unsigned too, and
 // sum_k x w = sum_k x (w + 128) - 128 sum_k x: four warps take the row sums of
@@ -447,12 +448,21 @@ __global__ void __launch_bounds__(kUnsigned ? 320 : 192, 1)
                     __syncwarp();
                     const uint32_t row0 = row - lane, rows = ep.m > row0 ? ep.m - row0 : 0;
                     Out* y = static_cast<Out*>(ep.y) + static_cast<int64_t>(row0) * ep.ld_y + col + c;
+                    auto staged = [&](uint32_t r, int j) { return out + r * 128 + (j / kPer ^ (r & 7)) * 16 + j % kPer * sizeof(Out); };
+                    if (sizeof(Out) == 2 && ep.ld_y % 2 == 0 && ep.n % 2 == 0 && reinterpret_cast<uintptr_t>(ep.y) % 4 == 0) {  // two columns a store
+                        const int j = lane * 2;
+                        if (col + c + j < ep.n) {
+#pragma unroll 16
+                            for (uint32_t r = 0; r < 32; ++r)
+                                if (r < rows) *reinterpret_cast<uint32_t*>(y + r * ep.ld_y + j) = *reinterpret_cast<const uint32_t*>(staged(r, j));
+                        }
+                    } else {
 #pragma unroll 8
-                    for (uint32_t r = 0; r < 32; ++r)
+                        for (uint32_t r = 0; r < 32; ++r)
 #pragma unroll
-                        for (int j = lane; j < kWide; j += 32)
-                            if (r < rows && col + c + j < ep.n)
-                                y[r * ep.ld_y + j] = reinterpret_cast<const Out*>(out + r * 128 + (j / kPer ^ (r & 7)) * 16)[j % kPer];
+                            for (int j = lane; j < kWide; j += 32)
+                                if (r < rows && col + c + j < ep.n) y[r * ep.ld_y + j] = *reinterpret_cast<const Out*>(staged(r, j));
+                    }
                     __syncwarp();
                 }
                 if constexpr (kTmaOut) {
