@@ -30,8 +30,9 @@ extern "C" {
 int nesle_ops_stalls(int device, uint32_t* count);
 
 /* Symmetric quantisation of each row to 8 bits: scale = max|x| / 127, q =
- * round-half-even(x / scale), both divisions in IEEE fp32; a row of zeros gets
- * scale 0 and zeros.  A row that holds a NaN or an infinity gets that scale, and
+ * round-half-even(x / scale) clamped to [-127, 127], both divisions in IEEE
+ * fp32 (the clamp acts where the scale is subnormal); a row whose scale is zero
+ * gets zeros.  A row that holds a NaN or an infinity gets that scale, and
  * zeros where x / scale is not a number.  Columns cols..ld_q-1 of q are set to
  * zero (ld_q - cols < 16).  ld_* in elements. */
 int nesle_quantize_rows(const void* x, int dtype, uint64_t rows, uint64_t cols, int64_t ld_x, int8_t* q, int64_t ld_q,

@@ -38,7 +38,9 @@ struct Chunk {
 // rint(x / s), the quotient rounded to fp32 first, of a row whose largest magnitude is 127 s.  x times the reciprocal of s is
 // within 3 roundings of the quotient, 127 * 3 * 2^-24 < 2^-14, so that only a chunk with a product this near to half an integer
 // is divided (and all where s is below the normal numbers, whose reciprocal may be infinite); and a sum with 1.5 * 2^23
-// has the nearest integer in its low bits.  65,536 x 1,024 bf16: 76 us by divisions and conversions, 64 so.
+// has the nearest integer in its low bits.  65,536 x 1,024 bf16: 76 us by divisions and conversions, 64 so.  Only a scale
+// below the normal numbers is rounded so coarsely that a quotient passes 127 (190 units over 127 round to one unit); such
+// rows are divided, and clamped there.
 struct Divisor {
     float value, reciprocal;
     __device__ __forceinline__ explicit Divisor(float s) : value(s), reciprocal(s >= 0x1p-120f ? 1.f / s : __builtin_nanf("")) {}
@@ -59,7 +61,7 @@ __device__ __forceinline__ void quantize(const float (&x)[N], const Divisor& d, 
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             const float q = __fdiv_rn(x[i], d.value);
-            bits[i] = __float_as_uint((q == q ? q : 0.f) + kRound);
+            bits[i] = __float_as_uint((q == q ? fminf(fmaxf(q, -127.f), 127.f) : 0.f) + kRound);
         }
     }
     if constexpr (N % 4 == 0) {

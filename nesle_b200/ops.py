@@ -83,8 +83,8 @@ def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
 
 def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """Symmetric 8-bit quantisation of the last dimension: ``(q, scale)`` with ``q = round(x / scale)`` (half to even)
-    in [-127, 127], ``scale = max|x| / 127`` in fp32, of shapes ``x.shape`` and ``x.shape[:-1]``.  A zero row has scale
-    0.  A NaN or an infinity in a row becomes the row's scale.  ``q``'s rows lie a multiple of 16 bytes apart, as
+    clamped to [-127, 127], ``scale = max|x| / 127`` in fp32, of shapes ``x.shape`` and ``x.shape[:-1]``.  A zero row has
+    scale 0.  A NaN or an infinity in a row becomes the row's scale.  ``q``'s rows lie a multiple of 16 bytes apart, as
     :func:`int8_linear` reads them best."""
     dev = _cuda_device(x, "x")
     dtype = _DTYPE.get(x.dtype)

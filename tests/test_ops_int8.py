@@ -267,3 +267,20 @@ def test_few_rows_that_start_anywhere(m, start):
         for x in (ram[:, start:start + k], ram.view(torch.int8)[:, start:start + k]):
             q, ws = _weight(21, k, start)
             _check(ops.int8_linear(x, ops.Int8Weight(q, ws), 0.5, out_dtype=torch.float32), x, 0.5, q, ws, None, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cols", [64, 63, 5000, 4999])
+def test_quantize_rows_clamps_where_the_scale_is_subnormal(cols):
+    """A scale of few units in the last place is rounded so coarsely that quotients pass 127: 190 units over 127 round to
+    one unit.  They end at 127, not at what is left of them in 8 bits."""
+    unit = 2.0 ** -149
+    most = torch.cat([torch.arange(1, 700, device="cuda"), torch.tensor([4000, 16129, 100000], device="cuda")]).double()
+    x = (torch.rand((len(most), cols), generator=_gen(4), device="cuda").double() * 2 - 1) * most[:, None]
+    x[:, 0], x[:, 1] = most, -most
+    x = (x.round() * unit).float()
+    q, s = ops.quantize_rows(x)
+    scale = ((most / 127).round() * unit).float()  # half to even, as IEEE division rounds it to a whole number of units
+    quotient = x.double() / torch.where(scale > 0, scale, 1.0).double()[:, None]
+    assert float(quotient.abs().max()) > 189
+    assert torch.equal(s, scale) and torch.equal(q, quotient.float().round().clamp(-127, 127).to(torch.int8))
