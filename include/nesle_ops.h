@@ -60,7 +60,7 @@ typedef struct nesle_int8_args {
 } nesle_int8_args;
 
 /* y[m][n] = act(x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]); the sum is exact in 32-bit integers, which
- * bounds k: 33,025 for unsigned x (255 * 255 k < 2^31), 131,072 for signed. */
+ * bounds k: 33,025 for unsigned x (255 * 255 k < 2^31), 131,071 for signed (128 * 128 k < 2^31). */
 int nesle_int8_linear(const nesle_int8_args* args, void* stream);
 /* Scratch bytes that the call needs (0 where x is 16-byte aligned with rows a multiple of 16 bytes apart). */
 uint64_t nesle_int8_workspace(const nesle_int8_args* args);

@@ -525,8 +525,8 @@ const char* check(const nesle_int8_args& a) {
     if (a.m > 0x7FFFFFFFull || a.n > 0x7FFFFFFFull) return "int8_linear: m and n must be below 2^31";
     if (a.m && a.n && (!a.y || !a.w_scale)) return "int8_linear: null argument";
     if (a.m && a.n && a.k && (!a.x || !a.w || (a.x_unsigned && !a.w_biased))) return "int8_linear: null argument";
-    if (a.k > (a.x_unsigned ? 33025ull : 131072ull))
-        return "int8_linear: k is above what 32-bit sums hold (33025 for uint8 tokens, 131072 for int8)";
+    if (a.k > (a.x_unsigned ? 33025ull : 131071ull))  // 255 * 255 k and 128 * 128 k are below 2^31
+        return "int8_linear: k is above what 32-bit sums hold (33025 for uint8 tokens, 131071 for int8)";
     if (a.ld_x < (int64_t)a.k || a.ld_w < (int64_t)a.k || a.ld_y < (int64_t)a.n) return "int8_linear: a leading dimension is shorter than its row";
     if (a.ld_w % 16 || reinterpret_cast<uintptr_t>(a.w) % 16 || reinterpret_cast<uintptr_t>(a.w_biased) % 16)
         return "int8_linear: weights must be 16-byte aligned with rows a multiple of 16 bytes apart";

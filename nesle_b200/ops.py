@@ -142,7 +142,8 @@ class Int8Weight:
 def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | float | None = None,
                 bias: torch.Tensor | None = None, *, relu: bool = False, out_dtype: torch.dtype = torch.bfloat16,
                 out: torch.Tensor | None = None) -> torch.Tensor:
-    """``act(x_scale * weight.scale * (x @ weight.q.T) + bias)`` with the integer product exact in 32 bits.
+    """``act(x_scale * weight.scale * (x @ weight.q.T) + bias)`` with the integer product exact in 32 bits, for which k
+    is at most 33,025 with uint8 tokens and 131,071 with others.
 
     ``x`` is ``(..., k)``: uint8 (RAM bytes) or int8 with ``x_scale`` a number or a float32 tensor ``x.shape[:-1]``; or
     floating, which is quantised per token first (:func:`quantize_rows`; ``x_scale`` stays None).  ``bias`` is float32

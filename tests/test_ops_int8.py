@@ -284,3 +284,26 @@ def test_quantize_rows_clamps_where_the_scale_is_subnormal(cols):
     quotient = x.double() / torch.where(scale > 0, scale, 1.0).double()[:, None]
     assert float(quotient.abs().max()) > 189
     assert torch.equal(s, scale) and torch.equal(q, quotient.float().round().clamp(-127, 127).to(torch.int8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 130])
+@pytest.mark.parametrize("dtype,k,value", [(torch.int8, 131071, -128), (torch.int8, 131056, -128), (torch.int8, 131071, 127),
+                                           (torch.uint8, 33025, 255), (torch.uint8, 33024, 255)])
+def test_extreme_sums_at_the_largest_k_are_exact(m, dtype, k, value):
+    """128 * 128 * 131,071 and 255 * 255 * 33,025 (weights + 128) are just below 2^31."""
+    x = torch.full((m, k), value, dtype=dtype, device="cuda")
+    q = torch.full((5, k), -128, dtype=torch.int8, device="cuda")
+    q[1::2] = 127
+    y = ops.int8_linear(x, ops.Int8Weight(q, torch.ones(5, device="cuda")), 1.0, out_dtype=torch.float32)
+    want = torch.tensor([float(k * value * int(w)) for w in q[:, 0]], device="cuda")  # rounded to fp32 once
+    assert torch.equal(y, want.expand(m, 5))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,k", [(torch.int8, 131072), (torch.uint8, 33026)])
+def test_sums_that_may_pass_32_bits_are_refused(dtype, k):
+    w = ops.Int8Weight(torch.zeros((5, k), dtype=torch.int8, device="cuda"), torch.ones(5, device="cuda"))
+    for m in (3, 130):
+        with pytest.raises(ValueError, match="32-bit sums"):
+            ops.int8_linear(torch.zeros((m, k), dtype=dtype, device="cuda"), w, 1.0)
