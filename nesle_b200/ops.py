@@ -53,6 +53,26 @@ def _no_grad_path(name: str, *tensors) -> None:
                 raise ValueError(f"{name} has no gradient; call it under torch.no_grad() or on detached tensors")
 
 
+def _span(x: torch.Tensor) -> tuple[int, int]:
+    """The first byte of a tensor and the one after its last."""
+    first = x.data_ptr()
+    if not x.numel():
+        return first, first
+    return first, first + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size()
+
+
+def _shares_memory(out: torch.Tensor, *others) -> bool:
+    """Whether ``out`` may lie on memory of the others, which a kernel may still read when it writes ``out``; such a call
+    writes elsewhere and copies."""
+    first, end = _span(out)
+    for x in others:
+        if x is not None:
+            a, b = _span(x)
+            if a < end and first < b:
+                return True
+    return False
+
+
 def _call(name: str, args: bytes, *rest: int) -> None:
     lib = _lib.load()
     rc = getattr(lib, name)(args, *rest)
@@ -147,7 +167,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
 
     ``x`` is ``(..., k)``: uint8 (RAM bytes) or int8 with ``x_scale`` a number or a float32 tensor ``x.shape[:-1]``; or
     floating, which is quantised per token first (:func:`quantize_rows`; ``x_scale`` stays None).  ``bias`` is float32
-    ``(n,)``.  The result is ``(..., n)`` in ``out_dtype`` (bfloat16, float16 or float32), or written to ``out``."""
+    ``(n,)``.  The result is ``(..., n)`` in ``out_dtype`` (bfloat16, float16 or float32), or written to ``out``, which may
+    lie on the memory of ``x``, ``x_scale`` and ``bias``."""
     dev = _cuda_device(x, "x")
     _require(isinstance(weight, Int8Weight) and weight._index == dev, f"weight must be an Int8Weight on cuda:{dev}")
     n, k = weight.n, weight.k
@@ -176,6 +197,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
         _require(bias.dtype == torch.float32 and bias.shape == (n,), f"bias must be float32 of shape ({n},)")
         bias = bias.detach().contiguous()
         bias_ptr = bias.data_ptr()
+    given = None
     if out is None:
         _require(out_dtype in _DTYPE, "out_dtype must be float32, bfloat16 or float16")
         out = torch.empty((*shape, n), dtype=out_dtype, device=x.device)
@@ -187,6 +209,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
         ld_y = out.stride(0) if out.dim() == 2 and m > 1 else max(n, 1)
         _require(out.dim() != 2 or out.stride(1) == 1 or n <= 1, "out must have unit column stride")
         _require(ld_y >= n, "out's rows must not overlap")
+        if _shares_memory(out, x, bias, x_scale if scale_ptr else None):
+            given, out, ld_y = out, torch.empty(out.shape, dtype=out.dtype, device=out.device), max(n, 1)
     x_ptr = x.data_ptr()
     # many rows that do not lie on 16 bytes are laid out again in scratch memory (as much as nesle_int8_workspace says)
     need = m * (-(-k // 16) * 16) if m > 64 and (x_ptr % 16 or ld_x % 16) else 0
@@ -195,7 +219,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
           _lib.INT8_ARGS.pack(x_ptr, unsigned, ld_x, scale_ptr, scale_value, weight.q.data_ptr(), weight.biased.data_ptr(),
                               weight.ld, weight.scale.data_ptr(), bias_ptr, out.data_ptr(), _DTYPE[out.dtype], ld_y, m, k, n,
                               relu, scratch.data_ptr() if need else 0, need, dev), _stream(dev))
-    return out
+    return out if given is None else given.copy_(out)
 
 
 # ------------------------------------------------------------------ Newton-Schulz
@@ -271,8 +295,9 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
 
     ``q, k``: (n, h, dk), ``v``: (n, h, dv), float32, bfloat16 or float16; ``g, beta``: (n, h) float32; ``state``:
     (n, h, dk, dv) float32 with contiguous matrices; ``reset``: (n,) bool or uint8.  ``scale`` is dk ** -0.5 unless
-    given.  Returns ``o`` (n, h, dv) in q's type, or writes it to ``out`` (contiguous).  Without gradients: for a
-    sequence with gradients see :func:`delta_scan`."""
+    given.  Returns ``o`` (n, h, dv) in q's type, or writes it to ``out`` (contiguous; it may lie on the memory of the
+    inputs, but ``state`` must share none with them).  Without gradients: for a sequence with gradients see
+    :func:`delta_scan`."""
     dev = _delta_inputs(q, k, v, g, beta, reset, "nh")
     _no_grad_path("delta_step", q, k, v, g, beta, state)
     n, h, dk = q.shape
@@ -283,12 +308,15 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     s_n, s_h, s_k, s_v = state.stride()
     _require((s_v == 1 or dv == 1) and (s_k == dv or dk == 1), "state's matrices must be contiguous")
     _require((n <= 1 or s_n >= dk * dv) and (h <= 1 or s_h >= dk * dv), "state's matrices must not overlap")
+    given = None
     if out is None:
         out = torch.empty((n, h, dv), dtype=q.dtype, device=q.device)
     else:
         _on(out, dev, "out")
         _require(out.dtype == q.dtype and out.shape == (n, h, dv) and out.is_contiguous(),
                  f"out must be contiguous {q.dtype} of shape {(n, h, dv)}")
+        if _shares_memory(out, q, k, v, g, beta, reset, state):
+            given, out = out, torch.empty_like(out)
     q, k, v = _unit(q), _unit(k), _unit(v)
     reset_ptr, reset_n = (0, 0) if reset is None else (reset.data_ptr(), reset.stride(0))
     _call("nesle_delta_step",
@@ -296,7 +324,7 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
                                     _DTYPE[q.dtype], g.data_ptr(), beta.data_ptr(), *g.stride(), *beta.stride(), reset_ptr,
                                     reset_n, state.data_ptr(), s_n, s_h, out.data_ptr(), n, h, dk, dv,
                                     dk ** -0.5 if scale is None else scale, dev), _stream(dev))
-    return out
+    return out if given is None else given.copy_(out)
 
 
 def _scan_args(q, k, v, g, beta, reset, state, scale, dev, *rest: int) -> bytes:

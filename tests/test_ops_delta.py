@@ -441,3 +441,24 @@ def test_refusals():
     ):
         with pytest.raises(ValueError):
             call()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("on", ["q", "k", "v", "q of another env", "state"])
+@pytest.mark.parametrize("dk", [32, 128])
+def test_step_writes_out_on_the_memory_of_an_input(on, dk):
+    """As if the output were written after everything has been read."""
+    x = inputs(1, 300, 2, dk, dk, torch.float32, 0.0, seed=30)
+    one = [x[i][0].clone() for i in NAMES[:5]]
+    state = x["state"].clone()
+    want = ops.delta_step(*one, state)
+    again = x["state"].clone()
+    if on == "q of another env":
+        room = torch.cat([one[0], one[0][:1]])
+        one[0], out = room[:-1], room[1:]
+    else:
+        out = again.view(-1)[5:5 + 300 * 2 * dk].view(300, 2, dk) if on == "state" else one["qkv".index(on)]
+    got = ops.delta_step(*one, again, out=out)
+    assert got is out and torch.equal(out, want)
+    if on != "state":
+        assert torch.equal(again, state)

@@ -307,3 +307,27 @@ def test_sums_that_may_pass_32_bits_are_refused(dtype, k):
     for m in (3, 130):
         with pytest.raises(ValueError, match="32-bit sums"):
             ops.int8_linear(torch.zeros((m, k), dtype=dtype, device="cuda"), w, 1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,k,n", [(40, 512, 256), (3000, 512, 256), (3000, 64, 32)])
+def test_out_on_the_memory_of_the_tokens(m, k, n):
+    """Other tiles still read the tokens when a tile's results are there."""
+    room = torch.randint(0, 256, (m, k), generator=_gen(6), device="cuda", dtype=torch.uint8)
+    x = room.clone()
+    q, ws = _weight(n, k, 7)
+    w = ops.Int8Weight(q, ws)
+    want = ops.int8_linear(x, w, 0.5)
+    out = room.view(torch.bfloat16)  # k bytes a row are k / 2 results
+    assert out.shape == want.shape
+    assert ops.int8_linear(room, w, 0.5, out=out) is out and torch.equal(out, want)
+    both = torch.cat([x, torch.empty((m, 2 * n), dtype=torch.uint8, device="cuda")], 1)  # side by side in one record
+    side = both[:, k:].view(torch.bfloat16)
+    ops.int8_linear(both[:, :k], w, 0.5, out=side)
+    assert torch.equal(side, want) and torch.equal(both[:, :k], x)
+    scales = torch.rand(m, generator=_gen(8), device="cuda") + 0.1
+    bias = torch.randn(n, generator=_gen(9), device="cuda")
+    want = ops.int8_linear(x, w, scales, bias, out_dtype=torch.float32)
+    store = torch.zeros((m, n), device="cuda")
+    store[0] = bias
+    assert torch.equal(ops.int8_linear(x, w, scales, store[0], out=store), want)
