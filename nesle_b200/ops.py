@@ -28,6 +28,8 @@ __all__ = ["Int8Weight", "delta_scan", "delta_step", "int8_linear", "orthogonali
 
 _DTYPE = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 _stream = torch._C._cuda_getCurrentRawStream
+# What a kernel writes in place has changed for autograd too: a gradient that saved the old values is then refused.
+_written = torch.autograd.graph.increment_version
 
 
 def _require(ok: bool, message: str) -> None:
@@ -197,8 +199,8 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
         _require(bias.dtype == torch.float32 and bias.shape == (n,), f"bias must be float32 of shape ({n},)")
         bias = bias.detach().contiguous()
         bias_ptr = bias.data_ptr()
-    given = None
-    if out is None:
+    given, fresh = None, out is None
+    if fresh:
         _require(out_dtype in _DTYPE, "out_dtype must be float32, bfloat16 or float16")
         out = torch.empty((*shape, n), dtype=out_dtype, device=x.device)
         ld_y = max(n, 1)
@@ -219,7 +221,11 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
           _lib.INT8_ARGS.pack(x_ptr, unsigned, ld_x, scale_ptr, scale_value, weight.q.data_ptr(), weight.biased.data_ptr(),
                               weight.ld, weight.scale.data_ptr(), bias_ptr, out.data_ptr(), _DTYPE[out.dtype], ld_y, m, k, n,
                               relu, scratch.data_ptr() if need else 0, need, dev), _stream(dev))
-    return out if given is None else given.copy_(out)
+    if given is not None:
+        return given.copy_(out)
+    if not fresh:
+        _written(out)
+    return out
 
 
 # ------------------------------------------------------------------ Newton-Schulz
@@ -236,7 +242,8 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, eps: float = 1e-7,
     _require(update.dim() >= 2, "update must have at least two dimensions")
     _no_grad_path("orthogonalize", update)
     rows, cols = update.shape[-2:]
-    if out is None:
+    fresh = out is None
+    if fresh:
         out = torch.empty(update.shape, dtype=torch.bfloat16, device=update.device)
     else:
         _on(out, dev, "out")
@@ -251,6 +258,8 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, eps: float = 1e-7,
     need = _lib.load().nesle_orth_workspace(args())
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device)
     _call("nesle_orthogonalize", args(scratch.data_ptr(), need), _stream(dev))
+    if not fresh:
+        _written(out)
     return out
 
 
@@ -308,8 +317,8 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     s_n, s_h, s_k, s_v = state.stride()
     _require((s_v == 1 or dv == 1) and (s_k == dv or dk == 1), "state's matrices must be contiguous")
     _require((n <= 1 or s_n >= dk * dv) and (h <= 1 or s_h >= dk * dv), "state's matrices must not overlap")
-    given = None
-    if out is None:
+    given, fresh = None, out is None
+    if fresh:
         out = torch.empty((n, h, dv), dtype=q.dtype, device=q.device)
     else:
         _on(out, dev, "out")
@@ -324,7 +333,11 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
                                     _DTYPE[q.dtype], g.data_ptr(), beta.data_ptr(), *g.stride(), *beta.stride(), reset_ptr,
                                     reset_n, state.data_ptr(), s_n, s_h, out.data_ptr(), n, h, dk, dv,
                                     dk ** -0.5 if scale is None else scale, dev), _stream(dev))
-    return out if given is None else given.copy_(out)
+    if given is not None:
+        _written(state)
+        return given.copy_(out)
+    _written(state if fresh else (state, out))
+    return out
 
 
 def _scan_args(q, k, v, g, beta, reset, state, scale, dev, *rest: int) -> bytes:

@@ -462,3 +462,28 @@ def test_step_writes_out_on_the_memory_of_an_input(on, dk):
     assert got is out and torch.equal(out, want)
     if on != "state":
         assert torch.equal(again, state)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("aliased", [False, True])
+def test_a_gradient_that_saved_the_state_or_out_is_refused_after_a_step(aliased):
+    """As after any torch operation in place; it would be that of the new values."""
+    x = inputs(1, 2, 1, 16, 16, seed=31)
+    one = [x[i][0] for i in NAMES[:5]]
+    state, out = x["state"], one[2] if aliased else torch.ones((2, 1, 16), device="cuda")
+    for written in (state, state[:1], out):  # a view is the same memory
+        a = torch.ones_like(written).requires_grad_()
+        saved = (a * written).sum()
+        ops.delta_step(*one, state, out=out)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            saved.backward()
+    a = torch.ones_like(one[0]).requires_grad_()
+    saved = (a * one[0]).sum()
+    ops.delta_step(*one, state)
+    saved.backward()  # inputs are not written
+    assert torch.equal(a.grad, one[0])
+    with torch.inference_mode():
+        state = x["state"].clone()
+        want = ops.delta_step(*one, state)
+    state.sum(), want.sum()
+    ops.delta_step(*one, state)  # has no version to raise

@@ -331,3 +331,14 @@ def test_out_on_the_memory_of_the_tokens(m, k, n):
     store = torch.zeros((m, n), device="cuda")
     store[0] = bias
     assert torch.equal(ops.int8_linear(x, w, scales, store[0], out=store), want)
+
+
+@pytest.mark.gpu
+def test_a_gradient_that_saved_out_is_refused_when_it_has_been_written():
+    q, ws = _weight(8, 32, 1)
+    x, out = torch.ones((4, 32), dtype=torch.uint8, device="cuda"), torch.ones((4, 8), device="cuda")
+    a = torch.ones_like(out).requires_grad_()
+    saved = (a * out).sum()
+    ops.int8_linear(x, ops.Int8Weight(q, ws), 1.0, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()

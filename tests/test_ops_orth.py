@@ -169,3 +169,14 @@ def test_in_a_thread_that_has_made_no_cuda_call():
     thread.join()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+@pytest.mark.gpu
+def test_a_gradient_that_saved_out_is_refused_when_it_has_been_written():
+    x = momentum(8, 12)
+    out = torch.ones((8, 12), device="cuda", dtype=torch.bfloat16)
+    a = torch.ones_like(out).requires_grad_()
+    saved = (a * out).sum()
+    ops.orthogonalize(x, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.backward()
