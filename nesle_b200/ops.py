@@ -176,7 +176,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
     n, k = weight.n, weight.k
     shape = x.shape
     _require(len(shape) >= 1 and shape[-1] == k, f"x must have {k} columns, has shape {tuple(shape)}")
-    _no_grad_path("int8_linear", x, bias)
+    _no_grad_path("int8_linear", x, bias, x_scale if isinstance(x_scale, torch.Tensor) else None)
     if x.dtype in _DTYPE:
         _require(x_scale is None, "x_scale is computed where x is floating")
         x, x_scale = quantize_rows(x)

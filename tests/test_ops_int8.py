@@ -342,3 +342,14 @@ def test_a_gradient_that_saved_out_is_refused_when_it_has_been_written():
     ops.int8_linear(x, ops.Int8Weight(q, ws), 1.0, out=out)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         saved.backward()
+
+
+@pytest.mark.gpu
+def test_a_scale_that_wants_a_gradient_is_refused():
+    q, ws = _weight(8, 32, 1)
+    x, w = torch.ones((4, 32), dtype=torch.uint8, device="cuda"), ops.Int8Weight(q, ws)
+    scale = torch.ones(4, device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        ops.int8_linear(x, w, scale)
+    with torch.no_grad():
+        assert torch.equal(ops.int8_linear(x, w, scale), ops.int8_linear(x, w, 1.0))
