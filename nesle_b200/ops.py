@@ -176,7 +176,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
     n, k = weight.n, weight.k
     shape = x.shape
     _require(len(shape) >= 1 and shape[-1] == k, f"x must have {k} columns, has shape {tuple(shape)}")
-    _no_grad_path("int8_linear", x, bias, x_scale if isinstance(x_scale, torch.Tensor) else None)
+    _no_grad_path("int8_linear", x, bias, x_scale if isinstance(x_scale, torch.Tensor) else None, out)
     if x.dtype in _DTYPE:
         _require(x_scale is None, "x_scale is computed where x is floating")
         x, x_scale = quantize_rows(x)
@@ -240,7 +240,7 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, eps: float = 1e-7,
     dev = _cuda_device(update, "update")
     _require(update.dtype in _DTYPE, "update must be float32, bfloat16 or float16")
     _require(update.dim() >= 2, "update must have at least two dimensions")
-    _no_grad_path("orthogonalize", update)
+    _no_grad_path("orthogonalize", update, out)
     rows, cols = update.shape[-2:]
     fresh = out is None
     if fresh:
@@ -308,7 +308,7 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     inputs, but ``state`` must share none with them).  Without gradients: for a sequence with gradients see
     :func:`delta_scan`."""
     dev = _delta_inputs(q, k, v, g, beta, reset, "nh")
-    _no_grad_path("delta_step", q, k, v, g, beta, state)
+    _no_grad_path("delta_step", q, k, v, g, beta, state, out)
     n, h, dk = q.shape
     dv = v.shape[-1]
     _on(state, dev, "state")

@@ -487,3 +487,14 @@ def test_a_gradient_that_saved_the_state_or_out_is_refused_after_a_step(aliased)
         want = ops.delta_step(*one, state)
     state.sum(), want.sum()
     ops.delta_step(*one, state)  # has no version to raise
+
+
+@pytest.mark.gpu
+def test_an_out_that_wants_a_gradient_is_refused():
+    x = inputs(1, 2, 1, 16, 16, seed=32)
+    out = torch.ones((2, 1, 16), device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        ops.delta_step(*(x[i][0] for i in NAMES[:5]), x["state"], out=out)
+    with torch.no_grad():
+        want = ops.delta_step(*(x[i][0] for i in NAMES[:5]), x["state"].clone())
+        assert torch.equal(ops.delta_step(*(x[i][0] for i in NAMES[:5]), x["state"], out=out), want)

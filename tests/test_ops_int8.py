@@ -353,3 +353,14 @@ def test_a_scale_that_wants_a_gradient_is_refused():
         ops.int8_linear(x, w, scale)
     with torch.no_grad():
         assert torch.equal(ops.int8_linear(x, w, scale), ops.int8_linear(x, w, 1.0))
+
+
+@pytest.mark.gpu
+def test_an_out_that_wants_a_gradient_is_refused():
+    q, ws = _weight(8, 32, 1)
+    x, w = torch.ones((4, 32), dtype=torch.uint8, device="cuda"), ops.Int8Weight(q, ws)
+    out = torch.ones((4, 8), device="cuda", requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        ops.int8_linear(x, w, 1.0, out=out)
+    with torch.no_grad():
+        assert torch.equal(ops.int8_linear(x, w, 1.0, out=out), ops.int8_linear(x, w, 1.0, out_dtype=torch.float32))

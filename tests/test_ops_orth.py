@@ -180,3 +180,12 @@ def test_a_gradient_that_saved_out_is_refused_when_it_has_been_written():
     ops.orthogonalize(x, out=out)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         saved.backward()
+
+
+@pytest.mark.gpu
+def test_an_out_that_wants_a_gradient_is_refused():
+    out = torch.ones((8, 12), device="cuda", dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match="no gradient"):
+        ops.orthogonalize(momentum(8, 12), out=out)
+    with torch.no_grad():
+        assert torch.equal(ops.orthogonalize(momentum(8, 12), out=out), ops.orthogonalize(momentum(8, 12)))
