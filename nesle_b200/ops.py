@@ -21,6 +21,7 @@ import ctypes
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -53,6 +54,10 @@ def _no_grad_path(name: str, *tensors) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise ValueError(f"{name} has no gradient; call it under torch.no_grad() or on detached tensors")
+    if forward_ad._current_level >= 0:  # within a dual_level()
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError(f"{name} has no forward-mode derivative; call it on primal tensors")
 
 
 def _span(x: torch.Tensor) -> tuple[int, int]:

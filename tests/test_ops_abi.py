@@ -105,3 +105,21 @@ def test_tensors_that_are_not_on_a_gpu_are_refused():
         ops.int8_linear(x, None)
     with pytest.raises(ValueError, match="CUDA"):
         ops.Int8Weight(torch.zeros((4, 4), dtype=torch.int8), torch.zeros(4))
+
+
+def test_tangents_are_refused_and_not_dropped():
+    """A dual tensor does not require grad; a call on it would go on without its tangent."""
+    torch = pytest.importorskip("torch")
+    from torch.autograd import forward_ad
+
+    from nesle_b200 import ops
+
+    x = torch.ones(3)
+    ops._no_grad_path("call", x, None)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, x)
+        with pytest.raises(ValueError, match="forward-mode"):
+            ops._no_grad_path("call", None, x, dual)
+        with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
+            ops._no_grad_path("call", dual)
+        ops._no_grad_path("call", x, forward_ad.unpack_dual(dual).primal)

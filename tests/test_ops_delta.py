@@ -498,3 +498,26 @@ def test_an_out_that_wants_a_gradient_is_refused():
     with torch.no_grad():
         want = ops.delta_step(*(x[i][0] for i in NAMES[:5]), x["state"].clone())
         assert torch.equal(ops.delta_step(*(x[i][0] for i in NAMES[:5]), x["state"], out=out), want)
+
+
+@pytest.mark.gpu
+def test_tangents_are_refused():
+    from torch.autograd import forward_ad
+
+    x = inputs(1, 2, 1, 16, 16, seed=33)
+    one = [x[i][0] for i in NAMES[:5]] + [x["state"]]
+    q = torch.ones((4, 16), dtype=torch.int8, device="cuda")
+    w = ops.Int8Weight(q, torch.ones(4, device="cuda"))
+    with forward_ad.dual_level():
+        for i in range(6):
+            args = [forward_ad.make_dual(y, torch.ones_like(y)) if i == j else y for j, y in enumerate(one)]
+            with pytest.raises(ValueError, match="forward-mode"):
+                ops.delta_step(*args)
+            with pytest.raises(NotImplementedError):
+                ops.delta_scan(*(y[None] for y in args[:5]), args[5])
+        ones = forward_ad.make_dual(torch.ones((4, 16), device="cuda"), torch.ones((4, 16), device="cuda"))
+        for call in (lambda: ops.orthogonalize(ones), lambda: ops.quantize_rows(ones), lambda: ops.int8_linear(ones, w),
+                     lambda: ops.int8_linear(q, w, 1.0, ones[0, :4]), lambda: ops.int8_linear(q, w, ones[:, 0])):
+            with pytest.raises(ValueError, match="forward-mode"):
+                call()
+        ops.delta_step(*one)
