@@ -574,6 +574,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                 decay = gates.decay();
                 starts = gates.starts();
                 if (aligned && !tc::mbar_wait_warp(&arrived[b % L::kBuffers], b / L::kBuffers & 1)) {
+                    for (int64_t x = b; x < blocks && x < b + 2; ++x) tc::mbar_drain(&arrived[x % L::kBuffers], x / L::kBuffers & 1);
                     if (lane == 0) {
                         atomicAdd(p.stalls, 1u);
                         ch.block = -1;
@@ -694,7 +695,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
         const Chunk& ch = chunks[turn & 1];
         const int64_t b = ch.block;
         if (b < 0) break;
-        if (aligned) tc::mbar_wait_warp(&arrived[b % L::kBuffers], b / L::kBuffers & 1);  // long since; it makes the copies visible here
+        if (aligned) tc::mbar_see(&arrived[b % L::kBuffers], b / L::kBuffers & 1);  // the helper waited for them
         const int r0 = ch.r0, r1 = ch.r1;
         if (!kEnds && p.checkpoints && r0 == 0) put_state(p.checkpoints + (seq * all + b0 + b) * dk * dv);
         if (ch.fresh) {
@@ -1149,6 +1150,18 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
         int64_t b = blocks, turn_of_block = -1;
         int r1 = 0;
         if (L::kBuffers == 3) fetch(blocks - 1);
+        // A wait has given up: no chunk follows the one at hand.  Block b, if it has not been waited for, and the one fetched
+        // ahead of it are still on their way.
+        uint32_t states = 0;  // fetched so far
+        auto give_up = [&](BackChunk& ch, int first) {
+            for (int x = first; aligned && x <= (L::kBuffers == 3) && b - x >= 0; ++x)
+                tc::mbar_drain(&sh.arrived[(b - x) % L::kBuffers], (turn_of_block + x) / L::kBuffers & 1);
+            if (lane == 0) {
+                atomicAdd(p.stalls, 1u);
+                ch.block = -1;
+            }
+            b = 0, r1 = 0;
+        };
         // the chunk before the last one prepared
         auto prepare = [&](BackChunk& ch) {
             if (r1 == 0) {
@@ -1166,11 +1179,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
                 starts = gates.starts();
                 // phases of a buffer's barrier count the blocks that it has held
                 if (aligned && !tc::mbar_wait_warp(&sh.arrived[b % L::kBuffers], turn_of_block / L::kBuffers & 1)) {
-                    if (lane == 0) {
-                        atomicAdd(p.stalls, 1u);
-                        ch.block = -1;
-                    }
-                    b = 0, r1 = 0;
+                    give_up(ch, 0);
                     return;
                 }
                 __syncwarp();
@@ -1290,7 +1299,12 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
             if (ch.block < 0) break;
             __syncwarp();
             __syncthreads();  // after U, ubar and dS are in shared memory
-            prepare(sh.chunk[(turn & 1) ^ 1]);
+            BackChunk& next = sh.chunk[(turn & 1) ^ 1];
+            prepare(next);
+            if (ch.state && fetch_state && !tc::mbar_wait_warp(&sh.state_arrived, states++ & 1)) {  // the warps read it by now
+                tc::mbar_drain(&sh.state_arrived, (states - 1) & 1);
+                give_up(next, 1);
+            }
             __syncthreads();  // after dA and dP are
         }
         return;
@@ -1328,7 +1342,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
         const uint32_t m0 = pair_mask(quad * 2, r0, r1), m1 = pair_mask(quad * 2 + 8, r0, r1);
         // the copies of this block were waited for by the helper; a wait that is over makes them visible here
         if constexpr (L::kInPlace)
-            if (aligned) tc::mbar_wait_warp(&sh.arrived[b % L::kBuffers], (blocks - 1 - b) / L::kBuffers & 1);
+            if (aligned) tc::mbar_see(&sh.arrived[b % L::kBuffers], (blocks - 1 - b) / L::kBuffers & 1);
 
         uint32_t xa[3][4];  // (-beta gamma ubar)^T for the update of dS
         if (has_v) {
@@ -1536,7 +1550,7 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
         for (int c = 0; c < 2; ++c) dq[c].zero(), dk[c].zero(), dku[c].zero();
         if (has_k) {
             const float* s0 = p.checkpoints + (seq * blocks + b) * dk_ * dv_;
-            if (fetch_state && state) tc::mbar_wait_warp(&sh.state_arrived, states & 1);
+            if (fetch_state && state) tc::mbar_see(&sh.state_arrived, states & 1);
             float dot = 0.f;
 #pragma unroll
             for (int s = 0; s < DV / 16; ++s) {

@@ -42,18 +42,22 @@ __device__ __forceinline__ bool mbar_try(uint64_t* b, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-// Waits for the phase with `parity` to end; false after kWaitClocks.
-__device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity) {
+// Waits for the phase with `parity` to end; false after `clocks`.  Whoever calls it says what a false means.
+[[nodiscard]] __device__ __forceinline__ bool mbar_wait(uint64_t* b, uint32_t parity, long long clocks = kWaitClocks) {
     if (mbar_try(b, parity)) return true;
     const long long t0 = clock64();
     while (!mbar_try(b, parity))
-        if (clock64() - t0 > kWaitClocks) return false;
+        if (clock64() - t0 > clocks) return false;
     return true;
 }
 // The same for a whole warp: all lanes go on, or none.
-__device__ __forceinline__ bool mbar_wait_warp(uint64_t* b, uint32_t parity) {
-    return __all_sync(0xffffffffu, mbar_wait(b, parity));
+[[nodiscard]] __device__ __forceinline__ bool mbar_wait_warp(uint64_t* b, uint32_t parity, long long clocks = kWaitClocks) {
+    return __all_sync(0xffffffffu, mbar_wait(b, parity, clocks));
 }
+// For a phase that another warp waits for as well and answers for: makes its copies visible to this one.
+__device__ __forceinline__ void mbar_see(uint64_t* b, uint32_t parity) { (void)mbar_wait_warp(b, parity); }
+// After a wait has given up: copies still on their way land, if they ever do, before their memory is given back.
+__device__ __forceinline__ void mbar_drain(uint64_t* b, uint32_t parity) { (void)mbar_wait_warp(b, parity); }
 
 __device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(m) : "memory");
