@@ -1150,25 +1150,14 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
         int64_t b = blocks, turn_of_block = -1;
         int r1 = 0;
         if (L::kBuffers == 3) fetch(blocks - 1);
-        // A wait has given up: no chunk follows the one at hand.  Block b, if it has not been waited for, and the one fetched
-        // ahead of it are still on their way.
         uint32_t states = 0;  // fetched so far
-        auto give_up = [&](BackChunk& ch, int first) {
-            for (int x = first; aligned && x <= (L::kBuffers == 3) && b - x >= 0; ++x)
-                tc::mbar_drain(&sh.arrived[(b - x) % L::kBuffers], (turn_of_block + x) / L::kBuffers & 1);
-            if (lane == 0) {
-                atomicAdd(p.stalls, 1u);
-                ch.block = -1;
-            }
-            b = 0, r1 = 0;
-        };
-        // the chunk before the last one prepared
-        auto prepare = [&](BackChunk& ch) {
+        // The chunk before the last one prepared; false where a wait has given up.
+        auto prepare = [&](BackChunk& ch) -> bool {
             if (r1 == 0) {
                 --b;
                 if (b < 0) {
                     if (lane == 0) ch.block = -1;
-                    return;
+                    return true;
                 }
                 ++turn_of_block;
                 r1 = (int)(p.t - b * kC < kC ? p.t - b * kC : kC);
@@ -1179,8 +1168,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
                 starts = gates.starts();
                 // phases of a buffer's barrier count the blocks that it has held
                 if (aligned && !tc::mbar_wait_warp(&sh.arrived[b % L::kBuffers], turn_of_block / L::kBuffers & 1)) {
-                    give_up(ch, 0);
-                    return;
+                    if (lane == 0) atomicAdd(p.stalls, 1u);
+                    return false;
                 }
                 __syncwarp();
                 if constexpr (!L::kInPlace) {
@@ -1242,6 +1231,13 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
             store_terms<3>(ch.n, hs.b, lane);
             __syncwarp();
             r1 = r0;
+            return true;
+        };
+        // After a wait that gave up no chunk follows the one at hand, and blocks on their way land before the block leaves.
+        auto give_up = [&](BackChunk& ch) {
+            for (int x = 0; aligned && x <= (L::kBuffers == 3) && b >= x; ++x)  // block b, and the one fetched ahead of it
+                tc::mbar_drain(&sh.arrived[(b - x) % L::kBuffers], (turn_of_block + x) / L::kBuffers & 1);
+            if (lane == 0) ch.block = -1;
         };
         // dg and dbeta of a chunk, from its sums
         auto finish = [&](const BackChunk& ch, const typename L::Sums& sums) {
@@ -1285,26 +1281,31 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
                 p.dbeta[to] = dbeta;
             }
         };
-        prepare(sh.chunk[0]);
+        bool ok = prepare(sh.chunk[0]);
+        if (!ok) give_up(sh.chunk[0]);
         __syncthreads();
         for (int turn = 0;; ++turn) {
             const BackChunk& ch = sh.chunk[turn & 1];
-            if (ch.block >= 0 && ch.state && fetch_state && lane == 0) {
-                tc::mbar_expect_tx(&sh.state_arrived, (uint32_t)L::kFetched);
+            if (states && !tc::mbar_wait_warp(&sh.state_arrived, (states - 1) & 1)) {  // the warps have read it
+                tc::mbar_drain(&sh.state_arrived, (states - 1) & 1);
+                if (lane == 0) atomicAdd(p.stalls, 1u);
+                ok = false;
+            }
+            if (ok && ch.block >= 0 && ch.state && fetch_state) {
+                ++states;
+                if (lane == 0) {
+                    tc::mbar_expect_tx(&sh.state_arrived, (uint32_t)L::kFetched);
 #pragma unroll
-                for (int i = 0; i < Fetch<float, DV>::kPanels; ++i)
-                    tc::tma_load_3d(fetched + i * DK * 32, &map_s, &sh.state_arrived, i * 32, 0, (int)(seq * blocks + ch.block));
+                    for (int i = 0; i < Fetch<float, DV>::kPanels; ++i)
+                        tc::tma_load_3d(fetched + i * DK * 32, &map_s, &sh.state_arrived, i * 32, 0, (int)(seq * blocks + ch.block));
+                }
             }
             if (turn) finish(sh.chunk[(turn & 1) ^ 1], sh.sums[(turn & 1) ^ 1]);
             if (ch.block < 0) break;
             __syncwarp();
             __syncthreads();  // after U, ubar and dS are in shared memory
             BackChunk& next = sh.chunk[(turn & 1) ^ 1];
-            prepare(next);
-            if (ch.state && fetch_state && !tc::mbar_wait_warp(&sh.state_arrived, states++ & 1)) {  // the warps read it by now
-                tc::mbar_drain(&sh.state_arrived, (states - 1) & 1);
-                give_up(next, 1);
-            }
+            if (!ok || !(ok = prepare(next))) give_up(next);
             __syncthreads();  // after dA and dP are
         }
         return;
