@@ -134,7 +134,8 @@ typedef struct nesle_delta_args {
 } nesle_delta_args;
 
 /* The same over t tokens; and its gradients, of all inputs, from those of o and of the final state.  The backward call
- * takes the forward call's inputs, errors and checkpoints.  The gradient of g is zero at tokens that start an episode. */
+ * takes the forward call's inputs, errors and checkpoints.  The gradient of g is zero at tokens that start an episode.
+ * A token that is not finite leaves outputs before it as they are; gradients of its whole episode may not be finite. */
 uint64_t nesle_delta_error_floats(const nesle_delta_args* args);
 uint64_t nesle_delta_checkpoint_floats(const nesle_delta_args* args);
 int nesle_delta_scan(const nesle_delta_args* args, void* stream);

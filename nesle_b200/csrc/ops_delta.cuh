@@ -448,6 +448,61 @@ struct Fetch {
     }
 };
 
+// Which tokens of fetched tiles hold a NaN or an infinity: 0 * x adds up to zero over all else.  A lane adds up its 16-byte
+// chunks, sum z those of token 4 z + lane / 8.
+template <class T>
+struct NotFinite {
+    using Two = std::conditional_t<sizeof(T) == 4, float, std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>>;
+    Two sum[4];
+    __device__ __forceinline__ NotFinite() {
+#pragma unroll
+        for (int z = 0; z < 4; ++z) sum[z] = zero();
+    }
+    static __device__ __forceinline__ Two zero() {
+        const uint32_t bits = 0;
+        return reinterpret_cast<const Two&>(bits);
+    }
+    static __device__ __forceinline__ bool bad(Two x) {
+        if constexpr (sizeof(T) == 4)
+            return x != x;
+        else
+            return !(to_f32(x.x) + to_f32(x.y) == 0.f);  // zeros but for a NaN
+    }
+    template <int D>
+    __device__ __forceinline__ void add(const T* tile, int lane) {
+        const uint4* chunks = reinterpret_cast<const uint4*>(tile);
+#pragma unroll
+        for (int i = 0; i < Fetch<T, D>::kPanels; ++i)
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                const uint4 x = chunks[i * kC * 8 + z * 32 + lane];
+                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (sizeof(T) == 4)
+                        sum[z] = fmaf(__uint_as_float(w[j]), 0.f, sum[z]);
+                    else
+                        sum[z] = __hfma2(reinterpret_cast<const Two&>(w[j]), zero(), sum[z]);
+                }
+            }
+    }
+    // Bit i for token i; `gate`, of lane i, is NaN where token i's gates are not finite.
+    __device__ __forceinline__ uint32_t tokens(float gate) const {
+        uint32_t out = 0;
+        const Two all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (__any_sync(0xffffffffu, bad(all) || gate != gate)) {
+            out = __ballot_sync(0xffffffffu, gate != gate);
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                const uint32_t lanes = __ballot_sync(0xffffffffu, bad(sum[z]));
+#pragma unroll
+                for (int g = 0; g < 4; ++g) out |= (lanes >> 8 * g & 0xFF ? 1u : 0u) << (z * 4 + g);
+            }
+        }
+        return out;
+    }
+};
+
 template <class T, int D>
 __device__ __forceinline__ void to_terms_warp(__nv_bfloat16* terms, int ld, const T* raw, int lane) {
     constexpr int N = Terms<T>::n;
@@ -555,7 +610,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
         const GatePointers get_gates(p, n, h, lane);
         Gates gates{}, next = get_gates.load(t0, p.t, lane);
         float decay = 1.f;
-        uint32_t starts = 0;
+        uint32_t starts = 0, cuts = 0;  // tokens that start an episode, and that begin a chunk for another reason
         int64_t b = -1;
         int r0 = 0, count = 0, restarts = 0;
         for (int turn = 0;; ++turn) {
@@ -584,6 +639,14 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                 }
                 __syncwarp();
                 fetch(b + 2);
+                if constexpr (!kEnds) {
+                    // A token whose key, value or gates are not finite begins a chunk: the products of a chunk multiply it by
+                    // the zeros that stand for "later" too, and would spoil the tokens before it.
+                    NotFinite<T> look;
+                    look.template add<DK>(raw_tile(b), lane);
+                    look.template add<L::kWidth>(raw_tile(b) + 2 * L::kTileK, lane);
+                    cuts = look.tokens((decay + gates.beta) * 0.f) & ((1u << count) - 1);
+                }
                 if constexpr (!L::kInPlace) {
                     __nv_bfloat16* to = terms + (b & 1) * 2 * NT * kC * L::kLdTerm;
                     to_terms_warp<T, DK>(to, L::kLdTerm, raw_tile(b), lane);
@@ -593,7 +656,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
             }
             const bool fresh = starts >> r0 & 1;
             restarts |= fresh;
-            const uint32_t later = starts & ~((2u << r0) - 1);
+            const uint32_t later = (starts | cuts) & ~((2u << r0) - 1);
             const int r1 = later ? min(count, __ffs(later) - 1) : count;
             chunk_decays(hs.d, ch.gamma, ch.eta, ch.beta, ch.keep, within(lane, r0, r1) ? decay : 1.f, gates.beta, r0, r1, fresh, lane);
             if (lane == 0) ch.block = (int)b, ch.r0 = r0, ch.r1 = r1, ch.fresh = fresh;

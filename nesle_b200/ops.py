@@ -425,7 +425,8 @@ def delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     ``q, k``: (t, n, h, dk), ``v``: (t, n, h, dv), one of float32, bfloat16 and float16, any strides (rows copied unless
     the last is 1); ``g, beta``: (t, n, h) float32; ``state``: (n, h, dk, dv) float32 before the first token, or None for
     zeros; ``reset``: (t, n) bool or uint8, True where a token starts an episode: nothing before it, not even a NaN,
-    reaches it, and no gradient passes.  States and sums are fp32 throughout.  With gradients a call keeps one state for
+    reaches it, and no gradient passes.  A NaN or an infinity in a token reaches no earlier one (in the gradients it may
+    spoil all tokens of its episode).  States and sums are fp32 throughout.  With gradients a call keeps one state for
     every 16 tokens until its backward pass."""
     dev = _delta_inputs(q, k, v, g, beta, reset, "tnh")
     t, n, h, dk = q.shape

@@ -521,3 +521,26 @@ def test_tangents_are_refused():
             with pytest.raises(ValueError, match="forward-mode"):
                 call()
         ops.delta_step(*one)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("name", ["q", "k", "v", "g", "beta"])
+@pytest.mark.parametrize("t,dk,dv,dtype", [(40, 64, 64, torch.bfloat16), (40, 64, 64, torch.float32), (40, 128, 128, torch.float16),
+                                           (40, 40, 72, torch.bfloat16), (40, 33, 65, torch.float32), (700, 64, 64, torch.bfloat16)])
+def test_what_is_not_finite_reaches_no_earlier_token(t, dk, dv, dtype, name, value):
+    """As in the recurrence, token by token: a token that is not finite leaves those before it, and columns of the state that
+    it does not reach, as they are; several in one block of 16, in the first token and in the last of the sequence."""
+    x = inputs(t, 2, 2, dk, dv, dtype, 0.0, seed=34)
+    assert is_cut(t, 2, 2, dk, dv) == (t == 700)
+    for at, n in ((13, 0), (t - 1, 1)):
+        x[name].view(t, 2, 2, -1)[at, n, 0, -1] = value
+    x["v"][9, 0, 1, 2], x["v"][15, 0, 1, 3], x["v"][22, 0, 1, 2] = value, value, value  # columns of their own
+    x["k"][16, 1, 1, 0] = value
+    want_o, want_s = reference({i: (y if i == "reset" else y.double()) for i, y in x.items()})
+    o, s = ops.delta_scan(*(x[i] for i in NAMES), x["reset"])
+    for got, want, what in ((o, want_o, "o"), (s, want_s, "state")):
+        finite = torch.isfinite(want)
+        assert bool(finite.any()) and not bool(finite.all())
+        assert torch.equal(torch.isfinite(got), finite), what
+        close(torch.where(finite, got, 0), torch.where(finite, want, 0), dk, dv, what)
