@@ -139,8 +139,8 @@ typedef struct nesle_delta_args {
 uint64_t nesle_delta_error_floats(const nesle_delta_args* args);
 uint64_t nesle_delta_checkpoint_floats(const nesle_delta_args* args);
 int nesle_delta_scan(const nesle_delta_args* args, void* stream);
-/* Where a few long sequences would leave most of the GPU idle, nesle_delta_split_floats is not 0, and a workspace of so many
- * floats (16-byte aligned for speed) lets the scan cut them into segments that run side by side.  NULL: one scan. */
+/* Where a few long sequences would leave most of the GPU idle, nesle_delta_split_floats (of the sizes, type and device) is not 0, and a workspace of
+ * so many floats (16-byte aligned for speed) lets the scan cut them into segments that run side by side.  NULL: one scan. */
 uint64_t nesle_delta_split_floats(const nesle_delta_args* args);
 int nesle_delta_scan_split(const nesle_delta_args* args, float* workspace, void* stream);
 int nesle_delta_scan_backward(const nesle_delta_args* args, void* stream);

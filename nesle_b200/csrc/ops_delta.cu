@@ -159,6 +159,12 @@ bool rows_aligned(const nesle_delta_args& x, const void* p, int64_t st, int64_t 
     return reinterpret_cast<uintptr_t>(p) % 16 == 0 && ok(x.t, st) && ok(x.n, sn) && ok(x.h, sh) && x.t <= 0x7FFFFFFFull;
 }
 
+int segments_of(const nesle_delta_args& a) {
+    const int dk = (int)a.dk;
+    const SplitCosts c = a.dtype == NESLE_F32 ? split_costs<float>(dk) : a.dtype == NESLE_BF16 ? split_costs<__nv_bfloat16>(dk) : split_costs<__half>(dk);
+    return count_segments((int64_t)a.t, (int64_t)(a.n * a.h), dk, (int)a.dv, sm_count(a.device), c);
+}
+
 Scan to_scan(const nesle_delta_args& a, bool backward) {
     Scan p{};
     p.q = a.q, p.k = a.k, p.v = a.v;
@@ -226,7 +232,7 @@ uint64_t nesle_delta_error_floats(const nesle_delta_args* a) {
 
 uint64_t nesle_delta_split_floats(const nesle_delta_args* a) {
     if (!a || delta::check_common(a->dtype, a->n, a->h, a->dk, a->dv) || !a->t || a->t > 0x7FFFFFFFull || !a->n || !a->h) return 0;
-    const int segments = delta::count_segments((int64_t)a->t, (int64_t)(a->n * a->h), (int)a->dk, (int)a->dv, sm_count(a->device));
+    const int segments = delta::segments_of(*a);
     return a->n * a->h * (uint64_t)(segments - 1) * (a->dk * (a->dk + a->dv) + 1);
 }
 
@@ -246,7 +252,7 @@ int nesle_delta_scan_split(const nesle_delta_args* args, float* workspace, void*
         if (reinterpret_cast<uintptr_t>(workspace) % 4) return invalid("delta_scan: workspace must be aligned");
         delta::Scan p = delta::to_scan(a, false);
         if (workspace && a.t && a.t <= 0x7FFFFFFFull) {
-            p.segments = delta::count_segments(p.t, p.n * p.h, p.dk, p.dv, sm_count(a.device));
+            p.segments = delta::segments_of(a);
             const int64_t all = (p.t + delta::kC - 1) / delta::kC;
             p.per = (all + p.segments - 1) / p.segments;
             p.ends = workspace;

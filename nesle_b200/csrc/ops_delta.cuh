@@ -30,6 +30,7 @@
 #pragma once
 #include <stddef.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "ops_common.h"
@@ -1827,20 +1828,43 @@ inline bool on_16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 ==
 // A sequence's chunks follow one another, so a few long ones leave most SMs idle.  The state after a segment is linear
 // in the state before it, S' = A S + B: so first every segment's A and B at once, as scans from a unit matrix without
 // values and from zero (outputs left out), then the ends in order, one small product each, then every segment's outputs
-// at once from the state before it.  That is two scans of 1 / G of the chunks and G joins, of a chunk's time each, in
-// place of one scan, as long as a pass's blocks are all on the GPU together.  bfloat16, cut and whole: 4 envs x 4 heads
-// x 4,096 tokens of 128 in 6 segments 250 and 525 us, of 64 in 14 107 and 420; 1 x 2 x 4,096 of 128 in 21 about 115 and
-// 521; 4 x 4 x 512 of 128 in 5 57 and 70, of 64 in 8 37 and 57; 8 x 4 x 1,024 of 64 in 8 57 and 109.  More segments than
-// the GPU holds at once are slower again: 306 us for 7 in the first.
-constexpr int kSplitCost = 10;  // of the two more launches, in chunks
+// at once from the state before it.  That is two passes of 1 / G of the chunks and G joins in place of one pass.  A pass
+// takes as long as the SM with most blocks; how many an SM holds at once goes by the type and by dk, and they slow one
+// another (kSharing).  Swept over 24 shapes and three types: the count chosen so is within 3% of the best on average, and
+// nowhere slower than the sequence whole by more than measurements differ.  Cut and whole, us:
+//
+//   envs x heads x tokens, dk = dv   bfloat16                  float16                    float32
+//   4 x 4 x 4,096 of 128             249 (6 segments) 523      696 (8) 1,318              834 (8) 1,626
+//   4 x 4 x 4,096 of 64              106 (15) 420              171 (18) 773               197 (18) 992
+//   4 x 4 x 512 of 128               58 (6) 70                 114 (3) 170                135 (3) 209
+//   4 x 4 x 512 of 64                37 (8) 58                 47 (8) 101                 51 (8) 129
+//   8 x 4 x 1,024 of 64              58 (8) 109                91 (6) 198                 105 (6) 252
+//   8 x 4 x 1,024 of 128             whole: 136, 3 would too   whole: 336, 3 take 394     whole: 414, 3 take 472
+//
+// Costs are in tenths of a chunk's time, which is 1.6 to 2 us in bfloat16 and two to three times that in the others; the
+// joins and the two more launches take the same time in all.
+struct SplitCosts {
+    int blocks;        // of the passes that an SM holds at once
+    int join, launch;  // of a segment, and of the two more launches
+};
+template <class T>
+inline SplitCosts split_costs(int dk) {
+    auto fit = [](size_t bytes, int most) { return std::min(most, (int)(228 * 1024 / (bytes + 1024))); };  // 1 KB a block is the system's
+    const int blocks = dk > 64 ? fit(ForwardSmem<T, 128>::kBytes, 2) : dk > 32 ? fit(ForwardSmem<T, 64>::kBytes, 3) : fit(ForwardSmem<T, 32>::kBytes, 3);
+    return Terms<T>::n == 1 ? SplitCosts{blocks, 10, 100} : SplitCosts{blocks, 5, 50};
+}
 
-inline int count_segments(int64_t t, int64_t heads, int dk, int dv, int sms) {
-    const int64_t all = (t + kC - 1) / kC, blocks = (int64_t)sms * (dk > 64 ? 2 : 3);
-    const int64_t value_blocks = (dv + 63) / 64, key_blocks = (dk + 63) / 64;
-    int64_t best = 1, best_cost = all;
-    for (int64_t g = 3; g <= all && g <= kMostSegments; ++g) {
-        if (heads * ((g - 1) * value_blocks + (g - 2) * key_blocks) > blocks || heads * g * value_blocks > blocks) break;
-        const int64_t cost = 2 * ((all + g - 1) / g) + g + kSplitCost;
+inline int count_segments(int64_t t, int64_t heads, int dk, int dv, int sms, const SplitCosts& c) {
+    constexpr int kSharing[2][4] = {{0, 10, 10, 12}, {0, 10, 13, 13}};  // a chunk's time where so many blocks share an SM; dk > 64
+    const int64_t all = (t + kC - 1) / kC, value_blocks = (dv + 63) / 64, key_blocks = (dk + 63) / 64;
+    auto pass = [&](int64_t blocks) {
+        const int64_t most = (blocks + sms - 1) / sms;
+        return most / c.blocks * kSharing[dk > 64][c.blocks] + kSharing[dk > 64][most % c.blocks];
+    };
+    int64_t best = 1, best_cost = all * pass(heads * value_blocks);
+    for (int64_t g = 3; g <= all && g <= kMostSegments && g * c.join + c.launch < best_cost; ++g) {
+        const int64_t cost = (all + g - 1) / g * (pass(heads * ((g - 1) * value_blocks + (g - 2) * key_blocks)) + pass(heads * g * value_blocks)) +
+                             g * c.join + c.launch;
         if (cost < best_cost) best = g, best_cost = cost;
     }
     const int64_t per = (all + best - 1) / best;

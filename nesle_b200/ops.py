@@ -363,9 +363,10 @@ def _scan_sizes(t: int, n: int, h: int, dk: int, dv: int) -> tuple[int, int]:
 
 
 @functools.lru_cache(maxsize=256)
-def _scan_split(t: int, n: int, h: int, dk: int, dv: int, dev: int) -> int:
+def _scan_split(t: int, n: int, h: int, dk: int, dv: int, dev: int, dtype: int = _lib.BF16) -> int:
     """Floats of the workspace with which a scan cuts its sequences into segments; 0 where it does not."""
-    return _lib.load().nesle_delta_split_floats(_lib.DELTA_ARGS.pack(*(0,) * 25, t, n, h, dk, dv, 0.0, *(0,) * 12, dev))
+    sizes = _lib.DELTA_ARGS.pack(*(0,) * 12, dtype, *(0,) * 12, t, n, h, dk, dv, 0.0, *(0,) * 12, dev)
+    return _lib.load().nesle_delta_split_floats(sizes)
 
 
 class _DeltaScan(torch.autograd.Function):
@@ -383,7 +384,7 @@ class _DeltaScan(torch.autograd.Function):
             ctx.save_for_backward(q, k, v, g, beta, reset, errors, checkpoints)
             ctx.scale, ctx.has_state, ctx.dev = scale, state is not None, dev
             ctx.set_materialize_grads(False)
-        split = _scan_split(t, n, h, dk, dv, dev)
+        split = _scan_split(t, n, h, dk, dv, dev, _DTYPE[q.dtype])
         ends = torch.empty(split, dtype=torch.float32, device=device) if split else None
         _call("nesle_delta_scan_split",
               _scan_args(q, k, v, g, beta, reset, state, scale, dev, o.data_ptr(), final.data_ptr(), *kept),

@@ -544,3 +544,25 @@ def test_what_is_not_finite_reaches_no_earlier_token(t, dk, dv, dtype, name, val
         assert bool(finite.any()) and not bool(finite.all())
         assert torch.equal(torch.isfinite(got), finite), what
         close(torch.where(finite, got, 0), torch.where(finite, want, 0), dk, dv, what)
+
+
+def segments(t, n, h, d, dtype):
+    floats = ops._scan_split(t, n, h, d, d, torch.cuda.current_device(), ops._DTYPE[dtype])
+    return 1 + floats // (n * h * (2 * d * d + 1))
+
+
+@pytest.mark.gpu
+def test_cutting_goes_by_what_an_sm_holds_of_the_type():
+    """Heads of 128 in 16 and 32 bits by terms leave room for one block on an SM, in bfloat16 for two: sequences whose
+    segments would come one after another anyway are left whole."""
+    if torch.cuda.get_device_properties(0).multi_processor_count != 148:
+        pytest.skip("the counts are those of 148 SMs")
+    wide = (torch.bfloat16, torch.float16, torch.float32)
+    assert [segments(4096, 4, 4, 128, x) for x in wide] == [6, 8, 8]
+    assert [segments(512, 4, 4, 128, x) for x in wide] == [6, 3, 3]
+    assert [segments(4096, 4, 4, 64, x) for x in wide] == [15, 18, 18]
+    assert [segments(1024, 8, 4, 128, x) for x in wide] == [1, 1, 1]
+    assert [segments(4096, 12, 4, 128, x) for x in wide] == [3, 1, 1]
+    for dtype in wide:  # what is cut so is the recurrence still
+        check(inputs(512, 4, 4, 128, 128, dtype, 0.003, seed=35), train=False)
+        check(inputs(1040, 1, 1, 64, 64, dtype, 0.003, seed=36), train=False)
