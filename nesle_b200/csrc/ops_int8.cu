@@ -573,18 +573,22 @@ int run(const nesle_int8_args& a, cudaStream_t st) {
     Epilogue ep{a.x_scale, a.x_scale_value, a.w_scale, a.bias, a.y, a.ld_y, (uint32_t)a.m, (uint32_t)a.k, (uint32_t)a.n, a.relu};
     const uint8_t* x = static_cast<const uint8_t*>(a.x);
     int64_t ld_x = a.ld_x;
-    if (a.m <= kFewTokens || !a.k) {  // k = 0 is the bias alone
-        const uint64_t gy = (a.m + 15) / 16;
-        if (gy > 65535) {  // only with k = 0
-            return invalid("int8_linear: k = 0 with more than a million tokens");
-        }
-        const dim3 grid(static_cast<unsigned>((a.n + 7) / 8), static_cast<unsigned>(gy));
+    if (a.m <= kFewTokens || !a.k) {  // k = 0 is the bias alone, of any number of tokens
         const uint8_t* w = reinterpret_cast<const uint8_t*>(a.w);
-        if (aligned_x(a))
-            int8_few_kernel<kUnsigned, Out, true><<<grid, 256, 0, st>>>(x, a.ld_x, w, a.ld_w, ep);
-        else
-            int8_few_kernel<kUnsigned, Out, false><<<grid, 256, 0, st>>>(x, a.ld_x, w, a.ld_w, ep);
-        return cuda_status(cudaGetLastError(), "int8_linear");
+        constexpr uint64_t kMost = 65535 * 16;  // tokens of a grid
+        for (uint64_t first = 0; first < a.m; first += kMost) {
+            Epilogue part = ep;
+            part.m = static_cast<uint32_t>(a.m - first < kMost ? a.m - first : kMost);
+            part.x_scale = ep.x_scale ? ep.x_scale + first : nullptr;
+            part.y = static_cast<Out*>(ep.y) + static_cast<int64_t>(first) * ep.ld_y;
+            const dim3 grid(static_cast<unsigned>((a.n + 7) / 8), (part.m + 15) / 16);
+            if (aligned_x(a))
+                int8_few_kernel<kUnsigned, Out, true><<<grid, 256, 0, st>>>(x, a.ld_x, w, a.ld_w, part);
+            else
+                int8_few_kernel<kUnsigned, Out, false><<<grid, 256, 0, st>>>(x, a.ld_x, w, a.ld_w, part);
+            if (int rc = cuda_status(cudaGetLastError(), "int8_linear")) return rc;
+        }
+        return NESLE_OK;
     }
     if (!aligned_x(a)) {
         ld_x = static_cast<int64_t>(padded(a.k));

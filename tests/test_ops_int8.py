@@ -364,3 +364,14 @@ def test_an_out_that_wants_a_gradient_is_refused():
         ops.int8_linear(x, w, 1.0, out=out)
     with torch.no_grad():
         assert torch.equal(ops.int8_linear(x, w, 1.0, out=out), ops.int8_linear(x, w, 1.0, out_dtype=torch.float32))
+
+
+@pytest.mark.gpu
+def test_no_columns_and_more_tokens_than_a_grid_holds():
+    m, n = 65535 * 16 + 21, 6
+    q, ws = _weight(n, 32, 1)
+    bias = torch.arange(float(n), device="cuda")
+    out = torch.full((m, 8), 7.0, device="cuda", dtype=torch.bfloat16)
+    ops.int8_linear(torch.empty((m, 0), dtype=torch.int8, device="cuda"), ops.Int8Weight(q[:, :0], ws), torch.ones(m, device="cuda"),
+                    bias, out=out[:, 1:7])
+    assert torch.equal(out[:, 1:7], bias.to(torch.bfloat16).expand(m, n)) and bool((out[:, 0] == 7).all() and (out[:, 7] == 7).all())
