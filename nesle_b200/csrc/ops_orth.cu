@@ -135,7 +135,8 @@ __global__ void __launch_bounds__(256) scale_kernel(const T* __restrict__ x, int
     sum = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += part[i];
-    const double factor = static_cast<double>(kScale) / (sqrt(sum) + eps);
+    const double norm = sqrt(sum) + eps;
+    const double factor = norm == 0 ? 0 : static_cast<double>(kScale) / norm;  // a matrix of zeros with eps = 0 stays zero
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
         const int i = threadIdx.x + k * 256, r = by_row ? i / 64 : i % 64, c = by_row ? i % 64 : i / 64;

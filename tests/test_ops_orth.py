@@ -189,3 +189,14 @@ def test_an_out_that_wants_a_gradient_is_refused():
         ops.orthogonalize(momentum(8, 12), out=out)
     with torch.no_grad():
         assert torch.equal(ops.orthogonalize(momentum(8, 12), out=out), ops.orthogonalize(momentum(8, 12)))
+
+
+@pytest.mark.gpu
+def test_a_zero_matrix_stays_zero_without_eps():
+    x = momentum(3, 40, 30, seed=13)
+    x[1] = 0
+    out = ops.orthogonalize(x, eps=0.0)
+    assert int((out[1] != 0).sum()) == 0
+    check(out[::2], x[::2])
+    x[1, 0, 0] = float("nan")
+    assert bool(torch.isnan(ops.orthogonalize(x, eps=0.0)[1]).all())
