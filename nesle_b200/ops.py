@@ -321,7 +321,9 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
         raise ValueError(f"state must be float32 of shape {(n, h, dk, dv)}")
     s_n, s_h, s_k, s_v = state.stride()
     _require((s_v == 1 or dv == 1) and (s_k == dv or dk == 1), "state's matrices must be contiguous")
-    _require((n <= 1 or s_n >= dk * dv) and (h <= 1 or s_h >= dk * dv), "state's matrices must not overlap")
+    inner, outer = (s_n * (n - 1), s_h) if h > 1 and (n <= 1 or s_n <= s_h) else (s_h * (h - 1), s_n)
+    _require((n <= 1 or s_n >= dk * dv) and (h <= 1 or s_h >= dk * dv) and (n * h <= 1 or outer >= inner + dk * dv),
+             "state's matrices must not overlap")
     given, fresh = None, out is None
     if fresh:
         out = torch.empty((n, h, dv), dtype=q.dtype, device=q.device)

@@ -566,3 +566,19 @@ def test_cutting_goes_by_what_an_sm_holds_of_the_type():
     for dtype in wide:  # what is cut so is the recurrence still
         check(inputs(512, 4, 4, 128, 128, dtype, 0.003, seed=35), train=False)
         check(inputs(1040, 1, 1, 64, 64, dtype, 0.003, seed=36), train=False)
+
+
+@pytest.mark.gpu
+def test_states_that_overlap_are_refused():
+    x = inputs(1, 3, 2, 4, 5, seed=37)
+    one = [x[i][0] for i in NAMES[:5]]
+    room = torch.zeros(200, device="cuda")
+    for strides in ((20, 20), (20, 40), (39, 20), (20, 50), (19, 100), (100, 19)):
+        with pytest.raises(ValueError, match="overlap"):
+            ops.delta_step(*one, room.as_strided((3, 2, 4, 5), (*strides, 5, 1)))
+    want = x["state"].clone()
+    o = ops.delta_step(*one, want)
+    for strides in ((40, 20), (20, 60), (41, 20), (21, 63)):  # either dimension may be the outer one
+        state = torch.zeros(200, device="cuda").as_strided((3, 2, 4, 5), (*strides, 5, 1))
+        state.copy_(x["state"])
+        assert torch.equal(ops.delta_step(*one, state), o) and torch.equal(state, want)
