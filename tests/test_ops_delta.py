@@ -572,7 +572,7 @@ def test_cutting_goes_by_what_an_sm_holds_of_the_type():
 def test_states_that_overlap_are_refused():
     x = inputs(1, 3, 2, 4, 5, seed=37)
     one = [x[i][0] for i in NAMES[:5]]
-    room = torch.zeros(200, device="cuda")
+    room = torch.zeros(300, device="cuda")
     for strides in ((20, 20), (20, 40), (39, 20), (20, 50), (19, 100), (100, 19)):
         with pytest.raises(ValueError, match="overlap"):
             ops.delta_step(*one, room.as_strided((3, 2, 4, 5), (*strides, 5, 1)))
