@@ -3,6 +3,7 @@
     m <- momentum m + grad;  u = grad + momentum m (nesterov) or m
     W <- (1 - lr weight_decay) W - lr sqrt(max(1, rows / cols)) orthogonalize(u)
 
+Momentum is a running sum and is kept in fp32 whatever the parameters' type.
 Matrices of one shape are orthogonalised as one batch
 (:func:`nesle_b200.ops.orthogonalize`).  Vectors, embeddings and output layers
 belong to another optimiser.  No counterpart in the reference.
@@ -33,6 +34,15 @@ class Muon(torch.optim.Optimizer):
                 if p.dim() != 2:
                     raise ValueError(f"Muon takes matrices, got a parameter of shape {tuple(p.shape)}")
 
+    def load_state_dict(self, state_dict) -> None:
+        super().load_state_dict(state_dict)
+        # torch has cast the state to the parameters' type
+        saved = [i for group in state_dict["param_groups"] for i in group["params"]]
+        for i, p in zip(saved, (p for group in self.param_groups for p in group["params"])):
+            momentum = state_dict["state"].get(i, {}).get("momentum")
+            if momentum is not None:
+                self.state[p]["momentum"] = momentum.to(device=p.device, dtype=torch.float32, copy=True)
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -50,7 +60,7 @@ class Muon(torch.optim.Optimizer):
                 for p in params:
                     state = self.state[p]
                     if "momentum" not in state:
-                        state["momentum"] = torch.zeros_like(p, memory_format=torch.contiguous_format)
+                        state["momentum"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                     buffers.append(state["momentum"])
                 torch._foreach_mul_(buffers, group["momentum"])
                 torch._foreach_add_(buffers, grads)

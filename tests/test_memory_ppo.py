@@ -134,3 +134,30 @@ def test_a_reset_clears_the_memory_of_its_env(cuda):
         assert torch.equal(x, y)
     # a memory decayed from nothing is nothing; the others are untouched by the flag
     assert torch.equal(kept, cleared)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_muon_keeps_its_momentum_in_32_bits(cuda, dtype):
+    """A running sum of 40 gradients: each step rounds it twice, to 2^-24 of at most 20 gradients of below 6."""
+    from nesle_b200.muon import Muon
+
+    gen = torch.Generator("cuda").manual_seed(5)
+    params = [torch.nn.Parameter(torch.randn(s, generator=gen, device="cuda").to(dtype)) for s in ((48, 96), (48, 96), (7, 5))]
+    opt = Muon(params, lr=0.01, momentum=0.95)
+    want = [torch.zeros(p.shape, device="cuda", dtype=torch.float64) for p in params]
+    for _ in range(40):
+        for i, p in enumerate(params):
+            p.grad = torch.randn(p.shape, generator=gen, device="cuda").to(dtype)
+            want[i] = 0.95 * want[i] + p.grad.double()
+        opt.step()
+    for p, x in zip(params, want):
+        got = opt.state[p]["momentum"]
+        assert got.dtype == torch.float32 and p.dtype == dtype and bool(torch.isfinite(p).all())
+        assert float((got.double() - x).abs().max()) <= 40 * 2 * 2.0 ** -24 * 120
+    again = Muon([torch.nn.Parameter(p.detach().clone()) for p in params], lr=0.5)
+    again.load_state_dict(opt.state_dict())
+    assert again.param_groups[0]["lr"] == 0.01
+    for p, x in zip(again.param_groups[0]["params"], params):
+        a, b = again.state[p]["momentum"], opt.state[x]["momentum"]
+        assert a.dtype == torch.float32 and torch.equal(a, b) and a.data_ptr() != b.data_ptr()
