@@ -212,12 +212,18 @@ class MemoryPPOTrainer(PPOTrainer):
 
 def train_memory_ppo(config: MemoryPPOConfig, iterations: int, workload: w.Workload | None = None,
                      device: int = 0) -> list[float]:
-    """Single-GPU training loop; returns the mean loss of every iteration."""
+    """Single-GPU training loop; returns the mean loss of every iteration.  Raises where an operator's kernel has given up
+    on a wait, whose outputs are invalid."""
+    from . import ops
+
     trainer = MemoryPPOTrainer(config, workload, device=device)
     out = []
+    stalls = ops.stalls(device)
     t0 = time.perf_counter()
     for it in range(iterations):
         out.append(float(trainer.iteration()["loss"]))
+        if ops.stalls(device) != stalls:  # beside the read of the loss, which has waited for the device
+            raise RuntimeError(f"a kernel gave up on an internal wait in iteration {it + 1}: its results are invalid")
         fps = trainer.global_step / max(1e-9, time.perf_counter() - t0)
         print(f"iteration={it + 1}/{iterations} step={trainer.global_step} loss={out[-1]:.4f} fps={fps:.0f}", flush=True)
     trainer.batch.synchronize()

@@ -161,3 +161,22 @@ def test_muon_keeps_its_momentum_in_32_bits(cuda, dtype):
     for p, x in zip(again.param_groups[0]["params"], params):
         a, b = again.state[p]["momentum"], opt.state[x]["momentum"]
         assert a.dtype == torch.float32 and torch.equal(a, b) and a.data_ptr() != b.data_ptr()
+
+
+def test_training_stops_where_a_kernel_has_given_up(monkeypatch):
+    """The counter is read once an iteration; what it held before does not count."""
+    from types import SimpleNamespace
+
+    from nesle_b200 import memory_ppo, ops
+
+    done = []
+    trainer = SimpleNamespace(iteration=lambda: done.append(1) or {"loss": 1.0}, global_step=0,
+                              batch=SimpleNamespace(synchronize=lambda: None))
+    monkeypatch.setattr(memory_ppo, "MemoryPPOTrainer", lambda *a, **k: trainer)
+    monkeypatch.setattr(ops, "stalls", lambda device: 3)
+    assert memory_ppo.train_memory_ppo(None, 4) == [1.0] * 4
+    done.clear()
+    monkeypatch.setattr(ops, "stalls", lambda device: 3 + (len(done) >= 2))
+    with pytest.raises(RuntimeError, match="iteration 2"):
+        memory_ppo.train_memory_ppo(None, 4)
+    assert len(done) == 2
