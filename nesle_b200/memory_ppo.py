@@ -234,11 +234,12 @@ def main(argv=None) -> int:
     ap = argparse.ArgumentParser(description="Recurrent PPO on the batched core")
     ap.add_argument("--envs", type=int, default=2048)
     ap.add_argument("--steps", type=int, default=128)
-    ap.add_argument("--batch", type=int, default=8192, help="samples of a minibatch: whole sequences of --steps")
+    ap.add_argument("--batch", type=int, default=8192, help="samples of a minibatch at most (one sequence at least): whole sequences of --steps")
     ap.add_argument("--iterations", type=int, default=4)
     ap.add_argument("--device", type=int, default=0)
     args = ap.parse_args(argv)
-    train_memory_ppo(MemoryPPOConfig(num_envs=args.envs, n_steps=args.steps, batch_size=min(args.batch, args.envs * args.steps)),
+    sequences = max(1, min(args.batch // args.steps, args.envs))
+    train_memory_ppo(MemoryPPOConfig(num_envs=args.envs, n_steps=args.steps, batch_size=sequences * args.steps),
                      args.iterations, device=args.device)
     return 0
 

@@ -180,3 +180,15 @@ def test_training_stops_where_a_kernel_has_given_up(monkeypatch):
     with pytest.raises(RuntimeError, match="iteration 2"):
         memory_ppo.train_memory_ppo(None, 4)
     assert len(done) == 2
+
+
+@pytest.mark.parametrize("envs,steps,batch,want", [(2048, 128, 8192, 8192), (2048, 100, 8192, 8100), (256, 32, 8192, 8192), (48, 5, 8192, 240),
+                                                   (3, 100, 64, 100)])
+def test_the_command_takes_any_number_of_steps(monkeypatch, envs, steps, batch, want):
+    """Minibatches of whole sequences, as many as --batch holds."""
+    from nesle_b200 import memory_ppo
+
+    seen = []
+    monkeypatch.setattr(memory_ppo, "train_memory_ppo", lambda config, iterations, device: seen.append(config))
+    assert memory_ppo.main(["--envs", str(envs), "--steps", str(steps), "--batch", str(batch)]) == 0
+    assert (seen[0].num_envs, seen[0].n_steps, seen[0].batch_size) == (envs, steps, want)
