@@ -6,7 +6,8 @@
  * policy a memory over time, and the Newton-Schulz orthogonalisation of matrix
  * updates.  No counterpart in the reference.
  *
- * All pointers are device memory of `device`.  Calls are asynchronous on
+ * All pointers are device memory of `device`, aligned to their elements (a
+ * pointer that is not is an invalid argument).  Calls are asynchronous on
  * `stream` (a cudaStream_t as void*, NULL = the legacy default stream), allocate
  * nothing and can be captured in a CUDA graph; scratch memory is the caller's.
  * Status codes and nesle_last_error() are those of nesle_b200.h.

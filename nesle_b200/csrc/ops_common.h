@@ -28,6 +28,13 @@ inline int cuda_status(cudaError_t e, const char* where) {
     return set_error(NESLE_ERR_CUDA, (std::string(where) + ": " + cudaGetErrorString(e)).c_str());
 }
 
+// Whether every pointer lies on `bytes`, as loads of elements of that size want it.
+template <class... P>
+bool all_on(uintptr_t bytes, P... pointers) {
+    return (... && (reinterpret_cast<uintptr_t>(pointers) % bytes == 0));
+}
+inline uintptr_t element_size(int dtype) { return dtype == NESLE_F32 ? 4 : 2; }
+
 // Runs a C entry's body: no C++ exception leaves the library.
 template <class F>
 int guarded(F&& body) noexcept {

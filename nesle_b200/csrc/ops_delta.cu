@@ -205,6 +205,8 @@ int nesle_delta_step(const nesle_delta_step_args* args, void* stream) {
         if (const char* why = delta::check_common(a.dtype, a.n, a.h, a.dk, a.dv)) return invalid(why);
         if (!a.n || !a.h) return NESLE_OK;
         if (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.state || !a.o) return invalid("delta_step: null argument");
+        if (!all_on(element_size(a.dtype), a.q, a.k, a.v, a.o) || !all_on(4, a.g, a.beta, a.state))
+            return invalid("delta_step: arguments must be aligned to their elements");
         OnDevice on(a.device);
         if (!on.ok) return invalid("delta_step: device ordinal out of range");
         const delta::Step p{a.q, a.k, a.v, a.q_n, a.q_h, a.k_n, a.k_h, a.v_n, a.v_h, a.g, a.beta, a.g_n, a.g_h, a.beta_n, a.beta_h,
@@ -245,11 +247,13 @@ int nesle_delta_scan_split(const nesle_delta_args* args, float* workspace, void*
         if (const char* why = delta::check_common(a.dtype, a.n, a.h, a.dk, a.dv)) return invalid(why);
         if (!a.n || !a.h) return NESLE_OK;
         if (a.t && (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.o)) return invalid("delta_scan: null argument");
+        if (!all_on(element_size(a.dtype), a.q, a.k, a.v, a.o) || !all_on(4, a.g, a.beta, a.state, a.final_state, a.checkpoints))
+            return invalid("delta_scan: arguments must be aligned to their elements");
+        if (!a.errors != !a.checkpoints) return invalid("delta_scan: errors and checkpoints go together");
+        if (!all_on(16, a.errors)) return invalid("delta_scan: errors must be 16-byte aligned");
+        if (!all_on(4, workspace)) return invalid("delta_scan: workspace must be aligned");
         OnDevice on(a.device);
         if (!on.ok) return invalid("delta_scan: device ordinal out of range");
-        if (!a.errors != !a.checkpoints) return invalid("delta_scan: errors and checkpoints go together");
-        if (reinterpret_cast<uintptr_t>(a.errors) % 16) return invalid("delta_scan: errors must be 16-byte aligned");
-        if (reinterpret_cast<uintptr_t>(workspace) % 4) return invalid("delta_scan: workspace must be aligned");
         delta::Scan p = delta::to_scan(a, false);
         if (workspace && a.t && a.t <= 0x7FFFFFFFull) {
             p.segments = delta::segments_of(a);
@@ -276,10 +280,12 @@ int nesle_delta_scan_backward(const nesle_delta_args* args, void* stream) {
         if (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.d_o || !a.errors || !a.checkpoints || !a.dq || !a.d_k || !a.d_v || !a.dg ||
             !a.dbeta)
             return invalid("delta_scan_backward: null argument");
+        if (!all_on(element_size(a.dtype), a.q, a.k, a.v, a.d_o, a.dq, a.d_k, a.d_v) ||
+            !all_on(4, a.g, a.beta, a.d_final, a.dg, a.dbeta, a.dstate))
+            return invalid("delta_scan_backward: arguments must be aligned to their elements");
+        if (!all_on(16, a.errors, a.checkpoints)) return invalid("delta_scan_backward: errors and checkpoints must be 16-byte aligned");
         OnDevice on(a.device);
         if (!on.ok) return invalid("delta_scan_backward: device ordinal out of range");
-        if (reinterpret_cast<uintptr_t>(a.errors) % 16 || reinterpret_cast<uintptr_t>(a.checkpoints) % 16)
-            return invalid("delta_scan_backward: errors and checkpoints must be 16-byte aligned");
         delta::Scan p = delta::to_scan(a, true);
         if (int rc = stall_counter(a.device, &p.stalls)) return rc;
         cudaStream_t st = static_cast<cudaStream_t>(stream);

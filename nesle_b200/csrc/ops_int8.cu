@@ -531,6 +531,7 @@ const char* check(const nesle_int8_args& a) {
     if (a.ld_w % 16 || reinterpret_cast<uintptr_t>(a.w) % 16 || reinterpret_cast<uintptr_t>(a.w_biased) % 16)
         return "int8_linear: weights must be 16-byte aligned with rows a multiple of 16 bytes apart";
     if (a.y_dtype != NESLE_F32 && a.y_dtype != NESLE_BF16 && a.y_dtype != NESLE_F16) return "int8_linear: unknown output type";
+    if (!all_on(4, a.x_scale, a.w_scale, a.bias) || !all_on(element_size(a.y_dtype), a.y)) return "int8_linear: scales, bias and y must be aligned to their elements";
     return nullptr;
 }
 
@@ -625,6 +626,7 @@ int nesle_quantize_rows(const void* x, int dtype, uint64_t rows, uint64_t cols, 
         if (ld_x < (int64_t)cols || ld_q < (int64_t)cols || ld_q - (int64_t)cols >= 16)
             return ops::invalid("quantize_rows: a leading dimension is shorter than its row, or ld_q 16 or more longer");
         if (rows > 0x7FFFFFFFull) return ops::invalid("quantize_rows: too many rows");
+        if (!ops::all_on(4, scale) || !ops::all_on(ops::element_size(dtype), x)) return ops::invalid("quantize_rows: x and scale must be aligned to their elements");
         ops::OnDevice on(device);
         if (!on.ok) return ops::invalid("quantize_rows: device ordinal out of range");
         cudaStream_t st = static_cast<cudaStream_t>(stream);

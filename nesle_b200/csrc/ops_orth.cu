@@ -900,6 +900,7 @@ int nesle_orthogonalize(const nesle_orth_args* args, void* stream) {
         if (!a.batch || !a.rows || !a.cols) return NESLE_OK;
         if (!a.x || !a.out) return ops::invalid("orthogonalize: null argument");
         if (reinterpret_cast<uintptr_t>(a.out) % 16) return ops::invalid("orthogonalize: out must be 16-byte aligned");
+        if (!ops::all_on(ops::element_size(a.dtype), a.x)) return ops::invalid("orthogonalize: x must be aligned to its elements");
         if (!a.workspace || a.workspace_bytes < nesle_orth_workspace(args) || reinterpret_cast<uintptr_t>(a.workspace) % 256)
             return ops::invalid("orthogonalize: the workspace is missing, too small or not 256-byte aligned");
         ops::OnDevice on(a.device);

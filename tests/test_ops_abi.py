@@ -123,3 +123,37 @@ def test_tangents_are_refused_and_not_dropped():
         with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):
             ops._no_grad_path("call", dual)
         ops._no_grad_path("call", x, forward_ad.unpack_dual(dual).primal)
+
+
+def test_pointers_off_their_elements_are_refused(lib):
+    """Before a device is touched: a load there would fault.  Every pointer in turn, one byte off, or two where it is to 4-byte
+    elements; the others are right, and sizes and strides those of a call that runs."""
+    P = 1 << 20  # a pointer that only its alignment is looked at of
+
+    def refused(call, names, elements):
+        for i, name in enumerate(names):
+            for off in {1, elements[i] // 2}:
+                args = [P + off if i == j else P for j in range(len(names))]
+                assert call(*args) == _lib.NESLE_ERR_INVALID, (name, off)
+                assert b"aligned" in lib.nesle_last_error(), (name, off, lib.nesle_last_error())
+
+    for dtype, size in ((0, 4), (1, 2), (2, 2)):
+        refused(lambda x, scale: lib.nesle_quantize_rows(x, dtype, 4, 8, 8, P, 16, scale, 0, None), ("x", "scale"), (size, 4))
+        refused(lambda xs, ws, bias, y: lib.nesle_int8_linear(
+            _lib.INT8_ARGS.pack(P, 1, 16, xs, 1.0, P, P, 16, ws, bias, y, dtype, 8, 4, 16, 8, 0, 0, 0, 0), None),
+            ("x_scale", "w_scale", "bias", "y"), (4, 4, 4, size))
+        refused(lambda x: lib.nesle_orthogonalize(_lib.ORTH_ARGS.pack(x, dtype, 16, 4, 1, 1, 4, 4, 5, 1e-7, P, P, 1 << 30, 0), None),
+                ("x",), (size,))
+        refused(lambda q, k, v, g, beta, state, o: lib.nesle_delta_step(
+            _lib.DELTA_STEP_ARGS.pack(q, k, v, *(16,) * 6, dtype, g, beta, *(1,) * 4, 0, 0, state, 256, 256, o, 2, 1, 16, 16, 1.0, 0), None),
+            ("q", "k", "v", "g", "beta", "state", "o"), (size, size, size, 4, 4, 4, size))
+
+        def scan(entry, q, k, v, g, beta, state, *rest):
+            return entry(_lib.DELTA_ARGS.pack(q, k, v, *(32, 16, 16) * 3, dtype, g, beta, *(2, 1, 1) * 2, 0, 0, 0, state, 4, 2, 1, 16, 16,
+                                              1.0, *rest, *(0,) * (12 - len(rest)), 0), None)
+
+        names = ("q", "k", "v", "g", "beta", "state", "o", "final_state", "errors", "checkpoints")
+        refused(lambda *p: scan(lib.nesle_delta_scan, *p), names, (size, size, size, 4, 4, 4, size, 4, 16, 4))
+        names = ("q", "k", "v", "g", "beta", "errors", "checkpoints", "d_o", "d_final", "dq", "d_k", "d_v", "dg", "dbeta", "dstate")
+        refused(lambda *p: scan(lib.nesle_delta_scan_backward, *p[:5], 0, 0, 0, *p[5:]), names,
+                (size, size, size, 4, 4, 16, 16, size, 4, size, size, size, 4, 4, 4))
