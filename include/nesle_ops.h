@@ -22,6 +22,10 @@
 extern "C" {
 #endif
 
+/* An output of nesle_int8_linear or nesle_delta_step lies on the memory of another argument, or may: it is told from the first
+ * and the last byte of each, and for rows as far apart as one another (two columns of one record) from their place in a row. */
+#define NESLE_ERR_OVERLAP 4
+
 #define NESLE_F32 0
 #define NESLE_BF16 1
 #define NESLE_F16 2
@@ -62,7 +66,7 @@ typedef struct nesle_int8_args {
 
 /* y[m][n] = act(x_scale[m] w_scale[n] sum_k x[m][k] w[n][k] + bias[n]); the sum is exact in 32-bit integers, which
  * bounds k: 33,025 for unsigned x (255 * 255 k < 2^31), 131,071 for signed (128 * 128 k < 2^31).  y shares no memory with the
- * other arguments. */
+ * other arguments (NESLE_ERR_OVERLAP). */
 int nesle_int8_linear(const nesle_int8_args* args, void* stream);
 /* Scratch bytes that the call needs (0 where x is 16-byte aligned with rows a multiple of 16 bytes apart). */
 uint64_t nesle_int8_workspace(const nesle_int8_args* args);
@@ -107,7 +111,8 @@ typedef struct nesle_delta_step_args {
 
 /* One token of every env and head, with the state updated in place:
  * S0 = reset ? 0 : exp(g) S;  u = beta (v - S0^T k);  S = S0 + k u^T;  o = scale S^T q.
- * state and o share no memory with one another or with the inputs: a head's q and k are read while others' o is written. */
+ * o shares no memory with the other arguments (NESLE_ERR_OVERLAP), and state none with the inputs: a head's q and k are read
+ * while others' o and state are written.  The states' matrices do not overlap. */
 int nesle_delta_step(const nesle_delta_step_args* args, void* stream);
 
 typedef struct nesle_delta_args {

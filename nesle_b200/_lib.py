@@ -14,7 +14,7 @@ import numpy as np
 PKG = Path(__file__).resolve().parent
 LIB_PATH = PKG / "libnesle_b200.so"
 
-NESLE_OK, NESLE_ERR_INVALID, NESLE_ERR_RUNTIME, NESLE_ERR_CUDA = 0, 1, 2, 3
+NESLE_OK, NESLE_ERR_INVALID, NESLE_ERR_RUNTIME, NESLE_ERR_CUDA, NESLE_ERR_OVERLAP = 0, 1, 2, 3, 4
 DONE_SMB, DONE_RAM_EQ, DONE_FRAME_LIMIT = 0, 1, 2
 ACTIONS_U8, ACTIONS_I64 = 0, 1
 RENDER_RGB, RENDER_INDEX, RENDER_GRAY84 = 0, 1, 2
@@ -189,7 +189,7 @@ def check(rc: int, lib=None) -> None:
         return
     lib = lib or load()
     msg = lib.nesle_last_error().decode()
-    if rc == NESLE_ERR_INVALID:
+    if rc in (NESLE_ERR_INVALID, NESLE_ERR_OVERLAP):
         raise ValueError(msg)
     raise RuntimeError(msg)
 

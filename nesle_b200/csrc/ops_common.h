@@ -33,6 +33,22 @@ template <class... P>
 bool all_on(uintptr_t bytes, P... pointers) {
     return (... && (reinterpret_cast<uintptr_t>(pointers) % bytes == 0));
 }
+// Memory of `rows` rows of `bytes`, `pitch` apart.
+struct Memory {
+    uintptr_t at;
+    uint64_t rows;
+    int64_t pitch;
+    uint64_t bytes;
+    Memory(const void* p, uint64_t rows_, int64_t pitch_, uint64_t bytes_) : at(reinterpret_cast<uintptr_t>(p)), rows(rows_), pitch(pitch_), bytes(bytes_) {}
+    uintptr_t end() const { return at && rows && bytes ? at + (rows - 1) * pitch + bytes : at; }
+};
+// Whether two may share a byte.
+inline bool may_overlap(const Memory& a, const Memory& b) {
+    if (a.at >= b.end() || b.at >= a.end()) return false;
+    if (a.pitch != b.pitch || a.pitch <= 0) return true;
+    const uint64_t pitch = a.pitch, d = b.at >= a.at ? (b.at - a.at) % pitch : (pitch - (a.at - b.at) % pitch) % pitch;
+    return d < a.bytes || d + b.bytes > pitch;  // b's rows begin d after a's, modulo the pitch
+}
 inline uintptr_t element_size(int dtype) { return dtype == NESLE_F32 ? 4 : 2; }
 
 // Runs a C entry's body: no C++ exception leaves the library.

@@ -207,6 +207,15 @@ int nesle_delta_step(const nesle_delta_step_args* args, void* stream) {
         if (!a.q || !a.k || !a.v || !a.g || !a.beta || !a.state || !a.o) return invalid("delta_step: null argument");
         if (!all_on(element_size(a.dtype), a.q, a.k, a.v, a.o) || !all_on(4, a.g, a.beta, a.state))
             return invalid("delta_step: arguments must be aligned to their elements");
+        const int64_t size = element_size(a.dtype);
+        auto heads = [&](const void* p, int64_t sn, int64_t sh, uint64_t bytes, int64_t element) {  // from the first to the last byte
+            return Memory(p, 1, 0, ((a.n - 1) * sn + (a.h - 1) * sh) * element + bytes);
+        };
+        const Memory o(a.o, 1, 0, a.n * a.h * a.dv * size);
+        for (const Memory& x : {heads(a.q, a.q_n, a.q_h, a.dk * size, size), heads(a.k, a.k_n, a.k_h, a.dk * size, size),
+                                heads(a.v, a.v_n, a.v_h, a.dv * size, size), heads(a.g, a.g_n, a.g_h, 4, 4), heads(a.beta, a.beta_n, a.beta_h, 4, 4),
+                                heads(a.state, a.state_n, a.state_h, a.dk * a.dv * 4, 4), Memory(a.reset, 1, 0, (a.n - 1) * a.reset_n + 1)})
+            if (may_overlap(o, x)) return set_error(NESLE_ERR_OVERLAP, "delta_step: o shares memory with another argument");
         OnDevice on(a.device);
         if (!on.ok) return invalid("delta_step: device ordinal out of range");
         const delta::Step p{a.q, a.k, a.v, a.q_n, a.q_h, a.k_n, a.k_h, a.v_n, a.v_h, a.g, a.beta, a.g_n, a.g_h, a.beta_n, a.beta_h,

@@ -651,6 +651,11 @@ int nesle_int8_linear(const nesle_int8_args* args, void* stream) {
         const nesle_int8_args& a = *args;
         if (const char* why = ops::check(a)) return ops::invalid(why);
         if (!a.m || !a.n) return NESLE_OK;
+        const int64_t size = ops::element_size(a.y_dtype);
+        const ops::Memory y(a.y, a.m, a.ld_y * size, a.n * size);
+        for (const ops::Memory& x : {ops::Memory(a.x, a.m, a.ld_x, a.k), ops::Memory(a.x_scale, 1, 0, a.m * 4), ops::Memory(a.bias, 1, 0, a.n * 4),
+                                     ops::Memory(a.w, a.n, a.ld_w, a.k), ops::Memory(a.w_biased, a.n, a.ld_w, a.k), ops::Memory(a.w_scale, 1, 0, a.n * 4)})
+            if (ops::may_overlap(y, x)) return set_error(NESLE_ERR_OVERLAP, "int8_linear: y shares memory with another argument");
         const uint64_t need = nesle_int8_workspace(args);
         if (need && (!a.workspace || a.workspace_bytes < need || reinterpret_cast<uintptr_t>(a.workspace) % 16))
             return ops::invalid("int8_linear: the workspace is missing, too small or not 16-byte aligned");

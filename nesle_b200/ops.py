@@ -60,29 +60,23 @@ def _no_grad_path(name: str, *tensors) -> None:
                 raise ValueError(f"{name} has no forward-mode derivative; call it on primal tensors")
 
 
-def _span(x: torch.Tensor) -> tuple[int, int]:
-    """The first byte of a tensor and the one after its last."""
-    first = x.data_ptr()
-    if not x.numel():
-        return first, first
-    return first, first + (1 + sum((n - 1) * s for n, s in zip(x.shape, x.stride()))) * x.element_size()
-
-
-def _shares_memory(out: torch.Tensor, *others) -> bool:
-    """Whether ``out`` may lie on memory of the others, which a kernel may still read when it writes ``out``; such a call
-    writes elsewhere and copies."""
-    first, end = _span(out)
-    for x in others:
-        if x is not None:
-            a, b = _span(x)
-            if a < end and first < b:
-                return True
-    return False
-
-
 def _call(name: str, args: bytes, *rest: int) -> None:
     lib = _lib.load()
     rc = getattr(lib, name)(args, *rest)
+    if rc:
+        _lib.check(rc, lib)
+
+
+def _call_out(name: str, args, out: torch.Tensor, ld: int, stream: int) -> None:
+    """``args(pointer, ld)`` is the call's block for an output there.  An ``out`` on the memory of an input, which the kernel
+    may still read when it writes, is written last: by a copy."""
+    lib = _lib.load()
+    rc = getattr(lib, name)(args(out.data_ptr(), ld), stream)
+    if rc == _lib.NESLE_ERR_OVERLAP:
+        elsewhere = torch.empty(out.shape, dtype=out.dtype, device=out.device)
+        rc = getattr(lib, name)(args(elsewhere.data_ptr(), max(elsewhere.shape[-1], 1)), stream)
+        if not rc:
+            out.copy_(elsewhere)
     if rc:
         _lib.check(rc, lib)
 
@@ -204,7 +198,7 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
         _require(bias.dtype == torch.float32 and bias.shape == (n,), f"bias must be float32 of shape ({n},)")
         bias = bias.detach().contiguous()
         bias_ptr = bias.data_ptr()
-    given, fresh = None, out is None
+    fresh = out is None
     if fresh:
         _require(out_dtype in _DTYPE, "out_dtype must be float32, bfloat16 or float16")
         out = torch.empty((*shape, n), dtype=out_dtype, device=x.device)
@@ -216,18 +210,17 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
         ld_y = out.stride(0) if out.dim() == 2 and m > 1 else max(n, 1)
         _require(out.dim() != 2 or out.stride(1) == 1 or n <= 1, "out must have unit column stride")
         _require(ld_y >= n, "out's rows must not overlap")
-        if _shares_memory(out, x, bias, x_scale if scale_ptr else None):
-            given, out, ld_y = out, torch.empty(out.shape, dtype=out.dtype, device=out.device), max(n, 1)
     x_ptr = x.data_ptr()
     # many rows that do not lie on 16 bytes are laid out again in scratch memory (as much as nesle_int8_workspace says)
     need = m * (-(-k // 16) * 16) if m > 64 and (x_ptr % 16 or ld_x % 16) else 0
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-    _call("nesle_int8_linear",
-          _lib.INT8_ARGS.pack(x_ptr, unsigned, ld_x, scale_ptr, scale_value, weight.q.data_ptr(), weight.biased.data_ptr(),
-                              weight.ld, weight.scale.data_ptr(), bias_ptr, out.data_ptr(), _DTYPE[out.dtype], ld_y, m, k, n,
-                              relu, scratch.data_ptr() if need else 0, need, dev), _stream(dev))
-    if given is not None:
-        return given.copy_(out)
+
+    def args(y, ld):
+        return _lib.INT8_ARGS.pack(x_ptr, unsigned, ld_x, scale_ptr, scale_value, weight.q.data_ptr(), weight.biased.data_ptr(), weight.ld,
+                                   weight.scale.data_ptr(), bias_ptr, y, _DTYPE[out.dtype], ld, m, k, n, relu,
+                                   scratch.data_ptr() if need else 0, need, dev)
+
+    _call_out("nesle_int8_linear", args, out, ld_y, _stream(dev))
     if not fresh:
         _written(out)
     return out
@@ -324,25 +317,22 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     inner, outer = (s_n * (n - 1), s_h) if h > 1 and (n <= 1 or s_n <= s_h) else (s_h * (h - 1), s_n)
     _require((n <= 1 or s_n >= dk * dv) and (h <= 1 or s_h >= dk * dv) and (n * h <= 1 or outer >= inner + dk * dv),
              "state's matrices must not overlap")
-    given, fresh = None, out is None
+    fresh = out is None
     if fresh:
         out = torch.empty((n, h, dv), dtype=q.dtype, device=q.device)
     else:
         _on(out, dev, "out")
         _require(out.dtype == q.dtype and out.shape == (n, h, dv) and out.is_contiguous(),
                  f"out must be contiguous {q.dtype} of shape {(n, h, dv)}")
-        if _shares_memory(out, q, k, v, g, beta, reset, state):
-            given, out = out, torch.empty_like(out)
     q, k, v = _unit(q), _unit(k), _unit(v)
     reset_ptr, reset_n = (0, 0) if reset is None else (reset.data_ptr(), reset.stride(0))
-    _call("nesle_delta_step",
-          _lib.DELTA_STEP_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
-                                    _DTYPE[q.dtype], g.data_ptr(), beta.data_ptr(), *g.stride(), *beta.stride(), reset_ptr,
-                                    reset_n, state.data_ptr(), s_n, s_h, out.data_ptr(), n, h, dk, dv,
-                                    dk ** -0.5 if scale is None else scale, dev), _stream(dev))
-    if given is not None:
-        _written(state)
-        return given.copy_(out)
+
+    def args(o, _):
+        return _lib.DELTA_STEP_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
+                                         _DTYPE[q.dtype], g.data_ptr(), beta.data_ptr(), *g.stride(), *beta.stride(), reset_ptr,
+                                         reset_n, state.data_ptr(), s_n, s_h, o, n, h, dk, dv, dk ** -0.5 if scale is None else scale, dev)
+
+    _call_out("nesle_delta_step", args, out, dv, _stream(dev))
     _written(state if fresh else (state, out))
     return out
 

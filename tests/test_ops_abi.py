@@ -157,3 +157,33 @@ def test_pointers_off_their_elements_are_refused(lib):
         names = ("q", "k", "v", "g", "beta", "errors", "checkpoints", "d_o", "d_final", "dq", "d_k", "d_v", "dg", "dbeta", "dstate")
         refused(lambda *p: scan(lib.nesle_delta_scan_backward, *p[:5], 0, 0, 0, *p[5:]), names,
                 (size, size, size, 4, 4, 16, 16, size, 4, size, size, size, 4, 4, 4))
+
+
+def test_outputs_on_the_memory_of_an_input_are_refused(lib):
+    """At the C boundary; ops.py writes such an output elsewhere and copies.  The calls that this refuses reach no device."""
+    far = 1 << 40
+
+    def int8(y, **at):
+        p = {"x": far, "x_scale": 2 * far, "w": 3 * far, "w_biased": 4 * far, "w_scale": 5 * far, "bias": 6 * far, **at}
+        return lib.nesle_int8_linear(_lib.INT8_ARGS.pack(p["x"], 1, 2048, p["x_scale"], 1.0, p["w"], p["w_biased"], 512, p["w_scale"], p["bias"],
+                                                         y, _lib.F32, 512, 40, 512, 100, 0, 0, 0, 0), None)
+
+    y = 7 * far  # 40 rows of 400 bytes, 2,048 apart
+    for name, size in (("x_scale", 160), ("w", 99 * 512 + 512), ("w_biased", 99 * 512 + 512), ("w_scale", 400), ("bias", 400)):
+        size = -(-size // 16) * 16
+        for at in (y, y + 39 * 2048 + 384, y - size + 16):
+            assert int8(y, **{name: at}) == _lib.NESLE_ERR_OVERLAP, (name, at - y)
+    # tokens, rows as far apart: bytes 0..511 of each against 0..399
+    for at in (y, y + 384, y - 496, y + 39 * 2048 + 384, y - 39 * 2048, y + 2048 - 496):
+        assert int8(y, x=at) == _lib.NESLE_ERR_OVERLAP, at - y
+    assert b"y shares memory" in lib.nesle_last_error()
+
+    def step(o, **at):  # 3 envs x 2 heads of 16 x 8, bf16
+        p = {"q": far, "k": 2 * far, "v": 3 * far, "g": 4 * far, "beta": 5 * far, "reset": 6 * far, "state": 7 * far, **at}
+        return lib.nesle_delta_step(_lib.DELTA_STEP_ARGS.pack(p["q"], p["k"], p["v"], 32, 16, 32, 16, 16, 8, _lib.BF16, p["g"], p["beta"], 2, 1, 2, 1,
+                                                              p["reset"], 1, p["state"], 256, 128, o, 3, 2, 16, 8, 1.0, 0), None)
+
+    o = 8 * far  # 96 bytes
+    for name, size in (("q", 192), ("k", 192), ("v", 96), ("g", 24), ("beta", 24), ("reset", 3), ("state", 3072)):
+        for at in (o, o + 92, o - (size - 1) // 4 * 4):
+            assert step(o, **{name: at}) == _lib.NESLE_ERR_OVERLAP, (name, at - o)
