@@ -67,20 +67,6 @@ def _call(name: str, args: bytes, *rest: int) -> None:
         _lib.check(rc, lib)
 
 
-def _call_out(name: str, args, out: torch.Tensor, ld: int, stream: int) -> None:
-    """``args(pointer, ld)`` is the call's block for an output there.  An ``out`` on the memory of an input, which the kernel
-    may still read when it writes, is written last: by a copy."""
-    lib = _lib.load()
-    rc = getattr(lib, name)(args(out.data_ptr(), ld), stream)
-    if rc == _lib.NESLE_ERR_OVERLAP:
-        elsewhere = torch.empty(out.shape, dtype=out.dtype, device=out.device)
-        rc = getattr(lib, name)(args(elsewhere.data_ptr(), max(elsewhere.shape[-1], 1)), stream)
-        if not rc:
-            out.copy_(elsewhere)
-    if rc:
-        _lib.check(rc, lib)
-
-
 def stalls(device: int = 0) -> int:
     """Times that a kernel gave up on an internal wait (0 unless something is broken); synchronises."""
     n = ctypes.c_uint32()
@@ -214,14 +200,18 @@ def int8_linear(x: torch.Tensor, weight: Int8Weight, x_scale: torch.Tensor | flo
     # many rows that do not lie on 16 bytes are laid out again in scratch memory (as much as nesle_int8_workspace says)
     need = m * (-(-k // 16) * 16) if m > 64 and (x_ptr % 16 or ld_x % 16) else 0
     scratch = torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
-
-    def args(y, ld):
-        return _lib.INT8_ARGS.pack(x_ptr, unsigned, ld_x, scale_ptr, scale_value, weight.q.data_ptr(), weight.biased.data_ptr(), weight.ld,
-                                   weight.scale.data_ptr(), bias_ptr, y, _DTYPE[out.dtype], ld, m, k, n, relu,
-                                   scratch.data_ptr() if need else 0, need, dev)
-
-    _call_out("nesle_int8_linear", args, out, ld_y, _stream(dev))
-    if not fresh:
+    lib = _lib.load()
+    rc = lib.nesle_int8_linear(
+        _lib.INT8_ARGS.pack(x_ptr, unsigned, ld_x, scale_ptr, scale_value, weight.q.data_ptr(), weight.biased.data_ptr(),
+                            weight.ld, weight.scale.data_ptr(), bias_ptr, out.data_ptr(), _DTYPE[out.dtype], ld_y, m, k, n,
+                            relu, scratch.data_ptr() if need else 0, need, dev), _stream(dev))
+    if rc:
+        if rc != _lib.NESLE_ERR_OVERLAP or fresh:
+            _lib.check(rc, lib)
+        # tiles still read the memory when others write it: the results go there last
+        y = int8_linear(x, weight, x_scale.flatten() if scale_ptr else x_scale, bias, relu=relu, out_dtype=out.dtype)
+        out.copy_(y.view(out.shape))
+    elif not fresh:
         _written(out)
     return out
 
@@ -326,14 +316,19 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
                  f"out must be contiguous {q.dtype} of shape {(n, h, dv)}")
     q, k, v = _unit(q), _unit(k), _unit(v)
     reset_ptr, reset_n = (0, 0) if reset is None else (reset.data_ptr(), reset.stride(0))
-
-    def args(o, _):
-        return _lib.DELTA_STEP_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
-                                         _DTYPE[q.dtype], g.data_ptr(), beta.data_ptr(), *g.stride(), *beta.stride(), reset_ptr,
-                                         reset_n, state.data_ptr(), s_n, s_h, o, n, h, dk, dv, dk ** -0.5 if scale is None else scale, dev)
-
-    _call_out("nesle_delta_step", args, out, dv, _stream(dev))
-    _written(state if fresh else (state, out))
+    lib = _lib.load()
+    rc = lib.nesle_delta_step(
+        _lib.DELTA_STEP_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), *q.stride()[:2], *k.stride()[:2], *v.stride()[:2],
+                                  _DTYPE[q.dtype], g.data_ptr(), beta.data_ptr(), *g.stride(), *beta.stride(), reset_ptr,
+                                  reset_n, state.data_ptr(), s_n, s_h, out.data_ptr(), n, h, dk, dv,
+                                  dk ** -0.5 if scale is None else scale, dev), _stream(dev))
+    if rc:
+        if rc != _lib.NESLE_ERR_OVERLAP or fresh:
+            _lib.check(rc, lib)
+        # a head's other warps still read q and k when one writes its columns: the results go there last
+        out.copy_(delta_step(q, k, v, g, beta, state, reset, scale=scale))
+    else:
+        _written(state if fresh else (state, out))
     return out
 
 
