@@ -449,56 +449,57 @@ struct Fetch {
     }
 };
 
-// Which tokens of fetched tiles hold a NaN or an infinity: 0 * x adds up to zero over all else.  A lane adds up its 16-byte
-// chunks, sum z those of token 4 z + lane / 8.
+// Whether fetched tiles hold a NaN or an infinity: 0 * x adds up to zero over all else.
 template <class T>
 struct NotFinite {
     using Two = std::conditional_t<sizeof(T) == 4, float, std::conditional_t<std::is_same_v<T, __half>, __half2, __nv_bfloat162>>;
-    Two sum[4];
-    __device__ __forceinline__ NotFinite() {
-#pragma unroll
-        for (int z = 0; z < 4; ++z) sum[z] = zero();
-    }
+    Two sum[4] = {zero(), zero(), zero(), zero()};
     static __device__ __forceinline__ Two zero() {
         const uint32_t bits = 0;
         return reinterpret_cast<const Two&>(bits);
-    }
-    static __device__ __forceinline__ bool bad(Two x) {
-        if constexpr (sizeof(T) == 4)
-            return x != x;
-        else
-            return !(to_f32(x.x) + to_f32(x.y) == 0.f);  // zeros but for a NaN
     }
     template <int D>
     __device__ __forceinline__ void add(const T* tile, int lane) {
         const uint4* chunks = reinterpret_cast<const uint4*>(tile);
 #pragma unroll
-        for (int i = 0; i < Fetch<T, D>::kPanels; ++i)
+        for (int i = 0; i < Fetch<T, D>::kPanels * 4; ++i) {
+            const uint4 x = chunks[i * 32 + lane];
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                const uint4 x = chunks[i * kC * 8 + z * 32 + lane];
-                const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    if constexpr (sizeof(T) == 4)
-                        sum[z] = fmaf(__uint_as_float(w[j]), 0.f, sum[z]);
-                    else
-                        sum[z] = __hfma2(reinterpret_cast<const Two&>(w[j]), zero(), sum[z]);
-                }
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (sizeof(T) == 4)
+                    sum[i % 4] = fmaf(__uint_as_float(w[j]), 0.f, sum[i % 4]);
+                else
+                    sum[i % 4] = __hfma2(reinterpret_cast<const Two&>(w[j]), zero(), sum[i % 4]);
             }
+        }
     }
-    // Bit i for token i; `gate`, of lane i, is NaN where token i's gates are not finite.
-    __device__ __forceinline__ uint32_t tokens(float gate) const {
+    static __device__ __forceinline__ float joined(Two x) {
+        if constexpr (sizeof(T) == 4)
+            return x;
+        else
+            return to_f32(x.x) + to_f32(x.y);
+    }
+    // Of the warp's lanes; `more` is a lane's own sum of this kind.
+    __device__ __forceinline__ bool any(float more) const {
+        more += joined((sum[0] + sum[1]) + (sum[2] + sum[3]));
+        return __any_sync(0xffffffffu, more != more);
+    }
+    // Which tokens of a tile, bit i for token i: a token's chunks are 8 lanes', those of four tokens a warp's.  Rare, and
+    // out of line for the registers of all else.
+    template <int D>
+    static __device__ __noinline__ uint32_t tokens(const T* tile, int lane) {
         uint32_t out = 0;
-        const Two all = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (__any_sync(0xffffffffu, bad(all) || gate != gate)) {
-            out = __ballot_sync(0xffffffffu, gate != gate);
+#pragma unroll 1
+        for (int i = 0; i < Fetch<T, D>::kPanels * 4; ++i) {
+            const uint4 x = reinterpret_cast<const uint4*>(tile)[i * 32 + lane];
+            const T* v = reinterpret_cast<const T*>(&x);
+            float f = 0.f;
 #pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                const uint32_t lanes = __ballot_sync(0xffffffffu, bad(sum[z]));
+            for (int j = 0; j < 16 / (int)sizeof(T); ++j) f = fmaf(to_f32(v[j]), 0.f, f);
+            const uint32_t lanes = __ballot_sync(0xffffffffu, f != f);
 #pragma unroll
-                for (int g = 0; g < 4; ++g) out |= (lanes >> 8 * g & 0xFF ? 1u : 0u) << (z * 4 + g);
-            }
+            for (int g = 0; g < 4; ++g) out |= (lanes >> 8 * g & 0xFF ? 1u : 0u) << (i % 4 * 4 + g);
         }
         return out;
     }
@@ -611,7 +612,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
         const GatePointers get_gates(p, n, h, lane);
         Gates gates{}, next = get_gates.load(t0, p.t, lane);
         float decay = 1.f;
-        uint32_t starts = 0, cuts = 0;  // tokens that start an episode, and that begin a chunk for another reason
+        uint32_t starts = 0;  // bit i: token i starts an episode; bit 16 + i: it begins a chunk for another reason
         int64_t b = -1;
         int r0 = 0, count = 0, restarts = 0;
         for (int turn = 0;; ++turn) {
@@ -643,10 +644,16 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
                 if constexpr (!kEnds) {
                     // A token whose key, value or gates are not finite begins a chunk: the products of a chunk multiply it by
                     // the zeros that stand for "later" too, and would spoil the tokens before it.
+                    const T *tk = raw_tile(b), *tv = tk + 2 * L::kTileK;
+                    const float gate = (decay + gates.beta) * 0.f;
                     NotFinite<T> look;
-                    look.template add<DK>(raw_tile(b), lane);
-                    look.template add<L::kWidth>(raw_tile(b) + 2 * L::kTileK, lane);
-                    cuts = look.tokens((decay + gates.beta) * 0.f) & ((1u << count) - 1);
+                    look.template add<DK>(tk, lane);
+                    look.template add<L::kWidth>(tv, lane);
+                    if (look.any(gate)) {
+                        const uint32_t bad = look.template tokens<DK>(tk, lane) | look.template tokens<L::kWidth>(tv, lane) |
+                                             __ballot_sync(0xffffffffu, gate != gate);
+                        starts |= (bad & ((1u << count) - 1)) << 16;
+                    }
                 }
                 if constexpr (!L::kInPlace) {
                     __nv_bfloat16* to = terms + (b & 1) * 2 * NT * kC * L::kLdTerm;
@@ -657,7 +664,7 @@ __global__ void __launch_bounds__((kForwardWarps + 1) * 32, DK == 128 ? 2 : 3)
             }
             const bool fresh = starts >> r0 & 1;
             restarts |= fresh;
-            const uint32_t later = (starts | cuts) & ~((2u << r0) - 1);
+            const uint32_t later = (starts | starts >> 16) & ~((2u << r0) - 1);
             const int r1 = later ? min(count, __ffs(later) - 1) : count;
             chunk_decays(hs.d, ch.gamma, ch.eta, ch.beta, ch.keep, within(lane, r0, r1) ? decay : 1.f, gates.beta, r0, r1, fresh, lane);
             if (lane == 0) ch.block = (int)b, ch.r0 = r0, ch.r1 = r1, ch.fresh = fresh;
