@@ -16,8 +16,8 @@ namespace {
 // A warp takes 32 columns of one state: a lane holds 4 neighbouring columns of
 // every fourth row, all loads in flight at once; S^T k and S^T q are summed in
 // one pass and joined over the 4 row groups by shuffles.  No shared memory but
-// the two vectors, no barrier.  2,048 envs x 4 heads of 64 x 64: 47.9 us,
-// 5.7 TB/s, 87% of a copy.
+// the two vectors, no barrier.  2,048 envs x 4 heads of 64 x 64: 49.4 us,
+// 5.5 TB/s, 84% of a copy.
 struct Step {
     const void *q, *k, *v;
     int64_t q_n, q_h, k_n, k_h, v_n, v_h;

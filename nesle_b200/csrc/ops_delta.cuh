@@ -313,10 +313,13 @@ __device__ __forceinline__ uint32_t pair_mask(int i, int r0, int r1) {
 // solve is a product too.  One barrier a chunk.
 //
 // 1,024 envs x 4 heads x 128 tokens of 64 x 64, keeping states and errors for
-// the gradients: 298 us, 3.6 TB/s; instruction issue bounds it (44% of the slots
-// at 13 warps an SM).  4 envs x 4 heads x 4,096 tokens of 128 x 128: 250 us in
-// 6 segments (count_segments), 525 in one: 2.05 us a chunk where a block has an SM
-// to itself, a chain of products as long as the helper's work.
+// the gradients: 298 us, 3.6 TB/s, 314 with an episode's end in 200 tokens (an end
+// makes two chunks of one).  No unit is full (44% of the issue slots at 13 warps an
+// SM): a chunk is a chain of dependent products, and that many warps hide no more
+// of it.  4 envs x 4 heads x 4,096 tokens of 128 x 128: 249 us in 6 segments
+// (count_segments), 523 in one: 2.05 us a chunk where a block has an SM to itself, a
+// chain of products as long as the helper's work.  The look for tokens that are not
+// finite costs nothing there, 1 to 2% with 16 and 32 bits by terms, 4% with ragged values.
 
 constexpr int kLdM = kC + 8;  // bf16 of a row of a 16 x 16 operand tile
 
@@ -1083,9 +1086,10 @@ __global__ void __launch_bounds__(kJoinThreads) scan_join_kernel(const Scan p) {
 // from the checkpoint.  A helper prepares the next chunk (decays, Q K^T, K K^T,
 // N) and finishes dg and dbeta of the last.  Two barriers a chunk.
 //
-// 1,024 envs x 4 heads x 128 tokens of 64 x 64: 769 us, bounded by instruction
-// latency at 10 warps an SM (168 registers a thread, 100 KB of shared memory a
-// block): 36% of the issue slots, tensor cores 20% busy.
+// 1,024 envs x 4 heads x 128 tokens of 64 x 64: 762 us, 831 with an episode's end in
+// 200 tokens.  No unit is full (36% of the issue slots, tensor cores 20% busy): 10
+// warps an SM (168 registers a thread, 100 KB of shared memory a block) wait for
+// their own chains of products.
 
 struct alignas(16) BackChunk {
     __nv_bfloat16 n[3][kC][kLdM];    // N, by terms
@@ -1785,8 +1789,9 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
                         for (int x = 0; x < 3; ++x) ya[x][z] = tmp[x];
                     }
                 }
-                // Of large heads dS comes back from shared memory: its registers are the others' in between (128 x 128: 364
-                // bytes of spills without, 196 with; 64 x 64 has few and is 8% faster without).
+                // Of large heads dS comes back from shared memory: its registers are the others' in between (128 x 128 spills
+                // 160 bytes a thread, 44 in the regular kernel, and spilled about twice as much without when that was measured;
+                // 64 x 64 has few and is 8% faster without).
                 constexpr bool kBack = DK > 64 || DV > 64;
 #pragma unroll
                 for (int i = 0; i < DK / 8; ++i)
@@ -1826,8 +1831,8 @@ __global__ void __launch_bounds__((DK > DV ? DK : DV) * 2 + 32, DK <= 64 && DV <
 
 // Heads that fill their tiles, of tensors a tiled copy may fetch and 16-byte stores may write, take the
 // kRegular kernels: the same code with every test of a ragged edge decided when it is compiled. 1,024 sequences
-// x 4 heads x 128 steps of 64 in bfloat16 take 298 and 769 us forwards and back, with the tests 307 and 814; 256
-// x 2 heads of 128 backwards 322 and 411.
+// x 4 heads x 128 steps of 64 in bfloat16 took 298 and 769 us forwards and back when that was split off, with the
+// tests 307 and 814; 256 x 2 heads of 128 backwards 322 and 411.
 inline bool on_16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // How many segments a few long sequences are cut into; 1 where that gains nothing.

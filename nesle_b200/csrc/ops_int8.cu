@@ -13,10 +13,11 @@ namespace {
 //
 // One pass: a row's 16-byte chunks stay in registers between the maximum and
 // the rounding (4 chunks a thread; longer rows are read again, from L2).
-// Memory bound: 65,536 x 1,024 bf16 64 us, 3.1 TB/s; small calls are a launch
-// (2,048 x 512 bf16: 6.8 us).  Rows that are not aligned come element by
-// element (65,536 x 1,021: 122 us; 32 elements a thread and a warp a row, to
-// do without the block's barrier, took 135).  The maximum is taken on the bit
+// 65,536 x 1,024 bf16: 62 us, 3.2 TB/s, half of what a copy reaches: the
+// conversions, products, roundings and tests of an element take 65% of the issue
+// slots.  Small calls are a launch (2,048 x 512 bf16: 6.4 us).  Rows that are not
+// aligned come element by element (65,536 x 1,021: 109 us; 32 elements a thread
+// and a warp a row, to do without the block's barrier, was a tenth slower).  The maximum is taken on the bit
 // patterns of |x|, where a NaN is above infinity and infinity above every
 // number, so that a row with either says so in its scale.
 
@@ -38,7 +39,7 @@ struct Chunk {
 // rint(x / s), the quotient rounded to fp32 first, of a row whose largest magnitude is 127 s.  x times the reciprocal of s is
 // within 3 roundings of the quotient, 127 * 3 * 2^-24 < 2^-14, so that only a chunk with a product this near to half an integer
 // is divided (and all where s is below the normal numbers, whose reciprocal may be infinite); and a sum with 1.5 * 2^23
-// has the nearest integer in its low bits.  65,536 x 1,024 bf16: 76 us by divisions and conversions, 64 so.  Only a scale
+// has the nearest integer in its low bits.  65,536 x 1,024 bf16: 76 us by divisions and conversions, 62 so.  Only a scale
 // below the normal numbers is rounded so coarsely that a quotient passes 127 (190 units over 127 round to one unit); such
 // rows are divided, and clamped there.
 struct Divisor {

@@ -422,8 +422,9 @@ __device__ __forceinline__ void emit_block(const Job& job, uint32_t batch, uint3
 
 // One tile by a cluster of kSplit blocks, each over its share of k; every block sends the others their columns of its
 // fp32 sums and adds up its own from all, in the order of the ranks.  (Fetching them from the others' shared memory took
-// 4,000 to 6,000 clocks, sending them takes 1,400.)  A product of a 256 x 256 matrix takes 6 to 8 us, of which its slices are 3,
-// the epilogue 1 to 2 and the rest starting and draining.
+// 4,000 to 6,000 clocks, sending them takes 1,400.)  A product of a 256 x 256 matrix takes 7 to 8 us by itself
+// (ncu) and 5.5 in its chain, where a launch starts under the one before: its slices are 3, the epilogue 1 to 2
+// and the rest starting and draining.
 template <int kProduct, int kBN, int kSplit>
 __global__ void __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, Job job, unsigned int* stalls) {
@@ -574,7 +575,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Large matrices: tiles of 256 x 256, one a block, two accumulators of 128 x 256 that fill tensor memory.  What bounds
 // the 128 x 128 tiles is their operands' way from L2 (48 bytes a clock and SM when all SMs read): 64 KB for 768 clocks of
 // products.  Here 64 KB, a slice of 32, feed 1,536 clocks.  2,048 x 2,048 by 2,048 x 4,096: 87 us for three products,
-// 1.2 PFLOP/s.
+// 1.2 PFLOP/s, 70% of what a bf16 library product reaches here.
 struct Wide {
     static constexpr uint32_t kSide = 256, kSlice = 32;
     static constexpr int kStages = 3;
