@@ -12,7 +12,9 @@ actor-critic on the batched core computes beside the env step.
 
 Calls go on the caller's current torch stream, return before the work is done,
 and never synchronise the host.  Argument errors raise ValueError, CUDA errors
-RuntimeError.  There is no CPU fallback: tensors must be on a CUDA device.
+RuntimeError.  There is no CPU fallback: tensors must be on a CUDA device.  They
+are read as they lie in memory: a lazily negated view (``Tensor.is_neg``) is to be
+resolved first.
 No counterpart in the reference.
 """
 from __future__ import annotations
@@ -118,7 +120,8 @@ def quantize_rows(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
 
 class Int8Weight:
     """A weight matrix ``(n, k)`` in 8 bits with a scale for each channel, laid out once for :func:`int8_linear`: rows
-    padded with zeros to a multiple of 16 bytes, and the same matrix + 128 as unsigned bytes for unsigned tokens."""
+    padded with zeros to a multiple of 16 bytes, and the same matrix + 128 as unsigned bytes for unsigned tokens.  A copy,
+    without gradients."""
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor):
         dev = _cuda_device(q, "q")
@@ -414,7 +417,8 @@ def delta_scan(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     the last is 1); ``g, beta``: (t, n, h) float32; ``state``: (n, h, dk, dv) float32 before the first token, or None for
     zeros; ``reset``: (t, n) bool or uint8, True where a token starts an episode: nothing before it, not even a NaN,
     reaches it, and no gradient passes.  A NaN or an infinity in a token reaches no earlier one (in the gradients it may
-    spoil all tokens of its episode).  States and sums are fp32 throughout.  With gradients a call keeps one state for
+    spoil all tokens of its episode).  States and sums are fp32 throughout; products take them as sums of bfloat16, whose
+    largest number, 3.39e38, is the largest that counts as finite.  With gradients a call keeps one state for
     every 16 tokens until its backward pass."""
     dev = _delta_inputs(q, k, v, g, beta, reset, "tnh")
     t, n, h, dk = q.shape
