@@ -82,7 +82,7 @@ def _rows(x: torch.Tensor) -> tuple[torch.Tensor, int]:
     """(..., cols) as (rows, cols) with unit column stride and rows that do not overlap, and the rows' distance; copies
     only where the layout has to change.  Where a stride carries no meaning (one row, or none) it is the row length."""
     if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1])
+        x = x.reshape(x.shape[:-1].numel(), x.shape[-1])  # not -1, which says nothing where there are no columns
     rows, cols = x.shape
     ld, unit = x.stride()
     if (unit != 1 and cols > 1) or (ld < cols and rows > 1):

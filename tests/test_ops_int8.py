@@ -375,3 +375,21 @@ def test_no_columns_and_more_tokens_than_a_grid_holds():
     ops.int8_linear(torch.empty((m, 0), dtype=torch.int8, device="cuda"), ops.Int8Weight(q[:, :0], ws), torch.ones(m, device="cuda"),
                     bias, out=out[:, 1:7])
     assert torch.equal(out[:, 1:7], bias.to(torch.bfloat16).expand(m, n)) and bool((out[:, 0] == 7).all() and (out[:, 7] == 7).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lead", [(), (3,), (2, 3), (2, 0, 4), (0,), (0, 5)])
+@pytest.mark.parametrize("k", [0, 1, 20])
+@pytest.mark.parametrize("dtype", [torch.uint8, torch.int8, torch.bfloat16])
+def test_any_leading_dimensions_and_none(lead, k, dtype):
+    q, ws = _weight(6, k, 3) if k else (torch.empty((6, 0), dtype=torch.int8, device="cuda"), torch.ones(6, device="cuda"))
+    w, bias = ops.Int8Weight(q, ws), torch.arange(6.0, device="cuda")
+    x = torch.randint(0, 50, (*lead, k), generator=_gen(2), device="cuda").to(dtype)
+    scale = None if dtype == torch.bfloat16 else torch.full(lead, 0.5, device="cuda")
+    y = ops.int8_linear(x, w, scale, bias, out_dtype=torch.float32)
+    assert y.shape == (*lead, 6)
+    xq, xs = (x, scale) if scale is not None else ops.quantize_rows(x)
+    assert xq.shape == x.shape and xs.shape == torch.Size(lead)
+    rows = max(1, torch.Size(lead).numel()) if not lead else torch.Size(lead).numel()
+    if rows:
+        _check(y.reshape(rows, 6), xq.reshape(rows, k), xs.reshape(rows, 1).double(), q, ws, bias, False)
