@@ -52,7 +52,7 @@ class Muon(torch.optim.Optimizer):
         for group in self.param_groups:
             alike: dict[tuple, list[torch.Tensor]] = {}
             for p in group["params"]:
-                if p.grad is not None:
+                if p.grad is not None and p.numel():
                     alike.setdefault((p.shape, p.dtype, p.device), []).append(p)
             for (shape, _, _), params in alike.items():
                 grads = [p.grad for p in params]

@@ -192,3 +192,15 @@ def test_the_command_takes_any_number_of_steps(monkeypatch, envs, steps, batch, 
     monkeypatch.setattr(memory_ppo, "train_memory_ppo", lambda config, iterations, device: seen.append(config))
     assert memory_ppo.main(["--envs", str(envs), "--steps", str(steps), "--batch", str(batch)]) == 0
     assert (seen[0].num_envs, seen[0].n_steps, seen[0].batch_size) == (envs, steps, want)
+
+
+@pytest.mark.gpu
+def test_muon_passes_over_matrices_without_elements(cuda):
+    from nesle_b200.muon import Muon
+
+    params = [torch.nn.Parameter(torch.randn(s, device="cuda")) for s in ((4, 0), (0, 4), (3, 5))]
+    before = params[2].detach().clone()
+    for p in params:
+        p.grad = torch.randn_like(p)
+    Muon(params).step()
+    assert not torch.equal(params[2].detach(), before)
