@@ -231,6 +231,7 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, eps: float = 1e-7,
     dev = _cuda_device(update, "update")
     _require(update.dtype in _DTYPE, "update must be float32, bfloat16 or float16")
     _require(update.dim() >= 2, "update must have at least two dimensions")
+    _require(1 <= steps < 1 << 31 and int(steps) == steps, "steps must be a whole number, at least 1")
     _no_grad_path("orthogonalize", update, out)
     rows, cols = update.shape[-2:]
     fresh = out is None
@@ -243,7 +244,7 @@ def orthogonalize(update: torch.Tensor, *, steps: int = 5, eps: float = 1e-7,
     x = update if update.dim() == 3 else update.reshape(-1, rows, cols) if out.numel() else update.new_empty((0, rows, cols))
 
     def args(scratch=0, size=0):
-        return _lib.ORTH_ARGS.pack(x.data_ptr(), _DTYPE[x.dtype], *x.stride(), *x.shape, steps, eps, out.data_ptr(), scratch,
+        return _lib.ORTH_ARGS.pack(x.data_ptr(), _DTYPE[x.dtype], *x.stride(), *x.shape, int(steps), eps, out.data_ptr(), scratch,
                                    size, dev)
 
     need = _lib.load().nesle_orth_workspace(args())

@@ -200,3 +200,12 @@ def test_a_zero_matrix_stays_zero_without_eps():
     check(out[::2], x[::2])
     x[1, 0, 0] = float("nan")
     assert bool(torch.isnan(ops.orthogonalize(x, eps=0.0)[1]).all())
+
+
+@pytest.mark.gpu
+def test_steps_that_are_no_count_are_refused():
+    x = momentum(8, 12)
+    for steps in (2.5, 0, -3, 1 << 40, float("nan")):
+        with pytest.raises(ValueError, match="steps"):
+            ops.orthogonalize(x, steps=steps)
+    assert torch.equal(ops.orthogonalize(x, steps=5.0), ops.orthogonalize(x))
